@@ -21,6 +21,7 @@
 #include "dbs.h"
 #include "dbs_device.h"
 #include "engine.h"
+#include "logits.h"
 
 using dbs_host::CallConstraints;
 using dbs_host::ExampleSpec;
@@ -1838,6 +1839,164 @@ DBS_EXPORT int dbs_device_backward_sparse_noalloc(DBSDecoderHandle* handle, int 
         dbs_host::backward_sparse_noalloc(opt, vocab_size, batch_size, steps, in, bo,
                                           static_cast<cudaStream_t>(cuda_stream));
         clear_error(handle);
+        return 0;
+    });
+}
+
+// ---------------------------------------------------------------------------
+// Operators on rows of logits
+// ---------------------------------------------------------------------------
+static dbs_logits::Rows logits_rows(const void* logits, int data_type, int64_t rows, int vocab_size,
+                                    int64_t row_stride) {
+    if (data_type != DBS_DTYPE_F32 && data_type != DBS_DTYPE_F16 && data_type != DBS_DTYPE_BF16)
+        throw std::invalid_argument("unknown data type");
+    const int64_t size = data_type == DBS_DTYPE_F32 ? 4 : 2;
+    if (rows < 0) throw std::invalid_argument("rows cannot be negative");
+    if (vocab_size <= 0) throw std::invalid_argument("vocab_size must be positive");
+    if (vocab_size * size > dbs_logits::kMaxRowBytes)
+        throw std::invalid_argument("a row of logits takes at most 3000000 bytes");
+    if (row_stride < 0) throw std::invalid_argument("row_stride cannot be negative");
+    if (rows > 0 && !logits) throw std::invalid_argument("logits cannot be null");
+    if (reinterpret_cast<uintptr_t>(logits) % static_cast<uintptr_t>(size) != 0)
+        throw std::invalid_argument("logits are not aligned to their type");
+    dbs_logits::Rows in;
+    in.x = logits;
+    in.dtype = data_type == DBS_DTYPE_F32 ? dbs_logits::kF32 : data_type == DBS_DTYPE_F16 ? dbs_logits::kF16
+                                                                                         : dbs_logits::kBF16;
+    in.rows = rows;
+    in.V = vocab_size;
+    in.stride = row_stride;
+    return in;
+}
+
+static void positive_temperature(float temperature) {
+    if (!(temperature > 0.0f) || !std::isfinite(temperature))
+        throw std::invalid_argument("temperature must be positive and finite");
+}
+
+DBS_EXPORT int dbs_device_sample(const void* logits, int data_type, int64_t rows, int vocab_size, int64_t row_stride,
+                                 const float* uniforms, const float* temperatures, float temperature,
+                                 const int32_t* top_ks, int top_k, const float* top_ps, float top_p,
+                                 const float* min_ps, float min_p, int32_t* tokens, void* cuda_stream) {
+    return guarded(nullptr, [&]() {
+        dbs_logits::SampleArgs a;
+        a.in = logits_rows(logits, data_type, rows, vocab_size, row_stride);
+        if (!temperatures && (!(temperature >= 0.0f) || !std::isfinite(temperature)))
+            throw std::invalid_argument("temperature must be finite and cannot be negative");
+        if (!top_ks && top_k < 0) throw std::invalid_argument("top_k cannot be negative");
+        if (!top_ps && !(top_p > 0.0f && top_p <= 1.0f)) throw std::invalid_argument("top_p must be in (0, 1]");
+        if (!min_ps && !(min_p >= 0.0f && min_p <= 1.0f)) throw std::invalid_argument("min_p must be in [0, 1]");
+        if (rows == 0) return 0;
+        if (!uniforms || !tokens) throw std::invalid_argument("uniforms and tokens cannot be null");
+        a.uniforms = uniforms;
+        a.temperature = temperatures;
+        a.temperature_all = temperature;
+        a.top_k = top_ks;
+        a.top_k_all = top_k;
+        a.top_p = top_ps;
+        a.top_p_all = top_p;
+        a.min_p = min_ps;
+        a.min_p_all = min_p;
+        a.tokens = tokens;
+        dbs_host::check_cuda(dbs_logits::launch_sample(a, static_cast<cudaStream_t>(cuda_stream)), "sample");
+        clear_error(nullptr);
+        return 0;
+    });
+}
+
+DBS_EXPORT int dbs_device_top_log_probs(const void* logits, int data_type, int64_t rows, int vocab_size,
+                                        int64_t row_stride, int n, float temperature, float* log_probs,
+                                        int32_t* tokens, void* cuda_stream) {
+    return guarded(nullptr, [&]() {
+        dbs_logits::TopArgs a;
+        a.in = logits_rows(logits, data_type, rows, vocab_size, row_stride);
+        positive_temperature(temperature);
+        if (n <= 0 || n > vocab_size || n > dbs_logits::kMaxTop)
+            throw std::invalid_argument("n must be in 1 .. min(vocab_size, 1024)");
+        if (rows == 0) return 0;
+        if (!log_probs || !tokens) throw std::invalid_argument("log_probs and tokens cannot be null");
+        a.n = n;
+        a.temperature = temperature;
+        a.log_probs = log_probs;
+        a.tokens = tokens;
+        dbs_host::check_cuda(dbs_logits::launch_top(a, static_cast<cudaStream_t>(cuda_stream)), "top_log_probs");
+        clear_error(nullptr);
+        return 0;
+    });
+}
+
+static dbs_logits::DistillArgs distill_args(const void* logits, int data_type, int64_t rows, int vocab_size,
+                                            int64_t row_stride, const float* teacher_log_probs,
+                                            const void* teacher_tokens, int token_bytes, int slots, float temperature,
+                                            int tail, int reduction, float scale, void* grad_logits) {
+    dbs_logits::DistillArgs a;
+    a.in = logits_rows(logits, data_type, rows, vocab_size, row_stride);
+    positive_temperature(temperature);
+    if (slots <= 0 || slots > dbs_logits::kMaxTop) throw std::invalid_argument("slots must be in 1 .. 1024");
+    if (token_bytes != 4 && token_bytes != 8) throw std::invalid_argument("token_bytes must be 4 or 8");
+    if (reduction != DBS_REDUCE_NONE && reduction != DBS_REDUCE_SUM && reduction != DBS_REDUCE_MEAN)
+        throw std::invalid_argument("unknown reduction");
+    if (!std::isfinite(scale)) throw std::invalid_argument("scale must be finite");
+    if (rows > 0 && (!teacher_log_probs || !teacher_tokens))
+        throw std::invalid_argument("teacher_log_probs and teacher_tokens cannot be null");
+    const uintptr_t size = data_type == DBS_DTYPE_F32 ? 4 : 2;
+    if (reinterpret_cast<uintptr_t>(grad_logits) % size != 0)
+        throw std::invalid_argument("grad_logits is not aligned to its type");
+    a.teacher_log_probs = teacher_log_probs;
+    a.teacher_tokens = teacher_tokens;
+    a.token_bytes = token_bytes;
+    a.n = slots;
+    a.temperature = temperature;
+    a.tail = tail;
+    a.reduction = reduction;
+    a.scale = scale;
+    a.grad = grad_logits;
+    return a;
+}
+
+DBS_EXPORT int dbs_device_distill(const void* logits, int data_type, int64_t rows, int vocab_size, int64_t row_stride,
+                                  const float* teacher_log_probs, const void* teacher_tokens, int token_bytes,
+                                  int slots, float temperature, int tail, int reduction, float scale,
+                                  float* row_losses, float* loss, int32_t* row_count, void* grad_logits,
+                                  void* cuda_stream) {
+    return guarded(nullptr, [&]() {
+        dbs_logits::DistillArgs a =
+            distill_args(logits, data_type, rows, vocab_size, row_stride, teacher_log_probs, teacher_tokens,
+                         token_bytes, slots, temperature, tail, reduction, scale, grad_logits);
+        if (rows > 0 && !row_losses) throw std::invalid_argument("row_losses cannot be null");
+        if (reduction != DBS_REDUCE_NONE && !loss) throw std::invalid_argument("a reduced loss needs a place");
+        if (reduction == DBS_REDUCE_MEAN && !row_count) throw std::invalid_argument("a mean needs a place for row_count");
+        a.row_losses = row_losses;
+        a.loss = loss;
+        a.row_count = row_count;
+        dbs_host::check_cuda(dbs_logits::launch_distill(a, static_cast<cudaStream_t>(cuda_stream)), "distill");
+        clear_error(nullptr);
+        return 0;
+    });
+}
+
+DBS_EXPORT int dbs_device_distill_backward(const void* logits, int data_type, int64_t rows, int vocab_size,
+                                           int64_t row_stride, const float* teacher_log_probs,
+                                           const void* teacher_tokens, int token_bytes, int slots, float temperature,
+                                           int tail, int reduction, float scale, const int32_t* row_count,
+                                           const float* grad_loss, int64_t grad_loss_stride, int flags,
+                                           void* grad_logits, void* cuda_stream) {
+    return guarded(nullptr, [&]() {
+        dbs_logits::DistillArgs a =
+            distill_args(logits, data_type, rows, vocab_size, row_stride, teacher_log_probs, teacher_tokens,
+                         token_bytes, slots, temperature, tail, reduction, scale, grad_logits);
+        if (grad_loss_stride < 0) throw std::invalid_argument("grad_loss_stride cannot be negative");
+        if ((flags & ~DBS_DEVICE_GRAD_UNIT) != 0) throw std::invalid_argument("unknown flags");
+        if (rows == 0) return 0;
+        if (!grad_loss || !grad_logits) throw std::invalid_argument("grad_loss and grad_logits cannot be null");
+        if (reduction == DBS_REDUCE_MEAN && !row_count) throw std::invalid_argument("a mean needs its row_count");
+        a.row_count = const_cast<int32_t*>(row_count);
+        a.grad_loss = grad_loss;
+        a.grad_loss_stride = grad_loss_stride;
+        a.skip_unit = (flags & DBS_DEVICE_GRAD_UNIT) != 0 ? 1 : 0;
+        dbs_host::check_cuda(dbs_logits::launch_distill_backward(a, static_cast<cudaStream_t>(cuda_stream)),
+                             "distill backward");
+        clear_error(nullptr);
         return 0;
     });
 }

@@ -190,6 +190,8 @@ bool compact_merge_applies(int max_K, int max_C, int max_ext, int max_N, bool ne
 // Kernel launches made by this library in this process (every launcher
 // counts the launches it queues).
 long long kernel_launch_count();
+// Counts one launch queued by another file's launcher; passes `err` on.
+cudaError_t count_launch(cudaError_t err);
 cudaError_t launch_weights(const DecodeParams& p, int max_T, int max_K, int max_P,
                            cudaStream_t stream);
 // Fused decode of a uniform batch without sequence constraints (rows

@@ -3934,6 +3934,7 @@ static cudaError_t counted(cudaError_t err) {
     return err;
 }
 long long kernel_launch_count() { return g_kernel_launches.load(std::memory_order_relaxed); }
+cudaError_t count_launch(cudaError_t err) { return counted(err); }
 
 static cudaError_t prefer_shared(const void* fn);
 

@@ -1,0 +1,81 @@
+// Operators on rows of raw logits [rows, V]: sampling, the best log-probs of
+// a row, and the distillation loss from a teacher's best log-probs.
+//
+// Every kernel gives one row to one thread-block cluster. The row is cut into
+// equal slices, one per CTA, each read from HBM once into that CTA's shared
+// memory; whatever needs the whole row (maximum, sums, thresholds, candidate
+// counts) crosses the cluster through distributed shared memory. Clusters are
+// persistent: cluster c takes rows c, c + n, c + 2n, ...
+#pragma once
+
+#include <cstdint>
+
+#include <cuda_runtime.h>
+
+namespace dbs_logits {
+
+enum DataType : int { kF32 = 0, kF16 = 1, kBF16 = 2 };
+
+// Limits of this implementation.
+constexpr int kMaxTop = 1024;                 // entries of a top list, slots of a teacher's row
+constexpr int64_t kMaxRowBytes = 3000000;      // a row has to fit 16 CTAs' shared memory
+
+struct Rows {
+    const void* x = nullptr;
+    int dtype = kF32;
+    int64_t rows = 0;
+    int V = 0;
+    int64_t stride = 0;   // elements between rows
+};
+
+struct SampleArgs {
+    Rows in;
+    const float* uniforms = nullptr;      // [rows]
+    // per-row settings (device, [rows]); null: the scalar below
+    const float* temperature = nullptr;
+    const int32_t* top_k = nullptr;
+    const float* top_p = nullptr;
+    const float* min_p = nullptr;
+    float temperature_all = 1.0f;
+    int top_k_all = 0;
+    float top_p_all = 1.0f;
+    float min_p_all = 0.0f;
+    int32_t* tokens = nullptr;            // [rows]
+};
+
+struct TopArgs {
+    Rows in;
+    int n = 0;
+    float temperature = 1.0f;
+    float* log_probs = nullptr;           // [rows, n]
+    int32_t* tokens = nullptr;            // [rows, n]
+};
+
+enum Reduction : int { kNone = 0, kSum = 1, kMean = 2 };
+
+struct DistillArgs {
+    Rows in;
+    const float* teacher_log_probs = nullptr;   // [rows, n]
+    const void* teacher_tokens = nullptr;       // [rows, n], int32 or int64
+    int token_bytes = 4;
+    int n = 0;
+    float temperature = 1.0f;
+    int tail = 1;
+    int reduction = kSum;
+    float scale = 1.0f;
+    float* row_losses = nullptr;                // [rows]; null: not written
+    float* loss = nullptr;                      // the reduced loss; null with kNone
+    int32_t* row_count = nullptr;               // kMean: rows with a teacher (written forward, read backward)
+    void* grad = nullptr;                       // [rows, V] contiguous, the logits' type; null: none
+    // backward: gradient of the loss (one value, or one for each row)
+    const float* grad_loss = nullptr;
+    int64_t grad_loss_stride = 0;
+    int skip_unit = 0;                          // grad holds the gradient for grad_loss = 1 already
+};
+
+cudaError_t launch_sample(const SampleArgs& a, cudaStream_t stream);
+cudaError_t launch_top(const TopArgs& a, cudaStream_t stream);
+cudaError_t launch_distill(const DistillArgs& a, cudaStream_t stream);
+cudaError_t launch_distill_backward(const DistillArgs& a, cudaStream_t stream);
+
+}  // namespace dbs_logits

@@ -1,0 +1,1556 @@
+// sm_100a kernels of the operators on rows of raw logits (see logits.h):
+// sampling, the best log-probs of a row, and the distillation loss.
+#include "logits.h"
+
+#include <cooperative_groups.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <algorithm>
+#include <cfloat>
+#include <cmath>
+#include <mutex>
+#include <tuple>
+#include <vector>
+
+#include "dbs_engine.h"
+
+namespace cg = cooperative_groups;
+
+namespace dbs_logits {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kWarps = kThreads / 32;
+constexpr int kMaxCluster = 16;
+constexpr int kBins = 4 * kThreads;
+constexpr int kSampleList = 512;   // longest top-k that goes through a candidate list
+constexpr uint32_t kAll = 0xFFFFFFFFu;
+
+// ---------------------------------------------------------------------------
+// Element types. A vector is 16 bytes; `Elem<E>::max` is the elementwise
+// maximum of two vectors, which drops NaN for the other operand.
+// ---------------------------------------------------------------------------
+template <class E>
+struct Elem;
+
+template <>
+struct Elem<float> {
+    static constexpr int kVec = 4;
+    static constexpr int kKeyShift = 0;
+    static constexpr uint32_t kNegInf = 0xFF800000u;   // two packed values for the 16-bit types
+    __device__ static float widen(float v) { return v; }
+    __device__ static float narrow(float v) { return v; }
+    __device__ static void unpack(const uint4& v, float (&f)[4]) {
+        f[0] = __uint_as_float(v.x);
+        f[1] = __uint_as_float(v.y);
+        f[2] = __uint_as_float(v.z);
+        f[3] = __uint_as_float(v.w);
+    }
+    __device__ static uint4 pack(const float (&f)[4]) {
+        return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+    }
+    __device__ static uint32_t max1(uint32_t a, uint32_t b) {
+        return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
+    }
+};
+
+template <>
+struct Elem<__half> {
+    static constexpr int kVec = 8;
+    static constexpr int kKeyShift = 13;   // a widened half has 13 zero low bits
+    static constexpr uint32_t kNegInf = 0xFC00FC00u;
+    __device__ static float widen(__half v) { return __half2float(v); }
+    __device__ static __half narrow(float v) { return __float2half_rn(v); }
+    __device__ static void unpack(const uint4& v, float (&f)[8]) {
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float2 p = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+            f[2 * i] = p.x;
+            f[2 * i + 1] = p.y;
+        }
+    }
+    __device__ static uint4 pack(const float (&f)[8]) {
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const __half2 p = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
+            w[i] = *reinterpret_cast<const uint32_t*>(&p);
+        }
+        return make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    __device__ static uint32_t max1(uint32_t a, uint32_t b) {
+        const __half2 r = __hmax2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
+        return *reinterpret_cast<const uint32_t*>(&r);
+    }
+};
+
+template <>
+struct Elem<__nv_bfloat16> {
+    static constexpr int kVec = 8;
+    static constexpr int kKeyShift = 16;
+    static constexpr uint32_t kNegInf = 0xFF80FF80u;
+    __device__ static float widen(__nv_bfloat16 v) { return __bfloat162float(v); }
+    __device__ static __nv_bfloat16 narrow(float v) { return __float2bfloat16_rn(v); }
+    __device__ static void unpack(const uint4& v, float (&f)[8]) {
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            f[2 * i] = __uint_as_float(w[i] << 16);
+            f[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+        }
+    }
+    __device__ static uint4 pack(const float (&f)[8]) {
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const __nv_bfloat162 p = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+            w[i] = *reinterpret_cast<const uint32_t*>(&p);
+        }
+        return make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    __device__ static uint32_t max1(uint32_t a, uint32_t b) {
+        const __nv_bfloat162 r =
+            __hmax2(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
+        return *reinterpret_cast<const uint32_t*>(&r);
+    }
+};
+
+template <class E>
+__device__ __forceinline__ uint4 vmax(const uint4& a, const uint4& b) {
+    return make_uint4(Elem<E>::max1(a.x, b.x), Elem<E>::max1(a.y, b.y), Elem<E>::max1(a.z, b.z),
+                      Elem<E>::max1(a.w, b.w));
+}
+
+template <class E>
+__device__ __forceinline__ uint4 vneg_inf() {
+    return make_uint4(Elem<E>::kNegInf, Elem<E>::kNegInf, Elem<E>::kNegInf, Elem<E>::kNegInf);
+}
+
+__device__ __forceinline__ uint4 ldg_once(const uint4* p) {
+    uint4 r;
+    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w)
+                 : "l"(p));
+    return r;
+}
+
+__device__ __forceinline__ float neg_inf() { return __uint_as_float(0xFF800000u); }
+
+__device__ __forceinline__ float ex2(float v) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+    return r;
+}
+
+// Monotone map of a float to an unsigned key (-0 as +0); the 16-bit types'
+// widened values differ in the bits above kKeyShift only.
+__device__ __forceinline__ uint32_t ord(float f) {
+    const uint32_t u = __float_as_uint(__fadd_rn(f, 0.0f));
+    return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+}
+__device__ __forceinline__ float unord(uint32_t k) {
+    return __uint_as_float((k & 0x80000000u) ? (k & 0x7FFFFFFFu) : ~k);
+}
+template <class E>
+__device__ __forceinline__ uint32_t key_of(float f) {
+    return ord(f) >> Elem<E>::kKeyShift;
+}
+template <class E>
+__device__ __forceinline__ float value_of(uint32_t key) {
+    const uint32_t top = key << Elem<E>::kKeyShift;
+    // a negative value's key is complemented, its zero low bits included
+    return (top & 0x80000000u) ? unord(top) : unord(top | ((1u << Elem<E>::kKeyShift) - 1u));
+}
+
+// ---------------------------------------------------------------------------
+// Block reductions. `scratch` holds kWarps values; every thread gets the
+// result, summed in one order.
+// ---------------------------------------------------------------------------
+template <class T, class Op>
+__device__ __forceinline__ T block_reduce(T v, Op op, T* scratch) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v = op(v, __shfl_xor_sync(kAll, v, o));
+    if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = v;
+    __syncthreads();
+    v = scratch[0];
+#pragma unroll
+    for (int w = 1; w < kWarps; ++w) v = op(v, scratch[w]);
+    __syncthreads();
+    return v;
+}
+struct Add {
+    template <class T>
+    __device__ T operator()(T a, T b) const { return a + b; }
+};
+struct Max {
+    template <class T>
+    __device__ T operator()(T a, T b) const { return a > b ? a : b; }
+};
+struct Min {
+    template <class T>
+    __device__ T operator()(T a, T b) const { return a < b ? a : b; }
+};
+
+// Sum of the values of the threads before this one.
+template <class T>
+__device__ __forceinline__ T block_before(T v, T* scratch) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    T incl = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const T up = __shfl_up_sync(kAll, incl, o);
+        if (lane >= o) incl += up;
+    }
+    if (lane == 31) scratch[warp] = incl;
+    __syncthreads();
+    T base = T(0);
+    for (int w = 0; w < warp; ++w) base += scratch[w];
+    __syncthreads();
+    T excl = __shfl_up_sync(kAll, incl, 1);
+    if (lane == 0) excl = T(0);
+    return base + excl;
+}
+
+__device__ __forceinline__ void cluster_sync(int size) {
+    if (size > 1) {
+        cg::this_cluster().sync();
+    } else {
+        __syncthreads();
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Slices. Positions count from the 16-byte boundary at or before the row's
+// first element (`phase` elements ahead of it); CTA c of the cluster holds
+// positions [c*S, (c+1)*S) in `buf`, and what lies outside the row is -inf.
+// ---------------------------------------------------------------------------
+struct Slice {
+    int nv;      // vectors in buf
+    int first;   // token of buf's element 0 (negative where the row starts later)
+};
+
+// Loads the slice and adds it to the elementwise maximum `acc`. kClean: NaN
+// is stored as -inf.
+template <class E, bool kClean>
+__device__ __forceinline__ Slice load_slice(const E* row, int V, int S, int c, uint4* buf, uint4& acc) {
+    constexpr int kVec = Elem<E>::kVec;
+    constexpr int kBatch = 8;
+    const int phase = static_cast<int>((reinterpret_cast<uintptr_t>(row) & 15u) / sizeof(E));
+    const int a0 = c * S;
+    const int len = max(0, min(S, V + phase - a0));
+    const int nv = (len + kVec - 1) / kVec;
+    const int v0 = (a0 == 0 && phase > 0) ? 1 : 0;
+    const int v1 = len / kVec;
+    const uint4* src = reinterpret_cast<const uint4*>(reinterpret_cast<uintptr_t>(row) -
+                                                      static_cast<uintptr_t>(phase) * sizeof(E)) + a0 / kVec;
+    const uint4 none = vneg_inf<E>();
+    for (int base = v0 + static_cast<int>(threadIdx.x); base < v1; base += kBatch * kThreads) {
+        uint4 r[kBatch];
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+            const int v = base + i * kThreads;
+            r[i] = v < v1 ? ldg_once(src + v) : none;
+        }
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+            const int v = base + i * kThreads;
+            if (kClean) r[i] = vmax<E>(r[i], none);
+            acc = vmax<E>(acc, r[i]);
+            if (v < v1) buf[v] = r[i];
+        }
+    }
+    // the row's ragged ends, element by element
+    int edge = -1;
+    if (threadIdx.x == 0 && v0 == 1 && nv > 0) edge = 0;
+    if (threadIdx.x == 32 && v1 < nv && !(v0 == 1 && v1 == 0)) edge = v1;
+    if (edge >= 0) {
+        float f[kVec];
+#pragma unroll
+        for (int e = 0; e < kVec; ++e) {
+            const int i = a0 + edge * kVec + e - phase;
+            f[e] = (i >= 0 && i < V) ? Elem<E>::widen(row[i]) : neg_inf();
+        }
+        uint4 r = Elem<E>::pack(f);
+        if (kClean) r = vmax<E>(r, none);
+        acc = vmax<E>(acc, r);
+        buf[edge] = r;
+    }
+    return Slice{nv, a0 - phase};
+}
+
+template <class E>
+__device__ __forceinline__ float lanes_max(const uint4& v) {
+    float f[Elem<E>::kVec];
+    Elem<E>::unpack(v, f);
+    float m = f[0];
+#pragma unroll
+    for (int i = 1; i < Elem<E>::kVec; ++i) m = fmaxf(m, f[i]);
+    return m;
+}
+
+// Descending sort of n keys in shared memory: a bitonic network whose runs
+// all have the same direction, so n need not be a power of two.
+__device__ void block_sort(uint64_t* a, int n) {
+    int n2 = 1;
+    while (n2 < n) n2 <<= 1;
+    const int half = n2 >> 1;
+    __syncthreads();
+    for (int size = 2; size <= n2; size <<= 1) {
+        for (int st = size >> 1; st > 0; st >>= 1) {
+            for (int p = threadIdx.x; p < half; p += kThreads) {
+                const int i = ((p & ~(st - 1)) << 1) | (p & (st - 1));
+                // the first step of a size compares mirrored places
+                const int j = st == (size >> 1) ? (i ^ (size - 1)) : i + st;
+                if (j < n) {
+                    const uint64_t x = a[i], y = a[j];
+                    if (x < y) {
+                        a[i] = y;
+                        a[j] = x;
+                    }
+                }
+            }
+            __syncthreads();
+        }
+    }
+}
+
+__device__ __forceinline__ uint64_t entry(float x, int token) {
+    return (static_cast<uint64_t>(ord(x)) << 32) | static_cast<uint64_t>(~static_cast<uint32_t>(token));
+}
+__device__ __forceinline__ float entry_value(uint64_t e) { return unord(static_cast<uint32_t>(e >> 32)); }
+__device__ __forceinline__ int entry_token(uint64_t e) {
+    return static_cast<int>(~static_cast<uint32_t>(e & 0xFFFFFFFFu));
+}
+
+// ---------------------------------------------------------------------------
+// What the sampling and top-list kernels keep in shared memory beside the
+// slice and the two lists.
+// ---------------------------------------------------------------------------
+struct Packet {        // one CTA's share of what the cluster adds up
+    double sum;
+    float best;
+    float tau;
+    int index;
+};
+struct Shared {
+    Packet box[kMaxCluster];       // written by every CTA of the cluster
+    int counts[kMaxCluster];
+    double masses[kMaxCluster];
+    int ties[kMaxCluster];
+    double d8[kWarps];
+    unsigned long long u8[kWarps];
+    float f8[kWarps];
+    int i8[kWarps];
+    double range_mass[kWarps];
+    int range_ties[kWarps];
+    int listed;
+    int found_bin;
+    unsigned long long found_above;
+};
+
+struct Team {      // a CTA's place in its cluster
+    int size;
+    int rank;
+    __device__ Team() {
+        auto c = cg::this_cluster();
+        size = static_cast<int>(c.num_blocks());
+        rank = static_cast<int>(c.block_rank());
+    }
+    // Gives `value` to every CTA of the cluster, at its own place.
+    template <class T>
+    __device__ void tell(T* place, const T& value) const {
+        if (static_cast<int>(threadIdx.x) < size)
+            *cg::this_cluster().map_shared_rank(place + rank, threadIdx.x) = value;
+    }
+    template <class T>
+    __device__ const T* of(const T* place, int other) const {
+        return cg::this_cluster().map_shared_rank(const_cast<T*>(place), other);
+    }
+};
+
+// ---------------------------------------------------------------------------
+// Weights of sampling: exp((x - m) / T) in 64 bits, because tokens have to be
+// the ones that exact sums give: with V borders between tokens, sums in 32
+// bits would pick another token about once in a hundred flat rows.
+// 2^(n/32 + r/32), n the nearest whole number: a table of 2^(j/32) held one
+// entry per lane, and the Taylor polynomial of 2^(r/32), |r| <= 1/2, to the
+// fourth power (relative error below 1.3e-12).
+// ---------------------------------------------------------------------------
+struct Weights {
+    float mf;
+    float cf;
+    double m;
+    double c;
+    double tab;    // 2^(lane/32)
+    __device__ Weights(float best, float temperature) {
+        mf = best;
+        m = static_cast<double>(best);
+        c = 46.166241308446828384 / static_cast<double>(temperature);   // 32 / ln 2
+        cf = static_cast<float>(c);
+        tab = exp2(static_cast<double>(threadIdx.x & 31) * 0.03125);
+    }
+    // All 32 lanes of the warp call it together.
+    __device__ __forceinline__ double operator()(float x) const {
+        // 0 * inf and inf - inf come out as NaN, which fmaxf drops
+        const float t = fmaxf((x - mf) * cf, -40000.0f);
+        const int n = __float_as_int(t + 12582912.0f) - 0x4B400000;
+        const double nd = __hiloint2double(0x43300000, n ^ static_cast<int>(0x80000000)) - 4503601774854144.0;
+        const double r = fma(static_cast<double>(x) - m, c, -nd);
+        constexpr double kL = 0.021660849392498290;   // ln 2 / 32
+        double p = fma(r, kL * kL * kL * kL / 24.0, kL * kL * kL / 6.0);
+        p = fma(r, p, kL * kL / 2.0);
+        p = fma(r, p, kL);
+        p = fma(r, p, 1.0);
+        p *= __shfl_sync(kAll, tab, n & 31);
+        p = __hiloint2double(__double2hiint(p) + ((n >> 5) << 20), __double2loint(p));
+        return x == mf ? 1.0 : (n < -32686 ? 0.0 : p);   // exp(-708) and below count as nothing
+    }
+};
+
+// A weight as a whole number of 2^-43: sums of these do not depend on their
+// order, and 2^20 of them stay below 2^63.
+__device__ __forceinline__ unsigned long long fixed(double w) {
+    return static_cast<unsigned long long>(__double_as_longlong(w + 512.0) - 0x4080000000000000LL);
+}
+
+// Where an ordered row is cut: every key above `key` is kept, and of those
+// equal to it the first `ties` by index.
+struct Cut {
+    uint32_t key;
+    int ties;
+};
+
+// Visits the slice's elements a warp at a time, all lanes together; lanes
+// past the end see -inf.
+template <class E, class F>
+__device__ __forceinline__ void for_elements(const uint4* buf, const Slice& s, F&& f) {
+    const int lane = threadIdx.x & 31;
+    for (int base = (threadIdx.x >> 5) * 32; base < s.nv; base += kThreads) {
+        const int v = base + lane;
+        float x[Elem<E>::kVec];
+        Elem<E>::unpack(v < s.nv ? buf[v] : vneg_inf<E>(), x);
+#pragma unroll
+        for (int e = 0; e < Elem<E>::kVec; ++e) f(x[e], v * Elem<E>::kVec + e);
+    }
+}
+
+// Finds the value at which the descending row reaches `target`: a count of
+// elements (kMass false) or a sum of fixed() weights. Elements with keys at or
+// below `floor_key` stay out. A round counts or adds up the members of 1024
+// bins per CTA, adds the cluster's bins and keeps the bin that reaches the
+// target; the first round's bins are equal steps of the value over
+// [best - span, best] (a last one holds the rest), later ones equal steps of
+// the key, until a bin is one value.
+// For kMass, `target` comes in as the share p, and becomes p * (all members'
+// mass + extra); where the members fall short of it, ok is false.
+// Returns the key reached, and the count or mass above it.
+struct Found {
+    uint32_t key;
+    double above;
+    double target;
+    double total;
+    bool ok;
+};
+
+template <class E, bool kMass>
+__device__ Found search(const Team& team, Shared& sh, unsigned long long* hist, const uint4* buf, const Slice& s,
+                        const Weights& weight, float span, uint32_t floor_key, double target, double extra) {
+    const float scale = static_cast<float>(kBins - 1) / span;
+    const float best = weight.mf;
+    int lin = -1;                 // the first round's bin, once known
+    uint32_t lo = floor_key + 1, hi = key_of<E>(best);
+    int shift = 0;
+    unsigned long long above = 0;
+    Found out;
+    out.total = 0.0;
+    auto lin_bin = [&](float x) {
+        // also right for infinite operands: inf - inf is NaN, and fminf drops it
+        const float b = x == best ? 0.0f : fminf((best - x) * scale, static_cast<float>(kBins - 1));
+        return static_cast<int>(b);
+    };
+    for (int round = 0;; ++round) {
+        for (int b = threadIdx.x; b < kBins; b += kThreads) hist[b] = 0;
+        __syncthreads();
+        unsigned long long rest = 0;
+        for_elements<E>(buf, s, [&](float x, int) {
+            const uint32_t k = key_of<E>(x);
+            const int l = lin_bin(x);
+            bool in = k > floor_key;
+            if (round > 0) in = in && l == lin && k >= lo && k <= hi;
+            if (!__any_sync(kAll, in)) return;
+            const unsigned long long w = kMass ? fixed(weight(x)) : 1ull;
+            if (in) {
+                const int b = round == 0 ? l : static_cast<int>((hi - k) >> shift);
+                if (round == 0 && b == kBins - 1)
+                    rest += w;
+                else
+                    atomicAdd(&hist[b], w);
+            }
+        });
+        if (round == 0 && rest) atomicAdd(&hist[kBins - 1], rest);
+        cluster_sync(team.size);
+        unsigned long long h[4] = {0, 0, 0, 0};
+        for (int c = 0; c < team.size; ++c) {
+            const unsigned long long* theirs = team.of(hist, c) + 4 * threadIdx.x;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) h[q] += theirs[q];
+        }
+        const unsigned long long own = h[0] + h[1] + h[2] + h[3];
+        const unsigned long long before = above + block_before<unsigned long long>(own, sh.u8);
+        if (round == 0) {
+            const unsigned long long total = block_reduce(own, Add(), sh.u8);
+            if (kMass) {
+                out.total = static_cast<double>(total) + extra;
+                target *= out.total;
+            }
+            out.target = target;
+            out.ok = static_cast<double>(total) >= target && total > 0;
+            if (!out.ok) {
+                cluster_sync(team.size);
+                out.key = floor_key;
+                out.above = static_cast<double>(total);
+                return out;
+            }
+        }
+        if (static_cast<double>(before) < target && static_cast<double>(before + own) >= target) {
+            unsigned long long run = before;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const bool here = static_cast<double>(run) < target && static_cast<double>(run + h[q]) >= target;
+                if (here) {
+                    sh.found_bin = 4 * static_cast<int>(threadIdx.x) + q;
+                    sh.found_above = run;
+                }
+                run += h[q];
+            }
+        }
+        cluster_sync(team.size);   // also: everybody has read the bins
+        const int b = sh.found_bin;
+        above = sh.found_above;
+        __syncthreads();
+        if (round == 0) {
+            lin = b;
+            // the bin's keys, its ends widened for the rounding of (best - x) * scale
+            if (b < kBins - 1 && best < FLT_MAX) {
+                const float width = span / static_cast<float>(kBins - 1);
+                const float slack = 0.01f * width + 1e-5f * fmaxf(fabsf(best), span);
+                if (b > 0) hi = min(hi, key_of<E>(best - static_cast<float>(b) * width + slack));
+                lo = max(lo, key_of<E>(best - static_cast<float>(b + 1) * width - slack));
+            }
+        } else {
+            if (shift == 0) {
+                out.key = hi - static_cast<uint32_t>(b);
+                out.above = static_cast<double>(above);
+                return out;
+            }
+            hi = hi - (static_cast<uint32_t>(b) << shift);
+            const uint32_t wide = (1u << shift) - 1u;
+            lo = hi - lo > wide ? hi - wide : lo;
+        }
+        const uint32_t width = hi - lo;
+        shift = 0;
+        while ((width >> shift) >= static_cast<uint32_t>(kBins)) ++shift;
+    }
+}
+
+// Appends every element that reaches `low` (and is above -inf) to the CTA's
+// list; `listed` counts on where the list is full.
+template <class E>
+__device__ __forceinline__ void append_from(Shared& sh, const uint4* buf, const Slice& s, float low, uint64_t* list,
+                                            int cap) {
+    for (int v = threadIdx.x; v < s.nv; v += kThreads) {
+        const uint4 r = buf[v];
+        if (lanes_max<E>(r) < low) continue;
+        float x[Elem<E>::kVec];
+        Elem<E>::unpack(r, x);
+#pragma unroll
+        for (int e = 0; e < Elem<E>::kVec; ++e) {
+            if (x[e] >= low && x[e] > neg_inf()) {
+                const int at = atomicAdd(&sh.listed, 1);
+                if (at < cap) list[at] = entry(x[e], s.first + v * Elem<E>::kVec + e);
+            }
+        }
+    }
+}
+
+// The row's best entries, n of them (fewer where fewer are above -inf), in
+// the leader's `sorted`, best first; the number of entries there, 0 in the
+// other CTAs. box[] holds every CTA's `tau` below which it needs to list
+// nothing. Every CTA lists what is at or above the least of these; where ties
+// make that too many, the exact cut is searched.
+template <class E>
+__device__ int gather_best(const Team& team, Shared& sh, const uint4* buf, const Slice& s, float best, int n,
+                           uint64_t* list, uint64_t* sorted, int cap, int leader) {
+    float tau = sh.box[0].tau;
+    for (int c = 1; c < team.size; ++c) tau = fminf(tau, sh.box[c].tau);
+    append_from<E>(sh, buf, s, tau, list, cap);
+    __syncthreads();
+    team.tell(sh.counts, sh.listed);
+    cluster_sync(team.size);
+    int total = 0;
+    for (int c = 0; c < team.size; ++c) total += sh.counts[c];
+    if (total > cap) {
+        // Too many: find the n-th value itself. All of the row's elements
+        // above -inf are members, and they are more than n.
+        const Weights weight(best, 1.0f);
+        float low = best;
+        for_elements<E>(buf, s, [&](float x, int) { low = x > neg_inf() ? fminf(low, x) : low; });
+        low = block_reduce(low, Min(), sh.f8);
+        cluster_sync(team.size);          // box is read by everybody
+        team.tell(sh.box, Packet{0.0, 0.0f, low, 0});
+        cluster_sync(team.size);
+        for (int c = 0; c < team.size; ++c) low = fminf(low, sh.box[c].tau);
+        float span = best - low;
+        if (!(span > 0.0f)) span = 1.0f;
+        if (!(span < FLT_MAX)) span = FLT_MAX;
+        // both lists' space holds the bins: what was listed is listed again below
+        const Found f = search<E, false>(team, sh, reinterpret_cast<unsigned long long*>(list), buf, s, weight, span,
+                                         key_of<E>(neg_inf()), static_cast<double>(n), 0.0);
+        const int need = n - static_cast<int>(f.above);
+        if (threadIdx.x == 0) sh.listed = 0;
+        __syncthreads();
+        append_from<E>(sh, buf, s, value_of<E>(f.key + 1), list, cap);
+        // the first `need` of the equal ones, by index: a stretch of
+        // neighbouring vectors per thread
+        const int per = (s.nv + kThreads - 1) / kThreads;
+        const int begin = min(s.nv, per * static_cast<int>(threadIdx.x)), end = min(s.nv, begin + per);
+        int mine = 0;
+        for (int v = begin; v < end; ++v) {
+            float x[Elem<E>::kVec];
+            Elem<E>::unpack(buf[v], x);
+#pragma unroll
+            for (int e = 0; e < Elem<E>::kVec; ++e) mine += key_of<E>(x[e]) == f.key;
+        }
+        const int all = block_reduce(mine, Add(), sh.i8);
+        int at = block_before(mine, sh.i8);
+        team.tell(sh.ties, all);
+        cluster_sync(team.size);
+        int ahead = 0;
+        for (int c = 0; c < team.rank; ++c) ahead += sh.ties[c];
+        const int keep = max(0, min(all, need - ahead));
+        const int listed = sh.listed;
+        for (int v = begin; v < end && at < keep; ++v) {
+            float x[Elem<E>::kVec];
+            Elem<E>::unpack(buf[v], x);
+#pragma unroll
+            for (int e = 0; e < Elem<E>::kVec; ++e) {
+                if (key_of<E>(x[e]) == f.key && at < keep) {
+                    list[listed + at] = entry(x[e], s.first + v * Elem<E>::kVec + e);
+                    ++at;
+                }
+            }
+        }
+        __syncthreads();
+        team.tell(sh.counts, listed + keep);
+        cluster_sync(team.size);
+        total = n;
+    }
+    if (team.rank != leader) return 0;
+    int at = 0;
+    for (int c = 0; c < team.size; ++c) {
+        const int count = sh.counts[c];
+        const uint64_t* theirs = team.of(list, c);
+        for (int i = threadIdx.x; i < count; i += kThreads) sorted[at + i] = theirs[i];
+        at += count;
+    }
+    block_sort(sorted, total);
+    return min(n, total);
+}
+
+// A value at or below the t-th largest of this CTA's element-place maxima
+// (kVec of them per thread), so that at least t of its elements reach it;
+// -inf where fewer than t are above -inf.
+template <class E>
+__device__ float threshold(Shared& sh, const uint4& acc, float best, int t) {
+    float g[Elem<E>::kVec];
+    Elem<E>::unpack(acc, g);
+    auto count = [&](float low) {
+        int c = 0;
+#pragma unroll
+        for (int e = 0; e < Elem<E>::kVec; ++e) c += g[e] >= low ? 1 : 0;
+        return block_reduce(c, Add(), sh.i8);
+    };
+    // the least of the threads' maxima that are above -inf
+    const float mine = lanes_max<E>(acc);
+    float lo = block_reduce(mine > neg_inf() ? mine : FLT_MAX, Min(), sh.f8);
+    if (count(lo) < t) {
+        lo = FLT_MAX;
+#pragma unroll
+        for (int e = 0; e < Elem<E>::kVec; ++e)
+            if (g[e] > neg_inf()) lo = fminf(lo, g[e]);
+        lo = block_reduce(lo, Min(), sh.f8);
+        if (count(lo) < t) return neg_inf();
+    }
+    // count(lo) >= t throughout; halves the values between, or the keys where
+    // the values' range is too wide for that (masks of the lowest value)
+    float hi = best;
+    const int enough = t + t / 2 + 8;
+    for (int i = 0; i < 40; ++i) {
+        const float mid = hi - lo < 1.0e4f ? 0.5f * lo + 0.5f * hi : unord(ord(lo) + ((ord(hi) - ord(lo)) >> 1));
+        if (!(mid > lo && mid < hi)) break;
+        const int c = count(mid);
+        if (c >= t) {
+            lo = mid;
+            if (c <= enough) break;
+        } else {
+            hi = mid;
+        }
+    }
+    return lo;
+}
+
+// ---------------------------------------------------------------------------
+// Softmax sums in 32 bits. An exponent is x c2 - B in one fused step, with a
+// whole number B near the maximum that the sum goes by: changing from one
+// CTA's B to the row's is a power of two, and a common rounding of c2 cancels
+// between a term and the sum. Where the maximum is so large (a mask of the
+// type's lowest value) that x c2 could overflow, a term is 1 at the maximum
+// and 0 below it, as neighbouring values there are further apart than any
+// exponent reaches.
+// ---------------------------------------------------------------------------
+struct Reference {
+    float best;
+    float B;
+    bool wide;
+    __device__ Reference(float best_, float c2) : best(best_), B(0.0f), wide(false) {
+        if (best > neg_inf()) {
+            const float b = best * c2;
+            wide = !(fabsf(b) < 1.0e30f) && fabsf(best) <= FLT_MAX;
+            B = wide || !(fabsf(b) < 1.0e30f) ? 0.0f : rintf(b);
+        }
+    }
+    __device__ __forceinline__ float exponent(float x, float c2) const {
+        return wide ? (x == best ? 0.0f : (x < best ? neg_inf() : x - x)) : fmaf(x, c2, -B);
+    }
+    // what a sum taken by `part` is multiplied by to go by this one
+    __device__ double factor(const Reference& part) const {
+        if (!(part.best > neg_inf())) return 1.0;   // nothing, or NaN
+        if (wide || part.wide) return part.best == best ? 1.0 : 0.0;
+        return exp2(static_cast<double>(part.B) - static_cast<double>(B));
+    }
+    // the reference in units of log2
+    __device__ double log2_of(float c2) const {
+        return wide ? static_cast<double>(best) * static_cast<double>(c2) : static_cast<double>(B);
+    }
+};
+
+// This thread's share of the slice's sum.
+template <class E>
+__device__ __forceinline__ float sum_exp(const uint4* buf, int nv, float c2, const Reference& ref) {
+    float p0 = 0.0f, p1 = 0.0f;
+    if (ref.wide) {
+        for (int v = threadIdx.x; v < nv; v += kThreads) {
+            float x[Elem<E>::kVec];
+            Elem<E>::unpack(buf[v], x);
+#pragma unroll
+            for (int e = 0; e < Elem<E>::kVec; ++e) p0 += ex2(ref.exponent(x[e], c2));
+        }
+        return p0;
+    }
+    for (int v = threadIdx.x; v < nv; v += kThreads) {
+        float x[Elem<E>::kVec];
+        Elem<E>::unpack(buf[v], x);
+#pragma unroll
+        for (int e = 0; e < Elem<E>::kVec; e += 2) {
+            p0 += ex2(fmaf(x[e], c2, -ref.B));
+            p1 += ex2(fmaf(x[e + 1], c2, -ref.B));
+        }
+    }
+    return p0 + p1;
+}
+
+// ---------------------------------------------------------------------------
+// The best log-probs of a row
+// ---------------------------------------------------------------------------
+template <class E>
+__global__ void __launch_bounds__(kThreads, 3) top_kernel(TopArgs a, int S, int cap) {
+    extern __shared__ uint4 dyn[];
+    __shared__ Shared sh;
+    const Team team;
+    uint4* buf = dyn;
+    uint64_t* list = reinterpret_cast<uint64_t*>(reinterpret_cast<char*>(dyn) + static_cast<size_t>(S) * sizeof(E));
+    uint64_t* sorted = list + cap;
+    const int64_t step = gridDim.x / team.size;
+    const int n = a.n;
+    const float c2 = 1.4426950408889634f / a.temperature;
+    int leader = 0;
+    cluster_sync(team.size);   // everybody's shared memory exists from here on
+    for (int64_t row = blockIdx.x / team.size; row < a.in.rows; row += step) {
+        __syncthreads();
+        if (threadIdx.x == 0) sh.listed = 0;
+        uint4 acc = vneg_inf<E>();
+        const Slice s = load_slice<E, true>(static_cast<const E*>(a.in.x) + row * a.in.stride, a.in.V, S, team.rank,
+                                            buf, acc);
+        const float mine = block_reduce(lanes_max<E>(acc), Max(), sh.f8);
+        const Reference ref(mine, c2);
+        const float part = sum_exp<E>(buf, s.nv, c2, ref);
+        const double sum = block_reduce(static_cast<double>(part), Add(), sh.d8);
+        const float tau = threshold<E>(sh, acc, mine, (n + team.size - 1) / team.size);
+        team.tell(sh.box, Packet{sum, mine, tau, 0});
+        cluster_sync(team.size);
+        float best = sh.box[0].best;
+        for (int c = 1; c < team.size; ++c) best = fmaxf(best, sh.box[c].best);
+        // the sum of 2^((x - best) c2)
+        const Reference all(best, c2);
+        double Z = 0.0;
+        for (int c = 0; c < team.size; ++c) Z += sh.box[c].sum * all.factor(Reference(sh.box[c].best, c2));
+        if (!all.wide) Z *= exp2(static_cast<double>(all.B) - static_cast<double>(best) * static_cast<double>(c2));
+        const int got = gather_best<E>(team, sh, buf, s, best, n, list, sorted, cap, leader);
+        if (team.rank == leader) {
+            const double log_z = log(Z);
+            for (int i = threadIdx.x; i < n; i += kThreads) {
+                float value = neg_inf();
+                int token = -1;
+                if (i < got) {
+                    const float x = entry_value(sorted[i]);
+                    token = entry_token(sorted[i]);
+                    value = static_cast<float>((static_cast<double>(x) - static_cast<double>(best)) /
+                                                   static_cast<double>(a.temperature) - log_z);
+                }
+                a.log_probs[row * n + i] = value;
+                a.tokens[row * n + i] = token;
+            }
+        }
+        leader = leader + 1 == team.size ? 0 : leader + 1;
+    }
+    cluster_sync(team.size);   // nobody leaves while its list is being read
+}
+
+// ---------------------------------------------------------------------------
+// Sampling
+// ---------------------------------------------------------------------------
+
+// The token that index order and the uniform number give among the elements
+// that the cut keeps. `out` is written by the CTA that holds it.
+template <class E>
+__device__ void pick(const Team& team, Shared& sh, const uint4* buf, const Slice& s, const Weights& weight, Cut cut,
+                     double u, int32_t* out) {
+    constexpr int kVec = Elem<E>::kVec;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const double tie = weight(value_of<E>(cut.key));
+    // a stretch of the slice per warp
+    const int per = ((s.nv + kWarps - 1) / kWarps + 31) & ~31;
+    const int begin = min(s.nv, per * warp), end = min(s.nv, begin + per);
+    double mass = 0.0;
+    int ties = 0;
+    for (int base = begin; base < end; base += 32) {
+        const int v = base + lane;
+        float x[kVec];
+        Elem<E>::unpack(v < end ? buf[v] : vneg_inf<E>(), x);
+#pragma unroll
+        for (int e = 0; e < kVec; ++e) {
+            const uint32_t k = key_of<E>(x[e]);
+            ties += k == cut.key ? 1 : 0;
+            const bool in = k > cut.key;
+            if (__any_sync(kAll, in)) {
+                const double w = weight(x[e]);
+                mass += in ? w : 0.0;
+            }
+        }
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        mass += __shfl_xor_sync(kAll, mass, o);
+        ties += __shfl_xor_sync(kAll, ties, o);
+    }
+    if (lane == 0) {
+        sh.range_mass[warp] = mass;
+        sh.range_ties[warp] = ties;
+    }
+    __syncthreads();
+    double cta_mass = 0.0;
+    int cta_ties = 0;
+    for (int w = 0; w < kWarps; ++w) {
+        cta_mass += sh.range_mass[w];
+        cta_ties += sh.range_ties[w];
+    }
+    team.tell(sh.masses, cta_mass);
+    team.tell(sh.ties, cta_ties);
+    cluster_sync(team.size);
+    auto at = [&](double m, int t) { return m + static_cast<double>(min(t, cut.ties)) * tie; };
+    // the first part whose running sum passes the target, else the last that adds anything
+    double m_all = 0.0;
+    int t_all = 0;
+    for (int c = 0; c < team.size; ++c) {
+        m_all += sh.masses[c];
+        t_all += sh.ties[c];
+    }
+    // a uniform number of 1 or more lies behind every sum, whatever its rounding
+    const double target = u < 1.0 ? u * at(m_all, t_all) : HUGE_VAL;
+    auto adds = [&](double mass, int t_before, int count) {
+        return mass > 0.0 || (tie > 0.0 && min(t_before + count, cut.ties) > min(t_before, cut.ties));
+    };
+    auto choose = [&](const double* masses, const int* counts, int parts, double& m, int& t) {
+        double m_run = m, m_best = m;
+        int t_run = t, t_best = t, chosen = -1;
+        for (int i = 0; i < parts; ++i) {
+            if (adds(masses[i], t_run, counts[i])) {
+                chosen = i;
+                m_best = m_run;
+                t_best = t_run;
+                if (at(m_run + masses[i], t_run + counts[i]) > target) break;
+            }
+            m_run += masses[i];
+            t_run += counts[i];
+        }
+        m = m_best;
+        t = t_best;
+        return chosen;
+    };
+    double m = 0.0;
+    int t = 0;
+    const int owner = choose(sh.masses, sh.ties, team.size, m, t);
+    if (owner == team.rank) {
+        const int w = choose(sh.range_mass, sh.range_ties, kWarps, m, t);
+        // that stretch again, by the whole CTA: neighbouring vectors per thread
+        const int w_begin = min(s.nv, per * max(w, 0)), w_end = min(s.nv, w_begin + per);
+        const int each = (per + kThreads - 1) / kThreads;
+        const int t_begin = min(w_end, w_begin + each * static_cast<int>(threadIdx.x));
+        const int t_end = min(w_end, t_begin + each);
+        double my_mass = 0.0;
+        int my_ties = 0;
+        for (int i = 0; i < each; ++i) {
+            const int v = t_begin + i;
+            float x[kVec];
+            Elem<E>::unpack(v < t_end ? buf[v] : vneg_inf<E>(), x);
+#pragma unroll
+            for (int e = 0; e < kVec; ++e) {
+                const uint32_t k = key_of<E>(x[e]);
+                const double w8 = weight(x[e]);
+                my_mass += k > cut.key ? w8 : 0.0;
+                my_ties += k == cut.key ? 1 : 0;
+            }
+        }
+        const double m0 = m + block_before(my_mass, sh.d8);
+        const int t0 = t + block_before(my_ties, sh.i8);
+        const bool mine = adds(my_mass, t0, my_ties);
+        const bool past = mine && at(m0 + my_mass, t0 + my_ties) > target;
+        const int none = kThreads;
+        const int first = block_reduce(past ? static_cast<int>(threadIdx.x) : none, Min(), sh.i8);
+        const int last = block_reduce(mine ? static_cast<int>(threadIdx.x) : -1, Max(), sh.i8);
+        const int who = first < none ? first : last;
+        // its warp walks along its elements
+        if (warp == (who >> 5) && who >= 0) {
+            double m_run = m0;
+            int t_run = t0, token = -1;
+            bool done = false;
+            for (int i = 0; i < each; ++i) {
+                const int v = t_begin + i;
+                float x[kVec];
+                Elem<E>::unpack(v < t_end ? buf[v] : vneg_inf<E>(), x);
+#pragma unroll
+                for (int e = 0; e < kVec; ++e) {
+                    const uint32_t k = key_of<E>(x[e]);
+                    const double w8 = weight(x[e]);
+                    const bool some = adds(k > cut.key ? w8 : 0.0, t_run, k == cut.key ? 1 : 0);
+                    if (k > cut.key) m_run += w8;
+                    if (k == cut.key) ++t_run;
+                    if (!done && some) {
+                        token = s.first + v * kVec + e;
+                        done = at(m_run, t_run) > target;
+                    }
+                }
+            }
+            if (static_cast<int>(threadIdx.x) == who) *out = token;
+        }
+    }
+}
+
+// A top-k row: its k best entries in order are all that is needed.
+__device__ void pick_listed(Shared& sh, const uint64_t* sorted, int count, float best, float temperature, double p,
+                            double log_q, double u, double* weight, int* token, int32_t* out) {
+    // weights of the ordered entries; a thread holds neighbouring ones
+    const int each = (count + kThreads - 1) / kThreads;
+    const int begin = min(count, each * static_cast<int>(threadIdx.x)), end = min(count, begin + each);
+    double mine = 0.0;
+    for (int i = begin; i < end; ++i) {
+        const float x = entry_value(sorted[i]);
+        const double z = x == best ? 0.0 : (static_cast<double>(x) - static_cast<double>(best)) /
+                                               static_cast<double>(temperature);
+        const double w = z < -708.0 ? 0.0 : exp(z);
+        weight[i] = w;
+        token[i] = entry_token(sorted[i]);
+        mine += w;
+    }
+    const double total = block_reduce(mine, Add(), sh.d8);
+    double run = block_before(mine, sh.d8);
+    int keep = 0;
+    for (int i = begin; i < end; ++i) {
+        const float x = entry_value(sorted[i]);
+        const double z = x == best ? 0.0 : (static_cast<double>(x) - static_cast<double>(best)) /
+                                               static_cast<double>(temperature);
+        keep += (i == 0 || ((!(p < 1.0) || run < p * total) && z >= log_q)) ? 1 : 0;
+        run += weight[i];
+    }
+    keep = block_reduce(keep, Add(), sh.i8);   // the kept ones are the first
+    mine = 0.0;
+    for (int i = begin; i < min(end, keep); ++i) mine += weight[i];
+    const double kept = block_reduce(mine, Add(), sh.d8);
+    const double target = u < 1.0 ? u * kept : HUGE_VAL;   // as in pick()
+    // the least kept index whose sum of weights up to it passes the target
+    int first = 0x7FFFFFFF, last = -1;
+    for (int i = threadIdx.x; i < keep; i += kThreads) {
+        const int own = token[i];
+        double sum = 0.0;
+        for (int j = 0; j < keep; ++j) sum += token[j] <= own ? weight[j] : 0.0;
+        if (weight[i] > 0.0) {
+            last = max(last, own);
+            if (sum > target) first = min(first, own);
+        }
+    }
+    first = block_reduce(first, Min(), sh.i8);
+    last = block_reduce(last, Max(), sh.i8);
+    if (threadIdx.x == 0) *out = first < 0x7FFFFFFF ? first : last;
+}
+
+template <class E>
+__global__ void __launch_bounds__(kThreads, 3) sample_kernel(SampleArgs a, int S, int cap) {
+    extern __shared__ uint4 dyn[];
+    __shared__ Shared sh;
+    const Team team;
+    uint4* buf = dyn;
+    uint64_t* list = reinterpret_cast<uint64_t*>(reinterpret_cast<char*>(dyn) + static_cast<size_t>(S) * sizeof(E));
+    uint64_t* sorted = list + cap;
+    const int64_t step = gridDim.x / team.size;
+    const int V = a.in.V;
+    int leader = 0;
+    cluster_sync(team.size);
+    for (int64_t row = blockIdx.x / team.size; row < a.in.rows; row += step) {
+        __syncthreads();
+        if (threadIdx.x == 0) sh.listed = 0;
+        const float given = a.temperature ? a.temperature[row] : a.temperature_all;
+        const float temperature = given > FLT_MAX ? FLT_MAX : given;
+        const int k = a.top_k ? a.top_k[row] : a.top_k_all;
+        const double p = static_cast<double>(a.top_p ? a.top_p[row] : a.top_p_all);
+        const float q_given = a.min_p ? a.min_p[row] : a.min_p_all;
+        const double q = q_given > 1.0f ? 1.0 : static_cast<double>(q_given);
+        const double u = static_cast<double>(a.uniforms[row]);
+        const bool cut_k = k > 0 && k < V;
+        // one token is left: no temperature, the best one alone, or no mass
+        const bool greedy = !(given > 0.0f) || k == 1 || p <= 0.0;
+        const bool by_list = !greedy && cut_k && k <= kSampleList;
+        uint4 acc = vneg_inf<E>();
+        const Slice s = load_slice<E, true>(static_cast<const E*>(a.in.x) + row * a.in.stride, V, S, team.rank, buf,
+                                            acc);
+        const float mine = block_reduce(lanes_max<E>(acc), Max(), sh.f8);
+        float tau = neg_inf();
+        int index = 0x7FFFFFFF;
+        if (by_list) tau = threshold<E>(sh, acc, mine, (k + team.size - 1) / team.size);
+        if (greedy) {
+            for (int v = threadIdx.x; v < s.nv; v += kThreads) {
+                float x[Elem<E>::kVec];
+                Elem<E>::unpack(buf[v], x);
+#pragma unroll
+                for (int e = 0; e < Elem<E>::kVec; ++e)
+                    if (x[e] == mine) index = min(index, s.first + v * Elem<E>::kVec + e);
+            }
+            index = block_reduce(index, Min(), sh.i8);
+        }
+        team.tell(sh.box, Packet{0.0, mine, tau, index});
+        cluster_sync(team.size);
+        float best = sh.box[0].best;
+        for (int c = 1; c < team.size; ++c) best = fmaxf(best, sh.box[c].best);
+        int32_t* out = a.tokens + row;
+        if (!(best > neg_inf())) {
+            if (team.rank == leader && threadIdx.x == 0) *out = -1;
+            cluster_sync(team.size);   // box is free again
+        } else if (greedy) {
+            if (team.rank == leader && threadIdx.x == 0) {
+                int token = 0x7FFFFFFF;
+                for (int c = 0; c < team.size; ++c)
+                    if (sh.box[c].best == best) token = min(token, sh.box[c].index);
+                *out = token;
+            }
+            cluster_sync(team.size);
+        } else if (by_list) {
+            const int got = gather_best<E>(team, sh, buf, s, best, k, list, sorted, cap, leader);
+            if (team.rank == leader) {
+                // the leader's own list has been copied: its space holds the weights
+                double* weight = reinterpret_cast<double*>(list);
+                int* token = reinterpret_cast<int*>(weight + got);
+                pick_listed(sh, sorted, got, best, temperature, p, q > 0.0 ? log(q) : -HUGE_VAL, u, weight, token, out);
+            }
+        } else {
+            const Weights weight(best, temperature);
+            unsigned long long* hist = reinterpret_cast<unsigned long long*>(list);
+            const uint32_t none = key_of<E>(neg_inf());
+            Cut cut{none, 0};
+            double cut_mass = 0.0;   // of the equal ones at the top-k cut
+            if (cut_k) {
+                float low = best;
+                for_elements<E>(buf, s, [&](float x, int) { low = x > neg_inf() ? fminf(low, x) : low; });
+                low = block_reduce(low, Min(), sh.f8);
+                cluster_sync(team.size);
+                team.tell(sh.box, Packet{0.0, 0.0f, low, 0});
+                cluster_sync(team.size);
+                for (int c = 0; c < team.size; ++c) low = fminf(low, sh.box[c].tau);
+                float span = best - low;
+                if (!(span > 0.0f)) span = 1.0f;
+                if (!(span < FLT_MAX)) span = FLT_MAX;
+                const Found f = search<E, false>(team, sh, hist, buf, s, weight, span, none,
+                                                 static_cast<double>(k), 0.0);
+                if (f.ok) {
+                    cut.key = f.key;
+                    cut.ties = k - static_cast<int>(f.above);
+                    cut_mass = static_cast<double>(fixed(weight(value_of<E>(f.key))));
+                }
+            }
+            if (p < 1.0) {
+                const float span = fminf(fmaxf(32.0f * temperature, FLT_MIN), FLT_MAX);
+                const Found f = search<E, true>(team, sh, hist, buf, s, weight, span, cut.key, p,
+                                                static_cast<double>(cut.ties) * cut_mass);
+                if (f.ok) {
+                    cut.key = f.key;
+                    cut.ties = 0x7FFFFFFF;
+                    cut_mass = static_cast<double>(fixed(weight(value_of<E>(f.key))));
+                }
+                // of the equal ones, as many as reach the target
+                const double left = ceil((f.target - f.above) / cut_mass);
+                if (left < static_cast<double>(cut.ties)) cut.ties = max(1, static_cast<int>(left));
+            }
+            if (q > 0.0) {
+                // kept: x >= m + T ln q, rounded up to a float
+                const float low = __double2float_ru(static_cast<double>(best) +
+                                                    static_cast<double>(temperature) * log(q));
+                const uint32_t low_key = best < FLT_MAX ? (key_of<E>(fminf(low, best))) : key_of<E>(best);
+                // a 16-bit type's key drops low bits: the least key whose value reaches `low`
+                const uint32_t least = value_of<E>(low_key) >= low ? low_key : low_key + 1;
+                if (least > cut.key) {
+                    cut.key = least - 1;
+                    cut.ties = 0;
+                }
+            }
+            pick<E>(team, sh, buf, s, weight, cut, u, out);
+            cluster_sync(team.size);
+        }
+        leader = leader + 1 == team.size ? 0 : leader + 1;
+    }
+    cluster_sync(team.size);
+}
+
+// ---------------------------------------------------------------------------
+// Distillation
+// ---------------------------------------------------------------------------
+struct DistillPacket {
+    double cross;     // sum of q (l - ln 2 (x c2 - reference)) over the CTA's slots
+    double q;         // and of q
+    float rest;       // sum of the exponentials of what is not listed
+    float listed;     // and of what is listed
+    float best;
+};
+struct DistillShared {
+    DistillPacket box[2][kMaxCluster];
+    double d8[kWarps];
+    float f8[kWarps];
+    int i8[kWarps];
+};
+
+__device__ __forceinline__ int64_t teacher_token(const DistillArgs& a, int64_t at) {
+    return a.token_bytes == 8 ? static_cast<const int64_t*>(a.teacher_tokens)[at]
+                              : static_cast<int64_t>(static_cast<const int32_t*>(a.teacher_tokens)[at]);
+}
+
+// One pass over the row gives its loss and (kGrad) its gradient: the slice
+// stays in shared memory between the sums and the gradient's rows, so the
+// logits are read once and the gradient written once.
+template <class E, bool kGrad>
+__global__ void __launch_bounds__(kThreads, 3) distill_kernel(DistillArgs a, int S) {
+    constexpr int kVec = Elem<E>::kVec;
+    extern __shared__ uint4 dyn[];
+    __shared__ DistillShared sh;
+    const Team team;
+    const int n = a.n, V = a.in.V;
+    uint4* buf = dyn;
+    E* elems = reinterpret_cast<E*>(dyn);
+    const int words = (S + 31) / 32;
+    uint32_t* seen = reinterpret_cast<uint32_t*>(elems + S);   // a bit for each listed place
+    int* place = reinterpret_cast<int*>(seen + words);        // slot -> place in the slice, or -1
+    float* slot_x = reinterpret_cast<float*>(place + n);
+    float* slot_q = slot_x + n;
+    const int64_t step = gridDim.x / team.size;
+    const float c2 = 1.4426950408889634f / a.temperature;
+    constexpr double kLn2 = 0.69314718055994530942;
+    int parity = 0;
+    cluster_sync(team.size);
+    for (int64_t row = blockIdx.x / team.size; row < a.in.rows; row += step) {
+        float g = 1.0f;
+        if (a.grad_loss) {
+            g = a.grad_loss[row * a.grad_loss_stride];
+            if (a.skip_unit && g == 1.0f) continue;   // the same for the whole cluster
+        }
+        __syncthreads();
+        for (int w = threadIdx.x; w < words; w += kThreads) seen[w] = 0;
+        const E* x = static_cast<const E*>(a.in.x) + row * a.in.stride;
+        const int phase = static_cast<int>((reinterpret_cast<uintptr_t>(x) & 15u) / sizeof(E));
+        const int a0 = team.rank * S - phase;     // token of the slice's element 0
+        // the teacher's slots: their probabilities' sum, and which fall into this slice
+        double Q = 0.0;
+        int any = 0;
+        __syncthreads();
+        bool twice = false;
+        for (int j = threadIdx.x; j < n; j += kThreads) {
+            const int64_t i = teacher_token(a, row * n + j);
+            const float l = a.teacher_log_probs[row * n + j];
+            int at = -1;
+            float q = 0.0f;
+            if (i >= 0 && i < V) {
+                any = 1;
+                const double q64 = exp(static_cast<double>(l));
+                Q += q64;
+                q = static_cast<float>(q64);
+                const int64_t here = i - a0;
+                if (here >= 0 && here < S) {
+                    at = static_cast<int>(here);
+                    const uint32_t bit = 1u << (at & 31);
+                    twice = twice || (atomicOr(&seen[at >> 5], bit) & bit) != 0;
+                }
+            }
+            place[j] = at;
+            slot_q[j] = q;
+        }
+        any = __syncthreads_or(any);
+        E* out = static_cast<E*>(a.grad) + (kGrad ? row * V : 0);
+        const bool same_phase =
+            kGrad && static_cast<int>((reinterpret_cast<uintptr_t>(out) & 15u) / sizeof(E)) == phase;
+        const int len = max(0, min(S, V + phase - team.rank * S));
+        const int nv = (len + kVec - 1) / kVec;
+        const int v0 = (team.rank == 0 && phase > 0) ? 1 : 0, v1 = len / kVec;
+        if (!any) {
+            // a row without a teacher: loss 0 and gradient 0 whatever its logits hold
+            if (a.row_losses && team.rank == 0 && threadIdx.x == 0) a.row_losses[row] = 0.0f;
+            if (kGrad) {
+                if (same_phase) {
+                    uint4* dst = reinterpret_cast<uint4*>(reinterpret_cast<uintptr_t>(out) - phase * sizeof(E)) +
+                                 team.rank * S / kVec;
+                    for (int v = v0 + threadIdx.x; v < v1; v += kThreads) dst[v] = make_uint4(0, 0, 0, 0);
+                }
+                for (int e = threadIdx.x; e < len; e += kThreads) {
+                    const int v = e / kVec;
+                    if (a0 + e >= 0 && (!same_phase || v < v0 || v >= v1)) out[a0 + e] = Elem<E>::narrow(0.0f);
+                }
+            }
+            continue;
+        }
+        Q = block_reduce(Q, Add(), sh.d8);
+        uint4 acc = vneg_inf<E>();
+        load_slice<E, false>(x, V, S, team.rank, buf, acc);
+        const float mine = block_reduce(lanes_max<E>(acc), Max(), sh.f8);
+        const Reference ref(mine, c2);
+        const double ref2 = ref.log2_of(c2);
+        // where a token is listed twice, the first slot stands for it
+        twice = __syncthreads_or(twice);
+        double cross = 0.0, q_here = 0.0;
+        float listed = 0.0f;
+        for (int j = threadIdx.x; j < n; j += kThreads) {
+            const int at = place[j];
+            if (at < 0) continue;
+            const float xj = Elem<E>::widen(elems[at]);
+            slot_x[j] = xj;
+            const float q = slot_q[j];
+            q_here += static_cast<double>(q);
+            if (q != 0.0f)
+                cross += static_cast<double>(q) *
+                         (static_cast<double>(a.teacher_log_probs[row * n + j]) -
+                          kLn2 * (static_cast<double>(xj) * static_cast<double>(c2) - ref2));
+            bool owner = true;
+            if (twice)
+                for (int o = 0; o < j; ++o) owner = owner && place[o] != at;
+            if (owner) listed += ex2(ref.exponent(xj, c2));
+        }
+        __syncthreads();
+        for (int j = threadIdx.x; j < n; j += kThreads)
+            if (place[j] >= 0) elems[place[j]] = Elem<E>::narrow(neg_inf());
+        __syncthreads();
+        const float rest = block_reduce(sum_exp<E>(buf, nv, c2, ref), Add(), sh.f8);
+        listed = block_reduce(listed, Add(), sh.f8);
+        cross = block_reduce(cross, Add(), sh.d8);
+        q_here = block_reduce(q_here, Add(), sh.d8);
+        team.tell(sh.box[parity], DistillPacket{cross, q_here, rest, listed, mine});
+        cluster_sync(team.size);
+        const DistillPacket* box = sh.box[parity];
+        parity ^= 1;
+        float best = box[0].best;
+        for (int c = 1; c < team.size; ++c) best = fmaxf(best, box[c].best);
+        const Reference all(best, c2);
+        const double all2 = all.log2_of(c2);
+        double R = 0.0, L = 0.0, C = 0.0;
+        for (int c = 0; c < team.size; ++c) {
+            const Reference part(box[c].best, c2);
+            const double f = all.factor(part);
+            R += f * static_cast<double>(box[c].rest);
+            L += f * static_cast<double>(box[c].listed);
+            if (box[c].q != 0.0) C += box[c].cross + box[c].q * kLn2 * (all2 - part.log2_of(c2));
+        }
+        const double Z = R + L;
+        const double q_rest = a.tail && R > 0.0 ? fmax(0.0, 1.0 - Q) : 0.0;
+        if (a.row_losses && team.rank == 0 && threadIdx.x == 0) {
+            // log P = ln 2 (x c2 - all2) - log Z
+            double loss = C;
+            if (Q != 0.0) loss += Q * log(Z);
+            if (q_rest > 0.0) loss += q_rest * (log(q_rest) - log(R / Z));
+            if (Z == 0.0) loss = Q > 0.0 ? static_cast<double>(INFINITY) : 0.0;   // nothing above -inf
+            a.row_losses[row] = static_cast<float>(a.reduction == kNone ? loss * static_cast<double>(a.scale) : loss);
+        }
+        if (kGrad) {
+            double w = static_cast<double>(a.scale) / static_cast<double>(a.temperature) * static_cast<double>(g);
+            if (a.reduction == kMean) w /= static_cast<double>(max(1, *a.row_count));
+            const double inv = Z > 0.0 || Z != Z ? 1.0 / Z : 0.0;
+            const float on = static_cast<float>((Q + q_rest) * inv * w);
+            const float off = static_cast<float>(((Q + q_rest) * inv - (q_rest > 0.0 ? q_rest / R : 0.0)) * w);
+            const float wf = static_cast<float>(w);
+            auto element = [&](float f) { return ex2(all.exponent(f, c2)) * off; };
+            auto elements = [&](int begin, int end) {
+                for (int e = max(begin, -a0) + static_cast<int>(threadIdx.x); e < end; e += kThreads)
+                    out[a0 + e] = Elem<E>::narrow(element(Elem<E>::widen(elems[e])));
+            };
+            if (same_phase) {
+                uint4* dst = reinterpret_cast<uint4*>(reinterpret_cast<uintptr_t>(out) - phase * sizeof(E)) +
+                             team.rank * S / kVec;
+                if (all.wide) {
+                    for (int v = v0 + threadIdx.x; v < v1; v += kThreads) {
+                        float f[kVec];
+                        Elem<E>::unpack(buf[v], f);
+#pragma unroll
+                        for (int e = 0; e < kVec; ++e) f[e] = element(f[e]);
+                        dst[v] = Elem<E>::pack(f);
+                    }
+                } else {
+                    for (int v = v0 + threadIdx.x; v < v1; v += kThreads) {
+                        float f[kVec];
+                        Elem<E>::unpack(buf[v], f);
+#pragma unroll
+                        for (int e = 0; e < kVec; ++e) f[e] = ex2(fmaf(f[e], c2, -all.B)) * off;
+                        dst[v] = Elem<E>::pack(f);
+                    }
+                }
+                elements(0, min(len, v0 * kVec));
+                elements(max(v0, v1) * kVec, len);
+            } else {
+                elements(0, len);
+            }
+            __syncthreads();   // the listed places are written a second time
+            for (int j = threadIdx.x; j < n; j += kThreads) {
+                const int at = place[j];
+                if (at < 0) continue;
+                float q = slot_q[j];
+                bool owner = true;
+                if (twice) {
+                    q = 0.0f;
+                    for (int o = 0; o < n; ++o) {
+                        if (place[o] == at) {
+                            owner = owner && o >= j;
+                            q += slot_q[o];
+                        }
+                    }
+                }
+                if (owner) out[a0 + at] = Elem<E>::narrow(fmaf(ex2(all.exponent(slot_x[j], c2)), on, -q * wf));
+            }
+        }
+    }
+    cluster_sync(team.size);
+}
+
+// Rows with at least one slot inside the vocabulary. One cluster of 8 CTAs; a
+// warp stops at a row's first such slot, which is nearly always in its first 32.
+__global__ void __cluster_dims__(8, 1, 1) __launch_bounds__(1024) count_kernel(DistillArgs a) {
+    __shared__ int counts[32];
+    __shared__ int parts[8];
+    const Team team;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int rows = 0;
+    for (int64_t row = team.rank * 32 + warp; row < a.in.rows; row += 256) {
+        bool any = false;
+        for (int j = 0; j < a.n && !any; j += 32) {
+            int64_t i = -1;
+            if (j + lane < a.n) i = teacher_token(a, row * a.n + j + lane);
+            any = __any_sync(kAll, i >= 0 && i < a.in.V) != 0;
+        }
+        rows += any ? 1 : 0;
+    }
+    if (lane == 0) counts[warp] = rows;
+    __syncthreads();
+    int mine = 0;
+    for (int w = 0; w < 32; ++w) mine += counts[w];
+    cluster_sync(8);   // everybody has started
+    if (threadIdx.x == 0) *cg::this_cluster().map_shared_rank(parts + team.rank, 0) = mine;
+    cluster_sync(8);
+    if (team.rank == 0 && threadIdx.x == 0) {
+        int all = 0;
+        for (int c = 0; c < 8; ++c) all += parts[c];
+        *a.row_count = all;
+    }
+}
+
+// The rows' losses added up in 64 bits and one order.
+__global__ void __launch_bounds__(1024) reduce_kernel(DistillArgs a) {
+    __shared__ double parts[32];
+    double v = 0.0;
+    for (int64_t r = threadIdx.x; r < a.in.rows; r += 1024) v += static_cast<double>(a.row_losses[r]);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(kAll, v, o);
+    if ((threadIdx.x & 31) == 0) parts[threadIdx.x >> 5] = v;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        double all = 0.0;
+        for (int w = 0; w < 32; ++w) all += parts[w];
+        all *= static_cast<double>(a.scale);
+        if (a.reduction == kMean) all /= static_cast<double>(max(1, *a.row_count));
+        *a.loss = static_cast<float>(all);
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Launchers
+// ---------------------------------------------------------------------------
+std::mutex g_mu;
+std::vector<std::tuple<const void*, int, size_t>> g_smem;               // kernel, device: shared memory allowed
+std::vector<std::tuple<const void*, int, size_t, int, int>> g_clusters;   // kernel, device, smem, size: resident
+
+// How a row is cut: CTAs per row and elements per slice.
+struct Shape {
+    int size;
+    int S;
+};
+
+// Slices of up to 68 KB let three CTAs share an SM, so that one's loads, one's
+// arithmetic and one's stores overlap. Few rows are cut finer, down to 8 KB,
+// so that they reach more SMs; 16 CTAs (more than every GPU grants a cluster)
+// are taken only for rows that need them.
+Shape shape_of(const Rows& in, int es) {
+    const int vec = 16 / es;
+    auto slice = [&](int size) {
+        const int64_t per = (static_cast<int64_t>(in.V) + vec - 1 + size - 1) / size;
+        return static_cast<int>((per + 63) / 64 * 64);
+    };
+    int size = 1;
+    while (size < 16 && static_cast<int64_t>(slice(size)) * es > 68 * 1024) size *= 2;
+    while (size < 8 && in.rows * size * 2 <= 148 && static_cast<int64_t>(slice(size)) * es > 8 * 1024) size *= 2;
+    return Shape{size, slice(size)};
+}
+
+template <class Kernel, class... Args>
+cudaError_t launch_rows(Kernel kernel, const Rows& in, int size, size_t smem, cudaStream_t stream, Args... args) {
+    const void* fn = reinterpret_cast<const void*>(kernel);
+    int dev = 0;
+    cudaError_t err = cudaGetDevice(&dev);
+    if (err != cudaSuccess) return err;
+    cudaLaunchConfig_t cfg = {};
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = static_cast<unsigned>(size);
+    attr.val.clusterDim.y = 1;
+    attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    int resident = 0;
+    {
+        std::lock_guard<std::mutex> lock(g_mu);
+        bool known = false;
+        for (auto& e : g_smem) {
+            if (std::get<0>(e) != fn || std::get<1>(e) != dev) continue;
+            known = true;
+            if (std::get<2>(e) < smem) {
+                err = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+                if (err != cudaSuccess) return err;
+                std::get<2>(e) = smem;
+            }
+        }
+        if (!known) {
+            err = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+            if (err == cudaSuccess) err = cudaFuncSetAttribute(fn, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+            if (err == cudaSuccess)
+                err = cudaFuncSetAttribute(fn, cudaFuncAttributePreferredSharedMemoryCarveout,
+                                           static_cast<int>(cudaSharedmemCarveoutMaxShared));
+            if (err != cudaSuccess) return err;
+            g_smem.emplace_back(fn, dev, smem);
+        }
+        for (auto& e : g_clusters)
+            if (std::get<0>(e) == fn && std::get<1>(e) == dev && std::get<2>(e) == smem && std::get<3>(e) == size)
+                resident = std::get<4>(e);
+        if (resident == 0) {
+            cfg.gridDim = dim3(static_cast<unsigned>(size));
+            err = cudaOccupancyMaxActiveClusters(&resident, fn, &cfg);
+            if (err != cudaSuccess) return err;
+            if (resident <= 0) return cudaErrorInvalidConfiguration;
+            g_clusters.emplace_back(fn, dev, smem, size, resident);
+        }
+    }
+    const int64_t clusters = std::min<int64_t>(in.rows, resident);
+    cfg.gridDim = dim3(static_cast<unsigned>(clusters * size));
+    return dbs_dev::count_launch(cudaLaunchKernelEx(&cfg, kernel, args...));
+}
+
+int element_size(int dtype) { return dtype == kF32 ? 4 : 2; }
+
+int list_space(int n) {
+    int cap = kBins / 2;   // both lists' space also holds the bins of a search
+    while (cap < 2 * n) cap *= 2;
+    return cap;
+}
+
+template <class E>
+cudaError_t launch_distill_typed(const DistillArgs& a, cudaStream_t stream) {
+    const Shape sh = shape_of(a.in, sizeof(E));
+    const size_t smem = static_cast<size_t>(sh.S) * sizeof(E) + static_cast<size_t>((sh.S + 31) / 32) * 4 +
+                        static_cast<size_t>(a.n) * 12;
+    return a.grad ? launch_rows(distill_kernel<E, true>, a.in, sh.size, smem, stream, a, sh.S)
+                  : launch_rows(distill_kernel<E, false>, a.in, sh.size, smem, stream, a, sh.S);
+}
+
+cudaError_t launch_distill_any(const DistillArgs& a, cudaStream_t stream) {
+    switch (a.in.dtype) {
+        case kF32: return launch_distill_typed<float>(a, stream);
+        case kF16: return launch_distill_typed<__half>(a, stream);
+        default: return launch_distill_typed<__nv_bfloat16>(a, stream);
+    }
+}
+
+}  // namespace
+
+cudaError_t launch_sample(const SampleArgs& a, cudaStream_t stream) {
+    const int es = element_size(a.in.dtype);
+    const Shape sh = shape_of(a.in, es);
+    // lists for rows that may take that path, bins for the others
+    const int cap = list_space(a.top_k ? kSampleList : (a.top_k_all <= kSampleList ? std::max(a.top_k_all, 0) : 0));
+    const size_t smem = static_cast<size_t>(sh.S) * es + static_cast<size_t>(cap) * 16;
+    switch (a.in.dtype) {
+        case kF32: return launch_rows(sample_kernel<float>, a.in, sh.size, smem, stream, a, sh.S, cap);
+        case kF16: return launch_rows(sample_kernel<__half>, a.in, sh.size, smem, stream, a, sh.S, cap);
+        default: return launch_rows(sample_kernel<__nv_bfloat16>, a.in, sh.size, smem, stream, a, sh.S, cap);
+    }
+}
+
+cudaError_t launch_top(const TopArgs& a, cudaStream_t stream) {
+    const int es = element_size(a.in.dtype);
+    const Shape sh = shape_of(a.in, es);
+    const int cap = list_space(a.n);
+    const size_t smem = static_cast<size_t>(sh.S) * es + static_cast<size_t>(cap) * 16;
+    switch (a.in.dtype) {
+        case kF32: return launch_rows(top_kernel<float>, a.in, sh.size, smem, stream, a, sh.S, cap);
+        case kF16: return launch_rows(top_kernel<__half>, a.in, sh.size, smem, stream, a, sh.S, cap);
+        default: return launch_rows(top_kernel<__nv_bfloat16>, a.in, sh.size, smem, stream, a, sh.S, cap);
+    }
+}
+
+cudaError_t launch_distill(const DistillArgs& a, cudaStream_t stream) {
+    if (a.reduction == kMean) {
+        count_kernel<<<8, 1024, 0, stream>>>(a);
+        const cudaError_t err = dbs_dev::count_launch(cudaGetLastError());
+        if (err != cudaSuccess) return err;
+    }
+    cudaError_t err = a.in.rows > 0 ? launch_distill_any(a, stream) : cudaSuccess;
+    if (err != cudaSuccess || a.reduction == kNone) return err;
+    reduce_kernel<<<1, 1024, 0, stream>>>(a);
+    return dbs_dev::count_launch(cudaGetLastError());
+}
+
+cudaError_t launch_distill_backward(const DistillArgs& a, cudaStream_t stream) {
+    return launch_distill_any(a, stream);
+}
+
+}  // namespace dbs_logits

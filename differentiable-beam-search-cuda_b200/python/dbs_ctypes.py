@@ -208,10 +208,19 @@ DEVICE_FUNCTIONS = {
     "dbs_device_merge_rows": (_I, [_VP, _VP, _I, _I, _I, _VP, _VP, _VP, ctypes.POINTER(DBSDeviceDecodeOutputs), _VP]),
     "dbs_device_backward_sparse_noalloc": (
         _I, [_VP, _I, _I, _I, ctypes.POINTER(DBSDeviceDecodeOutputs), _VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP]),
+    "dbs_device_sample": (
+        _I, [_VP, _I, _I64, _I, _I64, _VP, _VP, _F, _VP, _I, _VP, _F, _VP, _F, _VP, _VP]),
+    "dbs_device_top_log_probs": (_I, [_VP, _I, _I64, _I, _I64, _I, _F, _VP, _VP, _VP]),
+    "dbs_device_distill": (
+        _I, [_VP, _I, _I64, _I, _I64, _VP, _VP, _I, _I, _F, _I, _I, _F, _VP, _VP, _VP, _VP, _VP]),
+    "dbs_device_distill_backward": (
+        _I, [_VP, _I, _I64, _I, _I64, _VP, _VP, _I, _I, _F, _I, _I, _F, _VP, _VP, _I64, _I, _VP, _VP]),
 }
 
 PROFILED_KERNELS = ("validate", "row_scan", "step_merge", "weights", "fill_zero", "backward")
 DBS_DEVICE_GRAD_PREZEROED = 1
+DBS_DEVICE_GRAD_UNIT = 2
+DBS_REDUCTIONS = {"none": 0, "sum": 1, "mean": 2}
 
 
 def load_library(path: Optional[str] = None, device_api: bool = True) -> ctypes.CDLL:

@@ -481,6 +481,266 @@ def decode(log_probs: torch.Tensor, options: DBSOptions) -> Tuple[torch.Tensor, 
 
 
 # ---------------------------------------------------------------------------
+# Operators on rows of raw logits: sampling, top log-probs, distillation
+# ---------------------------------------------------------------------------
+_DTYPES = {torch.float32: dbs_ctypes.DBS_DTYPE_F32, torch.float16: dbs_ctypes.DBS_DTYPE_F16,
+           torch.bfloat16: dbs_ctypes.DBS_DTYPE_BF16}
+_MAX_ROW_BYTES = 3_000_000
+_MAX_LIST = 1024
+
+
+def _check_global(rc: int, what: str) -> None:
+    if rc != 0:
+        raise RuntimeError(f"{what} failed: {_library().dbs_last_global_error().decode()}")
+
+
+def _validate_logits(logits: torch.Tensor) -> None:
+    if logits.dtype not in _DTYPES:
+        raise ValueError("logits must be float32, float16 or bfloat16")
+    if logits.dim() < 1:
+        raise ValueError("logits must have shape [..., V]")
+    _validate_positive_int_dim(logits.size(-1), "V")
+    if logits.size(-1) * logits.element_size() > _MAX_ROW_BYTES:
+        raise ValueError(f"a row of logits takes at most {_MAX_ROW_BYTES} bytes")
+
+
+def _logits_rows(logits: torch.Tensor) -> torch.Tensor:
+    """[..., V] as [rows, V] with neighbouring elements in a row: a view where
+    the strides allow it, else a copy."""
+    V = logits.size(-1)
+    x = logits.detach()
+    if V > 1 and x.stride(-1) != 1:
+        x = x.contiguous()
+    if x.dim() == 2:
+        return x
+    try:
+        return x.view(-1, V) if x.numel() else x.reshape(math.prod(x.shape[:-1]), V)
+    except RuntimeError:  # leading dimensions that do not merge
+        return x.contiguous().view(-1, V)
+
+
+def _rows_args(x: torch.Tensor):
+    return _vp(x), _DTYPES[x.dtype], x.size(0), x.size(1), x.stride(0) if x.size(0) > 1 else x.size(1)
+
+
+def _beside(t: torch.Tensor, name: str, device: torch.device, dtype: torch.dtype, shape) -> torch.Tensor:
+    """`t` broadcast to `shape`, contiguous on the logits' device; a tensor on another GPU is refused."""
+    if t.is_cuda and t.device != device:
+        raise ValueError(f"{name} is on {t.device}, the logits are on {device}")
+    try:
+        t = t.detach().to(device=device, dtype=dtype).expand(shape)
+    except RuntimeError:
+        raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}") from None
+    return t.contiguous()
+
+
+def _row_setting(value, name: str, device: torch.device, dtype: torch.dtype, lead, check):
+    """A sampling setting as (per-row tensor or None, scalar): numbers are checked, tensors are read on the device."""
+    if isinstance(value, torch.Tensor):
+        return _beside(value, name, device, dtype, lead), 0
+    check(value)
+    return None, value
+
+
+def _check_temperature(value) -> None:
+    _validate_finite_float(value, "temperature")
+    if value < 0.0:
+        raise ValueError("temperature cannot be negative")
+
+
+def _check_top_k(value) -> None:
+    if value != int(value) or value < 0:
+        raise ValueError("top_k must be a non-negative integer")
+
+
+def _check_top_p(value) -> None:
+    if not 0.0 < value <= 1.0:
+        raise ValueError("top_p must be in (0, 1]")
+
+
+def _check_min_p(value) -> None:
+    if not 0.0 <= value <= 1.0:
+        raise ValueError("min_p must be in [0, 1]")
+
+
+def _validate_positive_temperature(temperature: float) -> None:
+    _validate_finite_float(temperature, "temperature")
+    if not temperature > 0.0:
+        raise ValueError("temperature must be positive")
+
+
+def sample(logits: torch.Tensor, uniforms: torch.Tensor, *, temperature=1.0, top_k=0, top_p=1.0,
+           min_p=0.0) -> torch.Tensor:
+    """One token per row of raw logits [..., V] from uniform numbers [...] in [0, 1): int32 [...].
+
+    The tokens of a row are ordered by (logit desc, token asc). Kept are the
+    first `top_k` (0: all), of these those before which less than `top_p` of
+    their softmax mass lies (1: all), of these those whose probability is at
+    least `min_p` times the best one's; the best is always kept. The token is
+    the least kept one at which the running sum, by index, of the kept weights
+    exp((x - max) / temperature) exceeds u times their total. Sums are held in
+    64 bits, so tokens do not depend on their order. `temperature` 0 takes the
+    best token (ties: the lowest index). NaN counts as -inf; a row without a
+    value above -inf gives -1. Each setting is a number or a tensor of one
+    value per row, whose values are not checked: a temperature that is not
+    positive is 0, a top_k that is not positive keeps all, a top_p of 1 or more
+    keeps all and one of 0 or less the best, a min_p above 1 is 1.
+    """
+    _validate_logits(logits)
+    lead = logits.shape[:-1]
+    if uniforms.dtype != torch.float32:
+        raise ValueError("uniforms must be float32")
+    if uniforms.shape != lead:
+        raise ValueError(f"uniforms must have shape {tuple(lead)}, got {tuple(uniforms.shape)}")
+    device = _cuda_device_for(logits)
+    t_rows, t_all = _row_setting(temperature, "temperature", device, torch.float32, lead, _check_temperature)
+    k_rows, k_all = _row_setting(top_k, "top_k", device, torch.int32, lead, _check_top_k)
+    p_rows, p_all = _row_setting(top_p, "top_p", device, torch.float32, lead, _check_top_p)
+    q_rows, q_all = _row_setting(min_p, "min_p", device, torch.float32, lead, _check_min_p)
+    x = _logits_rows(logits.to(device))
+    u = _beside(uniforms, "uniforms", device, torch.float32, lead)
+    tokens = torch.empty(lead, dtype=torch.int32, device=device)
+    with torch.cuda.device(device):
+        rc = _library().dbs_device_sample(*_rows_args(x), _vp(u), _vp(t_rows), t_all, _vp(k_rows),
+                                          min(int(k_all), _INT_MAX), _vp(p_rows), p_all, _vp(q_rows), q_all,
+                                          _vp(tokens), _stream_ptr(device))
+    _check_global(rc, "sample")
+    return tokens.to(logits.device)
+
+
+def top_log_probs(logits: torch.Tensor, n: int, *, temperature: float = 1.0) -> Tuple[torch.Tensor, torch.Tensor]:
+    """The n best tokens of each row of raw logits [..., V] and their log-probs
+    under softmax(logits / temperature): (float32 [..., n], int32 [..., n]).
+
+    Best first, ties by the lowest token; NaN counts as -inf; n is at most
+    min(V, 1024). Places beyond the tokens above -inf hold -inf and -1, which
+    `distillation_loss` reads as empty. No gradient flows through it.
+    """
+    _validate_logits(logits)
+    if n != int(n) or not 1 <= n <= min(logits.size(-1), _MAX_LIST):
+        raise ValueError(f"n must be in 1 .. {min(logits.size(-1), _MAX_LIST)}")
+    _validate_positive_temperature(temperature)
+    device = _cuda_device_for(logits)
+    x = _logits_rows(logits.to(device))
+    shape = (*logits.shape[:-1], int(n))
+    log_probs = torch.empty(shape, dtype=torch.float32, device=device)
+    tokens = torch.empty(shape, dtype=torch.int32, device=device)
+    with torch.cuda.device(device):
+        rc = _library().dbs_device_top_log_probs(*_rows_args(x), int(n), temperature, _vp(log_probs), _vp(tokens),
+                                                 _stream_ptr(device))
+    _check_global(rc, "top_log_probs")
+    return log_probs.to(logits.device), tokens.to(logits.device)
+
+
+def _distill_args(x, log_probs, tokens, settings):
+    temperature, tail, reduction, scale = settings
+    return (*_rows_args(x), _vp(log_probs), _vp(tokens), tokens.element_size(), tokens.size(-1), temperature,
+            int(tail), reduction, scale)
+
+
+def _distill_forward(logits, log_probs, tokens, settings, need_grad):
+    """(loss, gradient for an incoming gradient of 1 or None, rows with a teacher or None)."""
+    x = _logits_rows(logits)
+    lead, device = logits.shape[:-1], logits.device
+    reduction = settings[2]
+    row_losses = torch.empty(lead, dtype=torch.float32, device=device)
+    loss = row_losses if reduction == 0 else torch.empty((), dtype=torch.float32, device=device)
+    rows = torch.empty((1,), dtype=torch.int32, device=device) if reduction == 2 else None
+    grad = torch.empty(logits.shape, dtype=logits.dtype, device=device) if need_grad else None
+    with torch.cuda.device(device):
+        rc = _library().dbs_device_distill(*_distill_args(x, log_probs, tokens, settings), _vp(row_losses),
+                                           None if reduction == 0 else _vp(loss), _vp(rows), _vp(grad),
+                                           _stream_ptr(device))
+    _check_global(rc, "distillation_loss")
+    return loss, grad, rows
+
+
+class _DBSDistillation(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits: torch.Tensor, log_probs: torch.Tensor, tokens: torch.Tensor, settings):
+        # The gradient for an incoming gradient of 1 is written in the same
+        # pass; the backward keeps it, or computes it again from the logits
+        # (one rounding) where the incoming gradient is another.
+        loss, ctx.grad, rows = _distill_forward(logits, log_probs, tokens, settings, True)
+        ctx.settings = settings
+        ctx.save_for_backward(logits, log_probs, tokens, rows)
+        return loss
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad_output: torch.Tensor):
+        logits, log_probs, tokens, rows = ctx.saved_tensors
+        # the forward's buffer serves the first backward; a repeated one
+        # (retain_graph) gets a buffer of its own
+        grad, ctx.grad = ctx.grad, None
+        flags = dbs_ctypes.DBS_DEVICE_GRAD_UNIT
+        if grad is None:
+            grad, flags = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device), 0
+        g = grad_output.detach().to(dtype=torch.float32)
+        stride = 1
+        if all(s == 0 for s in g.stride()):
+            stride = 0      # one value for all rows
+        else:
+            g = g.contiguous()
+        x = _logits_rows(logits)
+        with torch.cuda.device(logits.device):
+            rc = _library().dbs_device_distill_backward(*_distill_args(x, log_probs, tokens, ctx.settings), _vp(rows),
+                                                        _vp(g), stride, flags, _vp(grad), _stream_ptr(logits.device))
+        _check_global(rc, "distillation_loss backward")
+        return grad, None, None, None
+
+
+def distillation_loss(logits: torch.Tensor, teacher_log_probs: torch.Tensor, teacher_tokens: torch.Tensor, *,
+                      temperature: float = 1.0, tail: bool = True, reduction: str = "mean",
+                      scale: float = 1.0) -> torch.Tensor:
+    """Divergence of softmax(logits / temperature) from a teacher's listed
+    log-probs (as `top_log_probs` gives them), with its gradient in the logits.
+
+    logits [..., V]; teacher_log_probs and teacher_tokens (int32 or int64)
+    [..., n], n <= 1024, at the same temperature. A slot whose token is outside
+    [0, V) is empty. With P the student's probabilities and q the teacher's, a
+    row's loss is sum q (log q - log P) over its slots; with `tail`, all tokens
+    that are not listed make up one more class of mass 1 - sum q (without it,
+    that mass is left out). A row without slots has loss 0 and gradient 0
+    whatever its logits hold, and "mean" divides by the number of the others;
+    "sum" and "none" (each row's, [...]) are the other reductions. `scale`
+    multiplies the loss (temperature ** 2 is usual); a factor given here costs
+    nothing, while one applied to the loss afterwards makes the backward read
+    the logits a second time. The loss is float32; gradients flow to the logits
+    alone.
+    """
+    _validate_logits(logits)
+    lead = logits.shape[:-1]
+    if teacher_tokens.dtype not in (torch.int32, torch.int64):
+        raise ValueError("teacher_tokens must be int32 or int64")
+    if not teacher_log_probs.is_floating_point():
+        raise ValueError("teacher_log_probs must be floating-point")
+    if teacher_tokens.dim() < 1 or teacher_tokens.shape[:-1] != lead:
+        raise ValueError(f"teacher_tokens must have shape {(*lead, 'n')}, got {tuple(teacher_tokens.shape)}")
+    if teacher_log_probs.shape != teacher_tokens.shape:
+        raise ValueError("teacher_log_probs and teacher_tokens must have the same shape")
+    if not 1 <= teacher_tokens.size(-1) <= _MAX_LIST:
+        raise ValueError(f"a teacher's row must have 1 .. {_MAX_LIST} slots")
+    if reduction not in dbs_ctypes.DBS_REDUCTIONS:
+        raise ValueError("reduction must be 'none', 'sum' or 'mean'")
+    _validate_positive_temperature(temperature)
+    _validate_finite_float(scale, "scale")
+    grad_on = torch.is_grad_enabled()
+    if grad_on and teacher_log_probs.requires_grad:
+        raise ValueError("teacher_log_probs takes no gradient; detach it")
+    device = _cuda_device_for(logits)
+    x = logits.to(device)
+    log_probs = _beside(teacher_log_probs, "teacher_log_probs", device, torch.float32, teacher_log_probs.shape)
+    tokens = _beside(teacher_tokens, "teacher_tokens", device, teacher_tokens.dtype, teacher_tokens.shape)
+    settings = (float(temperature), bool(tail), dbs_ctypes.DBS_REDUCTIONS[reduction], float(scale))
+    if grad_on and x.requires_grad:
+        loss = _DBSDistillation.apply(x, log_probs, tokens, settings)
+    else:
+        loss = _distill_forward(x, log_probs, tokens, settings, False)[0]
+    return loss.to(logits.device)
+
+
+# ---------------------------------------------------------------------------
 # torch.ops.dbs.* with the reference's schemas (python/torch_extension.cpp:191-194)
 # ---------------------------------------------------------------------------
 def _op_options(*args) -> DBSOptions:

@@ -155,6 +155,74 @@ DBS_EXPORT int dbs_device_backward_sparse_noalloc(DBSDecoderHandle* handle, int 
                                                   float* sparse_values, int64_t* sparse_counts,
                                                   float* grad_initial_scores, void* cuda_stream);
 
+/* Operators on rows of raw logits (not log-probs), device data only. The
+ * reference has no counterpart: it starts at log-probs and has beam selection
+ * alone. Common arguments: `logits` holds `rows` rows of `vocab_size`
+ * elements of DBS_DTYPE_F32 / F16 / BF16 (`data_type`), row r at
+ * r * row_stride elements (0 repeats one row); rows need no alignment beyond
+ * their element's. A row holds at most 3000000 bytes. No handle: errors are
+ * in dbs_last_global_error. No call allocates, waits or keeps state, so calls
+ * may overlap on several streams and be captured into graphs. */
+
+/* One token per row from uniform numbers in [0, 1). With m the row's maximum
+ * (NaN counts as -inf) and weights w_i = exp((x_i - m) / temperature), 0 below
+ * exp(-708): order the tokens by (logit desc, token asc); keep the first top_k
+ * (all where top_k <= 0), of these those before which less than top_p of their
+ * mass lies (all where top_p >= 1), of these those with w >= min_p; the best
+ * always. The token is the least kept index at which the sum of kept weights
+ * up to and including it exceeds u times their total (the last kept one of
+ * positive weight where none does: u of 1 or more, or NaN). temperature <= 0 takes the best
+ * token, a row without a value above -inf gives -1. Sums are held in 64 bits.
+ * temperatures / top_ks / top_ps / min_ps are per-row settings [rows] or NULL
+ * for the value beside them. */
+DBS_EXPORT int dbs_device_sample(const void* logits, int data_type, int64_t rows, int vocab_size, int64_t row_stride,
+                                 const float* uniforms, const float* temperatures, float temperature,
+                                 const int32_t* top_ks, int top_k, const float* top_ps, float top_p,
+                                 const float* min_ps, float min_p, int32_t* tokens, void* cuda_stream);
+
+/* The n best tokens of each row (logit desc, token asc; NaN counts as -inf)
+ * and their log-probs under softmax(logits / temperature): log_probs and
+ * tokens [rows, n], n <= min(vocab_size, 1024). Places beyond the tokens above
+ * -inf hold -inf and -1. */
+DBS_EXPORT int dbs_device_top_log_probs(const void* logits, int data_type, int64_t rows, int vocab_size,
+                                        int64_t row_stride, int n, float temperature, float* log_probs,
+                                        int32_t* tokens, void* cuda_stream);
+
+/* Distillation from a teacher's listed log-probs. teacher_tokens [rows, slots]
+ * (int32 or int64: token_bytes 4 or 8) and teacher_log_probs [rows, slots],
+ * slots <= 1024; a slot whose token is outside [0, vocab_size) is empty. With
+ * P = softmax(logits / temperature), S the listed tokens, q_j = exp of a
+ * slot's log-prob, P_r = sum of P outside S, and q_r = max(0, 1 - sum q)
+ * where `tail` is set and P_r > 0, else 0, a row's loss is
+ *   sum_j q_j (log q_j - log P_j) + q_r (log q_r - log P_r),   0 log 0 = 0,
+ * and 0 for a row without slots, whatever its logits hold. `reduction`:
+ * DBS_REDUCE_NONE (row_losses [rows] alone; loss NULL), _SUM, or _MEAN over
+ * the rows with slots (row_count [1] is written); `scale` multiplies the
+ * result. row_losses [rows] is needed for every reduction. grad_logits
+ * ([rows, vocab_size] contiguous, the logits' type, or NULL) takes the
+ * gradient for an incoming gradient of 1, in the same pass over the logits. */
+#define DBS_REDUCE_NONE 0
+#define DBS_REDUCE_SUM 1
+#define DBS_REDUCE_MEAN 2
+DBS_EXPORT int dbs_device_distill(const void* logits, int data_type, int64_t rows, int vocab_size, int64_t row_stride,
+                                  const float* teacher_log_probs, const void* teacher_tokens, int token_bytes,
+                                  int slots, float temperature, int tail, int reduction, float scale,
+                                  float* row_losses, float* loss, int32_t* row_count, void* grad_logits,
+                                  void* cuda_stream);
+
+/* The gradient of dbs_device_distill for the incoming gradient grad_loss
+ * (device; row r's at r * grad_loss_stride, so 0 for one value). The other
+ * arguments are the forward call's, row_count as it wrote it. With
+ * DBS_DEVICE_GRAD_UNIT in `flags`, grad_logits is what the forward call wrote,
+ * and rows whose incoming gradient is 1 stay as they are. */
+#define DBS_DEVICE_GRAD_UNIT 2
+DBS_EXPORT int dbs_device_distill_backward(const void* logits, int data_type, int64_t rows, int vocab_size,
+                                           int64_t row_stride, const float* teacher_log_probs,
+                                           const void* teacher_tokens, int token_bytes, int slots, float temperature,
+                                           int tail, int reduction, float scale, const int32_t* row_count,
+                                           const float* grad_loss, int64_t grad_loss_stride, int flags,
+                                           void* grad_logits, void* cuda_stream);
+
 /* Diagnostics of the most recent device decode whose counters have been read
  * back (process-wide): rows the row scan read a second time from HBM (a
  * speculative threshold, learned from earlier rows, kept fewer entries than
