@@ -18,7 +18,8 @@ enum DataType : int { kF32 = 0, kF16 = 1, kBF16 = 2 };
 
 // Limits of this implementation.
 constexpr int kMaxTop = 1024;                 // entries of a top list, slots of a teacher's row
-constexpr int64_t kMaxRowBytes = 3000000;      // a row has to fit 16 CTAs' shared memory
+constexpr int64_t kMaxRowBytes = 3000000;      // a row has to fit 16 CTAs' shared memory,
+constexpr int64_t kMaxDistillBytes = 1040000;  // three times where it is distilled
 
 struct Rows {
     const void* x = nullptr;
@@ -65,7 +66,8 @@ struct DistillArgs {
     float scale = 1.0f;
     float* row_losses = nullptr;                // [rows]; null: not written
     float* loss = nullptr;                      // the reduced loss; null with kNone
-    int32_t* row_count = nullptr;               // kMean: rows with a teacher (written forward, read backward)
+    void* state = nullptr;                      // distill_state_bytes(); written forward, read backward
+    int skip_state = 0;                         // backward: the sums are there already
     void* grad = nullptr;                       // [rows, V] contiguous, the logits' type; null: none
     // backward: gradient of the loss (one value, or one for each row)
     const float* grad_loss = nullptr;
@@ -76,6 +78,7 @@ struct DistillArgs {
 cudaError_t launch_sample(const SampleArgs& a, cudaStream_t stream);
 cudaError_t launch_top(const TopArgs& a, cudaStream_t stream);
 cudaError_t launch_distill(const DistillArgs& a, cudaStream_t stream);
+int64_t distill_state_bytes(int64_t rows, int n);
 cudaError_t launch_distill_backward(const DistillArgs& a, cudaStream_t stream);
 
 }  // namespace dbs_logits

@@ -138,6 +138,23 @@ __device__ __forceinline__ uint4 ldg_once(const uint4* p) {
 
 __device__ __forceinline__ float neg_inf() { return __uint_as_float(0xFF800000u); }
 
+// Two floats in one register pair: sm_100a multiplies or adds both in one
+// instruction.
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 r;
+    asm("add.rn.f32x2 %0, %1, %2;"
+        : "=l"(reinterpret_cast<uint64_t&>(r))
+        : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)));
+    return r;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    float2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;"
+        : "=l"(reinterpret_cast<uint64_t&>(r))
+        : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)));
+    return r;
+}
+
 __device__ __forceinline__ float ex2(float v) {
     float r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
@@ -730,10 +747,6 @@ struct Reference {
         if (wide || part.wide) return part.best == best ? 1.0 : 0.0;
         return exp2(static_cast<double>(part.B) - static_cast<double>(B));
     }
-    // the reference in units of log2
-    __device__ double log2_of(float c2) const {
-        return wide ? static_cast<double>(best) * static_cast<double>(c2) : static_cast<double>(B);
-    }
 };
 
 // This thread's share of the slice's sum.
@@ -774,7 +787,7 @@ __global__ void __launch_bounds__(kThreads, 3) top_kernel(TopArgs a, int S, int 
     uint64_t* sorted = list + cap;
     const int64_t step = gridDim.x / team.size;
     const int n = a.n;
-    const float c2 = 1.4426950408889634f / a.temperature;
+    const float c2 = fminf(1.4426950408889634f / a.temperature, FLT_MAX);
     int leader = 0;
     cluster_sync(team.size);   // everybody's shared memory exists from here on
     for (int64_t row = blockIdx.x / team.size; row < a.in.rows; row += step) {
@@ -1133,270 +1146,499 @@ __global__ void __launch_bounds__(kThreads, 3) sample_kernel(SampleArgs a, int S
 // ---------------------------------------------------------------------------
 // Distillation
 // ---------------------------------------------------------------------------
-struct DistillPacket {
-    double cross;     // sum of q (l - ln 2 (x c2 - reference)) over the CTA's slots
-    double q;         // and of q
-    float rest;       // sum of the exponentials of what is not listed
-    float listed;     // and of what is listed
-    float best;
+// What a call keeps of its rows between its kernels (and for a backward).
+struct SlotState {     // a teacher's slot
+    int token;         // -1: empty, or another slot of this token stands for it
+    float x;           // the student's logit
+    float q;           // the token's probability, all its slots together
+    int unused;
 };
-struct DistillShared {
-    DistillPacket box[2][kMaxCluster];
-    double d8[kWarps];
-    float f8[kWarps];
-    int i8[kWarps];
+struct RowState {
+    double Q;          // sum of q
+    double C;          // sum of q (l - ln 2 c2 (x - best_listed)), slot by slot
+    float best_listed; // maximum of the listed logits, -inf without any
+    float listed;      // sum of their exponentials 2^(c2 (x - best_listed))
+    float best_rest;   // the same over all other logits
+    float rest;
 };
+struct DistillState {
+    SlotState* slots;  // [rows, n]
+    RowState* rows;    // [rows]
+    int* any;          // [rows]: the row has slots
+};
+
+__host__ __device__ __forceinline__ DistillState state_of(const DistillArgs& a) {
+    DistillState s;
+    char* p = static_cast<char*>(a.state);
+    s.slots = reinterpret_cast<SlotState*>(p);
+    p += static_cast<int64_t>(a.in.rows) * a.n * static_cast<int64_t>(sizeof(SlotState));
+    s.rows = reinterpret_cast<RowState*>(p);
+    p += a.in.rows * static_cast<int64_t>(sizeof(RowState));
+    s.any = reinterpret_cast<int*>(p);
+    return s;
+}
 
 __device__ __forceinline__ int64_t teacher_token(const DistillArgs& a, int64_t at) {
     return a.token_bytes == 8 ? static_cast<const int64_t*>(a.teacher_tokens)[at]
                               : static_cast<int64_t>(static_cast<const int32_t*>(a.teacher_tokens)[at]);
 }
 
-// One pass over the row gives its loss and (kGrad) its gradient: the slice
-// stays in shared memory between the sums and the gradient's rows, so the
-// logits are read once and the gradient written once.
-template <class E, bool kGrad>
-__global__ void __launch_bounds__(kThreads, 3) distill_kernel(DistillArgs a, int S) {
-    constexpr int kVec = Elem<E>::kVec;
-    extern __shared__ uint4 dyn[];
-    __shared__ DistillShared sh;
-    const Team team;
-    const int n = a.n, V = a.in.V;
-    uint4* buf = dyn;
-    E* elems = reinterpret_cast<E*>(dyn);
-    const int words = (S + 31) / 32;
-    uint32_t* seen = reinterpret_cast<uint32_t*>(elems + S);   // a bit for each listed place
-    int* place = reinterpret_cast<int*>(seen + words);        // slot -> place in the slice, or -1
-    float* slot_x = reinterpret_cast<float*>(place + n);
-    float* slot_q = slot_x + n;
-    const int64_t step = gridDim.x / team.size;
-    const float c2 = 1.4426950408889634f / a.temperature;
-    constexpr double kLn2 = 0.69314718055994530942;
-    int parity = 0;
-    cluster_sync(team.size);
-    for (int64_t row = blockIdx.x / team.size; row < a.in.rows; row += step) {
-        float g = 1.0f;
-        if (a.grad_loss) {
-            g = a.grad_loss[row * a.grad_loss_stride];
-            if (a.skip_unit && g == 1.0f) continue;   // the same for the whole cluster
+// 2^(c2 (x - best)) for x <= best; 0 where nothing is above -inf.
+__device__ __forceinline__ float share(float x, float best, float c2) {
+    return best > neg_inf() || best != best ? ex2((x - best) * c2) : 0.0f;
+}
+
+template <class T, class Op>
+__device__ __forceinline__ T reduce_block(T v, Op op, T* scratch) {   // any number of warps; scratch: 32 values
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v = op(v, __shfl_xor_sync(kAll, v, o));
+    if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = v;
+    __syncthreads();
+    v = scratch[0];
+    for (int w = 1; w < static_cast<int>(blockDim.x) / 32; ++w) v = op(v, scratch[w]);
+    __syncthreads();
+    return v;
+}
+
+// The teacher's slots, a CTA per row: everything that takes a thread a while
+// is done here, for all rows at once, and not between the barriers of the
+// rows' pass. A token listed twice is found in a hash table of `mask` + 1
+// places; its first slot stands for it with the sum of the probabilities.
+template <class E>
+__global__ void __launch_bounds__(256) slots_kernel(DistillArgs a, int mask) {
+    extern __shared__ int table[];      // tokens, then their first slots
+    __shared__ double d32[32];
+    __shared__ float f32[32];
+    int* first = table + mask + 1;
+    const DistillState state = state_of(a);
+    const int n = a.n, tid = threadIdx.x, threads = blockDim.x;
+    const float c2 = fminf(1.4426950408889634f / a.temperature, FLT_MAX);
+    for (int64_t row = blockIdx.x; row < a.in.rows; row += gridDim.x) {
+        const E* x = static_cast<const E*>(a.in.x) + row * a.in.stride;
+        SlotState* slots = state.slots + row * n;
+        for (int i = tid; i <= mask; i += threads) {
+            table[i] = -1;
+            first[i] = 0x7FFFFFFF;
         }
         __syncthreads();
-        for (int w = threadIdx.x; w < words; w += kThreads) seen[w] = 0;
-        const E* x = static_cast<const E*>(a.in.x) + row * a.in.stride;
-        const int phase = static_cast<int>((reinterpret_cast<uintptr_t>(x) & 15u) / sizeof(E));
-        const int a0 = team.rank * S - phase;     // token of the slice's element 0
-        // the teacher's slots: their probabilities' sum, and which fall into this slice
-        double Q = 0.0;
-        int any = 0;
-        __syncthreads();
-        bool twice = false;
-        for (int j = threadIdx.x; j < n; j += kThreads) {
-            const int64_t i = teacher_token(a, row * n + j);
-            const float l = a.teacher_log_probs[row * n + j];
-            int at = -1;
-            float q = 0.0f;
-            if (i >= 0 && i < V) {
-                any = 1;
-                const double q64 = exp(static_cast<double>(l));
-                Q += q64;
-                q = static_cast<float>(q64);
-                const int64_t here = i - a0;
-                if (here >= 0 && here < S) {
-                    at = static_cast<int>(here);
-                    const uint32_t bit = 1u << (at & 31);
-                    twice = twice || (atomicOr(&seen[at >> 5], bit) & bit) != 0;
-                }
+        auto find = [&](int token) {
+            uint32_t h = (static_cast<uint32_t>(token) * 2654435761u) >> 16;
+            while (true) {
+                h &= static_cast<uint32_t>(mask);
+                const int was = atomicCAS(&table[h], -1, token);
+                if (was == -1 || was == token) return h;
+                ++h;
             }
-            place[j] = at;
-            slot_q[j] = q;
+        };
+        float best = neg_inf();
+        double Q = 0.0;
+        bool any = false;
+        for (int j = tid; j < n; j += threads) {
+            const int64_t i = teacher_token(a, row * n + j);
+            SlotState slot = {-1, 0.0f, 0.0f, 0};
+            if (i >= 0 && i < a.in.V) {
+                any = true;
+                slot.token = static_cast<int>(i);
+                slot.x = Elem<E>::widen(x[i]);
+                const double q = exp(static_cast<double>(a.teacher_log_probs[row * n + j]));
+                slot.q = static_cast<float>(q);
+                Q += q;
+                best = fmaxf(best, slot.x);
+                atomicMin(&first[find(slot.token)], j);
+            }
+            slots[j] = slot;
         }
         any = __syncthreads_or(any);
+        best = reduce_block(best, Max(), f32);
+        Q = reduce_block(Q, Add(), d32);
+        double C = 0.0;
+        float listed = 0.0f;
+        bool twice = false;
+        for (int j = tid; j < n; j += threads) {
+            SlotState slot = slots[j];
+            if (slot.token < 0) continue;
+            const float l = a.teacher_log_probs[row * n + j];
+            if (slot.q != 0.0f) {
+                const double z = slot.x == best ? 0.0 : static_cast<double>(slot.x) - static_cast<double>(best);
+                C += static_cast<double>(slot.q) *
+                     (static_cast<double>(l) - 0.69314718055994530942 * static_cast<double>(c2) * z);
+            }
+            if (first[find(slot.token)] == j) {
+                listed += share(slot.x, best, c2);
+            } else {
+                twice = true;
+            }
+        }
+        listed = reduce_block(listed, Add(), f32);
+        C = reduce_block(C, Add(), d32);
+        if (__syncthreads_or(twice)) {
+            for (int j = tid; j < n; j += threads) {
+                const int token = slots[j].token;
+                if (token < 0 || first[find(token)] != j) continue;
+                float q = 0.0f;
+                for (int o = j; o < n; ++o)
+                    if (teacher_token(a, row * n + o) == token) q += slots[o].q;
+                slots[j].unused = __float_as_int(q);
+            }
+            __syncthreads();
+            for (int j = tid; j < n; j += threads) {
+                if (slots[j].token < 0) continue;
+                if (first[find(slots[j].token)] == j)
+                    slots[j].q = __int_as_float(slots[j].unused);
+                else
+                    slots[j].token = -1;
+            }
+        }
+        if (tid == 0) {
+            state.rows[row] = RowState{Q, C, best, listed, neg_inf(), 0.0f};
+            state.any[row] = any ? 1 : 0;
+        }
+        __syncthreads();
+    }
+}
+
+__device__ __forceinline__ void copy_async(uint4* to, const uint4* from) {
+    asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16;" ::"r"(
+                     static_cast<uint32_t>(__cvta_generic_to_shared(to))),
+                 "l"(from)
+                 : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int kLeft>
+__device__ __forceinline__ void copies_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(kLeft) : "memory");
+}
+// The cluster's barrier for threads that have nothing to show: their stores
+// need not have landed.
+__device__ __forceinline__ void cluster_arrive_relaxed() { asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory"); }
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
+
+template <int kW>
+struct DistillShared {
+    float2 box[2][kMaxCluster];   // maximum and sum of the CTAs' slices
+    float2 part[kW];              // and of the warps' vectors
+    float ends[32];               // the slice's elements that no whole vector holds
+    int i32[32];
+};
+
+// One pass over the row gives its sum and (kGrad) its gradient: the logits are
+// read once and the gradient written once. The slices of three rows are in
+// shared memory or on their way into it, so the memory works on while the
+// cluster exchanges its sums. A thread copies the same eight vectors that it
+// adds up by their own maximum; the exponentials stay in its registers, so the
+// gradient costs a multiplication each, and the buffer is free for another
+// row as soon as it was read.
+// What the teacher lists is not part of the sum, which must not be a
+// difference of two sums (a tail of 1e-6 would be lost in it): the listed
+// places become -inf in shared memory, and their gradients are written last.
+template <class E, bool kGrad, int kT>
+__global__ void __launch_bounds__(kT, 512 / kT) distill_kernel(DistillArgs a, int S) {
+    constexpr int kVec = Elem<E>::kVec;
+    constexpr int kRing = 3;
+    constexpr int kHold = 8;
+    constexpr int kW = kT / 32;
+    extern __shared__ uint4 dyn[];
+    __shared__ DistillShared<kW> sh;
+    // the backward of a loss that was not multiplied by anything: all is done
+    if (a.skip_unit && a.grad_loss_stride == 0 && *a.grad_loss == 1.0f) return;
+    const Team team;
+    const DistillState state = state_of(a);
+    const int n = a.n, V = a.in.V, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int slice_vecs = S / kVec;
+    const int64_t step = gridDim.x / team.size;
+    const float c2 = fminf(1.4426950408889634f / a.temperature, FLT_MAX);
+    const float2 cc = make_float2(c2, c2);
+    float unit = a.scale / a.temperature;
+    if (kGrad && a.reduction == kMean) {
+        int rows = 0;
+        for (int64_t r = tid; r < a.in.rows; r += kT) rows += state.any[r];
+        unit /= static_cast<float>(max(1, reduce_block(rows, Add(), sh.i32)));
+    }
+    cluster_sync(team.size);
+
+    const int64_t first_row = blockIdx.x / team.size;
+    const E* in = static_cast<const E*>(a.in.x);
+    // Where a row's slice lies: positions count from the 16-byte boundary at
+    // or before the row's first element; [v0, v1) are whole vectors.
+    struct View {
+        const uint4* src;
+        int phase, v0, v1, len;
+    };
+    auto view = [&](int64_t r) {
+        const uintptr_t x = reinterpret_cast<uintptr_t>(in + r * a.in.stride);
+        View w;
+        w.phase = static_cast<int>((x & 15u) / sizeof(E));
+        w.len = max(0, min(S, V + w.phase - team.rank * S));
+        w.v0 = team.rank == 0 && w.phase > 0 ? 1 : 0;
+        w.v1 = w.len / kVec;
+        w.src = reinterpret_cast<const uint4*>(x & ~static_cast<uintptr_t>(15)) + team.rank * slice_vecs;
+        return w;
+    };
+    auto start = [&](int64_t r, bool go, int buffer) {
+        if (go) {
+            const View w = view(r);
+            const int left = w.v1 - w.v0 - tid;
+            uint4* to = dyn + buffer * slice_vecs + w.v0 + tid;
+            const uint4* from = w.src + w.v0 + tid;
+#pragma unroll
+            for (int i = 0; i < kHold; ++i)
+                if (i * kT < left) copy_async(to + i * kT, from + i * kT);
+        }
+        copies_commit();
+    };
+    auto wanted = [&](int64_t r) { return r < a.in.rows && state.any[r] != 0; };
+    bool have[kRing];   // the rows of this turn and the next two
+#pragma unroll
+    for (int b = 0; b < kRing; ++b) {
+        have[b] = wanted(first_row + b * step);
+        start(first_row + b * step, have[b], b);
+    }
+    bool ahead = wanted(first_row + kRing * step);
+    SlotState slot = {-1, 0.0f, 0.0f, 0};   // this thread's first slot of the row to come
+    if (have[0] && tid < n) slot = state.slots[first_row * n + tid];
+    int buffer = 0, turn = 0;
+    for (int64_t row = first_row; row < a.in.rows; row += step) {
+        const bool any = have[0], go = ahead;
+        have[0] = have[1];
+        have[1] = have[2];
+        have[2] = ahead;
+        const int64_t later = row + kRing * step;
+        ahead = wanted(later + step);
+        const int buf_at = buffer;
+        buffer = buffer + 1 == kRing ? 0 : buffer + 1;
+        uint4* buf = dyn + buf_at * slice_vecs;
+        E* elems = reinterpret_cast<E*>(buf);
+        const View here = view(row);
+        const int v0 = here.v0, v1 = here.v1, len = here.len;
+        const int a0 = team.rank * S - here.phase;   // token of the slice's element 0
+        const SlotState mine = slot;
+        if (have[0] && tid < n) slot = state.slots[(row + step) * n + tid];
+        float g = 1.0f;
+        if (kGrad && a.grad_loss) g = a.grad_loss[row * a.grad_loss_stride];
         E* out = static_cast<E*>(a.grad) + (kGrad ? row * V : 0);
         const bool same_phase =
-            kGrad && static_cast<int>((reinterpret_cast<uintptr_t>(out) & 15u) / sizeof(E)) == phase;
-        const int len = max(0, min(S, V + phase - team.rank * S));
-        const int nv = (len + kVec - 1) / kVec;
-        const int v0 = (team.rank == 0 && phase > 0) ? 1 : 0, v1 = len / kVec;
-        if (!any) {
-            // a row without a teacher: loss 0 and gradient 0 whatever its logits hold
-            if (a.row_losses && team.rank == 0 && threadIdx.x == 0) a.row_losses[row] = 0.0f;
-            if (kGrad) {
-                if (same_phase) {
-                    uint4* dst = reinterpret_cast<uint4*>(reinterpret_cast<uintptr_t>(out) - phase * sizeof(E)) +
-                                 team.rank * S / kVec;
-                    for (int v = v0 + threadIdx.x; v < v1; v += kThreads) dst[v] = make_uint4(0, 0, 0, 0);
+            kGrad && static_cast<int>((reinterpret_cast<uintptr_t>(out) & 15u) / sizeof(E)) == here.phase;
+        uint4* dst = reinterpret_cast<uint4*>(reinterpret_cast<uintptr_t>(out) & ~static_cast<uintptr_t>(15)) +
+                     team.rank * slice_vecs + v0 + tid;
+        const int left = v1 - v0 - tid;   // of this thread's vectors, those with i * kT < left exist
+        // elements of the slice that no whole vector holds, [0, head) and
+        // [tail_at, len), are the last warp's
+        const int head = min(len, v0 * kVec), tail_at = max(head, v1 * kVec);
+        const int ragged = lane < head ? lane : tail_at + lane - head;
+        const bool at_end = warp == kW - 1 && ragged < len && a0 + ragged >= 0;
+        if (!any || (a.skip_unit && g == 1.0f)) {   // the same for the whole cluster
+            copies_wait<kRing - 1>();   // this buffer's copies, should there be any, before others go into it
+            start(later, go, buf_at);
+            if (kGrad && !any) {
+                // a row without a teacher: gradient 0 whatever its logits hold
+#pragma unroll
+                for (int i = 0; i < kHold; ++i) {
+                    if (i * kT >= left) continue;
+                    if (same_phase)
+                        __stcs(dst + i * kT, make_uint4(0, 0, 0, 0));
+                    else
+#pragma unroll
+                        for (int k = 0; k < kVec; ++k)
+                            out[a0 + (v0 + tid + i * kT) * kVec + k] = Elem<E>::narrow(0.0f);
                 }
-                for (int e = threadIdx.x; e < len; e += kThreads) {
-                    const int v = e / kVec;
-                    if (a0 + e >= 0 && (!same_phase || v < v0 || v >= v1)) out[a0 + e] = Elem<E>::narrow(0.0f);
-                }
+                if (at_end) out[a0 + ragged] = Elem<E>::narrow(0.0f);
             }
             continue;
         }
-        Q = block_reduce(Q, Add(), sh.d8);
-        uint4 acc = vneg_inf<E>();
-        load_slice<E, false>(x, V, S, team.rank, buf, acc);
-        const float mine = block_reduce(lanes_max<E>(acc), Max(), sh.f8);
-        const Reference ref(mine, c2);
-        const double ref2 = ref.log2_of(c2);
-        // where a token is listed twice, the first slot stands for it
-        twice = __syncthreads_or(twice);
-        double cross = 0.0, q_here = 0.0;
-        float listed = 0.0f;
-        for (int j = threadIdx.x; j < n; j += kThreads) {
-            const int at = place[j];
-            if (at < 0) continue;
-            const float xj = Elem<E>::widen(elems[at]);
-            slot_x[j] = xj;
-            const float q = slot_q[j];
-            q_here += static_cast<double>(q);
-            if (q != 0.0f)
-                cross += static_cast<double>(q) *
-                         (static_cast<double>(a.teacher_log_probs[row * n + j]) -
-                          kLn2 * (static_cast<double>(xj) * static_cast<double>(c2) - ref2));
-            bool owner = true;
-            if (twice)
-                for (int o = 0; o < j; ++o) owner = owner && place[o] != at;
-            if (owner) listed += ex2(ref.exponent(xj, c2));
-        }
+        const RowState known = state.rows[row];
+        copies_wait<kRing - 1>();
+        if (at_end) sh.ends[lane] = Elem<E>::widen(in[row * a.in.stride + a0 + ragged]);
+        __syncthreads();   // the slice is there
+        auto mark = [&](int token) {
+            const int e = token - a0;
+            if (token < 0 || e < 0 || e >= len) return;
+            if (e >= head && e < tail_at)
+                elems[e] = Elem<E>::narrow(neg_inf());
+            else
+                sh.ends[e < head ? e : e - tail_at + head] = neg_inf();
+        };
+        mark(tid < n ? mine.token : -1);
+        for (int j = tid + kT; j < n; j += kT) mark(state.slots[row * n + j].token);
         __syncthreads();
-        for (int j = threadIdx.x; j < n; j += kThreads)
-            if (place[j] >= 0) elems[place[j]] = Elem<E>::narrow(neg_inf());
-        __syncthreads();
-        const float rest = block_reduce(sum_exp<E>(buf, nv, c2, ref), Add(), sh.f8);
-        listed = block_reduce(listed, Add(), sh.f8);
-        cross = block_reduce(cross, Add(), sh.d8);
-        q_here = block_reduce(q_here, Add(), sh.d8);
-        team.tell(sh.box[parity], DistillPacket{cross, q_here, rest, listed, mine});
-        cluster_sync(team.size);
-        const DistillPacket* box = sh.box[parity];
-        parity ^= 1;
-        float best = box[0].best;
-        for (int c = 1; c < team.size; ++c) best = fmaxf(best, box[c].best);
-        const Reference all(best, c2);
-        const double all2 = all.log2_of(c2);
-        double R = 0.0, L = 0.0, C = 0.0;
-        for (int c = 0; c < team.size; ++c) {
-            const Reference part(box[c].best, c2);
-            const double f = all.factor(part);
-            R += f * static_cast<double>(box[c].rest);
-            L += f * static_cast<double>(box[c].listed);
-            if (box[c].q != 0.0) C += box[c].cross + box[c].q * kLn2 * (all2 - part.log2_of(c2));
+        const uint4 none = vneg_inf<E>();
+        uint4 r[kHold], top = none;
+#pragma unroll
+        for (int i = 0; i < kHold; ++i) {
+            r[i] = none;
+            if (i * kT < left) r[i] = buf[v0 + tid + i * kT];
+            top = vmax<E>(top, r[i]);
         }
-        const double Z = R + L;
-        const double q_rest = a.tail && R > 0.0 ? fmax(0.0, 1.0 - Q) : 0.0;
-        if (a.row_losses && team.rank == 0 && threadIdx.x == 0) {
-            // log P = ln 2 (x c2 - all2) - log Z
-            double loss = C;
-            if (Q != 0.0) loss += Q * log(Z);
-            if (q_rest > 0.0) loss += q_rest * (log(q_rest) - log(R / Z));
-            if (Z == 0.0) loss = Q > 0.0 ? static_cast<double>(INFINITY) : 0.0;   // nothing above -inf
-            a.row_losses[row] = static_cast<float>(a.reduction == kNone ? loss * static_cast<double>(a.scale) : loss);
+        float best = lanes_max<E>(top);
+        float end_f = neg_inf();
+        if (at_end) {
+            end_f = sh.ends[lane];
+            best = fmaxf(best, end_f);
+        }
+        const float from = best > neg_inf() ? -best : 0.0f;
+        const float2 ff = make_float2(from, from);
+        float2 p = make_float2(0.0f, 0.0f);
+        float e[kGrad ? kHold * kVec : 1];
+#pragma unroll
+        for (int i = 0; i < kHold; ++i) {
+            float f[kVec];
+            Elem<E>::unpack(r[i], f);
+#pragma unroll
+            for (int k = 0; k < kVec; k += 2) {
+                float2 t = mul2(add2(make_float2(f[k], f[k + 1]), ff), cc);
+                t.x = ex2(t.x);
+                t.y = ex2(t.y);
+                p = add2(p, t);
+                if (kGrad) {
+                    e[i * kVec + k] = t.x;
+                    e[i * kVec + k + 1] = t.y;
+                }
+            }
+        }
+        float sum = p.x + p.y;
+        const float end_e = at_end ? ex2((end_f + from) * c2) : 0.0f;
+        sum += end_e;
+        start(later, go, buf_at);   // a thread has read what it copies over
+        // over the warp, the CTA and the cluster: maxima, and sums by them
+        auto join = [&](float m, float v, int lanes) {
+            float all = m;
+            for (int o = lanes / 2; o > 0; o >>= 1) all = fmaxf(all, __shfl_xor_sync(kAll, all, o));
+            v = v == 0.0f ? 0.0f : v * share(m, all, c2);
+            for (int o = lanes / 2; o > 0; o >>= 1) v += __shfl_xor_sync(kAll, v, o);
+            return make_float2(all, v);
+        };
+        const float2 of_warp = join(best, sum, 32);
+        if (lane == 0) sh.part[warp] = of_warp;
+        __syncthreads();
+        float2 rest = make_float2(neg_inf(), 0.0f);
+        if (team.size == 1 || warp == 0) {
+            const float2 part = sh.part[lane % kW];
+            rest = join(part.x, part.y, kW);
+        }
+        if (team.size > 1) {
+            if (warp == 0) {
+                if (lane < team.size) *cg::this_cluster().map_shared_rank(&sh.box[turn][team.rank], lane) = rest;
+                cluster_arrive();
+            } else {
+                cluster_arrive_relaxed();
+            }
+            cluster_wait();
+            float2 part = make_float2(neg_inf(), 0.0f);
+            if (lane < team.size) part = sh.box[turn][lane];
+            rest = join(part.x, part.y, kMaxCluster);
+            // lanes 16 to 31 joined nothing
+            rest.x = __shfl_sync(kAll, rest.x, 0);
+            rest.y = __shfl_sync(kAll, rest.y, 0);
+            turn ^= 1;
+        }
+        if (tid == 0 && team.rank == 0 && !a.skip_state) {
+            state.rows[row].best_rest = rest.x;
+            state.rows[row].rest = rest.y;
         }
         if (kGrad) {
-            double w = static_cast<double>(a.scale) / static_cast<double>(a.temperature) * static_cast<double>(g);
-            if (a.reduction == kMean) w /= static_cast<double>(max(1, *a.row_count));
-            const double inv = Z > 0.0 || Z != Z ? 1.0 / Z : 0.0;
-            const float on = static_cast<float>((Q + q_rest) * inv * w);
-            const float off = static_cast<float>(((Q + q_rest) * inv - (q_rest > 0.0 ? q_rest / R : 0.0)) * w);
-            const float wf = static_cast<float>(w);
-            auto element = [&](float f) { return ex2(all.exponent(f, c2)) * off; };
-            auto elements = [&](int begin, int end) {
-                for (int e = max(begin, -a0) + static_cast<int>(threadIdx.x); e < end; e += kThreads)
-                    out[a0 + e] = Elem<E>::narrow(element(Elem<E>::widen(elems[e])));
-            };
-            if (same_phase) {
-                uint4* dst = reinterpret_cast<uint4*>(reinterpret_cast<uintptr_t>(out) - phase * sizeof(E)) +
-                             team.rank * S / kVec;
-                if (all.wide) {
-                    for (int v = v0 + threadIdx.x; v < v1; v += kThreads) {
-                        float f[kVec];
-                        Elem<E>::unpack(buf[v], f);
+            const float all = fmaxf(rest.x, known.best_listed);
+            const float Z = (rest.y == 0.0f ? 0.0f : rest.y * share(rest.x, all, c2)) +
+                            (known.listed == 0.0f ? 0.0f : known.listed * share(known.best_listed, all, c2));
+            const float q_rest =
+                a.tail && rest.y > 0.0f ? static_cast<float>(fmax(0.0, 1.0 - known.Q)) : 0.0f;
+            const float w = unit * g;
+            const float G = (static_cast<float>(known.Q) + q_rest) * (Z == 0.0f ? 0.0f : __fdividef(1.0f, Z));
+            // P = share by the row's maximum / Z, P / P_r = share by the rest's / its sum
+            float scale = G * share(best, all, c2);
+            if (q_rest > 0.0f) scale -= __fdividef(q_rest, rest.y) * share(best, rest.x, c2);
+            scale = best > neg_inf() ? scale * w : 0.0f;
+            const float2 ss = make_float2(scale, scale);
 #pragma unroll
-                        for (int e = 0; e < kVec; ++e) f[e] = element(f[e]);
-                        dst[v] = Elem<E>::pack(f);
-                    }
-                } else {
-                    for (int v = v0 + threadIdx.x; v < v1; v += kThreads) {
-                        float f[kVec];
-                        Elem<E>::unpack(buf[v], f);
+            for (int i = 0; i < kHold; ++i) {
+                float f[kVec];
 #pragma unroll
-                        for (int e = 0; e < kVec; ++e) f[e] = ex2(fmaf(f[e], c2, -all.B)) * off;
-                        dst[v] = Elem<E>::pack(f);
+                for (int k = 0; k < kVec; k += 2) {
+                    const float2 y = mul2(make_float2(e[i * kVec + k], e[i * kVec + k + 1]), ss);
+                    f[k] = y.x;
+                    f[k + 1] = y.y;
+                }
+                if (i * kT < left) {
+                    if (same_phase) {
+                        __stcs(dst + i * kT, Elem<E>::pack(f));
+                    } else {
+#pragma unroll
+                        for (int k = 0; k < kVec; ++k)
+                            out[a0 + (v0 + tid + i * kT) * kVec + k] = Elem<E>::narrow(f[k]);
                     }
                 }
-                elements(0, min(len, v0 * kVec));
-                elements(max(v0, v1) * kVec, len);
-            } else {
-                elements(0, len);
             }
+            if (at_end) out[a0 + ragged] = Elem<E>::narrow(end_e * scale);
             __syncthreads();   // the listed places are written a second time
-            for (int j = threadIdx.x; j < n; j += kThreads) {
-                const int at = place[j];
-                if (at < 0) continue;
-                float q = slot_q[j];
-                bool owner = true;
-                if (twice) {
-                    q = 0.0f;
-                    for (int o = 0; o < n; ++o) {
-                        if (place[o] == at) {
-                            owner = owner && o >= j;
-                            q += slot_q[o];
-                        }
-                    }
-                }
-                if (owner) out[a0 + at] = Elem<E>::narrow(fmaf(ex2(all.exponent(slot_x[j], c2)), on, -q * wf));
-            }
+            auto listed = [&](const SlotState& s) {
+                const int at = s.token - a0;
+                if (s.token >= 0 && at >= 0 && at < len)
+                    out[s.token] = Elem<E>::narrow(fmaf(share(s.x, all, c2), G * w, -s.q * w));
+            };
+            if (tid < n) listed(mine);
+            for (int j = tid + kT; j < n; j += kT) listed(state.slots[row * n + j]);
         }
     }
+    copies_wait<0>();
     cluster_sync(team.size);
 }
 
-// Rows with at least one slot inside the vocabulary. One cluster of 8 CTAs; a
-// warp stops at a row's first such slot, which is nearly always in its first 32.
-__global__ void __cluster_dims__(8, 1, 1) __launch_bounds__(1024) count_kernel(DistillArgs a) {
-    __shared__ int counts[32];
-    __shared__ int parts[8];
+// The rows' losses from their sums, and their sum in 64 bits and one order.
+// One cluster of 8 CTAs.
+__global__ void __cluster_dims__(8, 1, 1) __launch_bounds__(1024) losses_kernel(DistillArgs a) {
+    __shared__ double d32[32];
+    __shared__ int i32[32];
+    __shared__ double sums[8];
+    __shared__ int counts[8];
     const Team team;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    int rows = 0;
-    for (int64_t row = team.rank * 32 + warp; row < a.in.rows; row += 256) {
-        bool any = false;
-        for (int j = 0; j < a.n && !any; j += 32) {
-            int64_t i = -1;
-            if (j + lane < a.n) i = teacher_token(a, row * a.n + j + lane);
-            any = __any_sync(kAll, i >= 0 && i < a.in.V) != 0;
+    const DistillState state = state_of(a);
+    const double c = static_cast<double>(fminf(1.4426950408889634f / a.temperature, FLT_MAX)) * 0.69314718055994530942;
+    double sum = 0.0;
+    int count = 0;
+    for (int64_t row = team.rank * 1024 + static_cast<int>(threadIdx.x); row < a.in.rows; row += 8 * 1024) {
+        double loss = 0.0;
+        if (state.any[row]) {
+            ++count;
+            const RowState s = state.rows[row];
+            const float all = fmaxf(s.best_listed, s.best_rest);
+            auto by = [&](float best, float v) {   // a sum by the row's maximum
+                return v == 0.0f ? 0.0 : static_cast<double>(v) *
+                           (best == all ? 1.0 : exp(c * (static_cast<double>(best) - static_cast<double>(all))));
+            };
+            const double Z = by(s.best_rest, s.rest) + by(s.best_listed, s.listed);
+            const double left = a.tail && s.rest > 0.0f ? fmax(0.0, 1.0 - s.Q) : 0.0;
+            // log P = c (x - all) - log Z
+            loss = s.C;
+            if (s.Q != 0.0) {
+                const double up = all == s.best_listed ? 0.0 : static_cast<double>(all) - static_cast<double>(s.best_listed);
+                loss += s.Q * (log(Z) + c * up);
+            }
+            if (left > 0.0) {
+                const double down = all == s.best_rest ? 0.0 : static_cast<double>(all) - static_cast<double>(s.best_rest);
+                loss += left * (log(left) - log(static_cast<double>(s.rest)) + c * down + log(Z));
+            }
+            if (Z == 0.0) loss = s.Q > 0.0 ? static_cast<double>(INFINITY) : 0.0;   // nothing above -inf
         }
-        rows += any ? 1 : 0;
+        sum += static_cast<double>(static_cast<float>(loss));
+        a.row_losses[row] = static_cast<float>(a.reduction == kNone ? loss * static_cast<double>(a.scale) : loss);
     }
-    if (lane == 0) counts[warp] = rows;
-    __syncthreads();
-    int mine = 0;
-    for (int w = 0; w < 32; ++w) mine += counts[w];
+    if (a.reduction == kNone) return;
+    sum = reduce_block(sum, Add(), d32);
+    count = reduce_block(count, Add(), i32);
     cluster_sync(8);   // everybody has started
-    if (threadIdx.x == 0) *cg::this_cluster().map_shared_rank(parts + team.rank, 0) = mine;
+    if (threadIdx.x == 0) {
+        *cg::this_cluster().map_shared_rank(sums + team.rank, 0) = sum;
+        *cg::this_cluster().map_shared_rank(counts + team.rank, 0) = count;
+    }
     cluster_sync(8);
     if (team.rank == 0 && threadIdx.x == 0) {
-        int all = 0;
-        for (int c = 0; c < 8; ++c) all += parts[c];
-        *a.row_count = all;
-    }
-}
-
-// The rows' losses added up in 64 bits and one order.
-__global__ void __launch_bounds__(1024) reduce_kernel(DistillArgs a) {
-    __shared__ double parts[32];
-    double v = 0.0;
-    for (int64_t r = threadIdx.x; r < a.in.rows; r += 1024) v += static_cast<double>(a.row_losses[r]);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(kAll, v, o);
-    if ((threadIdx.x & 31) == 0) parts[threadIdx.x >> 5] = v;
-    __syncthreads();
-    if (threadIdx.x == 0) {
         double all = 0.0;
-        for (int w = 0; w < 32; ++w) all += parts[w];
+        int rows = 0;
+        for (int i = 0; i < 8; ++i) {
+            all += sums[i];
+            rows += counts[i];
+        }
         all *= static_cast<double>(a.scale);
-        if (a.reduction == kMean) all /= static_cast<double>(max(1, *a.row_count));
+        if (a.reduction == kMean) all /= static_cast<double>(max(1, rows));
         *a.loss = static_cast<float>(all);
     }
 }
@@ -1418,26 +1660,27 @@ struct Shape {
 // arithmetic and one's stores overlap. Few rows are cut finer, down to 8 KB,
 // so that they reach more SMs; 16 CTAs (more than every GPU grants a cluster)
 // are taken only for rows that need them.
-Shape shape_of(const Rows& in, int es) {
+Shape shape_of(const Rows& in, int es, int most) {
     const int vec = 16 / es;
     auto slice = [&](int size) {
         const int64_t per = (static_cast<int64_t>(in.V) + vec - 1 + size - 1) / size;
         return static_cast<int>((per + 63) / 64 * 64);
     };
     int size = 1;
-    while (size < 16 && static_cast<int64_t>(slice(size)) * es > 68 * 1024) size *= 2;
+    while (size < 16 && static_cast<int64_t>(slice(size)) * es > most) size *= 2;
     while (size < 8 && in.rows * size * 2 <= 148 && static_cast<int64_t>(slice(size)) * es > 8 * 1024) size *= 2;
     return Shape{size, slice(size)};
 }
 
 template <class Kernel, class... Args>
-cudaError_t launch_rows(Kernel kernel, const Rows& in, int size, size_t smem, cudaStream_t stream, Args... args) {
+cudaError_t launch_rows(Kernel kernel, const Rows& in, int size, size_t smem, cudaStream_t stream, int threads,
+                        Args... args) {
     const void* fn = reinterpret_cast<const void*>(kernel);
     int dev = 0;
     cudaError_t err = cudaGetDevice(&dev);
     if (err != cudaSuccess) return err;
     cudaLaunchConfig_t cfg = {};
-    cfg.blockDim = dim3(kThreads);
+    cfg.blockDim = dim3(static_cast<unsigned>(threads));
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
     cudaLaunchAttribute attr;
@@ -1493,13 +1736,26 @@ int list_space(int n) {
     return cap;
 }
 
+#ifndef DT
+#define DT 512
+#endif
+// Slices of three rows, of at most 8 vectors per thread.
 template <class E>
 cudaError_t launch_distill_typed(const DistillArgs& a, cudaStream_t stream) {
-    const Shape sh = shape_of(a.in, sizeof(E));
-    const size_t smem = static_cast<size_t>(sh.S) * sizeof(E) + static_cast<size_t>((sh.S + 31) / 32) * 4 +
-                        static_cast<size_t>(a.n) * 12;
-    return a.grad ? launch_rows(distill_kernel<E, true>, a.in, sh.size, smem, stream, a, sh.S)
-                  : launch_rows(distill_kernel<E, false>, a.in, sh.size, smem, stream, a, sh.S);
+    const Shape sh = shape_of(a.in, sizeof(E), DT * 8 * 16);
+    const size_t smem = static_cast<size_t>(sh.S) * sizeof(E) * 3;
+    return a.grad ? launch_rows(distill_kernel<E, true, DT>, a.in, sh.size, smem, stream, DT, a, sh.S)
+                  : launch_rows(distill_kernel<E, false, DT>, a.in, sh.size, smem, stream, DT, a, sh.S);
+}
+
+template <class E>
+cudaError_t launch_slots(const DistillArgs& a, cudaStream_t stream) {
+    int places = 64;
+    while (places < 2 * a.n) places *= 2;
+    const int threads = std::min(256, (a.n + 31) / 32 * 32);
+    const int64_t ctas = std::min<int64_t>(a.in.rows, 148 * 2048 / threads);
+    slots_kernel<E><<<static_cast<unsigned>(ctas), threads, places * 8, stream>>>(a, places - 1);
+    return dbs_dev::count_launch(cudaGetLastError());
 }
 
 cudaError_t launch_distill_any(const DistillArgs& a, cudaStream_t stream) {
@@ -1514,43 +1770,49 @@ cudaError_t launch_distill_any(const DistillArgs& a, cudaStream_t stream) {
 
 cudaError_t launch_sample(const SampleArgs& a, cudaStream_t stream) {
     const int es = element_size(a.in.dtype);
-    const Shape sh = shape_of(a.in, es);
+    const Shape sh = shape_of(a.in, es, 68 * 1024);
     // lists for rows that may take that path, bins for the others
     const int cap = list_space(a.top_k ? kSampleList : (a.top_k_all <= kSampleList ? std::max(a.top_k_all, 0) : 0));
     const size_t smem = static_cast<size_t>(sh.S) * es + static_cast<size_t>(cap) * 16;
     switch (a.in.dtype) {
-        case kF32: return launch_rows(sample_kernel<float>, a.in, sh.size, smem, stream, a, sh.S, cap);
-        case kF16: return launch_rows(sample_kernel<__half>, a.in, sh.size, smem, stream, a, sh.S, cap);
-        default: return launch_rows(sample_kernel<__nv_bfloat16>, a.in, sh.size, smem, stream, a, sh.S, cap);
+        case kF32: return launch_rows(sample_kernel<float>, a.in, sh.size, smem, stream, kThreads, a, sh.S, cap);
+        case kF16: return launch_rows(sample_kernel<__half>, a.in, sh.size, smem, stream, kThreads, a, sh.S, cap);
+        default: return launch_rows(sample_kernel<__nv_bfloat16>, a.in, sh.size, smem, stream, kThreads, a, sh.S, cap);
     }
 }
 
 cudaError_t launch_top(const TopArgs& a, cudaStream_t stream) {
     const int es = element_size(a.in.dtype);
-    const Shape sh = shape_of(a.in, es);
+    const Shape sh = shape_of(a.in, es, 68 * 1024);
     const int cap = list_space(a.n);
     const size_t smem = static_cast<size_t>(sh.S) * es + static_cast<size_t>(cap) * 16;
     switch (a.in.dtype) {
-        case kF32: return launch_rows(top_kernel<float>, a.in, sh.size, smem, stream, a, sh.S, cap);
-        case kF16: return launch_rows(top_kernel<__half>, a.in, sh.size, smem, stream, a, sh.S, cap);
-        default: return launch_rows(top_kernel<__nv_bfloat16>, a.in, sh.size, smem, stream, a, sh.S, cap);
+        case kF32: return launch_rows(top_kernel<float>, a.in, sh.size, smem, stream, kThreads, a, sh.S, cap);
+        case kF16: return launch_rows(top_kernel<__half>, a.in, sh.size, smem, stream, kThreads, a, sh.S, cap);
+        default: return launch_rows(top_kernel<__nv_bfloat16>, a.in, sh.size, smem, stream, kThreads, a, sh.S, cap);
     }
 }
 
 cudaError_t launch_distill(const DistillArgs& a, cudaStream_t stream) {
-    if (a.reduction == kMean) {
-        count_kernel<<<8, 1024, 0, stream>>>(a);
-        const cudaError_t err = dbs_dev::count_launch(cudaGetLastError());
+    if (a.in.rows > 0) {
+        cudaError_t err = a.in.dtype == kF32   ? launch_slots<float>(a, stream)
+                          : a.in.dtype == kF16 ? launch_slots<__half>(a, stream)
+                                               : launch_slots<__nv_bfloat16>(a, stream);
+        if (err == cudaSuccess) err = launch_distill_any(a, stream);
         if (err != cudaSuccess) return err;
+    } else if (a.reduction == kNone) {
+        return cudaSuccess;
     }
-    cudaError_t err = a.in.rows > 0 ? launch_distill_any(a, stream) : cudaSuccess;
-    if (err != cudaSuccess || a.reduction == kNone) return err;
-    reduce_kernel<<<1, 1024, 0, stream>>>(a);
+    losses_kernel<<<8, 1024, 0, stream>>>(a);
     return dbs_dev::count_launch(cudaGetLastError());
 }
 
 cudaError_t launch_distill_backward(const DistillArgs& a, cudaStream_t stream) {
     return launch_distill_any(a, stream);
+}
+
+int64_t distill_state_bytes(int64_t rows, int n) {
+    return rows * (n * static_cast<int64_t>(sizeof(SlotState)) + static_cast<int64_t>(sizeof(RowState)) + 4);
 }
 
 }  // namespace dbs_logits

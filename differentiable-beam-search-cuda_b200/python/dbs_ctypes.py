@@ -213,6 +213,7 @@ DEVICE_FUNCTIONS = {
     "dbs_device_top_log_probs": (_I, [_VP, _I, _I64, _I, _I64, _I, _F, _VP, _VP, _VP]),
     "dbs_device_distill": (
         _I, [_VP, _I, _I64, _I, _I64, _VP, _VP, _I, _I, _F, _I, _I, _F, _VP, _VP, _VP, _VP, _VP]),
+    "dbs_device_distill_state_bytes": (_I, [_I64, _I, ctypes.POINTER(_I64)]),
     "dbs_device_distill_backward": (
         _I, [_VP, _I, _I64, _I, _I64, _VP, _VP, _I, _I, _F, _I, _I, _F, _VP, _VP, _I64, _I, _VP, _VP]),
 }

@@ -486,6 +486,7 @@ def decode(log_probs: torch.Tensor, options: DBSOptions) -> Tuple[torch.Tensor, 
 _DTYPES = {torch.float32: dbs_ctypes.DBS_DTYPE_F32, torch.float16: dbs_ctypes.DBS_DTYPE_F16,
            torch.bfloat16: dbs_ctypes.DBS_DTYPE_BF16}
 _MAX_ROW_BYTES = 3_000_000
+_MAX_DISTILL_BYTES = 1_040_000
 _MAX_LIST = 1024
 
 
@@ -494,14 +495,14 @@ def _check_global(rc: int, what: str) -> None:
         raise RuntimeError(f"{what} failed: {_library().dbs_last_global_error().decode()}")
 
 
-def _validate_logits(logits: torch.Tensor) -> None:
+def _validate_logits(logits: torch.Tensor, most: int = _MAX_ROW_BYTES) -> None:
     if logits.dtype not in _DTYPES:
         raise ValueError("logits must be float32, float16 or bfloat16")
     if logits.dim() < 1:
         raise ValueError("logits must have shape [..., V]")
     _validate_positive_int_dim(logits.size(-1), "V")
-    if logits.size(-1) * logits.element_size() > _MAX_ROW_BYTES:
-        raise ValueError(f"a row of logits takes at most {_MAX_ROW_BYTES} bytes")
+    if logits.size(-1) * logits.element_size() > most:
+        raise ValueError(f"a row of logits takes at most {most} bytes")
 
 
 def _logits_rows(logits: torch.Tensor) -> torch.Tensor:
@@ -639,20 +640,22 @@ def _distill_args(x, log_probs, tokens, settings):
 
 
 def _distill_forward(logits, log_probs, tokens, settings, need_grad):
-    """(loss, gradient for an incoming gradient of 1 or None, rows with a teacher or None)."""
+    """(loss, gradient for an incoming gradient of 1 or None, the rows' state for a backward)."""
     x = _logits_rows(logits)
     lead, device = logits.shape[:-1], logits.device
     reduction = settings[2]
     row_losses = torch.empty(lead, dtype=torch.float32, device=device)
     loss = row_losses if reduction == 0 else torch.empty((), dtype=torch.float32, device=device)
-    rows = torch.empty((1,), dtype=torch.int32, device=device) if reduction == 2 else None
+    size = ctypes.c_int64()
+    _check_global(_library().dbs_device_distill_state_bytes(x.size(0), tokens.size(-1), size), "distillation_loss")
+    state = torch.empty((size.value,), dtype=torch.uint8, device=device)
     grad = torch.empty(logits.shape, dtype=logits.dtype, device=device) if need_grad else None
     with torch.cuda.device(device):
         rc = _library().dbs_device_distill(*_distill_args(x, log_probs, tokens, settings), _vp(row_losses),
-                                           None if reduction == 0 else _vp(loss), _vp(rows), _vp(grad),
+                                           None if reduction == 0 else _vp(loss), _vp(state), _vp(grad),
                                            _stream_ptr(device))
     _check_global(rc, "distillation_loss")
-    return loss, grad, rows
+    return loss, grad, state
 
 
 class _DBSDistillation(torch.autograd.Function):
@@ -661,15 +664,15 @@ class _DBSDistillation(torch.autograd.Function):
         # The gradient for an incoming gradient of 1 is written in the same
         # pass; the backward keeps it, or computes it again from the logits
         # (one rounding) where the incoming gradient is another.
-        loss, ctx.grad, rows = _distill_forward(logits, log_probs, tokens, settings, True)
+        loss, ctx.grad, state = _distill_forward(logits, log_probs, tokens, settings, True)
         ctx.settings = settings
-        ctx.save_for_backward(logits, log_probs, tokens, rows)
+        ctx.save_for_backward(logits, log_probs, tokens, state)
         return loss
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad_output: torch.Tensor):
-        logits, log_probs, tokens, rows = ctx.saved_tensors
+        logits, log_probs, tokens, state = ctx.saved_tensors
         # the forward's buffer serves the first backward; a repeated one
         # (retain_graph) gets a buffer of its own
         grad, ctx.grad = ctx.grad, None
@@ -684,7 +687,7 @@ class _DBSDistillation(torch.autograd.Function):
             g = g.contiguous()
         x = _logits_rows(logits)
         with torch.cuda.device(logits.device):
-            rc = _library().dbs_device_distill_backward(*_distill_args(x, log_probs, tokens, ctx.settings), _vp(rows),
+            rc = _library().dbs_device_distill_backward(*_distill_args(x, log_probs, tokens, ctx.settings), _vp(state),
                                                         _vp(g), stride, flags, _vp(grad), _stream_ptr(logits.device))
         _check_global(rc, "distillation_loss backward")
         return grad, None, None, None
@@ -709,7 +712,7 @@ def distillation_loss(logits: torch.Tensor, teacher_log_probs: torch.Tensor, tea
     the logits a second time. The loss is float32; gradients flow to the logits
     alone.
     """
-    _validate_logits(logits)
+    _validate_logits(logits, _MAX_DISTILL_BYTES)
     lead = logits.shape[:-1]
     if teacher_tokens.dtype not in (torch.int32, torch.int64):
         raise ValueError("teacher_tokens must be int32 or int64")

@@ -197,29 +197,32 @@ DBS_EXPORT int dbs_device_top_log_probs(const void* logits, int data_type, int64
  *   sum_j q_j (log q_j - log P_j) + q_r (log q_r - log P_r),   0 log 0 = 0,
  * and 0 for a row without slots, whatever its logits hold. `reduction`:
  * DBS_REDUCE_NONE (row_losses [rows] alone; loss NULL), _SUM, or _MEAN over
- * the rows with slots (row_count [1] is written); `scale` multiplies the
- * result. row_losses [rows] is needed for every reduction. grad_logits
- * ([rows, vocab_size] contiguous, the logits' type, or NULL) takes the
- * gradient for an incoming gradient of 1, in the same pass over the logits. */
+ * the rows with slots; `scale` multiplies the result. row_losses [rows] is
+ * needed for every reduction. grad_logits ([rows, vocab_size] contiguous, the
+ * logits' type, or NULL) takes the gradient for an incoming gradient of 1, in
+ * the same pass over the logits. `state` is dbs_device_distill_state_bytes
+ * bytes of device memory, 16-byte aligned, that the call fills and a backward
+ * of it reads. A row holds at most 1040000 bytes here. */
 #define DBS_REDUCE_NONE 0
 #define DBS_REDUCE_SUM 1
 #define DBS_REDUCE_MEAN 2
 DBS_EXPORT int dbs_device_distill(const void* logits, int data_type, int64_t rows, int vocab_size, int64_t row_stride,
                                   const float* teacher_log_probs, const void* teacher_tokens, int token_bytes,
                                   int slots, float temperature, int tail, int reduction, float scale,
-                                  float* row_losses, float* loss, int32_t* row_count, void* grad_logits,
+                                  float* row_losses, float* loss, void* state, void* grad_logits,
                                   void* cuda_stream);
+DBS_EXPORT int dbs_device_distill_state_bytes(int64_t rows, int slots, int64_t* bytes);
 
 /* The gradient of dbs_device_distill for the incoming gradient grad_loss
  * (device; row r's at r * grad_loss_stride, so 0 for one value). The other
- * arguments are the forward call's, row_count as it wrote it. With
+ * arguments are the forward call's, `state` as it wrote it. With
  * DBS_DEVICE_GRAD_UNIT in `flags`, grad_logits is what the forward call wrote,
  * and rows whose incoming gradient is 1 stay as they are. */
 #define DBS_DEVICE_GRAD_UNIT 2
 DBS_EXPORT int dbs_device_distill_backward(const void* logits, int data_type, int64_t rows, int vocab_size,
                                            int64_t row_stride, const float* teacher_log_probs,
                                            const void* teacher_tokens, int token_bytes, int slots, float temperature,
-                                           int tail, int reduction, float scale, const int32_t* row_count,
+                                           int tail, int reduction, float scale, const void* state,
                                            const float* grad_loss, int64_t grad_loss_stride, int flags,
                                            void* grad_logits, void* cuda_stream);
 

@@ -78,6 +78,7 @@ def test_top_log_probs_longest_list():
     (dict(temperature=0.0), "temperature must be positive"),
     (dict(scale=float("nan")), "scale must be finite"),
     (dict(logits=X.double()), "float32, float16 or bfloat16"),
+    (dict(logits=torch.empty(3, 260_001)), "takes at most 1040000 bytes"),
     (dict(teacher_log_probs=LQ.clone().requires_grad_(True)), "takes no gradient"),
 ])
 def test_distillation_arguments(change, message):
@@ -99,8 +100,8 @@ def test_no_cuda_device_fails_loudly():
 
 # Host memory stands in for the device's: every call here is refused before a kernel is launched.
 BUF = (ctypes.c_float * 64)()
-P = ctypes.cast(BUF, ctypes.c_void_p)
-ODD = ctypes.c_void_p(ctypes.addressof(BUF) + 1)
+P = ctypes.c_void_p((ctypes.addressof(BUF) + 15) // 16 * 16)
+ODD = ctypes.c_void_p(P.value + 1)
 
 
 def refused(lib, rc, message):
@@ -145,11 +146,18 @@ def test_c_arguments(libdbs):
     refused(libdbs, distill(*rows, P, P, 4, 2, 1.0, 1, 1, float("inf"), P, P, P, None, None), "scale")
     refused(libdbs, distill(*rows, P, P, 4, 2, 1.0, 1, 1, 1.0, None, P, P, None, None), "row_losses")
     refused(libdbs, distill(*rows, P, P, 4, 2, 1.0, 1, 1, 1.0, P, None, P, None, None), "needs a place")
-    refused(libdbs, distill(*rows, P, P, 4, 2, 1.0, 1, 2, 1.0, P, P, None, None, None), "row_count")
+    refused(libdbs, distill(*rows, P, P, 4, 2, 1.0, 1, 2, 1.0, P, P, None, None, None), "state cannot be null")
+    refused(libdbs, distill(*rows, P, P, 4, 2, 1.0, 1, 2, 1.0, P, P, ODD, None, None), "state is not aligned")
+    refused(libdbs, distill(P, 0, 1, 260_001, 260_001, P, P, 4, 2, 1.0, 1, 2, 1.0, P, P, P, None, None), "at most 1040000 bytes")
+    size = ctypes.c_int64()
+    assert libdbs.dbs_device_distill_state_bytes(3, 5, ctypes.byref(size)) == 0 and size.value >= 3 * 5 * 8
+    assert libdbs.dbs_device_distill_state_bytes(3, 0, ctypes.byref(size)) == -1
+    assert libdbs.dbs_device_distill_state_bytes(-1, 5, ctypes.byref(size)) == -1
+    assert libdbs.dbs_device_distill_state_bytes(1, 5, None) == -1
     refused(libdbs, distill(*rows, P, P, 4, 2, 1.0, 1, 1, 1.0, P, P, P, ODD, None), "aligned")
     backward = libdbs.dbs_device_distill_backward
     refused(libdbs, backward(*rows, P, P, 4, 2, 1.0, 1, 1, 1.0, P, None, 0, 0, P, None), "grad_loss")
     refused(libdbs, backward(*rows, P, P, 4, 2, 1.0, 1, 1, 1.0, P, P, -1, 0, P, None), "stride")
     refused(libdbs, backward(*rows, P, P, 4, 2, 1.0, 1, 1, 1.0, P, P, 0, 1, P, None), "flags")
-    refused(libdbs, backward(*rows, P, P, 4, 2, 1.0, 1, 2, 1.0, None, P, 0, 0, P, None), "row_count")
+    refused(libdbs, backward(*rows, P, P, 4, 2, 1.0, 1, 2, 1.0, None, P, 0, 0, P, None), "state")
     assert dc.DBS_REDUCTIONS == {"none": 0, "sum": 1, "mean": 2}

@@ -492,10 +492,13 @@ def test_rows_behind_the_last_stay_as_they_are():
     grad = torch.full((8, 333), 7.0, device="cuda")
     losses, loss = torch.full((8,), 7.0, device="cuda"), torch.empty((), device="cuda")
     at, lq = torch.zeros(5, 2, dtype=torch.int32, device="cuda"), torch.full((5, 2), -1.0, device="cuda")
+    size = ctypes.c_int64()
+    assert lib.dbs_device_distill_state_bytes(5, 2, size) == 0
+    state = torch.full((size.value + 64,), 7, dtype=torch.uint8, device="cuda")
     s = ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
     p = ext._vp
     assert lib.dbs_device_top_log_probs(p(x), 0, 5, 333, 333, 4, 1.0, p(values), p(tokens), s) == 0
-    assert lib.dbs_device_distill(p(x), 0, 5, 333, 333, p(lq), p(at), 4, 2, 1.0, 1, 1, 1.0, p(losses), p(loss), None, p(grad), s) == 0
+    assert lib.dbs_device_distill(p(x), 0, 5, 333, 333, p(lq), p(at), 4, 2, 1.0, 1, 1, 1.0, p(losses), p(loss), p(state), p(grad), s) == 0
     torch.cuda.synchronize()
     assert torch.all(values[5:] == 7.0) and torch.all(tokens[5:] == 7) and torch.all(grad[5:] == 7.0) and torch.all(losses[5:] == 7.0)
-    assert torch.all(tokens[:5] >= 0)
+    assert torch.all(tokens[:5] >= 0) and torch.all(state[size.value:] == 7)
