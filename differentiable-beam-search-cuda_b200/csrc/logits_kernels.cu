@@ -1314,38 +1314,38 @@ __device__ __forceinline__ void cluster_arrive_relaxed() { asm volatile("barrier
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
 
-template <int kW>
+constexpr int kHold = 16;   // vectors of a slice per thread
 struct DistillShared {
-    float2 box[2][kMaxCluster];   // maximum and sum of the CTAs' slices
-    float2 part[kW];              // and of the warps' vectors
+    float2 box[2][kMaxCluster];   // reference and sum of the CTAs' slices
+    float2 part[kWarps];          // and of the warps' vectors
     float ends[32];               // the slice's elements that no whole vector holds
+    uint32_t end_marks[2];        // which of these are listed
     int i32[32];
+    uint4 marks[2][kThreads];     // a bit for each of a thread's elements: those that are listed
 };
 
 // One pass over the row gives its sum and (kGrad) its gradient: the logits are
-// read once and the gradient written once. The slices of three rows are in
-// shared memory or on their way into it, so the memory works on while the
-// cluster exchanges its sums. A thread copies the same eight vectors that it
-// adds up by their own maximum; the exponentials stay in its registers, so the
-// gradient costs a multiplication each, and the buffer is free for another
-// row as soon as it was read.
+// read once and the gradient written once. A thread copies, adds up and turns
+// into gradients the same vectors of its CTA's slice in shared memory, and
+// starts the copy of the next row's vector as soon as it has used one, so
+// there are two barriers a row: for the row's sum, and before the listed
+// places are written a second time.
 // What the teacher lists is not part of the sum, which must not be a
-// difference of two sums (a tail of 1e-6 would be lost in it): the listed
-// places become -inf in shared memory, and their gradients are written last.
-template <class E, bool kGrad, int kT>
-__global__ void __launch_bounds__(kT, 512 / kT) distill_kernel(DistillArgs a, int S) {
+// difference of two sums (a tail of 1e-6 would be lost in it): a row ahead,
+// the slots' threads name the listed elements to the threads that hold them,
+// which make them -inf.
+template <class E, bool kGrad>
+__global__ void __launch_bounds__(kThreads, 3) distill_kernel(DistillArgs a, int S) {
     constexpr int kVec = Elem<E>::kVec;
-    constexpr int kRing = 3;
-    constexpr int kHold = 8;
-    constexpr int kW = kT / 32;
+    constexpr int kT = kThreads;
+    constexpr int kChunk = 4;
     extern __shared__ uint4 dyn[];
-    __shared__ DistillShared<kW> sh;
+    __shared__ DistillShared sh;
     // the backward of a loss that was not multiplied by anything: all is done
     if (a.skip_unit && a.grad_loss_stride == 0 && *a.grad_loss == 1.0f) return;
     const Team team;
     const DistillState state = state_of(a);
     const int n = a.n, V = a.in.V, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int slice_vecs = S / kVec;
     const int64_t step = gridDim.x / team.size;
     const float c2 = fminf(1.4426950408889634f / a.temperature, FLT_MAX);
     const float2 cc = make_float2(c2, c2);
@@ -1355,151 +1355,161 @@ __global__ void __launch_bounds__(kT, 512 / kT) distill_kernel(DistillArgs a, in
         for (int64_t r = tid; r < a.in.rows; r += kT) rows += state.any[r];
         unit /= static_cast<float>(max(1, reduce_block(rows, Add(), sh.i32)));
     }
+    sh.marks[0][tid] = sh.marks[1][tid] = make_uint4(0, 0, 0, 0);
+    if (tid < 2) sh.end_marks[tid] = 0;
     cluster_sync(team.size);
 
-    const int64_t first_row = blockIdx.x / team.size;
-    const E* in = static_cast<const E*>(a.in.x);
+    uint4* buf = dyn + tid;   // this thread's vectors, kT apart
     // Where a row's slice lies: positions count from the 16-byte boundary at
-    // or before the row's first element; [v0, v1) are whole vectors.
+    // or before the row's first element; [v0, v1) are whole vectors, counted
+    // from the slice's start, and elements outside them (`head` at its start,
+    // then those from tail_at on) are the last warp's.
     struct View {
         const uint4* src;
-        int phase, v0, v1, len;
+        int a0, v0, v1, len;
     };
-    auto view = [&](int64_t r) {
-        const uintptr_t x = reinterpret_cast<uintptr_t>(in + r * a.in.stride);
+    auto view = [&](const E* x) {
+        const uintptr_t at = reinterpret_cast<uintptr_t>(x);
+        const int phase = static_cast<int>((at & 15u) / sizeof(E));
         View w;
-        w.phase = static_cast<int>((x & 15u) / sizeof(E));
-        w.len = max(0, min(S, V + w.phase - team.rank * S));
-        w.v0 = team.rank == 0 && w.phase > 0 ? 1 : 0;
+        w.a0 = team.rank * S - phase;   // token of the slice's element 0
+        w.len = max(0, min(S, V - w.a0));
+        w.v0 = team.rank == 0 && phase > 0 ? 1 : 0;
         w.v1 = w.len / kVec;
-        w.src = reinterpret_cast<const uint4*>(x & ~static_cast<uintptr_t>(15)) + team.rank * slice_vecs;
+        w.src = reinterpret_cast<const uint4*>(at & ~static_cast<uintptr_t>(15)) + team.rank * (S / kVec);
         return w;
     };
-    auto start = [&](int64_t r, bool go, int buffer) {
-        if (go) {
-            const View w = view(r);
-            const int left = w.v1 - w.v0 - tid;
-            uint4* to = dyn + buffer * slice_vecs + w.v0 + tid;
-            const uint4* from = w.src + w.v0 + tid;
-#pragma unroll
-            for (int i = 0; i < kHold; ++i)
-                if (i * kT < left) copy_async(to + i * kT, from + i * kT);
+    const E* in = static_cast<const E*>(a.in.x);
+    auto name = [&](const SlotState& s, const View& w, int par) {
+        const int e = s.token - w.a0;
+        if (s.token < 0 || e < 0 || e >= w.len) return;
+        const int head = min(w.len, w.v0 * kVec), tail_at = max(head, w.v1 * kVec);
+        if (e < head || e >= tail_at) {
+            atomicOr(&sh.end_marks[par], 1u << (e < head ? e : e - tail_at + head));
+        } else {
+            const int v = e / kVec - w.v0, bit = v / kT * kVec + e % kVec;
+            atomicOr(reinterpret_cast<uint32_t*>(&sh.marks[par][v % kT]) + (bit >> 5), 1u << (bit & 31));
         }
-        copies_commit();
     };
-    auto wanted = [&](int64_t r) { return r < a.in.rows && state.any[r] != 0; };
-    bool have[kRing];   // the rows of this turn and the next two
-#pragma unroll
-    for (int b = 0; b < kRing; ++b) {
-        have[b] = wanted(first_row + b * step);
-        start(first_row + b * step, have[b], b);
+    SlotState slot = {-1, 0.0f, 0.0f, 0};   // this thread's first slot of the next row
+    auto name_all = [&](int64_t r, const View& w, int par) {
+        if (tid < n) name(slot, w, par);
+        for (int j = tid + kT; j < n; j += kT) name(state.slots[r * n + j], w, par);
+    };
+
+    const int64_t first_row = blockIdx.x / team.size;
+    bool any_next = first_row < a.in.rows && state.any[first_row] != 0;
+    bool any_after = first_row + step < a.in.rows && state.any[first_row + step] != 0;
+    View next = view(in + first_row * a.in.stride);
+    if (any_next) {
+        if (tid < n) slot = state.slots[first_row * n + tid];
+        for (int i = 0, v = next.v0 + tid; v < next.v1; v += kT, ++i) copy_async(buf + i * kT, next.src + v);
+        name_all(first_row, next, 0);
     }
-    bool ahead = wanted(first_row + kRing * step);
-    SlotState slot = {-1, 0.0f, 0.0f, 0};   // this thread's first slot of the row to come
-    if (have[0] && tid < n) slot = state.slots[first_row * n + tid];
-    int buffer = 0, turn = 0;
+    copies_commit();
+    __syncthreads();
+    int parity = 0, turn = 0;
     for (int64_t row = first_row; row < a.in.rows; row += step) {
-        const bool any = have[0], go = ahead;
-        have[0] = have[1];
-        have[1] = have[2];
-        have[2] = ahead;
-        const int64_t later = row + kRing * step;
-        ahead = wanted(later + step);
-        const int buf_at = buffer;
-        buffer = buffer + 1 == kRing ? 0 : buffer + 1;
-        uint4* buf = dyn + buf_at * slice_vecs;
-        E* elems = reinterpret_cast<E*>(buf);
-        const View here = view(row);
-        const int v0 = here.v0, v1 = here.v1, len = here.len;
-        const int a0 = team.rank * S - here.phase;   // token of the slice's element 0
+        const int par = parity;
+        parity ^= 1;
+        const bool any = any_next;
+        any_next = any_after;
+        any_after = row + 2 * step < a.in.rows && state.any[row + 2 * step] != 0;
+        const View here = next;
         const SlotState mine = slot;
-        if (have[0] && tid < n) slot = state.slots[(row + step) * n + tid];
+        next = view(in + (row + step) * a.in.stride);
+        if (any_next && tid < n) slot = state.slots[(row + step) * n + tid];
         float g = 1.0f;
         if (kGrad && a.grad_loss) g = a.grad_loss[row * a.grad_loss_stride];
         E* out = static_cast<E*>(a.grad) + (kGrad ? row * V : 0);
-        const bool same_phase =
-            kGrad && static_cast<int>((reinterpret_cast<uintptr_t>(out) & 15u) / sizeof(E)) == here.phase;
-        uint4* dst = reinterpret_cast<uint4*>(reinterpret_cast<uintptr_t>(out) & ~static_cast<uintptr_t>(15)) +
-                     team.rank * slice_vecs + v0 + tid;
-        const int left = v1 - v0 - tid;   // of this thread's vectors, those with i * kT < left exist
-        // elements of the slice that no whole vector holds, [0, head) and
-        // [tail_at, len), are the last warp's
-        const int head = min(len, v0 * kVec), tail_at = max(head, v1 * kVec);
+        uint4* dst = reinterpret_cast<uint4*>(out + here.a0);
+        const bool same_phase = kGrad && (reinterpret_cast<uintptr_t>(dst) & 15u) == 0;
+        dst += here.v0 + tid;
+        const int count = (here.v1 - here.v0 - tid + kT - 1) / kT;   // of this thread's vectors
+        const int next_count = any_next ? (next.v1 - next.v0 - tid + kT - 1) / kT : 0;
+        const uint4* src = next.src + next.v0 + tid;
+        const int head = min(here.len, here.v0 * kVec), tail_at = max(head, here.v1 * kVec);
         const int ragged = lane < head ? lane : tail_at + lane - head;
-        const bool at_end = warp == kW - 1 && ragged < len && a0 + ragged >= 0;
+        const bool at_end = warp == kWarps - 1 && ragged < here.len && here.a0 + ragged >= 0;
         if (!any || (a.skip_unit && g == 1.0f)) {   // the same for the whole cluster
-            copies_wait<kRing - 1>();   // this buffer's copies, should there be any, before others go into it
-            start(later, go, buf_at);
-            if (kGrad && !any) {
+            if (any) {
+                sh.marks[par][tid] = make_uint4(0, 0, 0, 0);
+                if (tid == 0) sh.end_marks[par] = 0;
+                copies_wait<0>();
+            } else if (kGrad) {
                 // a row without a teacher: gradient 0 whatever its logits hold
-#pragma unroll
-                for (int i = 0; i < kHold; ++i) {
-                    if (i * kT >= left) continue;
-                    if (same_phase)
-                        __stcs(dst + i * kT, make_uint4(0, 0, 0, 0));
-                    else
-#pragma unroll
-                        for (int k = 0; k < kVec; ++k)
-                            out[a0 + (v0 + tid + i * kT) * kVec + k] = Elem<E>::narrow(0.0f);
-                }
-                if (at_end) out[a0 + ragged] = Elem<E>::narrow(0.0f);
+                if (same_phase)
+                    for (int i = 0; i < count; ++i) __stcs(dst + i * kT, make_uint4(0, 0, 0, 0));
+                else
+                    for (int e = here.v0 * kVec + tid; e < here.v1 * kVec; e += kT)
+                        out[here.a0 + e] = Elem<E>::narrow(0.0f);
+                if (at_end) out[here.a0 + ragged] = Elem<E>::narrow(0.0f);
             }
+            for (int i = 0; i < next_count; ++i) copy_async(buf + i * kT, src + i * kT);
+            copies_commit();
+            if (any_next) {
+                __syncthreads();   // the marks of two rows ago are gone
+                name_all(row + step, next, parity);
+            }
+            __syncthreads();
             continue;
         }
         const RowState known = state.rows[row];
-        copies_wait<kRing - 1>();
-        if (at_end) sh.ends[lane] = Elem<E>::widen(in[row * a.in.stride + a0 + ragged]);
-        __syncthreads();   // the slice is there
-        auto mark = [&](int token) {
-            const int e = token - a0;
-            if (token < 0 || e < 0 || e >= len) return;
-            if (e >= head && e < tail_at)
-                elems[e] = Elem<E>::narrow(neg_inf());
-            else
-                sh.ends[e < head ? e : e - tail_at + head] = neg_inf();
-        };
-        mark(tid < n ? mine.token : -1);
-        for (int j = tid + kT; j < n; j += kT) mark(state.slots[row * n + j].token);
-        __syncthreads();
-        const uint4 none = vneg_inf<E>();
-        uint4 r[kHold], top = none;
+        copies_wait<0>();
+        const uint4 marks = sh.marks[par][tid];
+        if (marks.x | marks.y | marks.z | marks.w) {
+            sh.marks[par][tid] = make_uint4(0, 0, 0, 0);
+            const uint32_t word[4] = {marks.x, marks.y, marks.z, marks.w};
 #pragma unroll
-        for (int i = 0; i < kHold; ++i) {
-            r[i] = none;
-            if (i * kT < left) r[i] = buf[v0 + tid + i * kT];
-            top = vmax<E>(top, r[i]);
-        }
-        float best = lanes_max<E>(top);
-        float end_f = neg_inf();
-        if (at_end) {
-            end_f = sh.ends[lane];
-            best = fmaxf(best, end_f);
-        }
-        const float from = best > neg_inf() ? -best : 0.0f;
-        const float2 ff = make_float2(from, from);
-        float2 p = make_float2(0.0f, 0.0f);
-        float e[kGrad ? kHold * kVec : 1];
-#pragma unroll
-        for (int i = 0; i < kHold; ++i) {
-            float f[kVec];
-            Elem<E>::unpack(r[i], f);
-#pragma unroll
-            for (int k = 0; k < kVec; k += 2) {
-                float2 t = mul2(add2(make_float2(f[k], f[k + 1]), ff), cc);
-                t.x = ex2(t.x);
-                t.y = ex2(t.y);
-                p = add2(p, t);
-                if (kGrad) {
-                    e[i * kVec + k] = t.x;
-                    e[i * kVec + k + 1] = t.y;
+            for (int k = 0; k < 4; ++k) {
+                for (uint32_t left = word[k]; left; left &= left - 1) {
+                    const int bit = 32 * k + __ffs(left) - 1;
+                    reinterpret_cast<E*>(buf + bit / kVec * kT)[bit % kVec] = Elem<E>::narrow(neg_inf());
                 }
             }
         }
-        float sum = p.x + p.y;
-        const float end_e = at_end ? ex2((end_f + from) * c2) : 0.0f;
-        sum += end_e;
-        start(later, go, buf_at);   // a thread has read what it copies over
-        // over the warp, the CTA and the cluster: maxima, and sums by them
+        float end_x = neg_inf();
+        if (at_end && !(sh.end_marks[par] >> lane & 1u)) end_x = Elem<E>::widen(in[row * a.in.stride + here.a0 + ragged]);
+        // The sum goes by the maximum of the thread's first vectors; where the
+        // others run so far beyond it that the sum overflows, by all of them.
+        const uint4 none = vneg_inf<E>();
+        auto best_of = [&](int until) {
+            uint4 top = none;
+            for (int i = 0; i < until; ++i) top = vmax<E>(top, buf[i * kT]);
+            return lanes_max<E>(top);
+        };
+        float best = neg_inf(), sum = 0.0f;
+        auto add = [&](const uint4& r, float2 from, float2& p) {
+            float f[kVec];
+            Elem<E>::unpack(r, f);
+#pragma unroll
+            for (int k = 0; k < kVec; k += 2) {
+                const float2 t = mul2(add2(make_float2(f[k], f[k + 1]), from), cc);
+                p = add2(p, make_float2(ex2(t.x), ex2(t.y)));
+            }
+        };
+        auto add_up = [&]() {
+            const float from = best > neg_inf() ? -best : 0.0f;
+            const float2 ff = make_float2(from, from);
+            float2 p = make_float2(0.0f, 0.0f);
+            int i = 0;
+            for (; i + kChunk <= count; i += kChunk) {
+                uint4 r[kChunk];
+#pragma unroll
+                for (int k = 0; k < kChunk; ++k) r[k] = buf[(i + k) * kT];
+#pragma unroll
+                for (int k = 0; k < kChunk; ++k) add(r[k], ff, p);
+            }
+            for (; i < count; ++i) add(buf[i * kT], ff, p);
+            sum = p.x + p.y + (at_end ? ex2((end_x + from) * c2) : 0.0f);
+        };
+        best = fmaxf(best_of(min(count, kChunk)), end_x);
+        add_up();
+        if (!(best > neg_inf()) || !(sum < 1.0e30f)) {
+            best = fmaxf(best_of(count), end_x);
+            add_up();
+        }
+        // over the warp, the CTA and the cluster: references, and sums by them
         auto join = [&](float m, float v, int lanes) {
             float all = m;
             for (int o = lanes / 2; o > 0; o >>= 1) all = fmaxf(all, __shfl_xor_sync(kAll, all, o));
@@ -1510,10 +1520,11 @@ __global__ void __launch_bounds__(kT, 512 / kT) distill_kernel(DistillArgs a, in
         const float2 of_warp = join(best, sum, 32);
         if (lane == 0) sh.part[warp] = of_warp;
         __syncthreads();
+        if (tid == 0) sh.end_marks[par] = 0;
         float2 rest = make_float2(neg_inf(), 0.0f);
         if (team.size == 1 || warp == 0) {
-            const float2 part = sh.part[lane % kW];
-            rest = join(part.x, part.y, kW);
+            const float2 part = sh.part[lane % kWarps];
+            rest = join(part.x, part.y, kWarps);
         }
         if (team.size > 1) {
             if (warp == 0) {
@@ -1522,6 +1533,9 @@ __global__ void __launch_bounds__(kT, 512 / kT) distill_kernel(DistillArgs a, in
             } else {
                 cluster_arrive_relaxed();
             }
+        }
+        if (any_next) name_all(row + step, next, parity);
+        if (team.size > 1) {
             cluster_wait();
             float2 part = make_float2(neg_inf(), 0.0f);
             if (lane < team.size) part = sh.box[turn][lane];
@@ -1543,39 +1557,62 @@ __global__ void __launch_bounds__(kT, 512 / kT) distill_kernel(DistillArgs a, in
                 a.tail && rest.y > 0.0f ? static_cast<float>(fmax(0.0, 1.0 - known.Q)) : 0.0f;
             const float w = unit * g;
             const float G = (static_cast<float>(known.Q) + q_rest) * (Z == 0.0f ? 0.0f : __fdividef(1.0f, Z));
-            // P = share by the row's maximum / Z, P / P_r = share by the rest's / its sum
+            // by the thread's reference: P = exponential * share by the row's / Z,
+            // P / P_r = exponential * share by the rest's / its sum
             float scale = G * share(best, all, c2);
             if (q_rest > 0.0f) scale -= __fdividef(q_rest, rest.y) * share(best, rest.x, c2);
             scale = best > neg_inf() ? scale * w : 0.0f;
-            const float2 ss = make_float2(scale, scale);
-#pragma unroll
-            for (int i = 0; i < kHold; ++i) {
+            const float from = best > neg_inf() ? -best : 0.0f;
+            const float2 ff = make_float2(from, from), ss = make_float2(scale, scale);
+            auto gradient = [&](const uint4& r) {
                 float f[kVec];
+                Elem<E>::unpack(r, f);
 #pragma unroll
                 for (int k = 0; k < kVec; k += 2) {
-                    const float2 y = mul2(make_float2(e[i * kVec + k], e[i * kVec + k + 1]), ss);
+                    const float2 t = mul2(add2(make_float2(f[k], f[k + 1]), ff), cc);
+                    const float2 y = mul2(make_float2(ex2(t.x), ex2(t.y)), ss);
                     f[k] = y.x;
                     f[k + 1] = y.y;
                 }
-                if (i * kT < left) {
-                    if (same_phase) {
-                        __stcs(dst + i * kT, Elem<E>::pack(f));
-                    } else {
+                return Elem<E>::pack(f);
+            };
+            int i = 0;
+            if (same_phase) {
+                for (; i + kChunk <= min(count, next_count); i += kChunk) {
+                    uint4 r[kChunk];
 #pragma unroll
-                        for (int k = 0; k < kVec; ++k)
-                            out[a0 + (v0 + tid + i * kT) * kVec + k] = Elem<E>::narrow(f[k]);
-                    }
+                    for (int k = 0; k < kChunk; ++k) r[k] = buf[(i + k) * kT];
+#pragma unroll
+                    for (int k = 0; k < kChunk; ++k) r[k] = gradient(r[k]);
+#pragma unroll
+                    for (int k = 0; k < kChunk; ++k) copy_async(buf + (i + k) * kT, src + (i + k) * kT);
+#pragma unroll
+                    for (int k = 0; k < kChunk; ++k) __stcs(dst + (i + k) * kT, r[k]);
+                }
+                for (int k = i; k < count; ++k) __stcs(dst + k * kT, gradient(buf[k * kT]));
+            } else {
+                for (int k = i; k < count; ++k) {
+                    const uint4 r = gradient(buf[k * kT]);
+                    const E* f = reinterpret_cast<const E*>(&r);
+#pragma unroll
+                    for (int m = 0; m < kVec; ++m) out[here.a0 + (here.v0 + tid + k * kT) * kVec + m] = f[m];
                 }
             }
-            if (at_end) out[a0 + ragged] = Elem<E>::narrow(end_e * scale);
+            for (; i < next_count; ++i) copy_async(buf + i * kT, src + i * kT);
+            copies_commit();
+            if (at_end) out[here.a0 + ragged] = Elem<E>::narrow(ex2((end_x + from) * c2) * scale);
             __syncthreads();   // the listed places are written a second time
             auto listed = [&](const SlotState& s) {
-                const int at = s.token - a0;
-                if (s.token >= 0 && at >= 0 && at < len)
+                const int at = s.token - here.a0;
+                if (s.token >= 0 && at >= 0 && at < here.len)
                     out[s.token] = Elem<E>::narrow(fmaf(share(s.x, all, c2), G * w, -s.q * w));
             };
             if (tid < n) listed(mine);
             for (int j = tid + kT; j < n; j += kT) listed(state.slots[row * n + j]);
+        } else {
+            for (int i = 0; i < next_count; ++i) copy_async(buf + i * kT, src + i * kT);
+            copies_commit();
+            __syncthreads();
         }
     }
     copies_wait<0>();
@@ -1667,8 +1704,9 @@ Shape shape_of(const Rows& in, int es, int most) {
         return static_cast<int>((per + 63) / 64 * 64);
     };
     int size = 1;
-    while (size < 16 && static_cast<int64_t>(slice(size)) * es > most) size *= 2;
-    while (size < 8 && in.rows * size * 2 <= 148 && static_cast<int64_t>(slice(size)) * es > 8 * 1024) size *= 2;
+    while (size < 8 && static_cast<int64_t>(slice(size)) * es > most) ++size;
+    if (static_cast<int64_t>(slice(size)) * es > most) size = 16;
+    while (size <= 4 && in.rows * size * 2 <= 148 && static_cast<int64_t>(slice(size)) * es > 8 * 1024) size *= 2;
     return Shape{size, slice(size)};
 }
 
@@ -1736,16 +1774,12 @@ int list_space(int n) {
     return cap;
 }
 
-#ifndef DT
-#define DT 512
-#endif
-// Slices of three rows, of at most 8 vectors per thread.
 template <class E>
 cudaError_t launch_distill_typed(const DistillArgs& a, cudaStream_t stream) {
-    const Shape sh = shape_of(a.in, sizeof(E), DT * 8 * 16);
-    const size_t smem = static_cast<size_t>(sh.S) * sizeof(E) * 3;
-    return a.grad ? launch_rows(distill_kernel<E, true, DT>, a.in, sh.size, smem, stream, DT, a, sh.S)
-                  : launch_rows(distill_kernel<E, false, DT>, a.in, sh.size, smem, stream, DT, a, sh.S);
+    const Shape sh = shape_of(a.in, sizeof(E), kThreads * kHold * 16);
+    const size_t smem = static_cast<size_t>(kThreads) * kHold * 16;
+    return a.grad ? launch_rows(distill_kernel<E, true>, a.in, sh.size, smem, stream, kThreads, a, sh.S)
+                  : launch_rows(distill_kernel<E, false>, a.in, sh.size, smem, stream, kThreads, a, sh.S);
 }
 
 template <class E>
