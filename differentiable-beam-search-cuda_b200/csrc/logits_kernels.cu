@@ -387,13 +387,27 @@ struct Team {      // a CTA's place in its cluster
     }
 };
 
+// 2^(steps / 32) in 64 bits, relative error below 2e-12: 2^(n/32 + r/32) with n
+// the whole number nearest to `steps` (within -2^15 and 2^15), a table of 2^(j/32) (an entry per lane) and
+// the Taylor polynomial of 2^(r/32) to the fourth power. All 32 lanes of a
+// warp call it together.
+__device__ __forceinline__ double exp_table() { return exp2(static_cast<double>(threadIdx.x & 31) * 0.03125); }
+__device__ __forceinline__ double exp_by(double steps, int n, double tab) {
+    constexpr double kL = 0.021660849392498290;   // ln 2 / 32
+    const double nd = __hiloint2double(0x43300000, n ^ static_cast<int>(0x80000000)) - 4503601774854144.0;
+    const double r = steps - nd;
+    double p = fma(r, kL * kL * kL * kL / 24.0, kL * kL * kL / 6.0);
+    p = fma(r, p, kL * kL / 2.0);
+    p = fma(r, p, kL);
+    p = fma(r, p, 1.0);
+    p *= __shfl_sync(kAll, tab, n & 31);
+    return __hiloint2double(__double2hiint(p) + ((n >> 5) << 20), __double2loint(p));
+}
+
 // ---------------------------------------------------------------------------
 // Weights of sampling: exp((x - m) / T) in 64 bits, because tokens have to be
 // the ones that exact sums give: with V borders between tokens, sums in 32
 // bits would pick another token about once in a hundred flat rows.
-// 2^(n/32 + r/32), n the nearest whole number: a table of 2^(j/32) held one
-// entry per lane, and the Taylor polynomial of 2^(r/32), |r| <= 1/2, to the
-// fourth power (relative error below 1.3e-12).
 // ---------------------------------------------------------------------------
 struct Weights {
     float mf;
@@ -406,22 +420,14 @@ struct Weights {
         m = static_cast<double>(best);
         c = 46.166241308446828384 / static_cast<double>(temperature);   // 32 / ln 2
         cf = static_cast<float>(c);
-        tab = exp2(static_cast<double>(threadIdx.x & 31) * 0.03125);
+        tab = exp_table();
     }
     // All 32 lanes of the warp call it together.
     __device__ __forceinline__ double operator()(float x) const {
         // 0 * inf and inf - inf come out as NaN, which fmaxf drops
         const float t = fmaxf((x - mf) * cf, -40000.0f);
         const int n = __float_as_int(t + 12582912.0f) - 0x4B400000;
-        const double nd = __hiloint2double(0x43300000, n ^ static_cast<int>(0x80000000)) - 4503601774854144.0;
-        const double r = fma(static_cast<double>(x) - m, c, -nd);
-        constexpr double kL = 0.021660849392498290;   // ln 2 / 32
-        double p = fma(r, kL * kL * kL * kL / 24.0, kL * kL * kL / 6.0);
-        p = fma(r, p, kL * kL / 2.0);
-        p = fma(r, p, kL);
-        p = fma(r, p, 1.0);
-        p *= __shfl_sync(kAll, tab, n & 31);
-        p = __hiloint2double(__double2hiint(p) + ((n >> 5) << 20), __double2loint(p));
+        const double p = exp_by((static_cast<double>(x) - m) * c, n, tab);
         return x == mf ? 1.0 : (n < -32686 ? 0.0 : p);   // exp(-708) and below count as nothing
     }
 };
@@ -1200,100 +1206,154 @@ __device__ __forceinline__ T reduce_block(T v, Op op, T* scratch) {   // any num
     return v;
 }
 
-// The teacher's slots, a CTA per row: everything that takes a thread a while
-// is done here, for all rows at once, and not between the barriers of the
-// rows' pass. A token listed twice is found in a hash table of `mask` + 1
-// places; its first slot stands for it with the sum of the probabilities.
-template <class E>
-__global__ void __launch_bounds__(256) slots_kernel(DistillArgs a, int mask) {
-    extern __shared__ int table[];      // tokens, then their first slots
-    __shared__ double d32[32];
-    __shared__ float f32[32];
-    int* first = table + mask + 1;
+// The teacher's slots, kGroup threads a row with kPer slots each (a warp, or a
+// CTA where the slots are many): everything that takes a thread a while is
+// done here, for all rows at once, and not between the barriers of the rows'
+// pass. The first slot of a token stands for all of its slots. Two bit maps of
+// the tokens' hashes (a bit for each of `mask` + 1 values) tell that no token
+// is listed twice; where they cannot (one row in 250 with 64 slots), the
+// tokens are compared.
+template <class E, int kGroup, int kPer>
+__global__ void __launch_bounds__(256) slots_kernel(DistillArgs a, uint32_t mask) {
+    constexpr int kRows = 256 / kGroup;   // of a CTA
+    extern __shared__ uint32_t maps[];
+    __shared__ double d8[8];
+    __shared__ float f8[8];
+    const int group = threadIdx.x / kGroup, tid = threadIdx.x % kGroup;
+    uint32_t* map = maps + group * ((mask + 1) / 16);
+    uint32_t* map2 = map + (mask + 1) / 32;
     const DistillState state = state_of(a);
-    const int n = a.n, tid = threadIdx.x, threads = blockDim.x;
+    const int n = a.n;
     const float c2 = fminf(1.4426950408889634f / a.temperature, FLT_MAX);
-    for (int64_t row = blockIdx.x; row < a.in.rows; row += gridDim.x) {
+    const double tab = exp_table();
+    auto sync = [&]() {
+        if (kGroup == 32)
+            __syncwarp();
+        else
+            __syncthreads();
+    };
+    auto over = [&](auto v, auto op, auto* scratch) {
+        if (kGroup == 32) {
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) v = op(v, __shfl_xor_sync(kAll, v, o));
+            return v;
+        }
+        return block_reduce(v, op, scratch);
+    };
+    auto some = [&](bool v) { return kGroup == 32 ? __any_sync(kAll, v) != 0 : __syncthreads_or(v) != 0; };
+    for (int i = tid; i < static_cast<int>((mask + 1) / 16); i += kGroup) map[i] = 0;
+    sync();
+    for (int64_t row = blockIdx.x * static_cast<int64_t>(kRows) + group; row < a.in.rows;
+         row += gridDim.x * static_cast<int64_t>(kRows)) {
         const E* x = static_cast<const E*>(a.in.x) + row * a.in.stride;
-        SlotState* slots = state.slots + row * n;
-        for (int i = tid; i <= mask; i += threads) {
-            table[i] = -1;
-            first[i] = 0x7FFFFFFF;
-        }
-        __syncthreads();
-        auto find = [&](int token) {
-            uint32_t h = (static_cast<uint32_t>(token) * 2654435761u) >> 16;
-            while (true) {
-                h &= static_cast<uint32_t>(mask);
-                const int was = atomicCAS(&table[h], -1, token);
-                if (was == -1 || was == token) return h;
-                ++h;
+        // this thread's slots, their loads in flight together
+        int64_t i[kPer];
+        float l[kPer];
+        SlotState slot[kPer];
+#pragma unroll
+        for (int k = 0; k < kPer; ++k) {
+            const int j = tid + k * kGroup;
+            i[k] = -1;
+            l[k] = 0.0f;
+            if (j < n) {
+                i[k] = teacher_token(a, row * n + j);
+                l[k] = a.teacher_log_probs[row * n + j];
             }
-        };
+        }
         float best = neg_inf();
-        double Q = 0.0;
         bool any = false;
-        for (int j = tid; j < n; j += threads) {
-            const int64_t i = teacher_token(a, row * n + j);
-            SlotState slot = {-1, 0.0f, 0.0f, 0};
-            if (i >= 0 && i < a.in.V) {
+#pragma unroll
+        for (int k = 0; k < kPer; ++k) {
+            slot[k] = SlotState{-1, neg_inf(), 0.0f, 0};
+            if (i[k] >= 0 && i[k] < a.in.V) {
                 any = true;
-                slot.token = static_cast<int>(i);
-                slot.x = Elem<E>::widen(x[i]);
-                const double q = exp(static_cast<double>(a.teacher_log_probs[row * n + j]));
-                slot.q = static_cast<float>(q);
-                Q += q;
-                best = fmaxf(best, slot.x);
-                atomicMin(&first[find(slot.token)], j);
+                slot[k].token = static_cast<int>(i[k]);
+                slot[k].x = Elem<E>::widen(x[i[k]]);
             }
-            slots[j] = slot;
         }
-        any = __syncthreads_or(any);
-        best = reduce_block(best, Max(), f32);
-        Q = reduce_block(Q, Add(), d32);
+        double Q = 0.0;
+        bool maybe = false;
+        uint32_t h[kPer];
+#pragma unroll
+        for (int k = 0; k < kPer; ++k) {
+            // log-probs above 709 are infinite, those below -708 nothing
+            const float t = fminf(fmaxf(l[k] * 46.16624f, -40000.0f), 40000.0f);
+            const int steps = __float_as_int(t + 12582912.0f) - 0x4B400000;
+            double q = exp_by(static_cast<double>(l[k]) * 46.166241308446828384, steps, tab);
+            if (!(l[k] >= -708.0f)) q = l[k] < -708.0f ? 0.0 : static_cast<double>(l[k]);
+            if (l[k] > 709.0f) q = HUGE_VAL;
+            if (slot[k].token >= 0) {
+                slot[k].q = static_cast<float>(q);
+                Q += q;
+                h[k] = static_cast<uint32_t>(slot[k].token) * 2654435761u;
+                const uint32_t h1 = h[k] >> 7 & mask, h2 = h[k] >> 15 & mask;
+                const bool was1 = atomicOr(&map[h1 >> 5], 1u << (h1 & 31u)) >> (h1 & 31u) & 1u;
+                const bool was2 = atomicOr(&map2[h2 >> 5], 1u << (h2 & 31u)) >> (h2 & 31u) & 1u;
+                maybe = maybe || (was1 && was2);
+            }
+            best = fmaxf(best, slot[k].x);
+        }
+        any = some(any);
+        best = over(best, Max(), f8);
+        Q = over(Q, Add(), d8);
+        bool owner[kPer];
+#pragma unroll
+        for (int k = 0; k < kPer; ++k) owner[k] = slot[k].token >= 0;
+        if (some(maybe)) {
+            // owner: no earlier slot has the token; i: what its slots have together
+#pragma unroll
+            for (int k = 0; k < kPer; ++k) i[k] = 0;
+            auto meet = [&](int token, float q, int o) {
+#pragma unroll
+                for (int k = 0; k < kPer; ++k) {
+                    if (token < 0 || token != slot[k].token) continue;
+                    owner[k] = owner[k] && o >= tid + k * kGroup;
+                    i[k] = __float_as_int(__int_as_float(static_cast<int>(i[k])) + q);
+                }
+            };
+            if (kGroup == 32) {
+#pragma unroll
+                for (int k = 0; k < kPer; ++k)
+                    for (int o = 0; o < 32; ++o)
+                        meet(__shfl_sync(kAll, slot[k].token, o), __shfl_sync(kAll, slot[k].q, o), o + 32 * k);
+            } else {
+                for (int o = 0; o < n; ++o) {
+                    const int64_t token = teacher_token(a, row * n + o);
+                    if (token >= 0 && token < a.in.V)
+                        meet(static_cast<int>(token),
+                             static_cast<float>(exp(static_cast<double>(a.teacher_log_probs[row * n + o]))), o);
+                }
+            }
+        } else {
+#pragma unroll
+            for (int k = 0; k < kPer; ++k) i[k] = __float_as_int(slot[k].q);
+        }
         double C = 0.0;
         float listed = 0.0f;
-        bool twice = false;
-        for (int j = tid; j < n; j += threads) {
-            SlotState slot = slots[j];
-            if (slot.token < 0) continue;
-            const float l = a.teacher_log_probs[row * n + j];
-            if (slot.q != 0.0f) {
-                const double z = slot.x == best ? 0.0 : static_cast<double>(slot.x) - static_cast<double>(best);
-                C += static_cast<double>(slot.q) *
-                     (static_cast<double>(l) - 0.69314718055994530942 * static_cast<double>(c2) * z);
+#pragma unroll
+        for (int k = 0; k < kPer; ++k) {
+            if (slot[k].token < 0) continue;
+            map[(h[k] >> 7 & mask) >> 5] = 0;   // all bits of the maps have been looked at
+            map2[(h[k] >> 15 & mask) >> 5] = 0;
+            if (slot[k].q != 0.0f) {
+                const double z = slot[k].x == best ? 0.0 : static_cast<double>(slot[k].x) - static_cast<double>(best);
+                C += static_cast<double>(slot[k].q) *
+                     (static_cast<double>(l[k]) - 0.69314718055994530942 * static_cast<double>(c2) * z);
             }
-            if (first[find(slot.token)] == j) {
-                listed += share(slot.x, best, c2);
-            } else {
-                twice = true;
-            }
+            if (owner[k]) listed += share(slot[k].x, best, c2);
+            slot[k].q = __int_as_float(static_cast<int>(i[k]));
+            if (!owner[k]) slot[k].token = -1;
         }
-        listed = reduce_block(listed, Add(), f32);
-        C = reduce_block(C, Add(), d32);
-        if (__syncthreads_or(twice)) {
-            for (int j = tid; j < n; j += threads) {
-                const int token = slots[j].token;
-                if (token < 0 || first[find(token)] != j) continue;
-                float q = 0.0f;
-                for (int o = j; o < n; ++o)
-                    if (teacher_token(a, row * n + o) == token) q += slots[o].q;
-                slots[j].unused = __float_as_int(q);
-            }
-            __syncthreads();
-            for (int j = tid; j < n; j += threads) {
-                if (slots[j].token < 0) continue;
-                if (first[find(slots[j].token)] == j)
-                    slots[j].q = __int_as_float(slots[j].unused);
-                else
-                    slots[j].token = -1;
-            }
-        }
+        listed = over(listed, Add(), f8);
+        C = over(C, Add(), d8);
+#pragma unroll
+        for (int k = 0; k < kPer; ++k)
+            if (tid + k * kGroup < n) state.slots[row * n + tid + k * kGroup] = slot[k];
         if (tid == 0) {
             state.rows[row] = RowState{Q, C, best, listed, neg_inf(), 0.0f};
             state.any[row] = any ? 1 : 0;
         }
-        __syncthreads();
+        sync();
     }
 }
 
@@ -1391,6 +1451,7 @@ __global__ void __launch_bounds__(kThreads, 3) distill_kernel(DistillArgs a, int
             atomicOr(reinterpret_cast<uint32_t*>(&sh.marks[par][v % kT]) + (bit >> 5), 1u << (bit & 31));
         }
     };
+    const uint4 none = vneg_inf<E>();
     SlotState slot = {-1, 0.0f, 0.0f, 0};   // this thread's first slot of the next row
     auto name_all = [&](int64_t r, const View& w, int par) {
         if (tid < n) name(slot, w, par);
@@ -1403,7 +1464,12 @@ __global__ void __launch_bounds__(kThreads, 3) distill_kernel(DistillArgs a, int
     View next = view(in + first_row * a.in.stride);
     if (any_next) {
         if (tid < n) slot = state.slots[first_row * n + tid];
-        for (int i = 0, v = next.v0 + tid; v < next.v1; v += kT, ++i) copy_async(buf + i * kT, next.src + v);
+        for (int i = 0, v = next.v0 + tid; i < kHold; v += kT, ++i) {
+            if (v < next.v1)
+                copy_async(buf + i * kT, next.src + v);
+            else
+                buf[i * kT] = none;
+        }
         name_all(first_row, next, 0);
     }
     copies_commit();
@@ -1427,10 +1493,18 @@ __global__ void __launch_bounds__(kThreads, 3) distill_kernel(DistillArgs a, int
         dst += here.v0 + tid;
         const int count = (here.v1 - here.v0 - tid + kT - 1) / kT;   // of this thread's vectors
         const int next_count = any_next ? (next.v1 - next.v0 - tid + kT - 1) / kT : 0;
-        const uint4* src = next.src + next.v0 + tid;
+        const uint4* src = next.src + next.v0 + tid;   // only its first next_count vectors are read
         const int head = min(here.len, here.v0 * kVec), tail_at = max(head, here.v1 * kVec);
         const int ragged = lane < head ? lane : tail_at + lane - head;
         const bool at_end = warp == kWarps - 1 && ragged < here.len && here.a0 + ragged >= 0;
+        auto copy_next = [&]() {
+            for (int i = 0; i < kHold; ++i) {
+                if (i < next_count)
+                    copy_async(buf + i * kT, src + i * kT);
+                else
+                    buf[i * kT] = none;
+            }
+        };
         if (!any || (a.skip_unit && g == 1.0f)) {   // the same for the whole cluster
             if (any) {
                 sh.marks[par][tid] = make_uint4(0, 0, 0, 0);
@@ -1445,7 +1519,7 @@ __global__ void __launch_bounds__(kThreads, 3) distill_kernel(DistillArgs a, int
                         out[here.a0 + e] = Elem<E>::narrow(0.0f);
                 if (at_end) out[here.a0 + ragged] = Elem<E>::narrow(0.0f);
             }
-            for (int i = 0; i < next_count; ++i) copy_async(buf + i * kT, src + i * kT);
+            copy_next();
             copies_commit();
             if (any_next) {
                 __syncthreads();   // the marks of two rows ago are gone
@@ -1472,60 +1546,59 @@ __global__ void __launch_bounds__(kThreads, 3) distill_kernel(DistillArgs a, int
         if (at_end && !(sh.end_marks[par] >> lane & 1u)) end_x = Elem<E>::widen(in[row * a.in.stride + here.a0 + ragged]);
         // The sum goes by the maximum of the thread's first vectors; where the
         // others run so far beyond it that the sum overflows, by all of them.
-        const uint4 none = vneg_inf<E>();
-        auto best_of = [&](int until) {
+        auto best_of = [&](int chunks) {
             uint4 top = none;
-            for (int i = 0; i < until; ++i) top = vmax<E>(top, buf[i * kT]);
+            for (int i = 0; i < chunks * kChunk; ++i) top = vmax<E>(top, buf[i * kT]);
             return lanes_max<E>(top);
         };
+        const int chunks = (count + kChunk - 1) / kChunk;   // the last one is filled up with -inf
         float best = neg_inf(), sum = 0.0f;
-        auto add = [&](const uint4& r, float2 from, float2& p) {
-            float f[kVec];
-            Elem<E>::unpack(r, f);
-#pragma unroll
-            for (int k = 0; k < kVec; k += 2) {
-                const float2 t = mul2(add2(make_float2(f[k], f[k + 1]), from), cc);
-                p = add2(p, make_float2(ex2(t.x), ex2(t.y)));
-            }
-        };
         auto add_up = [&]() {
             const float from = best > neg_inf() ? -best : 0.0f;
             const float2 ff = make_float2(from, from);
             float2 p = make_float2(0.0f, 0.0f);
-            int i = 0;
-            for (; i + kChunk <= count; i += kChunk) {
+            const uint4* at = buf;
+            for (int i = 0; i < chunks; ++i, at += kChunk * kT) {
                 uint4 r[kChunk];
 #pragma unroll
-                for (int k = 0; k < kChunk; ++k) r[k] = buf[(i + k) * kT];
+                for (int k = 0; k < kChunk; ++k) r[k] = at[k * kT];
 #pragma unroll
-                for (int k = 0; k < kChunk; ++k) add(r[k], ff, p);
+                for (int k = 0; k < kChunk; ++k) {
+                    float f[kVec];
+                    Elem<E>::unpack(r[k], f);
+#pragma unroll
+                    for (int m = 0; m < kVec; m += 2) {
+                        const float2 t = mul2(add2(make_float2(f[m], f[m + 1]), ff), cc);
+                        p = add2(p, make_float2(ex2(t.x), ex2(t.y)));
+                    }
+                }
             }
-            for (; i < count; ++i) add(buf[i * kT], ff, p);
             sum = p.x + p.y + (at_end ? ex2((end_x + from) * c2) : 0.0f);
         };
-        best = fmaxf(best_of(min(count, kChunk)), end_x);
+        best = fmaxf(best_of(min(chunks, 1)), end_x);
         add_up();
         if (!(best > neg_inf()) || !(sum < 1.0e30f)) {
-            best = fmaxf(best_of(count), end_x);
+            best = fmaxf(best_of(chunks), end_x);
             add_up();
         }
         // over the warp, the CTA and the cluster: references, and sums by them
-        auto join = [&](float m, float v, int lanes) {
-            float all = m;
-            for (int o = lanes / 2; o > 0; o >>= 1) all = fmaxf(all, __shfl_xor_sync(kAll, all, o));
-            v = v == 0.0f ? 0.0f : v * share(m, all, c2);
-            for (int o = lanes / 2; o > 0; o >>= 1) v += __shfl_xor_sync(kAll, v, o);
-            return make_float2(all, v);
-        };
-        const float2 of_warp = join(best, sum, 32);
-        if (lane == 0) sh.part[warp] = of_warp;
+        float2 rest = make_float2(best, sum);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) rest.x = fmaxf(rest.x, __shfl_xor_sync(kAll, rest.x, o));
+        rest.y = sum == 0.0f ? 0.0f : sum * share(best, rest.x, c2);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) rest.y += __shfl_xor_sync(kAll, rest.y, o);
+        if (lane == 0) sh.part[warp] = rest;
         __syncthreads();
+        auto join = [&](const float2* parts, int size) {
+            float2 all = make_float2(neg_inf(), 0.0f);
+            for (int i = 0; i < size; ++i) all.x = fmaxf(all.x, parts[i].x);
+            const float from = all.x > neg_inf() ? -all.x : 0.0f;
+            for (int i = 0; i < size; ++i) all.y += parts[i].y * ex2((parts[i].x + from) * c2);
+            return all;
+        };
         if (tid == 0) sh.end_marks[par] = 0;
-        float2 rest = make_float2(neg_inf(), 0.0f);
-        if (team.size == 1 || warp == 0) {
-            const float2 part = sh.part[lane % kWarps];
-            rest = join(part.x, part.y, kWarps);
-        }
+        if (team.size == 1 || warp == 0) rest = join(sh.part, kWarps);
         if (team.size > 1) {
             if (warp == 0) {
                 if (lane < team.size) *cg::this_cluster().map_shared_rank(&sh.box[turn][team.rank], lane) = rest;
@@ -1537,12 +1610,7 @@ __global__ void __launch_bounds__(kThreads, 3) distill_kernel(DistillArgs a, int
         if (any_next) name_all(row + step, next, parity);
         if (team.size > 1) {
             cluster_wait();
-            float2 part = make_float2(neg_inf(), 0.0f);
-            if (lane < team.size) part = sh.box[turn][lane];
-            rest = join(part.x, part.y, kMaxCluster);
-            // lanes 16 to 31 joined nothing
-            rest.x = __shfl_sync(kAll, rest.x, 0);
-            rest.y = __shfl_sync(kAll, rest.y, 0);
+            rest = join(sh.box[turn], team.size);
             turn ^= 1;
         }
         if (tid == 0 && team.rank == 0 && !a.skip_state) {
@@ -1576,29 +1644,44 @@ __global__ void __launch_bounds__(kThreads, 3) distill_kernel(DistillArgs a, int
                 }
                 return Elem<E>::pack(f);
             };
-            int i = 0;
             if (same_phase) {
-                for (; i + kChunk <= min(count, next_count); i += kChunk) {
+                uint4* at = buf;
+                for (int i = 0; i < kHold; i += kChunk, at += kChunk * kT, dst += kChunk * kT, src += kChunk * kT) {
                     uint4 r[kChunk];
+                    if (i + kChunk <= min(count, next_count)) {
 #pragma unroll
-                    for (int k = 0; k < kChunk; ++k) r[k] = buf[(i + k) * kT];
+                        for (int k = 0; k < kChunk; ++k) r[k] = at[k * kT];
 #pragma unroll
-                    for (int k = 0; k < kChunk; ++k) r[k] = gradient(r[k]);
+                        for (int k = 0; k < kChunk; ++k) r[k] = gradient(r[k]);
 #pragma unroll
-                    for (int k = 0; k < kChunk; ++k) copy_async(buf + (i + k) * kT, src + (i + k) * kT);
+                        for (int k = 0; k < kChunk; ++k) {
+                            copy_async(at + k * kT, src + k * kT);
+                            __stcs(dst + k * kT, r[k]);
+                        }
+                    } else {
 #pragma unroll
-                    for (int k = 0; k < kChunk; ++k) __stcs(dst + (i + k) * kT, r[k]);
+                        for (int k = 0; k < kChunk; ++k) r[k] = i + k < count ? at[k * kT] : none;
+#pragma unroll
+                        for (int k = 0; k < kChunk; ++k) r[k] = gradient(r[k]);
+#pragma unroll
+                        for (int k = 0; k < kChunk; ++k) {
+                            if (i + k < next_count)
+                                copy_async(at + k * kT, src + k * kT);
+                            else
+                                at[k * kT] = none;
+                            if (i + k < count) __stcs(dst + k * kT, r[k]);
+                        }
+                    }
                 }
-                for (int k = i; k < count; ++k) __stcs(dst + k * kT, gradient(buf[k * kT]));
             } else {
-                for (int k = i; k < count; ++k) {
+                for (int k = 0; k < count; ++k) {
                     const uint4 r = gradient(buf[k * kT]);
                     const E* f = reinterpret_cast<const E*>(&r);
 #pragma unroll
                     for (int m = 0; m < kVec; ++m) out[here.a0 + (here.v0 + tid + k * kT) * kVec + m] = f[m];
                 }
+                copy_next();
             }
-            for (; i < next_count; ++i) copy_async(buf + i * kT, src + i * kT);
             copies_commit();
             if (at_end) out[here.a0 + ragged] = Elem<E>::narrow(ex2((end_x + from) * c2) * scale);
             __syncthreads();   // the listed places are written a second time
@@ -1610,7 +1693,7 @@ __global__ void __launch_bounds__(kThreads, 3) distill_kernel(DistillArgs a, int
             if (tid < n) listed(mine);
             for (int j = tid + kT; j < n; j += kT) listed(state.slots[row * n + j]);
         } else {
-            for (int i = 0; i < next_count; ++i) copy_async(buf + i * kT, src + i * kT);
+            copy_next();
             copies_commit();
             __syncthreads();
         }
@@ -1631,11 +1714,11 @@ __global__ void __cluster_dims__(8, 1, 1) __launch_bounds__(1024) losses_kernel(
     const double c = static_cast<double>(fminf(1.4426950408889634f / a.temperature, FLT_MAX)) * 0.69314718055994530942;
     double sum = 0.0;
     int count = 0;
-    for (int64_t row = team.rank * 1024 + static_cast<int>(threadIdx.x); row < a.in.rows; row += 8 * 1024) {
+    for (int64_t row = team.rank + static_cast<int64_t>(threadIdx.x) * 8; row < a.in.rows; row += 8 * blockDim.x) {
         double loss = 0.0;
+        const RowState s = state.rows[row];
         if (state.any[row]) {
             ++count;
-            const RowState s = state.rows[row];
             const float all = fmaxf(s.best_listed, s.best_rest);
             auto by = [&](float best, float v) {   // a sum by the row's maximum
                 return v == 0.0f ? 0.0 : static_cast<double>(v) *
@@ -1651,7 +1734,7 @@ __global__ void __cluster_dims__(8, 1, 1) __launch_bounds__(1024) losses_kernel(
             }
             if (left > 0.0) {
                 const double down = all == s.best_rest ? 0.0 : static_cast<double>(all) - static_cast<double>(s.best_rest);
-                loss += left * (log(left) - log(static_cast<double>(s.rest)) + c * down + log(Z));
+                loss += left * (log(left * Z / static_cast<double>(s.rest)) + c * down);
             }
             if (Z == 0.0) loss = s.Q > 0.0 ? static_cast<double>(INFINITY) : 0.0;   // nothing above -inf
         }
@@ -1784,11 +1867,18 @@ cudaError_t launch_distill_typed(const DistillArgs& a, cudaStream_t stream) {
 
 template <class E>
 cudaError_t launch_slots(const DistillArgs& a, cudaStream_t stream) {
-    int places = 64;
-    while (places < 2 * a.n) places *= 2;
-    const int threads = std::min(256, (a.n + 31) / 32 * 32);
-    const int64_t ctas = std::min<int64_t>(a.in.rows, 148 * 2048 / threads);
-    slots_kernel<E><<<static_cast<unsigned>(ctas), threads, places * 8, stream>>>(a, places - 1);
+    const unsigned warps = static_cast<unsigned>(std::min<int64_t>((a.in.rows + 7) / 8, 148 * 8));
+    if (a.n <= 32) {
+        slots_kernel<E, 32, 1><<<warps, 256, 8 * 2048, stream>>>(a, 8192 - 1);
+    } else if (a.n <= 64) {
+        slots_kernel<E, 32, 2><<<warps, 256, 8 * 2048, stream>>>(a, 8192 - 1);
+    } else if (a.n <= 128) {
+        slots_kernel<E, 32, 4><<<warps, 256, 8 * 2048, stream>>>(a, 8192 - 1);
+    } else {
+        static_assert(kMaxTop <= 4 * 256, "four slots per thread");
+        const unsigned ctas = static_cast<unsigned>(std::min<int64_t>(a.in.rows, 148 * 8));
+        slots_kernel<E, 256, 4><<<ctas, 256, 32768, stream>>>(a, 131072 - 1);
+    }
     return dbs_dev::count_launch(cudaGetLastError());
 }
 
@@ -1837,7 +1927,7 @@ cudaError_t launch_distill(const DistillArgs& a, cudaStream_t stream) {
     } else if (a.reduction == kNone) {
         return cudaSuccess;
     }
-    losses_kernel<<<8, 1024, 0, stream>>>(a);
+    losses_kernel<<<8, a.in.rows <= 4096 ? 256 : 1024, 0, stream>>>(a);
     return dbs_dev::count_launch(cudaGetLastError());
 }
 
