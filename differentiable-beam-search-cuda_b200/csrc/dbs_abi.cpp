@@ -1869,6 +1869,12 @@ static dbs_logits::Rows logits_rows(const void* logits, int data_type, int64_t r
     return in;
 }
 
+static void check_workspace(const void* workspace, int64_t bytes) {
+    if (bytes > 0 && !workspace) throw std::invalid_argument("workspace cannot be null");
+    if (reinterpret_cast<uintptr_t>(workspace) % 16 != 0)
+        throw std::invalid_argument("workspace is not aligned to 16 bytes");
+}
+
 static void positive_temperature(float temperature) {
     if (!(temperature > 0.0f) || !std::isfinite(temperature))
         throw std::invalid_argument("temperature must be positive and finite");
@@ -1877,7 +1883,8 @@ static void positive_temperature(float temperature) {
 DBS_EXPORT int dbs_device_sample(const void* logits, int data_type, int64_t rows, int vocab_size, int64_t row_stride,
                                  const float* uniforms, const float* temperatures, float temperature,
                                  const int32_t* top_ks, int top_k, const float* top_ps, float top_p,
-                                 const float* min_ps, float min_p, int32_t* tokens, void* cuda_stream) {
+                                 const float* min_ps, float min_p, int32_t* tokens, void* workspace,
+                                 void* cuda_stream) {
     return guarded(nullptr, [&]() {
         dbs_logits::SampleArgs a;
         a.in = logits_rows(logits, data_type, rows, vocab_size, row_stride);
@@ -1898,7 +1905,38 @@ DBS_EXPORT int dbs_device_sample(const void* logits, int data_type, int64_t rows
         a.min_p = min_ps;
         a.min_p_all = min_p;
         a.tokens = tokens;
+        a.space = workspace;
+        check_workspace(workspace, dbs_logits::sample_space(a));
         dbs_host::check_cuda(dbs_logits::launch_sample(a, static_cast<cudaStream_t>(cuda_stream)), "sample");
+        clear_error(nullptr);
+        return 0;
+    });
+}
+
+DBS_EXPORT int dbs_device_sample_workspace_bytes(int data_type, int64_t rows, int vocab_size, int top_k,
+                                                 int64_t* bytes) {
+    return guarded(nullptr, [&]() {
+        if (!bytes) throw std::invalid_argument("bytes cannot be null");
+        dbs_logits::SampleArgs a;
+        a.in = logits_rows(bytes, data_type, rows, vocab_size, 0);   // any pointer: the rows are not read
+        static const int32_t per_row = 0;
+        a.top_k = top_k < 0 ? &per_row : nullptr;
+        a.top_k_all = top_k;
+        *bytes = dbs_logits::sample_space(a);
+        clear_error(nullptr);
+        return 0;
+    });
+}
+
+DBS_EXPORT int dbs_device_top_log_probs_workspace_bytes(int data_type, int64_t rows, int vocab_size, int n,
+                                                        int64_t* bytes) {
+    return guarded(nullptr, [&]() {
+        if (!bytes) throw std::invalid_argument("bytes cannot be null");
+        dbs_logits::TopArgs a;
+        a.in = logits_rows(bytes, data_type, rows, vocab_size, 0);
+        if (n <= 0) throw std::invalid_argument("n must be positive");
+        a.n = n;
+        *bytes = dbs_logits::top_space(a);
         clear_error(nullptr);
         return 0;
     });
@@ -1906,7 +1944,7 @@ DBS_EXPORT int dbs_device_sample(const void* logits, int data_type, int64_t rows
 
 DBS_EXPORT int dbs_device_top_log_probs(const void* logits, int data_type, int64_t rows, int vocab_size,
                                         int64_t row_stride, int n, float temperature, float* log_probs,
-                                        int32_t* tokens, void* cuda_stream) {
+                                        int32_t* tokens, void* workspace, void* cuda_stream) {
     return guarded(nullptr, [&]() {
         dbs_logits::TopArgs a;
         a.in = logits_rows(logits, data_type, rows, vocab_size, row_stride);
@@ -1919,6 +1957,8 @@ DBS_EXPORT int dbs_device_top_log_probs(const void* logits, int data_type, int64
         a.temperature = temperature;
         a.log_probs = log_probs;
         a.tokens = tokens;
+        a.space = workspace;
+        check_workspace(workspace, dbs_logits::top_space(a));
         dbs_host::check_cuda(dbs_logits::launch_top(a, static_cast<cudaStream_t>(cuda_stream)), "top_log_probs");
         clear_error(nullptr);
         return 0;

@@ -42,6 +42,8 @@ struct SampleArgs {
     float top_p_all = 1.0f;
     float min_p_all = 0.0f;
     int32_t* tokens = nullptr;            // [rows]
+    void* space = nullptr;                // sample_space() bytes
+    const int* left = nullptr;            // set by the launcher: the rows a kernel takes, their number first
 };
 
 struct TopArgs {
@@ -50,6 +52,8 @@ struct TopArgs {
     float temperature = 1.0f;
     float* log_probs = nullptr;           // [rows, n]
     int32_t* tokens = nullptr;            // [rows, n]
+    void* space = nullptr;                // top_space() bytes
+    const int* left = nullptr;            // as above
 };
 
 enum Reduction : int { kNone = 0, kSum = 1, kMean = 2 };
@@ -75,6 +79,9 @@ struct DistillArgs {
     int skip_unit = 0;                          // grad holds the gradient for grad_loss = 1 already
 };
 
+// Device memory that a call needs for what passes between its kernels.
+int64_t sample_space(const SampleArgs& a);
+int64_t top_space(const TopArgs& a);
 cudaError_t launch_sample(const SampleArgs& a, cudaStream_t stream);
 cudaError_t launch_top(const TopArgs& a, cudaStream_t stream);
 cudaError_t launch_distill(const DistillArgs& a, cudaStream_t stream);

@@ -724,6 +724,28 @@ __device__ float threshold(Shared& sh, const uint4& acc, float best, int t) {
     return lo;
 }
 
+__device__ __forceinline__ void copy_async(uint4* to, const uint4* from) {
+    asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16;" ::"r"(
+                     static_cast<uint32_t>(__cvta_generic_to_shared(to))),
+                 "l"(from)
+                 : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int kLeft>
+__device__ __forceinline__ void copies_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(kLeft) : "memory");
+}
+// The cluster's barrier for threads that have nothing to show: their stores
+// need not have landed.
+__device__ __forceinline__ void cluster_arrive_relaxed() { asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory"); }
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
+
+// 2^(c2 (x - best)) for x <= best; 0 where nothing is above -inf.
+__device__ __forceinline__ float share(float x, float best, float c2) {
+    return best > neg_inf() || best != best ? ex2((x - best) * c2) : 0.0f;
+}
+
 // ---------------------------------------------------------------------------
 // Softmax sums in 32 bits. An exponent is x c2 - B in one fused step, with a
 // whole number B near the maximum that the sum goes by: changing from one
@@ -796,7 +818,9 @@ __global__ void __launch_bounds__(kThreads, 3) top_kernel(TopArgs a, int S, int 
     const float c2 = fminf(1.4426950408889634f / a.temperature, FLT_MAX);
     int leader = 0;
     cluster_sync(team.size);   // everybody's shared memory exists from here on
-    for (int64_t row = blockIdx.x / team.size; row < a.in.rows; row += step) {
+    const int64_t rows = a.left ? a.left[0] : a.in.rows;
+    for (int64_t at = blockIdx.x / team.size; at < rows; at += step) {
+        const int64_t row = a.left ? a.left[1 + at] : at;
         __syncthreads();
         if (threadIdx.x == 0) sh.listed = 0;
         uint4 acc = vneg_inf<E>();
@@ -1036,7 +1060,9 @@ __global__ void __launch_bounds__(kThreads, 3) sample_kernel(SampleArgs a, int S
     const int V = a.in.V;
     int leader = 0;
     cluster_sync(team.size);
-    for (int64_t row = blockIdx.x / team.size; row < a.in.rows; row += step) {
+    const int64_t rows = a.left ? a.left[0] : a.in.rows;
+    for (int64_t at = blockIdx.x / team.size; at < rows; at += step) {
+        const int64_t row = a.left ? a.left[1 + at] : at;
         __syncthreads();
         if (threadIdx.x == 0) sh.listed = 0;
         const float given = a.temperature ? a.temperature[row] : a.temperature_all;
@@ -1150,6 +1176,609 @@ __global__ void __launch_bounds__(kThreads, 3) sample_kernel(SampleArgs a, int S
 }
 
 // ---------------------------------------------------------------------------
+// Many rows: a scan that lists each row's candidates, then a kernel that
+// finishes the rows from their lists.
+//
+// A row's vectors are dealt to `parts` CTAs in chunks of one vector per thread
+// (chunk c to part c mod parts, so that tokens sorted by frequency spread
+// evenly). A part keeps its maximum, its sum and its candidates: the elements
+// at or above a threshold below which at least `take` of its threads' maxima
+// do not lie. No part waits for another, so that the scan runs at the memory's
+// pace. The finish accepts a list where its last wanted entry reaches every
+// part's threshold: then nothing unlisted could have come before it. Rows that
+// fail (or whose ties overflow a list) go to the cluster's kernel below, by
+// the list `left`.
+// ---------------------------------------------------------------------------
+struct PartState {
+    double sum;
+    float best;
+    float tau;     // everything at or above it is listed
+    int count;
+    int unused;
+};
+struct ScanState {
+    PartState* parts;    // [rows, parts]
+    uint64_t* lists;     // [rows, parts, cap]
+    double* chunks;      // [rows, parts * kHold, kWarps]: sums of a warp's vectors of a chunk
+    int* left;           // [1 + rows]: the number of rows for the cluster's kernel, and which
+};
+struct ScanShape {
+    int parts;
+    int cap;
+};
+constexpr int kHold = 16;       // chunks of a part
+constexpr int kScanBins = 128;
+constexpr int kNucleus = 192;   // candidates listed for a top-p without a top-k
+
+__host__ __device__ __forceinline__ ScanState scan_of(void* space, int64_t rows, ScanShape sh, bool chunks) {
+    ScanState s;
+    char* p = static_cast<char*>(space);
+    s.parts = reinterpret_cast<PartState*>(p);
+    p += rows * sh.parts * static_cast<int64_t>(sizeof(PartState));
+    s.lists = reinterpret_cast<uint64_t*>(p);
+    p += rows * sh.parts * sh.cap * 8;
+    s.chunks = reinterpret_cast<double*>(p);
+    if (chunks) p += rows * sh.parts * kHold * kWarps * 8;
+    s.left = reinterpret_cast<int*>(p);
+    return s;
+}
+
+// What a row needs of the scan.
+struct Plan {
+    int take;       // candidates; 0: none, or all from `low` on
+    bool sum;       // its mass in 64 bits
+    bool chunks;    // and that of each chunk
+    bool by_low;    // candidates are what reaches maximum + low
+    float temperature;
+    double low;     // T ln(min_p), at most 0
+    int k;          // 0: no cut by rank
+    double p, q;
+    bool left;      // the cluster's kernel takes the row
+};
+
+__device__ __forceinline__ Plan plan_of(const SampleArgs& a, int64_t row) {
+    Plan r;
+    const float given = a.temperature ? a.temperature[row] : a.temperature_all;
+    r.temperature = given > FLT_MAX ? FLT_MAX : given;
+    const int k = a.top_k ? a.top_k[row] : a.top_k_all;
+    r.p = static_cast<double>(a.top_p ? a.top_p[row] : a.top_p_all);
+    const float q_given = a.min_p ? a.min_p[row] : a.min_p_all;
+    r.q = q_given > 1.0f ? 1.0 : static_cast<double>(q_given);
+    r.k = k > 0 && k < a.in.V ? k : 0;
+    const bool greedy = !(given > 0.0f) || k == 1 || r.p <= 0.0;
+    const bool by_p = r.p < 1.0, by_q = r.q > 0.0;
+    r.low = by_q && !greedy ? static_cast<double>(r.temperature) * log(r.q) : -HUGE_VAL;
+    r.take = greedy ? 1 : r.k > 0 ? r.k : by_p ? kNucleus : 0;
+    if (greedy) r.k = 1;
+    r.sum = !greedy && r.k == 0 && (by_p || !by_q);
+    r.chunks = r.sum && !by_p;
+    // the mass of the first k needs all of them, whatever min_p leaves of them
+    r.by_low = by_q && !greedy && (r.k == 0 || !by_p);
+    r.left = r.k > kSampleList;
+    return r;
+}
+__device__ __forceinline__ Plan plan_of(const TopArgs& a, int64_t) {
+    Plan r = {};
+    r.take = r.k = a.n;
+    r.temperature = a.temperature;
+    return r;
+}
+
+template <class E, class Args, bool kTop>
+__global__ void __launch_bounds__(kThreads, 3) scan_kernel(Args a, ScanShape shape, void* space, bool with_chunks) {
+    constexpr int kVec = Elem<E>::kVec;
+    extern __shared__ uint4 dyn[];
+    __shared__ float2 part8[kWarps];
+    __shared__ float low8[kWarps];
+    __shared__ double d8[kWarps];
+    __shared__ __align__(16) int hist[kScanBins];
+    __shared__ int listed;
+    const ScanState state = scan_of(space, a.in.rows, shape, with_chunks);
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, V = a.in.V;
+    const uint4 none = vneg_inf<E>();
+    uint4* buf = dyn + tid;    // this thread's vectors, kThreads apart
+    const int64_t items = a.in.rows * shape.parts;
+    const int per = ((V + kVec - 2) / kVec + 1 + kThreads * shape.parts - 1) / (kThreads * shape.parts);   // chunks of a part
+    if (blockIdx.x == 0 && tid == 0) state.left[0] = 0;
+    auto copy = [&](int64_t item) {
+        const int64_t row = item / shape.parts;
+        const int part = static_cast<int>(item - row * shape.parts);
+        const E* x = static_cast<const E*>(a.in.x) + row * a.in.stride;
+        const int phase = static_cast<int>((reinterpret_cast<uintptr_t>(x) & 15u) / sizeof(E));
+        const uint4* src = reinterpret_cast<const uint4*>(reinterpret_cast<uintptr_t>(x) & ~static_cast<uintptr_t>(15));
+        const int v0 = phase > 0 ? 1 : 0, v1 = (V + phase) / kVec;
+        for (int i = 0, v = part * kThreads + tid; i < per; ++i, v += shape.parts * kThreads) {
+            if (v >= v0 && v < v1) {
+                copy_async(buf + i * kThreads, src + v);
+            } else {
+                float f[kVec];   // a ragged end of the row, or behind it
+#pragma unroll
+                for (int e = 0; e < kVec; ++e) {
+                    const int64_t token = static_cast<int64_t>(v) * kVec + e - phase;
+                    f[e] = token >= 0 && token < V ? Elem<E>::widen(x[token]) : neg_inf();
+                }
+                buf[i * kThreads] = Elem<E>::pack(f);
+            }
+        }
+        copies_commit();
+    };
+    if (blockIdx.x < items) copy(blockIdx.x);
+    for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
+        const int64_t row = item / shape.parts;
+        const int part = static_cast<int>(item - row * shape.parts);
+        const Plan plan = plan_of(a, row);
+        const uintptr_t x = reinterpret_cast<uintptr_t>(static_cast<const E*>(a.in.x) + row * a.in.stride);
+        const int phase = static_cast<int>((x & 15u) / sizeof(E));
+        if (tid < kScanBins) hist[tid] = 0;
+        if (tid == 0) listed = 0;
+        copies_wait<0>();
+        uint4 top = none;
+        for (int i = 0; i < per; ++i) top = vmax<E>(top, buf[i * kThreads]);
+        const float mine = lanes_max<E>(top);
+        float sum = 0.0f;
+        if (kTop) {
+            // the thread's exponentials by its own maximum
+            const float c2 = fminf(1.4426950408889634f / plan.temperature, FLT_MAX);
+            const float from = mine > neg_inf() ? -mine : 0.0f;
+            const float2 ff = make_float2(from, from), cc = make_float2(c2, c2);
+            float2 p = make_float2(0.0f, 0.0f);
+#pragma unroll 4
+            for (int i = 0; i < per; ++i) {
+                float f[kVec];
+                Elem<E>::unpack(vmax<E>(buf[i * kThreads], none), f);
+#pragma unroll
+                for (int e = 0; e < kVec; e += 2) {
+                    const float2 t = mul2(add2(make_float2(f[e], f[e + 1]), ff), cc);
+                    p = add2(p, make_float2(ex2(t.x), ex2(t.y)));
+                }
+            }
+            sum = p.x + p.y;
+        }
+        float2 of_warp = make_float2(mine, 0.0f);
+        float least = mine > neg_inf() ? mine : FLT_MAX;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            of_warp.x = fmaxf(of_warp.x, __shfl_xor_sync(kAll, of_warp.x, o));
+            least = fminf(least, __shfl_xor_sync(kAll, least, o));
+        }
+        if (kTop) {
+            const float c2 = fminf(1.4426950408889634f / plan.temperature, FLT_MAX);
+            of_warp.y = sum == 0.0f ? 0.0f : sum * share(mine, of_warp.x, c2);
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) of_warp.y += __shfl_xor_sync(kAll, of_warp.y, o);
+        }
+        if (lane == 0) {
+            part8[warp] = of_warp;
+            low8[warp] = least;
+        }
+        __syncthreads();
+        float best = part8[0].x;
+        least = low8[0];
+#pragma unroll
+        for (int w = 1; w < kWarps; ++w) {
+            best = fmaxf(best, part8[w].x);
+            least = fminf(least, low8[w]);
+        }
+        float tau = HUGE_VALF;   // nothing is listed
+        if (plan.take > 0 && !plan.left) {
+            // how many of the threads' maxima to pass: the part's share, and
+            // three times the spread of such shares
+            const float mean = static_cast<float>(plan.take) / static_cast<float>(shape.parts);
+            const int want = static_cast<int>(ceilf(mean + 3.0f * sqrtf(mean))) + (shape.parts > 1 ? 2 : 0);
+            const float span = fmaxf(best - least, 1.0e-30f);
+            const float scale = static_cast<float>(kScanBins - 1) / span;
+            if (mine > neg_inf()) atomicAdd(&hist[min(kScanBins - 1, static_cast<int>((best - mine) * scale))], 1);
+            __syncthreads();
+            const int4 four = reinterpret_cast<const int4*>(hist)[lane];
+            int run = four.x + four.y + four.z + four.w;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int up = __shfl_up_sync(kAll, run, o);
+                if (lane >= o) run += up;
+            }
+            int bin = kScanBins;   // the first bin up to which there are enough
+            const int before = run - (four.x + four.y + four.z + four.w);
+            if (run >= want) {
+                bin = 4 * lane;
+                int sum4 = before + four.x;
+                if (sum4 < want) { ++bin; sum4 += four.y; }
+                if (sum4 < want) { ++bin; sum4 += four.z; }
+                if (sum4 < want) ++bin;
+            }
+            bin = __reduce_min_sync(kAll, bin);
+            tau = bin < kScanBins - 1 && best < FLT_MAX ? best - static_cast<float>(bin + 1) / scale : neg_inf();
+        }
+        if (plan.by_low && !plan.left) {
+            const float low = __double2float_rd(static_cast<double>(best) + plan.low);
+            tau = plan.take > 0 ? fmaxf(tau, low) : low;
+        }
+        double mass = 0.0;
+        if (!kTop && plan.sum && best > neg_inf()) {
+            const Weights weight(best, plan.temperature);
+            for (int i = 0; i < per; ++i) {
+                float f[kVec];
+                Elem<E>::unpack(buf[i * kThreads], f);
+                double w = 0.0;
+#pragma unroll
+                for (int e = 0; e < kVec; ++e) w += weight(f[e]);
+                mass += w;
+                if (plan.chunks) {
+#pragma unroll
+                    for (int o = 16; o > 0; o >>= 1) w += __shfl_xor_sync(kAll, w, o);
+                    if (lane == 0)
+                        state.chunks[(row * shape.parts * kHold + i * shape.parts + part) * kWarps + warp] = w;
+                }
+            }
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) mass += __shfl_xor_sync(kAll, mass, o);
+            if (lane == 0) d8[warp] = mass;
+        }
+        // The warp looks through the vectors of each of its threads whose
+        // maximum reaches tau, an element per lane.
+        uint64_t* list = state.lists + item * shape.cap;
+        const E* elems = reinterpret_cast<const E*>(dyn);
+        for (unsigned have = __ballot_sync(kAll, mine >= tau && mine > neg_inf()); have; have &= have - 1) {
+            const int owner = warp * 32 + __ffs(have) - 1;
+            for (int at = lane; at < per * kVec; at += 32) {
+                const int i = at / kVec, e = at % kVec;
+                const float v = Elem<E>::widen(elems[(i * kThreads + owner) * kVec + e]);
+                if (v >= tau && v > neg_inf()) {
+                    const int place = atomicAdd(&listed, 1);
+                    if (place < shape.cap)
+                        list[place] = entry(v, ((i * shape.parts + part) * kThreads + owner) * kVec + e - phase);
+                }
+            }
+        }
+        __syncthreads();
+        if (tid == 0) {
+            PartState out = {0.0, best, tau, listed, 0};
+            if (kTop) {
+                const float c2 = fminf(1.4426950408889634f / plan.temperature, FLT_MAX);
+                float all = 0.0f;
+                for (int w = 0; w < kWarps; ++w)
+                    all += part8[w].y == 0.0f ? 0.0f : part8[w].y * share(part8[w].x, best, c2);
+                out.sum = static_cast<double>(all);
+            } else if (plan.sum && best > neg_inf()) {
+                for (int w = 0; w < kWarps; ++w) out.sum += d8[w];
+            }
+            state.parts[item] = out;
+        }
+        if (item + gridDim.x < items) copy(item + gridDim.x);
+        __syncthreads();   // listed and the bins are free again
+    }
+}
+
+// The parts' lists in `keys`, best first; how many entries, and from which
+// value on none is missing. -1: a list overflowed.
+struct Gathered {
+    int count;
+    int whole;     // of them, those that reach every part's threshold
+    float best;
+    float tau;     // the highest of the parts' thresholds
+    bool all;      // every element above -inf is there
+};
+template <int kT>
+__device__ Gathered gather_parts(const ScanState& state, ScanShape shape, int64_t row, uint64_t* keys, uint64_t* other,
+                                 int* places, int* counters) {
+    const PartState* parts = state.parts + row * shape.parts;
+    Gathered g = {0, 0, neg_inf(), neg_inf(), true};
+    float tau = neg_inf();
+    bool over = false;
+    for (int s = 0; s < shape.parts; ++s) {
+        const PartState p = parts[s];
+        if (threadIdx.x == 0) places[s] = g.count;
+        over = over || p.count > shape.cap;
+        g.count += min(p.count, shape.cap);
+        g.best = fmaxf(g.best, p.best);
+        if (p.best > neg_inf()) tau = fmaxf(tau, p.tau);
+    }
+    g.all = !(tau > neg_inf());
+    g.tau = tau;
+    if (over) {
+        g.count = -1;
+        return g;
+    }
+    if (threadIdx.x == 0) counters[0] = 0;
+    __syncthreads();
+    // a part's entries by a warp
+    for (int s = threadIdx.x / 32; s < shape.parts; s += kT / 32) {
+        const uint64_t* list = state.lists + (row * shape.parts + s) * shape.cap;
+        for (int i = threadIdx.x % 32; i < parts[s].count; i += 32) other[places[s] + i] = list[i];
+    }
+    __syncthreads();
+    // in order, by counting the better ones
+    int whole = 0;
+    for (int i = threadIdx.x; i < g.count; i += kT) {
+        const uint64_t mine = other[i];
+        int rank = 0;
+        int j = 0;
+        for (; j + 2 <= g.count; j += 2) {
+            const ulonglong2 two = *reinterpret_cast<const ulonglong2*>(other + j);
+            rank += (two.x > mine ? 1 : 0) + (two.y > mine ? 1 : 0);
+        }
+        if (j < g.count) rank += other[j] > mine ? 1 : 0;
+        keys[rank] = mine;
+        whole += entry_value(mine) >= tau ? 1 : 0;
+    }
+    whole = __reduce_add_sync(kAll, whole);
+    if (threadIdx.x % 32 == 0) atomicAdd(&counters[0], whole);
+    __syncthreads();
+    g.whole = counters[0];
+    return g;
+}
+
+constexpr int kFinish = 128;   // threads of a finishing CTA
+
+__global__ void __launch_bounds__(kFinish) top_finish_kernel(TopArgs a, ScanShape shape, void* space) {
+    extern __shared__ uint64_t keys_space[];
+    __shared__ int places[64];
+    __shared__ int counters[1];
+    const ScanState state = scan_of(space, a.in.rows, shape, false);
+    uint64_t* keys = keys_space;
+    uint64_t* other = keys + shape.parts * shape.cap;
+    const int n = a.n;
+    const double c = static_cast<double>(fminf(1.4426950408889634f / a.temperature, FLT_MAX));
+    for (int64_t row = blockIdx.x; row < a.in.rows; row += gridDim.x) {
+        const Gathered g = gather_parts<kFinish>(state, shape, row, keys, other, places, counters);
+        if (g.count < 0 || (!g.all && g.whole < n) || !(g.best < HUGE_VALF)) {
+            if (threadIdx.x == 0) state.left[1 + atomicAdd(&state.left[0], 1)] = static_cast<int>(row);
+            __syncthreads();
+            continue;
+        }
+        double Z = 0.0;
+        for (int s = 0; s < shape.parts; ++s) {
+            const PartState p = state.parts[row * shape.parts + s];
+            if (p.sum != 0.0)
+                Z += p.sum * (p.best == g.best ? 1.0 : exp2(c * (static_cast<double>(p.best) - static_cast<double>(g.best))));
+        }
+        const double log_z = log(Z);
+        for (int i = threadIdx.x; i < n; i += kFinish) {
+            float value = neg_inf();
+            int token = -1;
+            if (i < g.count) {
+                token = entry_token(keys[i]);
+                value = static_cast<float>((static_cast<double>(entry_value(keys[i])) - static_cast<double>(g.best)) /
+                                               static_cast<double>(a.temperature) - log_z);
+            }
+            a.log_probs[row * n + i] = value;
+            a.tokens[row * n + i] = token;
+        }
+        __syncthreads();
+    }
+}
+
+template <class E>
+__global__ void __launch_bounds__(kFinish) sample_finish_kernel(SampleArgs a, ScanShape shape, void* space) {
+    constexpr int kVec = Elem<E>::kVec;
+    constexpr int kW = kFinish / 32;
+    extern __shared__ uint64_t keys_space[];
+    __shared__ int places[64];
+    __shared__ int counters[1];
+    __shared__ double d8[kW];
+    __shared__ int i8[kW];
+    const ScanState state = scan_of(space, a.in.rows, shape, true);
+    uint64_t* keys = keys_space;
+    uint64_t* other = keys + shape.parts * shape.cap;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    auto total_of = [&](double v) {
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(kAll, v, o);
+        if (lane == 0) d8[warp] = v;
+        __syncthreads();
+        v = 0.0;
+        for (int w = 0; w < kW; ++w) v += d8[w];
+        __syncthreads();
+        return v;
+    };
+    auto before_of = [&](double v) {   // the sum of the threads before this one
+        double incl = v;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const double up = __shfl_up_sync(kAll, incl, o);
+            if (lane >= o) incl += up;
+        }
+        if (lane == 31) d8[warp] = incl;
+        __syncthreads();
+        double base = 0.0;
+        for (int w = 0; w < warp; ++w) base += d8[w];
+        __syncthreads();
+        const double excl = __shfl_up_sync(kAll, incl, 1);
+        return base + (lane == 0 ? 0.0 : excl);
+    };
+    auto over_ints = [&](int v, auto op) {
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) v = op(v, __shfl_xor_sync(kAll, v, o));
+        if (lane == 0) i8[warp] = v;
+        __syncthreads();
+        v = i8[0];
+        for (int w = 1; w < kW; ++w) v = op(v, i8[w]);
+        __syncthreads();
+        return v;
+    };
+    for (int64_t row = blockIdx.x; row < a.in.rows; row += gridDim.x) {
+        const Plan plan = plan_of(a, row);
+        const double u = static_cast<double>(a.uniforms[row]);
+        const PartState* parts = state.parts + row * shape.parts;
+        int32_t* out = a.tokens + row;
+        auto leave = [&]() {
+            if (tid == 0) state.left[1 + atomicAdd(&state.left[0], 1)] = static_cast<int>(row);
+            __syncthreads();
+        };
+        if (plan.left) {
+            leave();
+            continue;
+        }
+        float best = neg_inf();
+        for (int s = 0; s < shape.parts; ++s) best = fmaxf(best, parts[s].best);
+        if (!(best > neg_inf())) {
+            if (tid == 0) *out = -1;
+            continue;
+        }
+        const double T = static_cast<double>(plan.temperature), m = static_cast<double>(best);
+        if (best > FLT_MAX && plan.take != 1) {   // the cluster's kernel knows infinities
+            leave();
+            continue;
+        }
+        double W = 0.0;
+        if (plan.sum)
+            for (int s = 0; s < shape.parts; ++s)
+                if (parts[s].sum != 0.0)
+                    W += parts[s].sum * (parts[s].best == best ? 1.0 : exp((static_cast<double>(parts[s].best) - m) / T));
+        if (plan.chunks) {
+            // temperature alone: the first stretch of 32 vectors at which the
+            // running sum passes the target, then the element in it
+            const double target = u < 1.0 ? u * W : HUGE_VAL;
+            const int stretches = shape.parts * kHold * kWarps;
+            const int per = ((a.in.V + kVec - 2) / kVec + 1 + kThreads * shape.parts - 1) / (kThreads * shape.parts);
+            const int used = per * shape.parts * kWarps;
+            const double* sums = state.chunks + row * stretches;
+            const int each = (used + kFinish - 1) / kFinish;
+            const int begin = min(used, each * tid), end = min(used, begin + each);
+            auto stretch = [&](int i) {
+                const int s = i / kWarps % shape.parts;
+                if (!(parts[s].best > neg_inf())) return 0.0;
+                const double v = sums[i];
+                return v == 0.0 || parts[s].best == best ? v : v * exp((static_cast<double>(parts[s].best) - m) / T);
+            };
+            double mine = 0.0;
+            for (int i = begin; i < end; ++i) mine += stretch(i);
+            double run = before_of(mine);
+            int first = used, last = -1;
+            double first_run = 0.0, last_run = 0.0;
+            for (int i = begin; i < end; ++i) {
+                const double v = stretch(i);
+                if (v > 0.0) {
+                    last = i;
+                    last_run = run;
+                    if (first == used && run + v > target) {
+                        first = i;
+                        first_run = run;
+                    }
+                }
+                run += v;
+            }
+            const int first_all = over_ints(first, Min()), last_all = over_ints(last, Max());
+            const int chosen = first_all < used ? first_all : last_all;
+            if ((first_all < used && first == chosen) || (first_all >= used && last == chosen)) {
+                if (chosen >= 0) {
+                    d8[0] = first_all < used ? first_run : last_run;
+                    counters[0] = chosen;
+                }
+            }
+            __syncthreads();
+            if (warp == 0) {
+                const int at = counters[0];
+                double base = d8[0];
+                const E* x = static_cast<const E*>(a.in.x) + row * a.in.stride;
+                const int phase = static_cast<int>((reinterpret_cast<uintptr_t>(x) & 15u) / sizeof(E));
+                const int64_t start = (static_cast<int64_t>(at / kWarps) * kThreads + at % kWarps * 32 + lane) * kVec - phase;
+                const Weights weight(best, plan.temperature);
+                double w[kVec], own = 0.0;
+#pragma unroll
+                for (int e = 0; e < kVec; ++e) {
+                    const int64_t token = start + e;
+                    float v = token >= 0 && token < a.in.V ? Elem<E>::widen(x[token]) : neg_inf();
+                    w[e] = weight(v == v ? v : neg_inf());
+                    own += w[e];
+                }
+                double incl = own;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const double up = __shfl_up_sync(kAll, incl, o);
+                    if (lane >= o) incl += up;
+                }
+                const double up = __shfl_up_sync(kAll, incl, 1);
+                double at_run = base + (lane == 0 ? 0.0 : up);
+                int hit = 0x7FFFFFFF, end_token = -1;
+#pragma unroll
+                for (int e = 0; e < kVec; ++e) {
+                    at_run += w[e];
+                    if (w[e] > 0.0) {
+                        end_token = static_cast<int>(start) + e;
+                        if (hit == 0x7FFFFFFF && at_run > target) hit = end_token;
+                    }
+                }
+                hit = __reduce_min_sync(kAll, hit);
+                end_token = __reduce_max_sync(kAll, end_token);
+                if (lane == 0) *out = hit < 0x7FFFFFFF ? hit : end_token;
+            }
+            __syncthreads();
+            continue;
+        }
+        const Gathered g = gather_parts<kFinish>(state, shape, row, keys, other, places, counters);
+        if (g.count < 0) {
+            leave();
+            continue;
+        }
+        if (plan.take == 1) {
+            if (tid == 0) *out = entry_token(keys[0]);
+            __syncthreads();
+            continue;
+        }
+        // the first k, or as many as are known
+        const int whole = g.all ? g.count : g.whole;
+        const int count = plan.k > 0 ? min(plan.k, whole) : whole;
+        // Is what lies behind the known ranks out? By rank; as everything that
+        // reaches m + T ln q is known; or as p or q cut within the known ones.
+        // The mass that p goes by is the row's, or that of the first k.
+        const bool mass_known = plan.k == 0 || !(plan.p < 1.0);
+        const bool enough = g.all || (plan.k > 0 && whole >= plan.k) ||
+                            (mass_known && plan.q > 0.0 && static_cast<double>(g.tau) <= m + plan.low);
+        double* weight = reinterpret_cast<double*>(other);
+        const int each = (count + kFinish - 1) / kFinish;
+        const int begin = min(count, each * tid), end = min(count, begin + each);
+        double mine = 0.0;
+        auto z_of = [&](int i) {
+            const float x = entry_value(keys[i]);
+            return x == best ? 0.0 : (static_cast<double>(x) - m) / T;
+        };
+        for (int i = begin; i < end; ++i) {
+            const double z = z_of(i);
+            weight[i] = z < -708.0 ? 0.0 : exp(z);
+            mine += weight[i];
+        }
+        const double listed_mass = total_of(mine);
+        if (plan.k > 0) W = listed_mass;
+        double run = before_of(mine);
+        const double log_q = plan.q > 0.0 ? log(plan.q) : -HUGE_VAL;
+        int keep = 0;
+        bool cut = false;   // p or q has cut within what is known
+        for (int i = begin; i < end; ++i) {
+            const bool in = i == 0 || ((!(plan.p < 1.0) || run < plan.p * W) && z_of(i) >= log_q);
+            keep += in ? 1 : 0;
+            cut = cut || !in;
+            run += weight[i];
+        }
+        keep = over_ints(keep, Add());
+        // without a top-k, the rank behind the last known one has to be out as well
+        if (plan.p < 1.0 && plan.k == 0 && !(listed_mass < plan.p * W)) cut = true;
+        const bool settled = __syncthreads_or(cut && mass_known) || enough;
+        if (!settled) {
+            leave();
+            continue;
+        }
+        mine = 0.0;
+        for (int i = begin; i < min(end, keep); ++i) mine += weight[i];
+        const double kept = total_of(mine);
+        const double target = u < 1.0 ? u * kept : HUGE_VAL;
+        int first = 0x7FFFFFFF, last = -1;
+        for (int i = tid; i < keep; i += kFinish) {
+            const int own = entry_token(keys[i]);
+            double sum = 0.0;
+            for (int j = 0; j < keep; ++j) sum += entry_token(keys[j]) <= own ? weight[j] : 0.0;
+            if (weight[i] > 0.0) {
+                last = max(last, own);
+                if (sum > target) first = min(first, own);
+            }
+        }
+        first = over_ints(first, Min());
+        last = over_ints(last, Max());
+        if (tid == 0) *out = first < 0x7FFFFFFF ? first : last;
+        __syncthreads();
+    }
+}
+
+// ---------------------------------------------------------------------------
 // Distillation
 // ---------------------------------------------------------------------------
 // What a call keeps of its rows between its kernels (and for a backward).
@@ -1187,11 +1816,6 @@ __host__ __device__ __forceinline__ DistillState state_of(const DistillArgs& a) 
 __device__ __forceinline__ int64_t teacher_token(const DistillArgs& a, int64_t at) {
     return a.token_bytes == 8 ? static_cast<const int64_t*>(a.teacher_tokens)[at]
                               : static_cast<int64_t>(static_cast<const int32_t*>(a.teacher_tokens)[at]);
-}
-
-// 2^(c2 (x - best)) for x <= best; 0 where nothing is above -inf.
-__device__ __forceinline__ float share(float x, float best, float c2) {
-    return best > neg_inf() || best != best ? ex2((x - best) * c2) : 0.0f;
 }
 
 template <class T, class Op>
@@ -1357,24 +1981,6 @@ __global__ void __launch_bounds__(256) slots_kernel(DistillArgs a, uint32_t mask
     }
 }
 
-__device__ __forceinline__ void copy_async(uint4* to, const uint4* from) {
-    asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16;" ::"r"(
-                     static_cast<uint32_t>(__cvta_generic_to_shared(to))),
-                 "l"(from)
-                 : "memory");
-}
-__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int kLeft>
-__device__ __forceinline__ void copies_wait() {
-    asm volatile("cp.async.wait_group %0;" ::"n"(kLeft) : "memory");
-}
-// The cluster's barrier for threads that have nothing to show: their stores
-// need not have landed.
-__device__ __forceinline__ void cluster_arrive_relaxed() { asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory"); }
-__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
-__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
-
-constexpr int kHold = 16;   // vectors of a slice per thread
 struct DistillShared {
     float2 box[2][kMaxCluster];   // reference and sum of the CTAs' slices
     float2 part[kWarps];          // and of the warps' vectors
@@ -1892,7 +2498,82 @@ cudaError_t launch_distill_any(const DistillArgs& a, cudaStream_t stream) {
 
 }  // namespace
 
-cudaError_t launch_sample(const SampleArgs& a, cudaStream_t stream) {
+namespace {
+
+// Rows from which the scan is worth its three launches, and the least of a row
+// that it is worth for.
+constexpr int64_t kScanRows = 32;
+constexpr int kScanVocab = 8192;
+constexpr int kScanTop = 256;   // longer lists are ordered faster in the cluster's kernel
+
+// Parts of at most 16 chunks; more of them where the rows are few or the lists
+// long (a list of its part's share should take less than half of its threads).
+ScanShape scan_shape(const Rows& in, int es, int take) {
+    const int chunk = kThreads * 16 / es;
+    const int chunks = (in.V + 16 / es - 1 + chunk - 1) / chunk;
+    int parts = (chunks + kHold - 1) / kHold;
+    while (parts < chunks && parts < 64 && (parts * 100 < take || in.rows * parts < 148 * 2)) ++parts;
+    const float mean = static_cast<float>(take) / static_cast<float>(parts);
+    const int cap = (static_cast<int>(4.0f * mean + 12.0f * sqrtf(mean)) + 96) / 2 * 2;
+    return ScanShape{parts, cap};
+}
+
+int sample_take(const SampleArgs& a) {
+    return a.top_k ? 128 : a.top_k_all > 0 ? std::min(a.top_k_all, kSampleList) : kNucleus;
+}
+
+int64_t scan_bytes(const Rows& in, ScanShape sh, bool chunks) {
+    return in.rows * (sh.parts * (static_cast<int64_t>(sizeof(PartState)) + sh.cap * 8LL +
+                                  (chunks ? kHold * kWarps * 8LL : 0LL)) + 4) + 64;
+}
+
+template <class E, class Args, bool kTop>
+cudaError_t launch_scan(const Args& a, ScanShape sh, bool chunks, cudaStream_t stream) {
+    Rows items = a.in;   // a CTA takes a part at a time
+    items.rows *= sh.parts;
+    return launch_rows(scan_kernel<E, Args, kTop>, items, 1, static_cast<size_t>(kThreads) * kHold * 16, stream,
+                       kThreads, a, sh, a.space, chunks);
+}
+
+template <class Kernel, class Args>
+cudaError_t launch_finish(Kernel kernel, const Args& a, ScanShape sh, cudaStream_t stream) {
+    const size_t smem = static_cast<size_t>(sh.parts) * sh.cap * 16;
+    return launch_rows(kernel, a.in, 1, smem, stream, kFinish, a, sh, a.space);
+}
+
+}  // namespace
+
+int64_t sample_space(const SampleArgs& a) {
+    if (a.in.rows < kScanRows || a.in.V < kScanVocab) return 0;
+    return scan_bytes(a.in, scan_shape(a.in, element_size(a.in.dtype), sample_take(a)), true);
+}
+
+int64_t top_space(const TopArgs& a) {
+    if (a.in.rows < kScanRows || a.in.V < kScanVocab || a.n > kScanTop) return 0;
+    return scan_bytes(a.in, scan_shape(a.in, element_size(a.in.dtype), a.n), false);
+}
+
+cudaError_t launch_sample(const SampleArgs& given, cudaStream_t stream) {
+    SampleArgs a = given;
+    if (sample_space(a) > 0) {
+        const ScanShape scan = scan_shape(a.in, element_size(a.in.dtype), sample_take(a));
+        cudaError_t err;
+        switch (a.in.dtype) {
+            case kF32:
+                err = launch_scan<float, SampleArgs, false>(a, scan, true, stream);
+                if (err == cudaSuccess) err = launch_finish(sample_finish_kernel<float>, a, scan, stream);
+                break;
+            case kF16:
+                err = launch_scan<__half, SampleArgs, false>(a, scan, true, stream);
+                if (err == cudaSuccess) err = launch_finish(sample_finish_kernel<__half>, a, scan, stream);
+                break;
+            default:
+                err = launch_scan<__nv_bfloat16, SampleArgs, false>(a, scan, true, stream);
+                if (err == cudaSuccess) err = launch_finish(sample_finish_kernel<__nv_bfloat16>, a, scan, stream);
+        }
+        if (err != cudaSuccess) return err;
+        a.left = scan_of(a.space, a.in.rows, scan, true).left;
+    }
     const int es = element_size(a.in.dtype);
     const Shape sh = shape_of(a.in, es, 68 * 1024);
     // lists for rows that may take that path, bins for the others
@@ -1905,7 +2586,17 @@ cudaError_t launch_sample(const SampleArgs& a, cudaStream_t stream) {
     }
 }
 
-cudaError_t launch_top(const TopArgs& a, cudaStream_t stream) {
+cudaError_t launch_top(const TopArgs& given, cudaStream_t stream) {
+    TopArgs a = given;
+    if (top_space(a) > 0) {
+        const ScanShape scan = scan_shape(a.in, element_size(a.in.dtype), a.n);
+        cudaError_t err = a.in.dtype == kF32   ? launch_scan<float, TopArgs, true>(a, scan, false, stream)
+                          : a.in.dtype == kF16 ? launch_scan<__half, TopArgs, true>(a, scan, false, stream)
+                                               : launch_scan<__nv_bfloat16, TopArgs, true>(a, scan, false, stream);
+        if (err == cudaSuccess) err = launch_finish(top_finish_kernel, a, scan, stream);
+        if (err != cudaSuccess) return err;
+        a.left = scan_of(a.space, a.in.rows, scan, false).left;
+    }
     const int es = element_size(a.in.dtype);
     const Shape sh = shape_of(a.in, es, 68 * 1024);
     const int cap = list_space(a.n);

@@ -524,6 +524,13 @@ def _rows_args(x: torch.Tensor):
     return _vp(x), _DTYPES[x.dtype], x.size(0), x.size(1), x.stride(0) if x.size(0) > 1 else x.size(1)
 
 
+def _workspace(query, x: torch.Tensor, n: int) -> Optional[torch.Tensor]:
+    """Device memory for what passes between a call's kernels, or None."""
+    size = ctypes.c_int64()
+    _check_global(query(_DTYPES[x.dtype], x.size(0), x.size(1), n, size), "workspace")
+    return torch.empty((size.value,), dtype=torch.uint8, device=x.device) if size.value else None
+
+
 def _beside(t: torch.Tensor, name: str, device: torch.device, dtype: torch.dtype, shape) -> torch.Tensor:
     """`t` broadcast to `shape`, contiguous on the logits' device; a tensor on another GPU is refused."""
     if t.is_cuda and t.device != device:
@@ -601,10 +608,11 @@ def sample(logits: torch.Tensor, uniforms: torch.Tensor, *, temperature=1.0, top
     x = _logits_rows(logits.to(device))
     u = _beside(uniforms, "uniforms", device, torch.float32, lead)
     tokens = torch.empty(lead, dtype=torch.int32, device=device)
+    k_all = min(int(k_all), _INT_MAX)
+    space = _workspace(_library().dbs_device_sample_workspace_bytes, x, k_all if k_rows is None else -1)
     with torch.cuda.device(device):
-        rc = _library().dbs_device_sample(*_rows_args(x), _vp(u), _vp(t_rows), t_all, _vp(k_rows),
-                                          min(int(k_all), _INT_MAX), _vp(p_rows), p_all, _vp(q_rows), q_all,
-                                          _vp(tokens), _stream_ptr(device))
+        rc = _library().dbs_device_sample(*_rows_args(x), _vp(u), _vp(t_rows), t_all, _vp(k_rows), k_all, _vp(p_rows),
+                                          p_all, _vp(q_rows), q_all, _vp(tokens), _vp(space), _stream_ptr(device))
     _check_global(rc, "sample")
     return tokens.to(logits.device)
 
@@ -626,9 +634,10 @@ def top_log_probs(logits: torch.Tensor, n: int, *, temperature: float = 1.0) -> 
     shape = (*logits.shape[:-1], int(n))
     log_probs = torch.empty(shape, dtype=torch.float32, device=device)
     tokens = torch.empty(shape, dtype=torch.int32, device=device)
+    space = _workspace(_library().dbs_device_top_log_probs_workspace_bytes, x, int(n))
     with torch.cuda.device(device):
         rc = _library().dbs_device_top_log_probs(*_rows_args(x), int(n), temperature, _vp(log_probs), _vp(tokens),
-                                                 _stream_ptr(device))
+                                                 _vp(space), _stream_ptr(device))
     _check_global(rc, "top_log_probs")
     return log_probs.to(logits.device), tokens.to(logits.device)
 

@@ -162,7 +162,10 @@ DBS_EXPORT int dbs_device_backward_sparse_noalloc(DBSDecoderHandle* handle, int 
  * r * row_stride elements (0 repeats one row); rows need no alignment beyond
  * their element's. A row holds at most 3000000 bytes. No handle: errors are
  * in dbs_last_global_error. No call allocates, waits or keeps state, so calls
- * may overlap on several streams and be captured into graphs. */
+ * may overlap on several streams and be captured into graphs, each with a
+ * workspace of its own: device memory, 16-byte aligned, of at least the bytes
+ * that the function beside the call names (NULL where that is 0), whose
+ * contents mean nothing before and after the call. */
 
 /* One token per row from uniform numbers in [0, 1). With m the row's maximum
  * (NaN counts as -inf) and weights w_i = exp((x_i - m) / temperature), 0 below
@@ -178,7 +181,11 @@ DBS_EXPORT int dbs_device_backward_sparse_noalloc(DBSDecoderHandle* handle, int 
 DBS_EXPORT int dbs_device_sample(const void* logits, int data_type, int64_t rows, int vocab_size, int64_t row_stride,
                                  const float* uniforms, const float* temperatures, float temperature,
                                  const int32_t* top_ks, int top_k, const float* top_ps, float top_p,
-                                 const float* min_ps, float min_p, int32_t* tokens, void* cuda_stream);
+                                 const float* min_ps, float min_p, int32_t* tokens, void* workspace,
+                                 void* cuda_stream);
+/* top_k: the call's, or -1 where it gives top_ks. */
+DBS_EXPORT int dbs_device_sample_workspace_bytes(int data_type, int64_t rows, int vocab_size, int top_k,
+                                                 int64_t* bytes);
 
 /* The n best tokens of each row (logit desc, token asc; NaN counts as -inf)
  * and their log-probs under softmax(logits / temperature): log_probs and
@@ -186,7 +193,9 @@ DBS_EXPORT int dbs_device_sample(const void* logits, int data_type, int64_t rows
  * -inf hold -inf and -1. */
 DBS_EXPORT int dbs_device_top_log_probs(const void* logits, int data_type, int64_t rows, int vocab_size,
                                         int64_t row_stride, int n, float temperature, float* log_probs,
-                                        int32_t* tokens, void* cuda_stream);
+                                        int32_t* tokens, void* workspace, void* cuda_stream);
+DBS_EXPORT int dbs_device_top_log_probs_workspace_bytes(int data_type, int64_t rows, int vocab_size, int n,
+                                                        int64_t* bytes);
 
 /* Distillation from a teacher's listed log-probs. teacher_tokens [rows, slots]
  * (int32 or int64: token_bytes 4 or 8) and teacher_log_probs [rows, slots],

@@ -118,8 +118,8 @@ def test_c_rows(libdbs, change, message):
     a = dict(logits=P, dtype=0, rows=1, V=16, stride=16)
     a.update(change)
     rows = (a["logits"], a["dtype"], a["rows"], a["V"], a["stride"])
-    refused(libdbs, libdbs.dbs_device_sample(*rows, P, None, 1.0, None, 0, None, 1.0, None, 0.0, P, None), message)
-    refused(libdbs, libdbs.dbs_device_top_log_probs(*rows, 1, 1.0, P, P, None), message)
+    refused(libdbs, libdbs.dbs_device_sample(*rows, P, None, 1.0, None, 0, None, 1.0, None, 0.0, P, P, None), message)
+    refused(libdbs, libdbs.dbs_device_top_log_probs(*rows, 1, 1.0, P, P, P, None), message)
     refused(libdbs, libdbs.dbs_device_distill(*rows, P, P, 4, 2, 1.0, 1, 1, 1.0, P, P, P, None, None), message)
     refused(libdbs, libdbs.dbs_device_distill_backward(*rows, P, P, 4, 2, 1.0, 1, 1, 1.0, P, P, 0, 0, P, None), message)
 
@@ -127,17 +127,27 @@ def test_c_rows(libdbs, change, message):
 def test_c_arguments(libdbs):
     rows = (P, 0, 1, 16, 16)
     sample = libdbs.dbs_device_sample
-    refused(libdbs, sample(*rows, None, None, 1.0, None, 0, None, 1.0, None, 0.0, P, None), "uniforms and tokens")
-    refused(libdbs, sample(*rows, P, None, -1.0, None, 0, None, 1.0, None, 0.0, P, None), "temperature")
-    refused(libdbs, sample(*rows, P, None, 1.0, None, -1, None, 1.0, None, 0.0, P, None), "top_k")
-    refused(libdbs, sample(*rows, P, None, 1.0, None, 0, None, 0.0, None, 0.0, P, None), "top_p")
-    refused(libdbs, sample(*rows, P, None, 1.0, None, 0, None, 1.0, None, 2.0, P, None), "min_p")
-    assert sample(None, 0, 0, 16, 16, None, None, 1.0, None, 0, None, 1.0, None, 0.0, None, None) == 0
+    refused(libdbs, sample(*rows, None, None, 1.0, None, 0, None, 1.0, None, 0.0, P, P, None), "uniforms and tokens")
+    refused(libdbs, sample(*rows, P, None, -1.0, None, 0, None, 1.0, None, 0.0, P, P, None), "temperature")
+    refused(libdbs, sample(*rows, P, None, 1.0, None, -1, None, 1.0, None, 0.0, P, P, None), "top_k")
+    refused(libdbs, sample(*rows, P, None, 1.0, None, 0, None, 0.0, None, 0.0, P, P, None), "top_p")
+    refused(libdbs, sample(*rows, P, None, 1.0, None, 0, None, 1.0, None, 2.0, P, P, None), "min_p")
+    assert sample(None, 0, 0, 16, 16, None, None, 1.0, None, 0, None, 1.0, None, 0.0, None, None, None) == 0
     top = libdbs.dbs_device_top_log_probs
-    refused(libdbs, top(*rows, 0, 1.0, P, P, None), "n must be")
-    refused(libdbs, top(*rows, 17, 1.0, P, P, None), "n must be")
-    refused(libdbs, top(*rows, 4, 0.0, P, P, None), "temperature")
-    refused(libdbs, top(*rows, 4, 1.0, None, P, None), "cannot be null")
+    refused(libdbs, top(*rows, 0, 1.0, P, P, None, None), "n must be")
+    refused(libdbs, top(*rows, 17, 1.0, P, P, None, None), "n must be")
+    refused(libdbs, top(*rows, 4, 0.0, P, P, None, None), "temperature")
+    refused(libdbs, top(*rows, 4, 1.0, None, P, None, None), "cannot be null")
+    wide = (P, 0, 64, 32000, 32000)      # the rows' own scan passes its lists on
+    refused(libdbs, sample(*wide, P, None, 1.0, None, 0, None, 1.0, None, 0.0, P, None, None), "workspace cannot be null")
+    refused(libdbs, sample(*wide, P, None, 1.0, None, 0, None, 1.0, None, 0.0, P, ODD, None), "workspace is not aligned")
+    refused(libdbs, top(*wide, 4, 1.0, P, P, None, None), "workspace cannot be null")
+    size = ctypes.c_int64()
+    for query in (libdbs.dbs_device_sample_workspace_bytes, libdbs.dbs_device_top_log_probs_workspace_bytes):
+        assert query(0, 64, 32000, 8, ctypes.byref(size)) == 0 and size.value > 0
+        assert query(0, 1, 32000, 8, ctypes.byref(size)) == 0 and size.value == 0
+        refused(libdbs, query(0, 64, 32000, 8, None), "bytes cannot be null")
+        refused(libdbs, query(9, 64, 32000, 8, ctypes.byref(size)), "data type")
     distill = libdbs.dbs_device_distill
     refused(libdbs, distill(*rows, None, P, 4, 2, 1.0, 1, 1, 1.0, P, P, P, None, None), "teacher_log_probs")
     refused(libdbs, distill(*rows, P, P, 2, 2, 1.0, 1, 1, 1.0, P, P, P, None, None), "token_bytes")
@@ -149,7 +159,6 @@ def test_c_arguments(libdbs):
     refused(libdbs, distill(*rows, P, P, 4, 2, 1.0, 1, 2, 1.0, P, P, None, None, None), "state cannot be null")
     refused(libdbs, distill(*rows, P, P, 4, 2, 1.0, 1, 2, 1.0, P, P, ODD, None, None), "state is not aligned")
     refused(libdbs, distill(P, 0, 1, 260_001, 260_001, P, P, 4, 2, 1.0, 1, 2, 1.0, P, P, P, None, None), "at most 1040000 bytes")
-    size = ctypes.c_int64()
     assert libdbs.dbs_device_distill_state_bytes(3, 5, ctypes.byref(size)) == 0 and size.value >= 3 * 5 * 8
     assert libdbs.dbs_device_distill_state_bytes(3, 0, ctypes.byref(size)) == -1
     assert libdbs.dbs_device_distill_state_bytes(-1, 5, ctypes.byref(size)) == -1

@@ -52,14 +52,14 @@ SETTINGS = [
 
 @pytest.mark.parametrize("settings", SETTINGS, ids=str)
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("N,V", [(3, 1), (5, 2), (4, 7), (17, 100), (9, 999), (6, 32000), (3, 50257)])
+@pytest.mark.parametrize("N,V", [(3, 1), (5, 2), (4, 7), (17, 100), (9, 999), (6, 32000), (3, 50257), (40, 32000), (33, 50257), (35, 8193)])
 def test_sample(N, V, dtype, settings):
     seed = N * 31 + V
     check_sample(rows(N, V, dtype, seed), uniforms(N, seed), **settings)
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("N,V", [(40, 4096), (150, 1023), (400, 130)])
+@pytest.mark.parametrize("N,V", [(40, 4096), (150, 1023), (400, 130), (130, 9001), (300, 32000)])
 def test_sample_settings_of_each_row(N, V, dtype):
     g = torch.Generator().manual_seed(N)
     x, u = rows(N, V, dtype, N), uniforms(N, N)
@@ -77,8 +77,8 @@ def test_sample_settings_of_each_row(N, V, dtype):
 
 @pytest.mark.parametrize("settings", SETTINGS, ids=str)
 @pytest.mark.parametrize("dtype", DTYPES)
-def test_sample_ties_and_masks(dtype, settings):
-    V = 5000
+@pytest.mark.parametrize("V,times", [(5000, 1), (9001, 3)])
+def test_sample_ties_and_masks(V, times, dtype, settings):
     g = torch.Generator().manual_seed(5)
     x = torch.round(rows(12, V, torch.float32, 5))            # many equal values
     x[0] = 0.0                                                # all equal
@@ -94,14 +94,14 @@ def test_sample_ties_and_masks(dtype, settings):
     x[9] = torch.where(torch.rand(V, generator=g) < 0.5, -math.inf, 4.0)
     x[10] = torch.arange(V, 0, -1) / 100.0                    # in order
     x[11] = torch.where(torch.arange(V) < 300, 2.0, 1.0)
-    x = x.to(dtype)
+    x = x.to(dtype).repeat(times, 1)
     for u in (0.0, 0.25, 0.5, 1.0 - 2.0 ** -24, 1.0):
-        check_sample(x, torch.full((12,), u), **settings)
-    check_sample(x, uniforms(12, 3), **settings)
+        check_sample(x, torch.full((12 * times,), u), **settings)
+    check_sample(x, uniforms(12 * times, 3), **settings)
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("N", [1, 30])
+@pytest.mark.parametrize("N", [1, 30, 50])
 def test_sample_more_equal_values_than_a_list_holds(dtype, N):
     x = torch.zeros(N, 32003)
     x[:, 20000:20020] = 1.0
@@ -112,6 +112,10 @@ def test_sample_more_equal_values_than_a_list_holds(dtype, N):
 
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_sample_views(dtype):
+    wide = rows(80, 8801, dtype, 8).cuda().view(40, 2, 8801)
+    for view in (wide[:, -1], wide[:, 0, 1:], wide[:, 1, 3:-2], wide[1, 1].expand(40, 8801)):
+        check_sample(view.cpu(), uniforms(40, 9), k=20, p=0.9, dev=view)
+        check_sample(view.cpu(), uniforms(40, 9), dev=view)
     big = rows(6 * 3, 700, dtype, 8).cuda().view(6, 3, 700)
     u = uniforms(6, 8)
     for view in (big[:, -1, :], big[:, 1, 1:], big[:, 0, 5:-3], big[:, 0, :1].expand(6, 1), big[0, 0, :].expand(6, 700),
@@ -158,7 +162,8 @@ def check_top(x, n, temperature=1.0, dev=None):
 
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("N,V,n", [(3, 1, 1), (4, 7, 7), (5, 100, 20), (20, 1025, 1024), (2, 32000, 1), (7, 32000, 64), (300, 2000, 33),
-                                   (2, 50257, 1000), (1, 128256, 128), (2, 256000, 256)])
+                                   (2, 50257, 1000), (1, 128256, 128), (2, 256000, 256),
+                                   (40, 32000, 1), (50, 32000, 64), (33, 50257, 256), (34, 128256, 20), (32, 8200, 100)])
 def test_top_log_probs(N, V, n, dtype):
     check_top(rows(N, V, dtype, V + n), n)
     check_top(rows(N, V, dtype, V + n), n, temperature=1.7)
@@ -166,8 +171,8 @@ def test_top_log_probs(N, V, n, dtype):
 
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("n", [1, 13, 300])
-def test_top_log_probs_ties_and_masks(dtype, n):
-    V = 6001
+@pytest.mark.parametrize("V,times", [(6001, 1), (10001, 3)])
+def test_top_log_probs_ties_and_masks(V, times, dtype, n):
     x = torch.round(rows(11, V, torch.float32, 6))
     x[0] = 0.0
     x[1] = -math.inf
@@ -181,10 +186,13 @@ def test_top_log_probs_ties_and_masks(dtype, n):
     x[9] = -50.0
     x[9, 4321] = 60.0
     x[10] = torch.where(torch.arange(V) % 2048 < 5, 3.0, -1.0)   # the best ones in one thread's hands
-    check_top(x.to(dtype), n)
+    check_top(x.to(dtype).repeat(times, 1), n)
 
 
 def test_top_log_probs_views():
+    wide = rows(80, 8801, torch.bfloat16, 4).cuda().view(40, 2, 8801)
+    for view in (wide[:, -1], wide[:, 0, 1:], wide[:, 1, 3:-2], wide[1, 1].expand(40, 8801)):
+        check_top(view.cpu(), 17, dev=view)
     big = rows(30, 801, torch.bfloat16, 4).cuda().view(5, 6, 801)
     for view in (big[:, -1], big[:, 2, 1:], big[:, 2, 3:-2], big[1, 1].expand(4, 801)):
         check_top(view.cpu(), 17, dev=view)
@@ -427,7 +435,7 @@ def test_cpu_tensors_come_back_to_the_cpu():
 
 
 def test_another_stream_and_two_at_once():
-    x = rows(64, 5000, torch.bfloat16, 40).cuda()
+    x = rows(64, 9000, torch.bfloat16, 40).cuda()
     u = uniforms(64, 40).cuda()
     want = ext.sample(x, u, top_k=30), ext.top_log_probs(x, 30), ext.sample(x, u, top_p=0.9)
     side = [torch.cuda.Stream(), torch.cuda.Stream()]
@@ -443,9 +451,9 @@ def test_another_stream_and_two_at_once():
 
 
 def test_captured_and_replayed():
-    x = rows(16, 3000, torch.float32, 50).cuda()
-    u = uniforms(16, 50).cuda()
-    lq, at = (t.cuda() for t in teacher(16, 3000, 10, 50))
+    x = rows(36, 9000, torch.float32, 50).cuda()
+    u = uniforms(36, 50).cuda()
+    lq, at = (t.cuda() for t in teacher(36, 9000, 10, 50))
 
     def step():
         leaf = x.detach().requires_grad_(True)
@@ -462,8 +470,8 @@ def test_captured_and_replayed():
     with torch.cuda.graph(graph):
         held = step()
     for seed in (51, 52):
-        x.copy_(rows(16, 3000, torch.float32, seed))
-        u.copy_(uniforms(16, seed))
+        x.copy_(rows(36, 9000, torch.float32, seed))
+        u.copy_(uniforms(36, seed))
         graph.replay()
         want = step()
         torch.cuda.synchronize()
@@ -497,7 +505,7 @@ def test_rows_behind_the_last_stay_as_they_are():
     state = torch.full((size.value + 64,), 7, dtype=torch.uint8, device="cuda")
     s = ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
     p = ext._vp
-    assert lib.dbs_device_top_log_probs(p(x), 0, 5, 333, 333, 4, 1.0, p(values), p(tokens), s) == 0
+    assert lib.dbs_device_top_log_probs(p(x), 0, 5, 333, 333, 4, 1.0, p(values), p(tokens), None, s) == 0
     assert lib.dbs_device_distill(p(x), 0, 5, 333, 333, p(lq), p(at), 4, 2, 1.0, 1, 1, 1.0, p(losses), p(loss), p(state), p(grad), s) == 0
     torch.cuda.synchronize()
     assert torch.all(values[5:] == 7.0) and torch.all(tokens[5:] == 7) and torch.all(grad[5:] == 7.0) and torch.all(losses[5:] == 7.0)
