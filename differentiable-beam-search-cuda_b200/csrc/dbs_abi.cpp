@@ -1913,15 +1913,18 @@ DBS_EXPORT int dbs_device_sample(const void* logits, int data_type, int64_t rows
     });
 }
 
-DBS_EXPORT int dbs_device_sample_workspace_bytes(int data_type, int64_t rows, int vocab_size, int top_k,
+DBS_EXPORT int dbs_device_sample_workspace_bytes(int data_type, int64_t rows, int vocab_size, int top_k, float top_p,
                                                  int64_t* bytes) {
     return guarded(nullptr, [&]() {
         if (!bytes) throw std::invalid_argument("bytes cannot be null");
         dbs_logits::SampleArgs a;
         a.in = logits_rows(bytes, data_type, rows, vocab_size, 0);   // any pointer: the rows are not read
-        static const int32_t per_row = 0;
-        a.top_k = top_k < 0 ? &per_row : nullptr;
+        static const int32_t k_per_row = 0;   // only whether these are null is looked at
+        static const float p_per_row = 0.0f;
+        a.top_k = top_k < 0 ? &k_per_row : nullptr;
         a.top_k_all = top_k;
+        a.top_p = top_p < 0.0f ? &p_per_row : nullptr;
+        a.top_p_all = top_p;
         *bytes = dbs_logits::sample_space(a);
         clear_error(nullptr);
         return 0;

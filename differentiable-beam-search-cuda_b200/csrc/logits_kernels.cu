@@ -309,14 +309,15 @@ __device__ __forceinline__ float lanes_max(const uint4& v) {
 
 // Descending sort of n keys in shared memory: a bitonic network whose runs
 // all have the same direction, so n need not be a power of two.
-__device__ void block_sort(uint64_t* a, int n) {
+template <int kT>
+__device__ void sort_by(uint64_t* a, int n) {
     int n2 = 1;
     while (n2 < n) n2 <<= 1;
     const int half = n2 >> 1;
     __syncthreads();
     for (int size = 2; size <= n2; size <<= 1) {
         for (int st = size >> 1; st > 0; st >>= 1) {
-            for (int p = threadIdx.x; p < half; p += kThreads) {
+            for (int p = threadIdx.x; p < half; p += kT) {
                 const int i = ((p & ~(st - 1)) << 1) | (p & (st - 1));
                 // the first step of a size compares mirrored places
                 const int j = st == (size >> 1) ? (i ^ (size - 1)) : i + st;
@@ -387,15 +388,15 @@ struct Team {      // a CTA's place in its cluster
     }
 };
 
-// 2^(steps / 32) in 64 bits, relative error below 2e-12: 2^(n/32 + r/32) with n
-// the whole number nearest to `steps` (within -2^15 and 2^15), a table of 2^(j/32) (an entry per lane) and
+// 2^(d c / 32) in 64 bits, relative error below 2e-12: 2^(n/32 + r/32) with n
+// the whole number nearest to d c (within -2^15 and 2^15), a table of 2^(j/32) (an entry per lane) and
 // the Taylor polynomial of 2^(r/32) to the fourth power. All 32 lanes of a
 // warp call it together.
 __device__ __forceinline__ double exp_table() { return exp2(static_cast<double>(threadIdx.x & 31) * 0.03125); }
-__device__ __forceinline__ double exp_by(double steps, int n, double tab) {
+__device__ __forceinline__ double exp_by(double d, double c, int n, double tab) {
     constexpr double kL = 0.021660849392498290;   // ln 2 / 32
     const double nd = __hiloint2double(0x43300000, n ^ static_cast<int>(0x80000000)) - 4503601774854144.0;
-    const double r = steps - nd;
+    const double r = fma(d, c, -nd);
     double p = fma(r, kL * kL * kL * kL / 24.0, kL * kL * kL / 6.0);
     p = fma(r, p, kL * kL / 2.0);
     p = fma(r, p, kL);
@@ -427,7 +428,7 @@ struct Weights {
         // 0 * inf and inf - inf come out as NaN, which fmaxf drops
         const float t = fmaxf((x - mf) * cf, -40000.0f);
         const int n = __float_as_int(t + 12582912.0f) - 0x4B400000;
-        const double p = exp_by((static_cast<double>(x) - m) * c, n, tab);
+        const double p = exp_by(static_cast<double>(x) - m, c, n, tab);
         return x == mf ? 1.0 : (n < -32686 ? 0.0 : p);   // exp(-708) and below count as nothing
     }
 };
@@ -515,10 +516,24 @@ __device__ Found search(const Team& team, Shared& sh, unsigned long long* hist, 
         if (round == 0 && rest) atomicAdd(&hist[kBins - 1], rest);
         cluster_sync(team.size);
         unsigned long long h[4] = {0, 0, 0, 0};
-        for (int c = 0; c < team.size; ++c) {
-            const unsigned long long* theirs = team.of(hist, c) + 4 * threadIdx.x;
+        for (int c0 = 0; c0 < team.size; c0 += 8) {
+            ulonglong2 theirs[8][2];
 #pragma unroll
-            for (int q = 0; q < 4; ++q) h[q] += theirs[q];
+            for (int c = 0; c < 8; ++c) {
+                theirs[c][0] = theirs[c][1] = make_ulonglong2(0, 0);
+                if (c0 + c < team.size) {
+                    const ulonglong2* of = reinterpret_cast<const ulonglong2*>(team.of(hist, c0 + c)) + 2 * threadIdx.x;
+                    theirs[c][0] = of[0];
+                    theirs[c][1] = of[1];
+                }
+            }
+#pragma unroll
+            for (int c = 0; c < 8; ++c) {
+                h[0] += theirs[c][0].x;
+                h[1] += theirs[c][0].y;
+                h[2] += theirs[c][1].x;
+                h[3] += theirs[c][1].y;
+            }
         }
         const unsigned long long own = h[0] + h[1] + h[2] + h[3];
         const unsigned long long before = above + block_before<unsigned long long>(own, sh.u8);
@@ -678,7 +693,7 @@ __device__ int gather_best(const Team& team, Shared& sh, const uint4* buf, const
         for (int i = threadIdx.x; i < count; i += kThreads) sorted[at + i] = theirs[i];
         at += count;
     }
-    block_sort(sorted, total);
+    sort_by<kThreads>(sorted, total);
     return min(n, total);
 }
 
@@ -1208,7 +1223,7 @@ struct ScanShape {
 };
 constexpr int kHold = 16;       // chunks of a part
 constexpr int kScanBins = 128;
-constexpr int kNucleus = 192;   // candidates listed for a top-p without a top-k
+constexpr int kNucleus = 512;   // candidates listed for a top-p without a top-k
 
 __host__ __device__ __forceinline__ ScanState scan_of(void* space, int64_t rows, ScanShape sh, bool chunks) {
     ScanState s;
@@ -1313,27 +1328,47 @@ __global__ void __launch_bounds__(kThreads, 3) scan_kernel(Args a, ScanShape sha
         if (tid == 0) listed = 0;
         copies_wait<0>();
         uint4 top = none;
-        for (int i = 0; i < per; ++i) top = vmax<E>(top, buf[i * kThreads]);
-        const float mine = lanes_max<E>(top);
-        float sum = 0.0f;
+        float sum = 0.0f, from = 0.0f;
+        const float c2 = fminf(1.4426950408889634f / plan.temperature, FLT_MAX);
         if (kTop) {
-            // the thread's exponentials by its own maximum
-            const float c2 = fminf(1.4426950408889634f / plan.temperature, FLT_MAX);
-            const float from = mine > neg_inf() ? -mine : 0.0f;
-            const float2 ff = make_float2(from, from), cc = make_float2(c2, c2);
-            float2 p = make_float2(0.0f, 0.0f);
+            // The thread's exponentials by the maximum of its first vectors;
+            // where the others run so far beyond it that the sum overflows, by
+            // the maximum of all.
+            auto add_up = [&]() {
+                const float2 ff = make_float2(-from, -from), cc = make_float2(c2, c2);
+                float2 p = make_float2(0.0f, 0.0f);
 #pragma unroll 4
-            for (int i = 0; i < per; ++i) {
-                float f[kVec];
-                Elem<E>::unpack(vmax<E>(buf[i * kThreads], none), f);
+                for (int i = 0; i < per; ++i) {
+                    const uint4 r = vmax<E>(buf[i * kThreads], none);
+                    top = vmax<E>(top, r);
+                    float f[kVec];
+                    Elem<E>::unpack(r, f);
 #pragma unroll
-                for (int e = 0; e < kVec; e += 2) {
-                    const float2 t = mul2(add2(make_float2(f[e], f[e + 1]), ff), cc);
-                    p = add2(p, make_float2(ex2(t.x), ex2(t.y)));
+                    for (int e = 0; e < kVec; e += 2) {
+                        const float2 t = mul2(add2(make_float2(f[e], f[e + 1]), ff), cc);
+                        p = add2(p, make_float2(ex2(t.x), ex2(t.y)));
+                    }
                 }
+                sum = p.x + p.y;
+            };
+            for (int i = 0; i < min(per, 4); ++i) top = vmax<E>(top, buf[i * kThreads]);
+            const float first = lanes_max<E>(top);
+            from = first > neg_inf() ? first : 0.0f;
+            add_up();
+            if (!(first > neg_inf()) || !(sum < 1.0e30f)) {
+                from = lanes_max<E>(top);
+                from = from > neg_inf() ? from : 0.0f;
+                add_up();
             }
-            sum = p.x + p.y;
+        } else {
+#pragma unroll 4
+            for (int i = 0; i < per; ++i) top = vmax<E>(top, buf[i * kThreads]);
         }
+        const float mine = lanes_max<E>(top);
+        // the sums in 64 bits go over the vectors a second time
+        const bool again = !kTop && plan.sum;
+        const int64_t next = item + gridDim.x;
+        if (!again && next < items) copy(next);
         float2 of_warp = make_float2(mine, 0.0f);
         float least = mine > neg_inf() ? mine : FLT_MAX;
 #pragma unroll
@@ -1342,8 +1377,7 @@ __global__ void __launch_bounds__(kThreads, 3) scan_kernel(Args a, ScanShape sha
             least = fminf(least, __shfl_xor_sync(kAll, least, o));
         }
         if (kTop) {
-            const float c2 = fminf(1.4426950408889634f / plan.temperature, FLT_MAX);
-            of_warp.y = sum == 0.0f ? 0.0f : sum * share(mine, of_warp.x, c2);
+            of_warp.y = sum == 0.0f ? 0.0f : sum * ex2((from - of_warp.x) * c2);
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) of_warp.y += __shfl_xor_sync(kAll, of_warp.y, o);
         }
@@ -1393,14 +1427,33 @@ __global__ void __launch_bounds__(kThreads, 3) scan_kernel(Args a, ScanShape sha
             tau = plan.take > 0 ? fmaxf(tau, low) : low;
         }
         double mass = 0.0;
-        if (!kTop && plan.sum && best > neg_inf()) {
+        if (again && best > neg_inf()) {
+            // Where a warp's vectors hold only terms below e^-17 of the part's
+            // maximum, they are added up in 32 bits: their error, 2^-22 of that,
+            // is lost among the others' 2e-12.
             const Weights weight(best, plan.temperature);
+            const float small_from = best - 17.0f * plan.temperature;
             for (int i = 0; i < per; ++i) {
                 float f[kVec];
-                Elem<E>::unpack(buf[i * kThreads], f);
-                double w = 0.0;
+                Elem<E>::unpack(vmax<E>(buf[i * kThreads], none), f);
+                double w;
+                float large = f[0];
 #pragma unroll
-                for (int e = 0; e < kVec; ++e) w += weight(f[e]);
+                for (int e = 1; e < kVec; ++e) large = fmaxf(large, f[e]);
+                if (__any_sync(kAll, large > small_from)) {
+                    double w0 = 0.0, w1 = 0.0;
+#pragma unroll
+                    for (int e = 0; e < kVec; e += 2) {
+                        w0 += weight(f[e]);
+                        w1 += weight(f[e + 1]);
+                    }
+                    w = w0 + w1;
+                } else {
+                    float small = 0.0f;
+#pragma unroll
+                    for (int e = 0; e < kVec; ++e) small += ex2((f[e] - best) * c2);
+                    w = static_cast<double>(small);
+                }
                 mass += w;
                 if (plan.chunks) {
 #pragma unroll
@@ -1413,19 +1466,37 @@ __global__ void __launch_bounds__(kThreads, 3) scan_kernel(Args a, ScanShape sha
             for (int o = 16; o > 0; o >>= 1) mass += __shfl_xor_sync(kAll, mass, o);
             if (lane == 0) d8[warp] = mass;
         }
-        // The warp looks through the vectors of each of its threads whose
-        // maximum reaches tau, an element per lane.
+        if (again && next < items) copy(next);
+        // The warp looks through the vectors of those of its threads whose
+        // maximum reaches tau, two threads at a time and a vector per lane;
+        // they come from L2, as shared memory is on to the next rows.
         uint64_t* list = state.lists + item * shape.cap;
-        const E* elems = reinterpret_cast<const E*>(dyn);
-        for (unsigned have = __ballot_sync(kAll, mine >= tau && mine > neg_inf()); have; have &= have - 1) {
-            const int owner = warp * 32 + __ffs(have) - 1;
-            for (int at = lane; at < per * kVec; at += 32) {
-                const int i = at / kVec, e = at % kVec;
-                const float v = Elem<E>::widen(elems[(i * kThreads + owner) * kVec + e]);
-                if (v >= tau && v > neg_inf()) {
+        const uint4* src = reinterpret_cast<const uint4*>(x & ~static_cast<uintptr_t>(15));
+        const E* elems = static_cast<const E*>(a.in.x) + row * a.in.stride;
+        const int v0 = phase > 0 ? 1 : 0, v1 = (V + phase) / kVec;
+        for (unsigned have = __ballot_sync(kAll, mine >= tau && mine > neg_inf()); have;) {
+            int owner = __ffs(have) - 1;
+            have &= have - 1;
+            const int other = have ? __ffs(have) - 1 : -1;
+            have &= have - 1;
+            if (lane >= kHold) owner = other;
+            const int i = lane % kHold, v = (i * shape.parts + part) * kThreads + warp * 32 + owner;
+            if (owner < 0 || i >= per || v >= (V + phase + kVec - 1) / kVec) continue;
+            float f[kVec];
+            if (v >= v0 && v < v1) {
+                Elem<E>::unpack(ldg_once(src + v), f);
+            } else {
+#pragma unroll
+                for (int e = 0; e < kVec; ++e) {
+                    const int token = v * kVec + e - phase;
+                    f[e] = token >= 0 && token < V ? Elem<E>::widen(elems[token]) : neg_inf();
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < kVec; ++e) {
+                if (f[e] >= tau && f[e] > neg_inf()) {
                     const int place = atomicAdd(&listed, 1);
-                    if (place < shape.cap)
-                        list[place] = entry(v, ((i * shape.parts + part) * kThreads + owner) * kVec + e - phase);
+                    if (place < shape.cap) list[place] = entry(f[e], v * kVec + e - phase);
                 }
             }
         }
@@ -1433,7 +1504,6 @@ __global__ void __launch_bounds__(kThreads, 3) scan_kernel(Args a, ScanShape sha
         if (tid == 0) {
             PartState out = {0.0, best, tau, listed, 0};
             if (kTop) {
-                const float c2 = fminf(1.4426950408889634f / plan.temperature, FLT_MAX);
                 float all = 0.0f;
                 for (int w = 0; w < kWarps; ++w)
                     all += part8[w].y == 0.0f ? 0.0f : part8[w].y * share(part8[w].x, best, c2);
@@ -1443,7 +1513,6 @@ __global__ void __launch_bounds__(kThreads, 3) scan_kernel(Args a, ScanShape sha
             }
             state.parts[item] = out;
         }
-        if (item + gridDim.x < items) copy(item + gridDim.x);
         __syncthreads();   // listed and the bins are free again
     }
 }
@@ -1459,19 +1528,29 @@ struct Gathered {
 };
 template <int kT>
 __device__ Gathered gather_parts(const ScanState& state, ScanShape shape, int64_t row, uint64_t* keys, uint64_t* other,
-                                 int* places, int* counters) {
+                                 int* counters) {
     const PartState* parts = state.parts + row * shape.parts;
     Gathered g = {0, 0, neg_inf(), neg_inf(), true};
-    float tau = neg_inf();
-    bool over = false;
-    for (int s = 0; s < shape.parts; ++s) {
-        const PartState p = parts[s];
-        if (threadIdx.x == 0) places[s] = g.count;
-        over = over || p.count > shape.cap;
-        g.count += min(p.count, shape.cap);
-        g.best = fmaxf(g.best, p.best);
-        if (p.best > neg_inf()) tau = fmaxf(tau, p.tau);
+    // a part per lane, by every warp
+    const int lane = threadIdx.x % 32;
+    PartState mine = {0.0, neg_inf(), neg_inf(), 0, 0};
+    if (lane < shape.parts) mine = parts[lane];
+    const bool over = __any_sync(kAll, mine.count > shape.cap) != 0;
+    float tau = mine.best > neg_inf() ? mine.tau : neg_inf();
+    g.best = mine.best;
+    int before = mine.count;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        g.best = fmaxf(g.best, __shfl_xor_sync(kAll, g.best, o));
+        tau = fmaxf(tau, __shfl_xor_sync(kAll, tau, o));
     }
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int up = __shfl_up_sync(kAll, before, o);
+        if (lane >= o) before += up;
+    }
+    g.count = __shfl_sync(kAll, before, 31);
+    before -= mine.count;
     g.all = !(tau > neg_inf());
     g.tau = tau;
     if (over) {
@@ -1481,14 +1560,21 @@ __device__ Gathered gather_parts(const ScanState& state, ScanShape shape, int64_
     if (threadIdx.x == 0) counters[0] = 0;
     __syncthreads();
     // a part's entries by a warp
-    for (int s = threadIdx.x / 32; s < shape.parts; s += kT / 32) {
+    for (int s = 0; s < shape.parts; ++s) {
+        const int to = __shfl_sync(kAll, before, s), count = __shfl_sync(kAll, mine.count, s);
+        if (s % (kT / 32) != static_cast<int>(threadIdx.x) / 32) continue;
         const uint64_t* list = state.lists + (row * shape.parts + s) * shape.cap;
-        for (int i = threadIdx.x % 32; i < parts[s].count; i += 32) other[places[s] + i] = list[i];
+        for (int i = lane; i < count; i += 32) other[to + i] = list[i];
     }
     __syncthreads();
-    // in order, by counting the better ones
     int whole = 0;
-    for (int i = threadIdx.x; i < g.count; i += kT) {
+    for (int i = threadIdx.x; i < g.count; i += kT) whole += entry_value(other[i]) >= tau ? 1 : 0;
+    if (g.count > kT) {
+        sort_by<kT>(other, g.count);
+        for (int i = threadIdx.x; i < g.count; i += kT) keys[i] = other[i];
+    }
+    // a short list in order by counting the better ones
+    for (int i = threadIdx.x; i < g.count && g.count <= kT; i += kT) {
         const uint64_t mine = other[i];
         int rank = 0;
         int j = 0;
@@ -1498,7 +1584,6 @@ __device__ Gathered gather_parts(const ScanState& state, ScanShape shape, int64_
         }
         if (j < g.count) rank += other[j] > mine ? 1 : 0;
         keys[rank] = mine;
-        whole += entry_value(mine) >= tau ? 1 : 0;
     }
     whole = __reduce_add_sync(kAll, whole);
     if (threadIdx.x % 32 == 0) atomicAdd(&counters[0], whole);
@@ -1507,30 +1592,31 @@ __device__ Gathered gather_parts(const ScanState& state, ScanShape shape, int64_
     return g;
 }
 
-constexpr int kFinish = 128;   // threads of a finishing CTA
 
-__global__ void __launch_bounds__(kFinish) top_finish_kernel(TopArgs a, ScanShape shape, void* space) {
+__global__ void __launch_bounds__(256) top_finish_kernel(TopArgs a, ScanShape shape, void* space) {
     extern __shared__ uint64_t keys_space[];
-    __shared__ int places[64];
     __shared__ int counters[1];
+    constexpr int kFinish = 256;
     const ScanState state = scan_of(space, a.in.rows, shape, false);
     uint64_t* keys = keys_space;
     uint64_t* other = keys + shape.parts * shape.cap;
     const int n = a.n;
     const double c = static_cast<double>(fminf(1.4426950408889634f / a.temperature, FLT_MAX));
     for (int64_t row = blockIdx.x; row < a.in.rows; row += gridDim.x) {
-        const Gathered g = gather_parts<kFinish>(state, shape, row, keys, other, places, counters);
+        const Gathered g = gather_parts<kFinish>(state, shape, row, keys, other, counters);
         if (g.count < 0 || (!g.all && g.whole < n) || !(g.best < HUGE_VALF)) {
             if (threadIdx.x == 0) state.left[1 + atomicAdd(&state.left[0], 1)] = static_cast<int>(row);
             __syncthreads();
             continue;
         }
-        double Z = 0.0;
-        for (int s = 0; s < shape.parts; ++s) {
-            const PartState p = state.parts[row * shape.parts + s];
+        double Z = 0.0;   // a part per lane, by every warp
+        if (static_cast<int>(threadIdx.x) % 32 < shape.parts) {
+            const PartState p = state.parts[row * shape.parts + threadIdx.x % 32];
             if (p.sum != 0.0)
-                Z += p.sum * (p.best == g.best ? 1.0 : exp2(c * (static_cast<double>(p.best) - static_cast<double>(g.best))));
+                Z = p.sum * (p.best == g.best ? 1.0 : exp2(c * (static_cast<double>(p.best) - static_cast<double>(g.best))));
         }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) Z += __shfl_xor_sync(kAll, Z, o);
         const double log_z = log(Z);
         for (int i = threadIdx.x; i < n; i += kFinish) {
             float value = neg_inf();
@@ -1548,11 +1634,11 @@ __global__ void __launch_bounds__(kFinish) top_finish_kernel(TopArgs a, ScanShap
 }
 
 template <class E>
-__global__ void __launch_bounds__(kFinish) sample_finish_kernel(SampleArgs a, ScanShape shape, void* space) {
+__global__ void __launch_bounds__(512) sample_finish_kernel(SampleArgs a, ScanShape shape, void* space) {
     constexpr int kVec = Elem<E>::kVec;
+    constexpr int kFinish = 512;
     constexpr int kW = kFinish / 32;
     extern __shared__ uint64_t keys_space[];
-    __shared__ int places[64];
     __shared__ int counters[1];
     __shared__ double d8[kW];
     __shared__ int i8[kW];
@@ -1608,8 +1694,12 @@ __global__ void __launch_bounds__(kFinish) sample_finish_kernel(SampleArgs a, Sc
             leave();
             continue;
         }
-        float best = neg_inf();
-        for (int s = 0; s < shape.parts; ++s) best = fmaxf(best, parts[s].best);
+        // a part per lane, by every warp
+        PartState own_part = {0.0, neg_inf(), 0.0f, 0, 0};
+        if (lane < shape.parts) own_part = parts[lane];
+        float best = own_part.best;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) best = fmaxf(best, __shfl_xor_sync(kAll, best, o));
         if (!(best > neg_inf())) {
             if (tid == 0) *out = -1;
             continue;
@@ -1619,11 +1709,15 @@ __global__ void __launch_bounds__(kFinish) sample_finish_kernel(SampleArgs a, Sc
             leave();
             continue;
         }
+        // what a part's sums are multiplied by to go by the row's maximum
+        const double factor = own_part.best == best ? 1.0
+                              : own_part.best > neg_inf() ? exp((static_cast<double>(own_part.best) - m) / T) : 0.0;
         double W = 0.0;
-        if (plan.sum)
-            for (int s = 0; s < shape.parts; ++s)
-                if (parts[s].sum != 0.0)
-                    W += parts[s].sum * (parts[s].best == best ? 1.0 : exp((static_cast<double>(parts[s].best) - m) / T));
+        if (plan.sum) {
+            W = factor == 0.0 ? 0.0 : own_part.sum * factor;
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) W += __shfl_xor_sync(kAll, W, o);
+        }
         if (plan.chunks) {
             // temperature alone: the first stretch of 32 vectors at which the
             // running sum passes the target, then the element in it
@@ -1632,13 +1726,18 @@ __global__ void __launch_bounds__(kFinish) sample_finish_kernel(SampleArgs a, Sc
             const int per = ((a.in.V + kVec - 2) / kVec + 1 + kThreads * shape.parts - 1) / (kThreads * shape.parts);
             const int used = per * shape.parts * kWarps;
             const double* sums = state.chunks + row * stretches;
+            if (!(u > 0.0)) {   // the first weight above 0 is wanted, however small
+                leave();
+                continue;
+            }
+            __shared__ double factors[32];
+            if (warp == 0) factors[lane] = factor;
+            __syncthreads();
             const int each = (used + kFinish - 1) / kFinish;
             const int begin = min(used, each * tid), end = min(used, begin + each);
             auto stretch = [&](int i) {
-                const int s = i / kWarps % shape.parts;
-                if (!(parts[s].best > neg_inf())) return 0.0;
-                const double v = sums[i];
-                return v == 0.0 || parts[s].best == best ? v : v * exp((static_cast<double>(parts[s].best) - m) / T);
+                const double f = factors[i / kWarps % shape.parts];
+                return f == 0.0 ? 0.0 : sums[i] * f;
             };
             double mine = 0.0;
             for (int i = begin; i < end; ++i) mine += stretch(i);
@@ -1705,7 +1804,7 @@ __global__ void __launch_bounds__(kFinish) sample_finish_kernel(SampleArgs a, Sc
             __syncthreads();
             continue;
         }
-        const Gathered g = gather_parts<kFinish>(state, shape, row, keys, other, places, counters);
+        const Gathered g = gather_parts<kFinish>(state, shape, row, keys, other, counters);
         if (g.count < 0) {
             leave();
             continue;
@@ -1762,7 +1861,28 @@ __global__ void __launch_bounds__(kFinish) sample_finish_kernel(SampleArgs a, Sc
         const double kept = total_of(mine);
         const double target = u < 1.0 ? u * kept : HUGE_VAL;
         int first = 0x7FFFFFFF, last = -1;
-        for (int i = tid; i < keep; i += kFinish) {
+        if (keep > kFinish / 4) {
+            // by index: token and rank in one key, then running sums
+            __syncthreads();
+            for (int i = tid; i < keep; i += kFinish) {
+                const uint64_t token = static_cast<uint64_t>(entry_token(keys[i]));
+                keys[i] = ~(token << 32 | static_cast<uint64_t>(i));
+            }
+            sort_by<kFinish>(keys, keep);
+            const int some = (keep + kFinish - 1) / kFinish;
+            const int from = min(keep, some * tid), until = min(keep, from + some);
+            double own = 0.0;
+            for (int i = from; i < until; ++i) own += weight[~keys[i] & 0xFFFFFFFFu];
+            double at = before_of(own);
+            for (int i = from; i < until; ++i) {
+                const double w = weight[~keys[i] & 0xFFFFFFFFu];
+                at += w;
+                if (w > 0.0) {
+                    last = static_cast<int>(~keys[i] >> 32);
+                    if (first == 0x7FFFFFFF && at > target) first = last;
+                }
+            }
+        } else for (int i = tid; i < keep; i += kFinish) {
             const int own = entry_token(keys[i]);
             double sum = 0.0;
             for (int j = 0; j < keep; ++j) sum += entry_token(keys[j]) <= own ? weight[j] : 0.0;
@@ -1903,7 +2023,7 @@ __global__ void __launch_bounds__(256) slots_kernel(DistillArgs a, uint32_t mask
             // log-probs above 709 are infinite, those below -708 nothing
             const float t = fminf(fmaxf(l[k] * 46.16624f, -40000.0f), 40000.0f);
             const int steps = __float_as_int(t + 12582912.0f) - 0x4B400000;
-            double q = exp_by(static_cast<double>(l[k]) * 46.166241308446828384, steps, tab);
+            double q = exp_by(static_cast<double>(l[k]), 46.166241308446828384, steps, tab);
             if (!(l[k] >= -708.0f)) q = l[k] < -708.0f ? 0.0 : static_cast<double>(l[k]);
             if (l[k] > 709.0f) q = HUGE_VAL;
             if (slot[k].token >= 0) {
@@ -2386,7 +2506,7 @@ struct Shape {
 // arithmetic and one's stores overlap. Few rows are cut finer, down to 8 KB,
 // so that they reach more SMs; 16 CTAs (more than every GPU grants a cluster)
 // are taken only for rows that need them.
-Shape shape_of(const Rows& in, int es, int most) {
+Shape shape_of(const Rows& in, int es, int most, bool few = false) {
     const int vec = 16 / es;
     auto slice = [&](int size) {
         const int64_t per = (static_cast<int64_t>(in.V) + vec - 1 + size - 1) / size;
@@ -2395,6 +2515,7 @@ Shape shape_of(const Rows& in, int es, int most) {
     int size = 1;
     while (size < 8 && static_cast<int64_t>(slice(size)) * es > most) ++size;
     if (static_cast<int64_t>(slice(size)) * es > most) size = 16;
+    if (few && size < 8) size = 8;   // a handful of rows out of many: one row's time counts
     while (size <= 4 && in.rows * size * 2 <= 148 && static_cast<int64_t>(slice(size)) * es > 8 * 1024) size *= 2;
     return Shape{size, slice(size)};
 }
@@ -2512,14 +2633,15 @@ ScanShape scan_shape(const Rows& in, int es, int take) {
     const int chunk = kThreads * 16 / es;
     const int chunks = (in.V + 16 / es - 1 + chunk - 1) / chunk;
     int parts = (chunks + kHold - 1) / kHold;
-    while (parts < chunks && parts < 64 && (parts * 100 < take || in.rows * parts < 148 * 2)) ++parts;
+    while (parts < chunks && parts < 32 && (parts * 100 < take || in.rows * parts < 148 * 2)) ++parts;
     const float mean = static_cast<float>(take) / static_cast<float>(parts);
     const int cap = (static_cast<int>(4.0f * mean + 12.0f * sqrtf(mean)) + 96) / 2 * 2;
     return ScanShape{parts, cap};
 }
 
 int sample_take(const SampleArgs& a) {
-    return a.top_k ? 128 : a.top_k_all > 0 ? std::min(a.top_k_all, kSampleList) : kNucleus;
+    const bool by_p = a.top_p || a.top_p_all < 1.0f;
+    return a.top_k ? (by_p ? 384 : 128) : a.top_k_all > 0 ? std::min(a.top_k_all, kSampleList) : by_p ? kNucleus : 1;
 }
 
 int64_t scan_bytes(const Rows& in, ScanShape sh, bool chunks) {
@@ -2536,9 +2658,9 @@ cudaError_t launch_scan(const Args& a, ScanShape sh, bool chunks, cudaStream_t s
 }
 
 template <class Kernel, class Args>
-cudaError_t launch_finish(Kernel kernel, const Args& a, ScanShape sh, cudaStream_t stream) {
+cudaError_t launch_finish(Kernel kernel, const Args& a, ScanShape sh, int threads, cudaStream_t stream) {
     const size_t smem = static_cast<size_t>(sh.parts) * sh.cap * 16;
-    return launch_rows(kernel, a.in, 1, smem, stream, kFinish, a, sh, a.space);
+    return launch_rows(kernel, a.in, 1, smem, stream, threads, a, sh, a.space);
 }
 
 }  // namespace
@@ -2561,21 +2683,21 @@ cudaError_t launch_sample(const SampleArgs& given, cudaStream_t stream) {
         switch (a.in.dtype) {
             case kF32:
                 err = launch_scan<float, SampleArgs, false>(a, scan, true, stream);
-                if (err == cudaSuccess) err = launch_finish(sample_finish_kernel<float>, a, scan, stream);
+                if (err == cudaSuccess) err = launch_finish(sample_finish_kernel<float>, a, scan, 512, stream);
                 break;
             case kF16:
                 err = launch_scan<__half, SampleArgs, false>(a, scan, true, stream);
-                if (err == cudaSuccess) err = launch_finish(sample_finish_kernel<__half>, a, scan, stream);
+                if (err == cudaSuccess) err = launch_finish(sample_finish_kernel<__half>, a, scan, 512, stream);
                 break;
             default:
                 err = launch_scan<__nv_bfloat16, SampleArgs, false>(a, scan, true, stream);
-                if (err == cudaSuccess) err = launch_finish(sample_finish_kernel<__nv_bfloat16>, a, scan, stream);
+                if (err == cudaSuccess) err = launch_finish(sample_finish_kernel<__nv_bfloat16>, a, scan, 512, stream);
         }
         if (err != cudaSuccess) return err;
         a.left = scan_of(a.space, a.in.rows, scan, true).left;
     }
     const int es = element_size(a.in.dtype);
-    const Shape sh = shape_of(a.in, es, 68 * 1024);
+    const Shape sh = shape_of(a.in, es, 68 * 1024, a.left != nullptr);
     // lists for rows that may take that path, bins for the others
     const int cap = list_space(a.top_k ? kSampleList : (a.top_k_all <= kSampleList ? std::max(a.top_k_all, 0) : 0));
     const size_t smem = static_cast<size_t>(sh.S) * es + static_cast<size_t>(cap) * 16;
@@ -2593,12 +2715,12 @@ cudaError_t launch_top(const TopArgs& given, cudaStream_t stream) {
         cudaError_t err = a.in.dtype == kF32   ? launch_scan<float, TopArgs, true>(a, scan, false, stream)
                           : a.in.dtype == kF16 ? launch_scan<__half, TopArgs, true>(a, scan, false, stream)
                                                : launch_scan<__nv_bfloat16, TopArgs, true>(a, scan, false, stream);
-        if (err == cudaSuccess) err = launch_finish(top_finish_kernel, a, scan, stream);
+        if (err == cudaSuccess) err = launch_finish(top_finish_kernel, a, scan, 256, stream);
         if (err != cudaSuccess) return err;
         a.left = scan_of(a.space, a.in.rows, scan, false).left;
     }
     const int es = element_size(a.in.dtype);
-    const Shape sh = shape_of(a.in, es, 68 * 1024);
+    const Shape sh = shape_of(a.in, es, 68 * 1024, a.left != nullptr);
     const int cap = list_space(a.n);
     const size_t smem = static_cast<size_t>(sh.S) * es + static_cast<size_t>(cap) * 16;
     switch (a.in.dtype) {

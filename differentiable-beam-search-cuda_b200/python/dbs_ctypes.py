@@ -210,7 +210,7 @@ DEVICE_FUNCTIONS = {
         _I, [_VP, _I, _I, _I, ctypes.POINTER(DBSDeviceDecodeOutputs), _VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP]),
     "dbs_device_sample": (
         _I, [_VP, _I, _I64, _I, _I64, _VP, _VP, _F, _VP, _I, _VP, _F, _VP, _F, _VP, _VP, _VP]),
-    "dbs_device_sample_workspace_bytes": (_I, [_I, _I64, _I, _I, ctypes.POINTER(_I64)]),
+    "dbs_device_sample_workspace_bytes": (_I, [_I, _I64, _I, _I, _F, ctypes.POINTER(_I64)]),
     "dbs_device_top_log_probs": (_I, [_VP, _I, _I64, _I, _I64, _I, _F, _VP, _VP, _VP, _VP]),
     "dbs_device_top_log_probs_workspace_bytes": (_I, [_I, _I64, _I, _I, ctypes.POINTER(_I64)]),
     "dbs_device_distill": (

@@ -524,10 +524,10 @@ def _rows_args(x: torch.Tensor):
     return _vp(x), _DTYPES[x.dtype], x.size(0), x.size(1), x.stride(0) if x.size(0) > 1 else x.size(1)
 
 
-def _workspace(query, x: torch.Tensor, n: int) -> Optional[torch.Tensor]:
+def _workspace(query, x: torch.Tensor, *settings) -> Optional[torch.Tensor]:
     """Device memory for what passes between a call's kernels, or None."""
     size = ctypes.c_int64()
-    _check_global(query(_DTYPES[x.dtype], x.size(0), x.size(1), n, size), "workspace")
+    _check_global(query(_DTYPES[x.dtype], x.size(0), x.size(1), *settings, size), "workspace")
     return torch.empty((size.value,), dtype=torch.uint8, device=x.device) if size.value else None
 
 
@@ -609,7 +609,8 @@ def sample(logits: torch.Tensor, uniforms: torch.Tensor, *, temperature=1.0, top
     u = _beside(uniforms, "uniforms", device, torch.float32, lead)
     tokens = torch.empty(lead, dtype=torch.int32, device=device)
     k_all = min(int(k_all), _INT_MAX)
-    space = _workspace(_library().dbs_device_sample_workspace_bytes, x, k_all if k_rows is None else -1)
+    space = _workspace(_library().dbs_device_sample_workspace_bytes, x, k_all if k_rows is None else -1,
+                       p_all if p_rows is None else -1.0)
     with torch.cuda.device(device):
         rc = _library().dbs_device_sample(*_rows_args(x), _vp(u), _vp(t_rows), t_all, _vp(k_rows), k_all, _vp(p_rows),
                                           p_all, _vp(q_rows), q_all, _vp(tokens), _vp(space), _stream_ptr(device))

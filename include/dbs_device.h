@@ -183,8 +183,8 @@ DBS_EXPORT int dbs_device_sample(const void* logits, int data_type, int64_t rows
                                  const int32_t* top_ks, int top_k, const float* top_ps, float top_p,
                                  const float* min_ps, float min_p, int32_t* tokens, void* workspace,
                                  void* cuda_stream);
-/* top_k: the call's, or -1 where it gives top_ks. */
-DBS_EXPORT int dbs_device_sample_workspace_bytes(int data_type, int64_t rows, int vocab_size, int top_k,
+/* top_k and top_p: the call's, or -1 where it gives top_ks or top_ps. */
+DBS_EXPORT int dbs_device_sample_workspace_bytes(int data_type, int64_t rows, int vocab_size, int top_k, float top_p,
                                                  int64_t* bytes);
 
 /* The n best tokens of each row (logit desc, token asc; NaN counts as -inf)

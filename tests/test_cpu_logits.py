@@ -143,11 +143,11 @@ def test_c_arguments(libdbs):
     refused(libdbs, sample(*wide, P, None, 1.0, None, 0, None, 1.0, None, 0.0, P, ODD, None), "workspace is not aligned")
     refused(libdbs, top(*wide, 4, 1.0, P, P, None, None), "workspace cannot be null")
     size = ctypes.c_int64()
-    for query in (libdbs.dbs_device_sample_workspace_bytes, libdbs.dbs_device_top_log_probs_workspace_bytes):
-        assert query(0, 64, 32000, 8, ctypes.byref(size)) == 0 and size.value > 0
-        assert query(0, 1, 32000, 8, ctypes.byref(size)) == 0 and size.value == 0
-        refused(libdbs, query(0, 64, 32000, 8, None), "bytes cannot be null")
-        refused(libdbs, query(9, 64, 32000, 8, ctypes.byref(size)), "data type")
+    for query, given in ((libdbs.dbs_device_sample_workspace_bytes, (8, 0.9)), (libdbs.dbs_device_top_log_probs_workspace_bytes, (8,))):
+        assert query(0, 64, 32000, *given, ctypes.byref(size)) == 0 and size.value > 0
+        assert query(0, 1, 32000, *given, ctypes.byref(size)) == 0 and size.value == 0
+        refused(libdbs, query(0, 64, 32000, *given, None), "bytes cannot be null")
+        refused(libdbs, query(9, 64, 32000, *given, ctypes.byref(size)), "data type")
     distill = libdbs.dbs_device_distill
     refused(libdbs, distill(*rows, None, P, 4, 2, 1.0, 1, 1, 1.0, P, P, P, None, None), "teacher_log_probs")
     refused(libdbs, distill(*rows, P, P, 2, 2, 1.0, 1, 1, 1.0, P, P, P, None, None), "token_bytes")
