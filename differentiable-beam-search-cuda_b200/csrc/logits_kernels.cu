@@ -1286,61 +1286,98 @@ __global__ void __launch_bounds__(kThreads, 3) scan_kernel(Args a, ScanShape sha
     __shared__ float2 part8[kWarps];
     __shared__ float low8[kWarps];
     __shared__ double d8[kWarps];
-    __shared__ __align__(16) int hist[kScanBins];
-    __shared__ int listed;
+    // the bins and the list's length of this part and the next
+    __shared__ __align__(16) int hist2[2 * kScanBins];
+    __shared__ int listed2[2];
     const ScanState state = scan_of(space, a.in.rows, shape, with_chunks);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, V = a.in.V;
     const uint4 none = vneg_inf<E>();
     uint4* buf = dyn + tid;    // this thread's vectors, kThreads apart
-    const int64_t items = a.in.rows * shape.parts;
     const int per = ((V + kVec - 2) / kVec + 1 + kThreads * shape.parts - 1) / (kThreads * shape.parts);   // chunks of a part
     if (blockIdx.x == 0 && tid == 0) state.left[0] = 0;
-    auto copy = [&](int64_t item) {
-        const int64_t row = item / shape.parts;
-        const int part = static_cast<int>(item - row * shape.parts);
-        const E* x = static_cast<const E*>(a.in.x) + row * a.in.stride;
-        const int phase = static_cast<int>((reinterpret_cast<uintptr_t>(x) & 15u) / sizeof(E));
-        const uint4* src = reinterpret_cast<const uint4*>(reinterpret_cast<uintptr_t>(x) & ~static_cast<uintptr_t>(15));
-        const int v0 = phase > 0 ? 1 : 0, v1 = (V + phase) / kVec;
-        for (int i = 0, v = part * kThreads + tid; i < per; ++i, v += shape.parts * kThreads) {
-            if (v >= v0 && v < v1) {
-                copy_async(buf + i * kThreads, src + v);
-            } else {
-                float f[kVec];   // a ragged end of the row, or behind it
+    // A part at a time: row and part, and how far the next one is.
+    int64_t row = blockIdx.x / shape.parts;
+    int part = static_cast<int>(blockIdx.x % shape.parts);
+    const int64_t row_step = gridDim.x / shape.parts;
+    const int part_step = static_cast<int>(gridDim.x % shape.parts);
+    struct View {
+        const E* x;
+        const uint4* src;
+        int phase, v0, v1;
+    };
+    auto view = [&](int64_t r) {
+        View w;
+        w.x = static_cast<const E*>(a.in.x) + r * a.in.stride;
+        const uintptr_t at = reinterpret_cast<uintptr_t>(w.x);
+        w.phase = static_cast<int>((at & 15u) / sizeof(E));
+        w.src = reinterpret_cast<const uint4*>(at & ~static_cast<uintptr_t>(15));
+        w.v0 = w.phase > 0 ? 1 : 0;
+        w.v1 = (V + w.phase) / kVec;
+        return w;
+    };
+    // a vector that the row fills only in part
+    auto ragged = [&](const View& w, int v) {
+        float f[kVec];
 #pragma unroll
-                for (int e = 0; e < kVec; ++e) {
-                    const int64_t token = static_cast<int64_t>(v) * kVec + e - phase;
-                    f[e] = token >= 0 && token < V ? Elem<E>::widen(x[token]) : neg_inf();
-                }
-                buf[i * kThreads] = Elem<E>::pack(f);
+        for (int e = 0; e < kVec; ++e) {
+            const int token = v * kVec + e - w.phase;
+            f[e] = token >= 0 && token < V ? Elem<E>::widen(w.x[token]) : neg_inf();
+        }
+        return Elem<E>::pack(f);
+    };
+    const int stride = shape.parts * kThreads;
+    auto copy = [&](const View& w, int p) {
+        int v = p * kThreads + tid;
+        if (w.v0 == 0 && (p + 1) * kThreads + (per - 1) * stride <= w.v1) {
+            const uint4* from = w.src + v;
+#pragma unroll 4
+            for (int i = 0; i < per; ++i, from += stride) copy_async(buf + i * kThreads, from);
+        } else {
+            for (int i = 0; i < per; ++i, v += stride) {
+                if (v >= w.v0 && v < w.v1)
+                    copy_async(buf + i * kThreads, w.src + v);
+                else
+                    buf[i * kThreads] = v * kVec < V + w.phase ? ragged(w, v) : none;
             }
         }
         copies_commit();
     };
-    if (blockIdx.x < items) copy(blockIdx.x);
-    for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
-        const int64_t row = item / shape.parts;
-        const int part = static_cast<int>(item - row * shape.parts);
+    View here = view(row);
+    if (tid < 2 * kScanBins) hist2[tid] = 0;
+    if (tid < 2) listed2[tid] = 0;
+    int parity = 0;
+    if (row < a.in.rows) copy(here, part);
+    __syncthreads();
+    while (row < a.in.rows) {
+        int64_t next_row = row + row_step;
+        int next_part = part + part_step;
+        if (next_part >= shape.parts) {
+            next_part -= shape.parts;
+            ++next_row;
+        }
+        const View next = view(next_row);
+        const bool more = next_row < a.in.rows;
         const Plan plan = plan_of(a, row);
-        const uintptr_t x = reinterpret_cast<uintptr_t>(static_cast<const E*>(a.in.x) + row * a.in.stride);
-        const int phase = static_cast<int>((x & 15u) / sizeof(E));
-        if (tid < kScanBins) hist[tid] = 0;
-        if (tid == 0) listed = 0;
+        const int phase = here.phase;
+        int* hist = hist2 + parity * kScanBins;
+        int* listed = listed2 + parity;
+        parity ^= 1;
         copies_wait<0>();
         uint4 top = none;
         float sum = 0.0f, from = 0.0f;
         const float c2 = fminf(1.4426950408889634f / plan.temperature, FLT_MAX);
         if (kTop) {
             // The thread's exponentials by the maximum of its first vectors;
-            // where the others run so far beyond it that the sum overflows, by
-            // the maximum of all.
-            auto add_up = [&]() {
+            // where the others run so far beyond it that the sum overflows, or
+            // where there is a NaN, by the maximum of all and without NaN.
+            auto add_up = [&](bool clean) {
                 const float2 ff = make_float2(-from, -from), cc = make_float2(c2, c2);
                 float2 p = make_float2(0.0f, 0.0f);
 #pragma unroll 4
                 for (int i = 0; i < per; ++i) {
-                    const uint4 r = vmax<E>(buf[i * kThreads], none);
+                    uint4 r = buf[i * kThreads];
                     top = vmax<E>(top, r);
+                    if (clean) r = vmax<E>(r, none);
                     float f[kVec];
                     Elem<E>::unpack(r, f);
 #pragma unroll
@@ -1354,11 +1391,11 @@ __global__ void __launch_bounds__(kThreads, 3) scan_kernel(Args a, ScanShape sha
             for (int i = 0; i < min(per, 4); ++i) top = vmax<E>(top, buf[i * kThreads]);
             const float first = lanes_max<E>(top);
             from = first > neg_inf() ? first : 0.0f;
-            add_up();
+            add_up(false);
             if (!(first > neg_inf()) || !(sum < 1.0e30f)) {
                 from = lanes_max<E>(top);
                 from = from > neg_inf() ? from : 0.0f;
-                add_up();
+                add_up(true);
             }
         } else {
 #pragma unroll 4
@@ -1367,8 +1404,7 @@ __global__ void __launch_bounds__(kThreads, 3) scan_kernel(Args a, ScanShape sha
         const float mine = lanes_max<E>(top);
         // the sums in 64 bits go over the vectors a second time
         const bool again = !kTop && plan.sum;
-        const int64_t next = item + gridDim.x;
-        if (!again && next < items) copy(next);
+        if (!again && more) copy(next, next_part);
         float2 of_warp = make_float2(mine, 0.0f);
         float least = mine > neg_inf() ? mine : FLT_MAX;
 #pragma unroll
@@ -1466,14 +1502,12 @@ __global__ void __launch_bounds__(kThreads, 3) scan_kernel(Args a, ScanShape sha
             for (int o = 16; o > 0; o >>= 1) mass += __shfl_xor_sync(kAll, mass, o);
             if (lane == 0) d8[warp] = mass;
         }
-        if (again && next < items) copy(next);
+        if (again && more) copy(next, next_part);
         // The warp looks through the vectors of those of its threads whose
         // maximum reaches tau, two threads at a time and a vector per lane;
         // they come from L2, as shared memory is on to the next rows.
+        const int64_t item = row * shape.parts + part;
         uint64_t* list = state.lists + item * shape.cap;
-        const uint4* src = reinterpret_cast<const uint4*>(x & ~static_cast<uintptr_t>(15));
-        const E* elems = static_cast<const E*>(a.in.x) + row * a.in.stride;
-        const int v0 = phase > 0 ? 1 : 0, v1 = (V + phase) / kVec;
         for (unsigned have = __ballot_sync(kAll, mine >= tau && mine > neg_inf()); have;) {
             int owner = __ffs(have) - 1;
             have &= have - 1;
@@ -1483,38 +1517,39 @@ __global__ void __launch_bounds__(kThreads, 3) scan_kernel(Args a, ScanShape sha
             const int i = lane % kHold, v = (i * shape.parts + part) * kThreads + warp * 32 + owner;
             if (owner < 0 || i >= per || v >= (V + phase + kVec - 1) / kVec) continue;
             float f[kVec];
-            if (v >= v0 && v < v1) {
-                Elem<E>::unpack(ldg_once(src + v), f);
-            } else {
-#pragma unroll
-                for (int e = 0; e < kVec; ++e) {
-                    const int token = v * kVec + e - phase;
-                    f[e] = token >= 0 && token < V ? Elem<E>::widen(elems[token]) : neg_inf();
-                }
-            }
+            Elem<E>::unpack(v >= here.v0 && v < here.v1 ? ldg_once(here.src + v) : ragged(here, v), f);
 #pragma unroll
             for (int e = 0; e < kVec; ++e) {
                 if (f[e] >= tau && f[e] > neg_inf()) {
-                    const int place = atomicAdd(&listed, 1);
+                    const int place = atomicAdd(listed, 1);
                     if (place < shape.cap) list[place] = entry(f[e], v * kVec + e - phase);
                 }
             }
         }
+        float all = 0.0f;
+        if (kTop && tid < 32) {   // the warps' sums, a warp per lane
+            const float2 of = lane < kWarps ? part8[lane] : make_float2(neg_inf(), 0.0f);
+            all = of.y == 0.0f ? 0.0f : of.y * share(of.x, best, c2);
+#pragma unroll
+            for (int o = kWarps / 2; o > 0; o >>= 1) all += __shfl_xor_sync(kAll, all, o);
+        }
+        // this part's bins were read before, the other ones are in use next
         __syncthreads();
+        if (tid < kScanBins) hist[tid] = 0;
         if (tid == 0) {
-            PartState out = {0.0, best, tau, listed, 0};
-            if (kTop) {
-                float all = 0.0f;
-                for (int w = 0; w < kWarps; ++w)
-                    all += part8[w].y == 0.0f ? 0.0f : part8[w].y * share(part8[w].x, best, c2);
-                out.sum = static_cast<double>(all);
-            } else if (plan.sum && best > neg_inf()) {
+            PartState out = {static_cast<double>(all), best, tau, *listed, 0};
+            if (!kTop && plan.sum && best > neg_inf()) {
+                out.sum = 0.0;
                 for (int w = 0; w < kWarps; ++w) out.sum += d8[w];
             }
             state.parts[item] = out;
+            *listed = 0;
         }
-        __syncthreads();   // listed and the bins are free again
+        row = next_row;
+        part = next_part;
+        here = next;
     }
+    copies_wait<0>();
 }
 
 // The parts' lists in `keys`, best first; how many entries, and from which
