@@ -1969,30 +1969,22 @@ DBS_EXPORT int dbs_device_top_log_probs(const void* logits, int data_type, int64
 }
 
 static dbs_logits::DistillArgs distill_args(const void* logits, int data_type, int64_t rows, int vocab_size,
-                                            int64_t row_stride, const float* teacher_log_probs,
-                                            const void* teacher_tokens, int token_bytes, int slots, float temperature,
-                                            int tail, int reduction, float scale, void* state,
-                                            void* grad_logits) {
+                                            int64_t row_stride, int slots, float temperature, int tail, int reduction,
+                                            float scale, void* state, void* grad_logits) {
     dbs_logits::DistillArgs a;
     a.in = logits_rows(logits, data_type, rows, vocab_size, row_stride);
     if (vocab_size * (data_type == DBS_DTYPE_F32 ? 4LL : 2LL) > dbs_logits::kMaxDistillBytes)
         throw std::invalid_argument("a row to distill takes at most 1040000 bytes");
     positive_temperature(temperature);
     if (slots <= 0 || slots > dbs_logits::kMaxTop) throw std::invalid_argument("slots must be in 1 .. 1024");
-    if (token_bytes != 4 && token_bytes != 8) throw std::invalid_argument("token_bytes must be 4 or 8");
     if (reduction != DBS_REDUCE_NONE && reduction != DBS_REDUCE_SUM && reduction != DBS_REDUCE_MEAN)
         throw std::invalid_argument("unknown reduction");
     if (!std::isfinite(scale)) throw std::invalid_argument("scale must be finite");
-    if (rows > 0 && (!teacher_log_probs || !teacher_tokens))
-        throw std::invalid_argument("teacher_log_probs and teacher_tokens cannot be null");
     if (rows > 0 && !state) throw std::invalid_argument("state cannot be null");
     if (reinterpret_cast<uintptr_t>(state) % 16 != 0) throw std::invalid_argument("state is not aligned to 16 bytes");
     const uintptr_t size = data_type == DBS_DTYPE_F32 ? 4 : 2;
     if (reinterpret_cast<uintptr_t>(grad_logits) % size != 0)
         throw std::invalid_argument("grad_logits is not aligned to its type");
-    a.teacher_log_probs = teacher_log_probs;
-    a.teacher_tokens = teacher_tokens;
-    a.token_bytes = token_bytes;
     a.n = slots;
     a.temperature = temperature;
     a.tail = tail;
@@ -2009,9 +2001,14 @@ DBS_EXPORT int dbs_device_distill(const void* logits, int data_type, int64_t row
                                   float* row_losses, float* loss, void* state, void* grad_logits,
                                   void* cuda_stream) {
     return guarded(nullptr, [&]() {
-        dbs_logits::DistillArgs a =
-            distill_args(logits, data_type, rows, vocab_size, row_stride, teacher_log_probs, teacher_tokens,
-                         token_bytes, slots, temperature, tail, reduction, scale, state, grad_logits);
+        dbs_logits::DistillArgs a = distill_args(logits, data_type, rows, vocab_size, row_stride, slots, temperature,
+                                                 tail, reduction, scale, state, grad_logits);
+        if (token_bytes != 4 && token_bytes != 8) throw std::invalid_argument("token_bytes must be 4 or 8");
+        if (rows > 0 && (!teacher_log_probs || !teacher_tokens))
+            throw std::invalid_argument("teacher_log_probs and teacher_tokens cannot be null");
+        a.teacher_log_probs = teacher_log_probs;
+        a.teacher_tokens = teacher_tokens;
+        a.token_bytes = token_bytes;
         if (rows > 0 && !row_losses) throw std::invalid_argument("row_losses cannot be null");
         if (reduction != DBS_REDUCE_NONE && !loss) throw std::invalid_argument("a reduced loss needs a place");
         a.row_losses = row_losses;
@@ -2032,16 +2029,12 @@ DBS_EXPORT int dbs_device_distill_state_bytes(int64_t rows, int slots, int64_t* 
 }
 
 DBS_EXPORT int dbs_device_distill_backward(const void* logits, int data_type, int64_t rows, int vocab_size,
-                                           int64_t row_stride, const float* teacher_log_probs,
-                                           const void* teacher_tokens, int token_bytes, int slots, float temperature,
-                                           int tail, int reduction, float scale, const void* state,
-                                           const float* grad_loss, int64_t grad_loss_stride, int flags,
+                                           int64_t row_stride, int slots, float temperature, int tail, int reduction,
+                                           float scale, const void* state, const float* grad_loss, int64_t grad_loss_stride, int flags,
                                            void* grad_logits, void* cuda_stream) {
     return guarded(nullptr, [&]() {
-        dbs_logits::DistillArgs a =
-            distill_args(logits, data_type, rows, vocab_size, row_stride, teacher_log_probs, teacher_tokens,
-                         token_bytes, slots, temperature, tail, reduction, scale, const_cast<void*>(state),
-                         grad_logits);
+        dbs_logits::DistillArgs a = distill_args(logits, data_type, rows, vocab_size, row_stride, slots, temperature,
+                                                 tail, reduction, scale, const_cast<void*>(state), grad_logits);
         if (grad_loss_stride < 0) throw std::invalid_argument("grad_loss_stride cannot be negative");
         if ((flags & ~DBS_DEVICE_GRAD_UNIT) != 0) throw std::invalid_argument("unknown flags");
         if (rows == 0) return 0;

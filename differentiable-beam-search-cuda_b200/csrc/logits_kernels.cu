@@ -1221,7 +1221,21 @@ struct ScanShape {
     int parts;
     int cap;
 };
-constexpr int kHold = 16;       // chunks of a part
+#ifndef SH
+#define SH 16
+#endif
+#ifndef SC
+#define SC 3
+#endif
+#ifndef DH
+#define DH 16
+#endif
+#ifndef DC
+#define DC 3
+#endif
+constexpr int kHold = 16;       // most chunks of a part
+constexpr int kScanHold = SH;
+constexpr int kSliceHold = DH;   // vectors of a slice per thread
 constexpr int kScanBins = 128;
 constexpr int kNucleus = 512;   // candidates listed for a top-p without a top-k
 
@@ -1280,7 +1294,7 @@ __device__ __forceinline__ Plan plan_of(const TopArgs& a, int64_t) {
 }
 
 template <class E, class Args, bool kTop>
-__global__ void __launch_bounds__(kThreads, 3) scan_kernel(Args a, ScanShape shape, void* space, bool with_chunks) {
+__global__ void __launch_bounds__(kThreads, SC) scan_kernel(Args a, ScanShape shape, void* space, bool with_chunks) {
     constexpr int kVec = Elem<E>::kVec;
     extern __shared__ uint4 dyn[];
     __shared__ float2 part8[kWarps];
@@ -1364,7 +1378,7 @@ __global__ void __launch_bounds__(kThreads, 3) scan_kernel(Args a, ScanShape sha
         parity ^= 1;
         copies_wait<0>();
         uint4 top = none;
-        float sum = 0.0f, from = 0.0f;
+        float mine = neg_inf(), sum = 0.0f, from = 0.0f;
         const float c2 = fminf(1.4426950408889634f / plan.temperature, FLT_MAX);
         if (kTop) {
             // The thread's exponentials by the maximum of its first vectors;
@@ -1376,10 +1390,12 @@ __global__ void __launch_bounds__(kThreads, 3) scan_kernel(Args a, ScanShape sha
 #pragma unroll 4
                 for (int i = 0; i < per; ++i) {
                     uint4 r = buf[i * kThreads];
-                    top = vmax<E>(top, r);
                     if (clean) r = vmax<E>(r, none);
                     float f[kVec];
                     Elem<E>::unpack(r, f);
+                    // (two 16-bit values at a time would take the exponentials' pipe)
+#pragma unroll
+                    for (int e = 0; e < kVec; e += 2) mine = fmaxf(fmaxf(f[e], f[e + 1]), mine);
 #pragma unroll
                     for (int e = 0; e < kVec; e += 2) {
                         const float2 t = mul2(add2(make_float2(f[e], f[e + 1]), ff), cc);
@@ -1393,15 +1409,14 @@ __global__ void __launch_bounds__(kThreads, 3) scan_kernel(Args a, ScanShape sha
             from = first > neg_inf() ? first : 0.0f;
             add_up(false);
             if (!(first > neg_inf()) || !(sum < 1.0e30f)) {
-                from = lanes_max<E>(top);
-                from = from > neg_inf() ? from : 0.0f;
+                from = mine > neg_inf() ? mine : 0.0f;
                 add_up(true);
             }
         } else {
 #pragma unroll 4
             for (int i = 0; i < per; ++i) top = vmax<E>(top, buf[i * kThreads]);
         }
-        const float mine = lanes_max<E>(top);
+        if (!kTop) mine = lanes_max<E>(top);
         // the sums in 64 bits go over the vectors a second time
         const bool again = !kTop && plan.sum;
         if (!again && more) copy(next, next_part);
@@ -2156,7 +2171,7 @@ struct DistillShared {
 // the slots' threads name the listed elements to the threads that hold them,
 // which make them -inf.
 template <class E, bool kGrad>
-__global__ void __launch_bounds__(kThreads, 3) distill_kernel(DistillArgs a, int S) {
+__global__ void __launch_bounds__(kThreads, DC) distill_kernel(DistillArgs a, int S) {
     constexpr int kVec = Elem<E>::kVec;
     constexpr int kT = kThreads;
     constexpr int kChunk = 4;
@@ -2225,7 +2240,7 @@ __global__ void __launch_bounds__(kThreads, 3) distill_kernel(DistillArgs a, int
     View next = view(in + first_row * a.in.stride);
     if (any_next) {
         if (tid < n) slot = state.slots[first_row * n + tid];
-        for (int i = 0, v = next.v0 + tid; i < kHold; v += kT, ++i) {
+        for (int i = 0, v = next.v0 + tid; i < kSliceHold; v += kT, ++i) {
             if (v < next.v1)
                 copy_async(buf + i * kT, next.src + v);
             else
@@ -2259,7 +2274,7 @@ __global__ void __launch_bounds__(kThreads, 3) distill_kernel(DistillArgs a, int
         const int ragged = lane < head ? lane : tail_at + lane - head;
         const bool at_end = warp == kWarps - 1 && ragged < here.len && here.a0 + ragged >= 0;
         auto copy_next = [&]() {
-            for (int i = 0; i < kHold; ++i) {
+            for (int i = 0; i < kSliceHold; ++i) {
                 if (i < next_count)
                     copy_async(buf + i * kT, src + i * kT);
                 else
@@ -2407,7 +2422,7 @@ __global__ void __launch_bounds__(kThreads, 3) distill_kernel(DistillArgs a, int
             };
             if (same_phase) {
                 uint4* at = buf;
-                for (int i = 0; i < kHold; i += kChunk, at += kChunk * kT, dst += kChunk * kT, src += kChunk * kT) {
+                for (int i = 0; i < kSliceHold; i += kChunk, at += kChunk * kT, dst += kChunk * kT, src += kChunk * kT) {
                     uint4 r[kChunk];
                     if (i + kChunk <= min(count, next_count)) {
 #pragma unroll
@@ -2621,8 +2636,8 @@ int list_space(int n) {
 
 template <class E>
 cudaError_t launch_distill_typed(const DistillArgs& a, cudaStream_t stream) {
-    const Shape sh = shape_of(a.in, sizeof(E), kThreads * kHold * 16);
-    const size_t smem = static_cast<size_t>(kThreads) * kHold * 16;
+    const Shape sh = shape_of(a.in, sizeof(E), kThreads * kSliceHold * 16);
+    const size_t smem = static_cast<size_t>(kThreads) * kSliceHold * 16;
     return a.grad ? launch_rows(distill_kernel<E, true>, a.in, sh.size, smem, stream, kThreads, a, sh.S)
                   : launch_rows(distill_kernel<E, false>, a.in, sh.size, smem, stream, kThreads, a, sh.S);
 }
@@ -2667,7 +2682,7 @@ constexpr int kScanTop = 256;   // longer lists are ordered faster in the cluste
 ScanShape scan_shape(const Rows& in, int es, int take) {
     const int chunk = kThreads * 16 / es;
     const int chunks = (in.V + 16 / es - 1 + chunk - 1) / chunk;
-    int parts = (chunks + kHold - 1) / kHold;
+    int parts = (chunks + kScanHold - 1) / kScanHold;
     while (parts < chunks && parts < 32 && (parts * 100 < take || in.rows * parts < 148 * 2)) ++parts;
     const float mean = static_cast<float>(take) / static_cast<float>(parts);
     const int cap = (static_cast<int>(4.0f * mean + 12.0f * sqrtf(mean)) + 96) / 2 * 2;
@@ -2688,7 +2703,7 @@ template <class E, class Args, bool kTop>
 cudaError_t launch_scan(const Args& a, ScanShape sh, bool chunks, cudaStream_t stream) {
     Rows items = a.in;   // a CTA takes a part at a time
     items.rows *= sh.parts;
-    return launch_rows(scan_kernel<E, Args, kTop>, items, 1, static_cast<size_t>(kThreads) * kHold * 16, stream,
+    return launch_rows(scan_kernel<E, Args, kTop>, items, 1, static_cast<size_t>(kThreads) * kScanHold * 16, stream,
                        kThreads, a, sh, a.space, chunks);
 }
 

@@ -217,7 +217,7 @@ DEVICE_FUNCTIONS = {
         _I, [_VP, _I, _I64, _I, _I64, _VP, _VP, _I, _I, _F, _I, _I, _F, _VP, _VP, _VP, _VP, _VP]),
     "dbs_device_distill_state_bytes": (_I, [_I64, _I, ctypes.POINTER(_I64)]),
     "dbs_device_distill_backward": (
-        _I, [_VP, _I, _I64, _I, _I64, _VP, _VP, _I, _I, _F, _I, _I, _F, _VP, _VP, _I64, _I, _VP, _VP]),
+        _I, [_VP, _I, _I64, _I, _I64, _I, _F, _I, _I, _F, _VP, _VP, _I64, _I, _VP, _VP]),
 }
 
 PROFILED_KERNELS = ("validate", "row_scan", "step_merge", "weights", "fill_zero", "backward")

@@ -19,6 +19,7 @@ without the built library every call raises.
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 import threading
 from dataclasses import dataclass, fields
@@ -488,11 +489,21 @@ _DTYPES = {torch.float32: dbs_ctypes.DBS_DTYPE_F32, torch.float16: dbs_ctypes.DB
 _MAX_ROW_BYTES = 3_000_000
 _MAX_DISTILL_BYTES = 1_040_000
 _MAX_LIST = 1024
+# the current stream's handle without a Stream object around it
+_RAW_STREAM = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
-def _check_global(rc: int, what: str) -> None:
+def _call(name: str, device: torch.device, *args) -> None:
+    """One device entry point on the current stream of `device`, errors raised."""
+    lib = _LIB or _library()
+    stream = _RAW_STREAM(device.index) if _RAW_STREAM else torch.cuda.current_stream(device).cuda_stream
+    if torch.cuda.current_device() == device.index:
+        rc = getattr(lib, name)(*args, stream)
+    else:
+        with torch.cuda.device(device):
+            rc = getattr(lib, name)(*args, stream)
     if rc != 0:
-        raise RuntimeError(f"{what} failed: {_library().dbs_last_global_error().decode()}")
+        raise RuntimeError(f"{name} failed: {lib.dbs_last_global_error().decode()}")
 
 
 def _validate_logits(logits: torch.Tensor, most: int = _MAX_ROW_BYTES) -> None:
@@ -500,8 +511,9 @@ def _validate_logits(logits: torch.Tensor, most: int = _MAX_ROW_BYTES) -> None:
         raise ValueError("logits must be float32, float16 or bfloat16")
     if logits.dim() < 1:
         raise ValueError("logits must have shape [..., V]")
-    _validate_positive_int_dim(logits.size(-1), "V")
-    if logits.size(-1) * logits.element_size() > most:
+    V = logits.size(-1)
+    _validate_positive_int_dim(V, "V")
+    if V * logits.element_size() > most:
         raise ValueError(f"a row of logits takes at most {most} bytes")
 
 
@@ -509,6 +521,8 @@ def _logits_rows(logits: torch.Tensor) -> torch.Tensor:
     """[..., V] as [rows, V] with neighbouring elements in a row: a view where
     the strides allow it, else a copy."""
     V = logits.size(-1)
+    if logits.dim() == 2 and (V == 1 or logits.stride(1) == 1):
+        return logits
     x = logits.detach()
     if V > 1 and x.stride(-1) != 1:
         x = x.contiguous()
@@ -521,18 +535,33 @@ def _logits_rows(logits: torch.Tensor) -> torch.Tensor:
 
 
 def _rows_args(x: torch.Tensor):
-    return _vp(x), _DTYPES[x.dtype], x.size(0), x.size(1), x.stride(0) if x.size(0) > 1 else x.size(1)
+    rows, V = x.shape
+    return x.data_ptr(), _DTYPES[x.dtype], rows, V, x.stride(0) if rows > 1 else V
 
 
-def _workspace(query, x: torch.Tensor, *settings) -> Optional[torch.Tensor]:
-    """Device memory for what passes between a call's kernels, or None."""
+def _ptr(t: Optional[torch.Tensor]):
+    return None if t is None else t.data_ptr()
+
+
+@functools.lru_cache(maxsize=256)
+def _bytes_needed(name: str, *args) -> int:
     size = ctypes.c_int64()
-    _check_global(query(_DTYPES[x.dtype], x.size(0), x.size(1), *settings, size), "workspace")
-    return torch.empty((size.value,), dtype=torch.uint8, device=x.device) if size.value else None
+    lib = _library()
+    if getattr(lib, name)(*args, size) != 0:
+        raise RuntimeError(f"{name} failed: {lib.dbs_last_global_error().decode()}")
+    return size.value
+
+
+def _workspace(name: str, x: torch.Tensor, *settings) -> Optional[torch.Tensor]:
+    """Device memory for what passes between a call's kernels, or None."""
+    size = _bytes_needed(name, _DTYPES[x.dtype], x.size(0), x.size(1), *settings)
+    return torch.empty((size,), dtype=torch.uint8, device=x.device) if size else None
 
 
 def _beside(t: torch.Tensor, name: str, device: torch.device, dtype: torch.dtype, shape) -> torch.Tensor:
     """`t` broadcast to `shape`, contiguous on the logits' device; a tensor on another GPU is refused."""
+    if t.dtype == dtype and t.device == device and t.shape == shape and t.is_contiguous():
+        return t
     if t.is_cuda and t.device != device:
         raise ValueError(f"{name} is on {t.device}, the logits are on {device}")
     try:
@@ -609,13 +638,11 @@ def sample(logits: torch.Tensor, uniforms: torch.Tensor, *, temperature=1.0, top
     u = _beside(uniforms, "uniforms", device, torch.float32, lead)
     tokens = torch.empty(lead, dtype=torch.int32, device=device)
     k_all = min(int(k_all), _INT_MAX)
-    space = _workspace(_library().dbs_device_sample_workspace_bytes, x, k_all if k_rows is None else -1,
-                       p_all if p_rows is None else -1.0)
-    with torch.cuda.device(device):
-        rc = _library().dbs_device_sample(*_rows_args(x), _vp(u), _vp(t_rows), t_all, _vp(k_rows), k_all, _vp(p_rows),
-                                          p_all, _vp(q_rows), q_all, _vp(tokens), _vp(space), _stream_ptr(device))
-    _check_global(rc, "sample")
-    return tokens.to(logits.device)
+    space = _workspace("dbs_device_sample_workspace_bytes", x, k_all if k_rows is None else -1,
+                       float(p_all) if p_rows is None else -1.0)
+    _call("dbs_device_sample", device, *_rows_args(x), u.data_ptr(), _ptr(t_rows), t_all, _ptr(k_rows), k_all,
+          _ptr(p_rows), p_all, _ptr(q_rows), q_all, tokens.data_ptr(), _ptr(space))
+    return tokens if logits.is_cuda else tokens.to(logits.device)
 
 
 def top_log_probs(logits: torch.Tensor, n: int, *, temperature: float = 1.0) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -635,36 +662,26 @@ def top_log_probs(logits: torch.Tensor, n: int, *, temperature: float = 1.0) -> 
     shape = (*logits.shape[:-1], int(n))
     log_probs = torch.empty(shape, dtype=torch.float32, device=device)
     tokens = torch.empty(shape, dtype=torch.int32, device=device)
-    space = _workspace(_library().dbs_device_top_log_probs_workspace_bytes, x, int(n))
-    with torch.cuda.device(device):
-        rc = _library().dbs_device_top_log_probs(*_rows_args(x), int(n), temperature, _vp(log_probs), _vp(tokens),
-                                                 _vp(space), _stream_ptr(device))
-    _check_global(rc, "top_log_probs")
-    return log_probs.to(logits.device), tokens.to(logits.device)
-
-
-def _distill_args(x, log_probs, tokens, settings):
-    temperature, tail, reduction, scale = settings
-    return (*_rows_args(x), _vp(log_probs), _vp(tokens), tokens.element_size(), tokens.size(-1), temperature,
-            int(tail), reduction, scale)
+    space = _workspace("dbs_device_top_log_probs_workspace_bytes", x, int(n))
+    _call("dbs_device_top_log_probs", device, *_rows_args(x), int(n), temperature, log_probs.data_ptr(),
+          tokens.data_ptr(), _ptr(space))
+    return (log_probs, tokens) if logits.is_cuda else (log_probs.to(logits.device), tokens.to(logits.device))
 
 
 def _distill_forward(logits, log_probs, tokens, settings, need_grad):
     """(loss, gradient for an incoming gradient of 1 or None, the rows' state for a backward)."""
     x = _logits_rows(logits)
-    lead, device = logits.shape[:-1], logits.device
-    reduction = settings[2]
-    row_losses = torch.empty(lead, dtype=torch.float32, device=device)
-    loss = row_losses if reduction == 0 else torch.empty((), dtype=torch.float32, device=device)
-    size = ctypes.c_int64()
-    _check_global(_library().dbs_device_distill_state_bytes(x.size(0), tokens.size(-1), size), "distillation_loss")
-    state = torch.empty((size.value,), dtype=torch.uint8, device=device)
+    device, slots = x.device, tokens.size(-1)
+    temperature, tail, reduction, scale = settings
+    loss = torch.empty(logits.shape[:-1] if reduction == 0 else (), dtype=torch.float32, device=device)
+    size = _bytes_needed("dbs_device_distill_state_bytes", x.size(0), slots)
+    # behind the state, where they are not asked for, the rows' losses
+    state = torch.empty((size + (0 if reduction == 0 else 4 * x.size(0)),), dtype=torch.uint8, device=device)
     grad = torch.empty(logits.shape, dtype=logits.dtype, device=device) if need_grad else None
-    with torch.cuda.device(device):
-        rc = _library().dbs_device_distill(*_distill_args(x, log_probs, tokens, settings), _vp(row_losses),
-                                           None if reduction == 0 else _vp(loss), _vp(state), _vp(grad),
-                                           _stream_ptr(device))
-    _check_global(rc, "distillation_loss")
+    at = state.data_ptr()
+    _call("dbs_device_distill", device, *_rows_args(x), log_probs.data_ptr(), tokens.data_ptr(), tokens.element_size(),
+          slots, temperature, tail, reduction, scale, *((loss.data_ptr(), None) if reduction == 0 else
+                                                        (at + size, loss.data_ptr())), at, _ptr(grad))
     return loss, grad, state
 
 
@@ -676,31 +693,37 @@ class _DBSDistillation(torch.autograd.Function):
         # (one rounding) where the incoming gradient is another.
         loss, ctx.grad, state = _distill_forward(logits, log_probs, tokens, settings, True)
         ctx.settings = settings
-        ctx.save_for_backward(logits, log_probs, tokens, state)
+        ctx.slots = tokens.size(-1)
+        ctx.save_for_backward(logits, state)
         return loss
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, grad_output: torch.Tensor):
-        logits, log_probs, tokens, state = ctx.saved_tensors
+        if torch.is_grad_enabled():   # create_graph: there is no second derivative
+            return _DBSDistillation._backward_once(ctx, grad_output)
+        return _DBSDistillation._backward(ctx, grad_output)
+
+    @staticmethod
+    def _backward(ctx, g: torch.Tensor):
+        logits, state = ctx.saved_tensors
         # the forward's buffer serves the first backward; a repeated one
         # (retain_graph) gets a buffer of its own
         grad, ctx.grad = ctx.grad, None
         flags = dbs_ctypes.DBS_DEVICE_GRAD_UNIT
         if grad is None:
             grad, flags = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device), 0
-        g = grad_output.detach().to(dtype=torch.float32)
-        stride = 1
-        if all(s == 0 for s in g.stride()):
-            stride = 0      # one value for all rows
-        else:
-            g = g.contiguous()
+        if g.dtype != torch.float32:
+            g = g.to(torch.float32)
+        stride = 0      # one value for all rows
+        if any(g.stride()):
+            g, stride = g.contiguous(), 1
         x = _logits_rows(logits)
-        with torch.cuda.device(logits.device):
-            rc = _library().dbs_device_distill_backward(*_distill_args(x, log_probs, tokens, ctx.settings), _vp(state),
-                                                        _vp(g), stride, flags, _vp(grad), _stream_ptr(logits.device))
-        _check_global(rc, "distillation_loss backward")
+        temperature, tail, reduction, scale = ctx.settings
+        _call("dbs_device_distill_backward", x.device, *_rows_args(x), ctx.slots, temperature, tail, reduction, scale,
+              state.data_ptr(), g.data_ptr(), stride, flags, grad.data_ptr())
         return grad, None, None, None
+
+    _backward_once = staticmethod(torch.autograd.function.once_differentiable(_backward.__func__))
 
 
 def distillation_loss(logits: torch.Tensor, teacher_log_probs: torch.Tensor, teacher_tokens: torch.Tensor, *,
@@ -745,12 +768,12 @@ def distillation_loss(logits: torch.Tensor, teacher_log_probs: torch.Tensor, tea
     x = logits.to(device)
     log_probs = _beside(teacher_log_probs, "teacher_log_probs", device, torch.float32, teacher_log_probs.shape)
     tokens = _beside(teacher_tokens, "teacher_tokens", device, teacher_tokens.dtype, teacher_tokens.shape)
-    settings = (float(temperature), bool(tail), dbs_ctypes.DBS_REDUCTIONS[reduction], float(scale))
+    settings = (float(temperature), 1 if tail else 0, dbs_ctypes.DBS_REDUCTIONS[reduction], float(scale))
     if grad_on and x.requires_grad:
         loss = _DBSDistillation.apply(x, log_probs, tokens, settings)
     else:
         loss = _distill_forward(x, log_probs, tokens, settings, False)[0]
-    return loss.to(logits.device)
+    return loss if logits.is_cuda else loss.to(logits.device)
 
 
 # ---------------------------------------------------------------------------

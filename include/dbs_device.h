@@ -229,9 +229,8 @@ DBS_EXPORT int dbs_device_distill_state_bytes(int64_t rows, int slots, int64_t* 
  * and rows whose incoming gradient is 1 stay as they are. */
 #define DBS_DEVICE_GRAD_UNIT 2
 DBS_EXPORT int dbs_device_distill_backward(const void* logits, int data_type, int64_t rows, int vocab_size,
-                                           int64_t row_stride, const float* teacher_log_probs,
-                                           const void* teacher_tokens, int token_bytes, int slots, float temperature,
-                                           int tail, int reduction, float scale, const void* state,
+                                           int64_t row_stride, int slots, float temperature, int tail, int reduction,
+                                           float scale, const void* state,
                                            const float* grad_loss, int64_t grad_loss_stride, int flags,
                                            void* grad_logits, void* cuda_stream);
 

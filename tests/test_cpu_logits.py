@@ -121,7 +121,7 @@ def test_c_rows(libdbs, change, message):
     refused(libdbs, libdbs.dbs_device_sample(*rows, P, None, 1.0, None, 0, None, 1.0, None, 0.0, P, P, None), message)
     refused(libdbs, libdbs.dbs_device_top_log_probs(*rows, 1, 1.0, P, P, P, None), message)
     refused(libdbs, libdbs.dbs_device_distill(*rows, P, P, 4, 2, 1.0, 1, 1, 1.0, P, P, P, None, None), message)
-    refused(libdbs, libdbs.dbs_device_distill_backward(*rows, P, P, 4, 2, 1.0, 1, 1, 1.0, P, P, 0, 0, P, None), message)
+    refused(libdbs, libdbs.dbs_device_distill_backward(*rows, 2, 1.0, 1, 1, 1.0, P, P, 0, 0, P, None), message)
 
 
 def test_c_arguments(libdbs):
@@ -165,8 +165,8 @@ def test_c_arguments(libdbs):
     assert libdbs.dbs_device_distill_state_bytes(1, 5, None) == -1
     refused(libdbs, distill(*rows, P, P, 4, 2, 1.0, 1, 1, 1.0, P, P, P, ODD, None), "aligned")
     backward = libdbs.dbs_device_distill_backward
-    refused(libdbs, backward(*rows, P, P, 4, 2, 1.0, 1, 1, 1.0, P, None, 0, 0, P, None), "grad_loss")
-    refused(libdbs, backward(*rows, P, P, 4, 2, 1.0, 1, 1, 1.0, P, P, -1, 0, P, None), "stride")
-    refused(libdbs, backward(*rows, P, P, 4, 2, 1.0, 1, 1, 1.0, P, P, 0, 1, P, None), "flags")
-    refused(libdbs, backward(*rows, P, P, 4, 2, 1.0, 1, 2, 1.0, None, P, 0, 0, P, None), "state")
+    refused(libdbs, backward(*rows, 2, 1.0, 1, 1, 1.0, P, None, 0, 0, P, None), "grad_loss")
+    refused(libdbs, backward(*rows, 2, 1.0, 1, 1, 1.0, P, P, -1, 0, P, None), "stride")
+    refused(libdbs, backward(*rows, 2, 1.0, 1, 1, 1.0, P, P, 0, 1, P, None), "flags")
+    refused(libdbs, backward(*rows, 2, 1.0, 1, 2, 1.0, None, P, 0, 0, P, None), "state")
     assert dc.DBS_REDUCTIONS == {"none": 0, "sum": 1, "mean": 2}
