@@ -72,6 +72,7 @@ struct DistillArgs {
     float* loss = nullptr;                      // the reduced loss; null with kNone
     void* state = nullptr;                      // distill_state_bytes(); written forward, read backward
     int skip_state = 0;                         // backward: the sums are there already
+    int join_losses = 0;                        // set by the launcher: the pass adds up the losses at its end
     void* grad = nullptr;                       // [rows, V] contiguous, the logits' type; null: none
     // backward: gradient of the loss (one value, or one for each row)
     const float* grad_loss = nullptr;

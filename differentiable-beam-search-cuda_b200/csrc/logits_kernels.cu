@@ -1221,21 +1221,7 @@ struct ScanShape {
     int parts;
     int cap;
 };
-#ifndef SH
-#define SH 16
-#endif
-#ifndef SC
-#define SC 3
-#endif
-#ifndef DH
-#define DH 16
-#endif
-#ifndef DC
-#define DC 3
-#endif
-constexpr int kHold = 16;       // most chunks of a part
-constexpr int kScanHold = SH;
-constexpr int kSliceHold = DH;   // vectors of a slice per thread
+constexpr int kHold = 16;       // most chunks of a part, and most vectors of a slice per thread
 constexpr int kScanBins = 128;
 constexpr int kNucleus = 512;   // candidates listed for a top-p without a top-k
 
@@ -1294,7 +1280,7 @@ __device__ __forceinline__ Plan plan_of(const TopArgs& a, int64_t) {
 }
 
 template <class E, class Args, bool kTop>
-__global__ void __launch_bounds__(kThreads, SC) scan_kernel(Args a, ScanShape shape, void* space, bool with_chunks) {
+__global__ void __launch_bounds__(kThreads, 3) scan_kernel(Args a, ScanShape shape, void* space, bool with_chunks) {
     constexpr int kVec = Elem<E>::kVec;
     extern __shared__ uint4 dyn[];
     __shared__ float2 part8[kWarps];
@@ -1970,6 +1956,7 @@ struct DistillState {
     SlotState* slots;  // [rows, n]
     RowState* rows;    // [rows]
     int* any;          // [rows]: the row has slots
+    int* done;         // clusters that have finished their rows
 };
 
 __host__ __device__ __forceinline__ DistillState state_of(const DistillArgs& a) {
@@ -1980,6 +1967,7 @@ __host__ __device__ __forceinline__ DistillState state_of(const DistillArgs& a) 
     s.rows = reinterpret_cast<RowState*>(p);
     p += a.in.rows * static_cast<int64_t>(sizeof(RowState));
     s.any = reinterpret_cast<int*>(p);
+    s.done = s.any + a.in.rows;
     return s;
 }
 
@@ -2036,6 +2024,7 @@ __global__ void __launch_bounds__(256) slots_kernel(DistillArgs a, uint32_t mask
     };
     auto some = [&](bool v) { return kGroup == 32 ? __any_sync(kAll, v) != 0 : __syncthreads_or(v) != 0; };
     for (int i = tid; i < static_cast<int>((mask + 1) / 16); i += kGroup) map[i] = 0;
+    if (blockIdx.x == 0 && threadIdx.x == 0) *state.done = 0;
     sync();
     for (int64_t row = blockIdx.x * static_cast<int64_t>(kRows) + group; row < a.in.rows;
          row += gridDim.x * static_cast<int64_t>(kRows)) {
@@ -2151,6 +2140,85 @@ __global__ void __launch_bounds__(256) slots_kernel(DistillArgs a, uint32_t mask
     }
 }
 
+// A row's loss from its sums. Other CTAs have written them: past L1.
+__device__ double row_loss(const DistillArgs& a, const DistillState& state, int64_t row, double c) {
+    const RowState* at = state.rows + row;
+    const RowState s = {__ldcg(&at->Q), __ldcg(&at->C), __ldcg(&at->best_listed), __ldcg(&at->listed),
+                        __ldcg(&at->best_rest), __ldcg(&at->rest)};
+    const float all = fmaxf(s.best_listed, s.best_rest);
+    auto by = [&](float best, float v) {   // a sum by the row's maximum
+        return v == 0.0f ? 0.0 : static_cast<double>(v) *
+                   (best == all ? 1.0 : exp(c * (static_cast<double>(best) - static_cast<double>(all))));
+    };
+    const double Z = by(s.best_rest, s.rest) + by(s.best_listed, s.listed);
+    if (Z == 0.0) return s.Q > 0.0 ? static_cast<double>(INFINITY) : 0.0;   // nothing above -inf
+    const double left = a.tail && s.rest > 0.0f ? fmax(0.0, 1.0 - s.Q) : 0.0;
+    // log P = c (x - all) - log Z
+    double loss = s.C;
+    if (s.Q != 0.0) {
+        const double up = all == s.best_listed ? 0.0 : static_cast<double>(all) - static_cast<double>(s.best_listed);
+        loss += s.Q * (log(Z) + c * up);
+    }
+    if (left > 0.0) {
+        const double down = all == s.best_rest ? 0.0 : static_cast<double>(all) - static_cast<double>(s.best_rest);
+        loss += left * (log(left * Z / static_cast<double>(s.rest)) + c * down);
+    }
+    return loss;
+}
+
+// The losses of rows first, first + step, ..., and this CTA's part of their
+// sum and number.
+__device__ void add_losses(const DistillArgs& a, const DistillState& state, int64_t first, int64_t step, double* d32,
+                           int* i32, double& sum, int& count) {
+    const double c = static_cast<double>(fminf(1.4426950408889634f / a.temperature, FLT_MAX)) * 0.69314718055994530942;
+    sum = 0.0;
+    count = 0;
+    for (int64_t row = first; row < a.in.rows; row += step) {
+        const bool any = state.any[row] != 0;
+        const double loss = any ? row_loss(a, state, row, c) : 0.0;
+        count += any ? 1 : 0;
+        sum += static_cast<double>(static_cast<float>(loss));
+        a.row_losses[row] = static_cast<float>(a.reduction == kNone ? loss * static_cast<double>(a.scale) : loss);
+    }
+    sum = reduce_block(sum, Add(), d32);
+    count = reduce_block(count, Add(), i32);
+}
+
+__device__ float reduced_loss(const DistillArgs& a, double sum, int count) {
+    sum *= static_cast<double>(a.scale);
+    return static_cast<float>(a.reduction == kMean ? sum / static_cast<double>(max(1, count)) : sum);
+}
+
+// Many rows' losses, and their sum in 64 bits and one order. One cluster of 8
+// CTAs.
+__global__ void __cluster_dims__(8, 1, 1) __launch_bounds__(1024) losses_kernel(DistillArgs a) {
+    __shared__ double d32[32];
+    __shared__ int i32[32];
+    __shared__ double sums[8];
+    __shared__ int counts[8];
+    const Team team;
+    const DistillState state = state_of(a);
+    double sum;
+    int count;
+    add_losses(a, state, team.rank + static_cast<int64_t>(threadIdx.x) * 8, 8 * 1024, d32, i32, sum, count);
+    if (a.reduction == kNone) return;
+    cluster_sync(8);   // everybody has started
+    if (threadIdx.x == 0) {
+        *cg::this_cluster().map_shared_rank(sums + team.rank, 0) = sum;
+        *cg::this_cluster().map_shared_rank(counts + team.rank, 0) = count;
+    }
+    cluster_sync(8);
+    if (team.rank == 0 && threadIdx.x == 0) {
+        sum = 0.0;
+        count = 0;
+        for (int i = 0; i < 8; ++i) {
+            sum += sums[i];
+            count += counts[i];
+        }
+        *a.loss = reduced_loss(a, sum, count);
+    }
+}
+
 struct DistillShared {
     float2 box[2][kMaxCluster];   // reference and sum of the CTAs' slices
     float2 part[kWarps];          // and of the warps' vectors
@@ -2158,6 +2226,8 @@ struct DistillShared {
     uint32_t end_marks[2];        // which of these are listed
     int i32[32];
     uint4 marks[2][kThreads];     // a bit for each of a thread's elements: those that are listed
+    double d32[32];
+    int last;
 };
 
 // One pass over the row gives its sum and (kGrad) its gradient: the logits are
@@ -2171,7 +2241,7 @@ struct DistillShared {
 // the slots' threads name the listed elements to the threads that hold them,
 // which make them -inf.
 template <class E, bool kGrad>
-__global__ void __launch_bounds__(kThreads, DC) distill_kernel(DistillArgs a, int S) {
+__global__ void __launch_bounds__(kThreads, 3) distill_kernel(DistillArgs a, int S) {
     constexpr int kVec = Elem<E>::kVec;
     constexpr int kT = kThreads;
     constexpr int kChunk = 4;
@@ -2240,7 +2310,7 @@ __global__ void __launch_bounds__(kThreads, DC) distill_kernel(DistillArgs a, in
     View next = view(in + first_row * a.in.stride);
     if (any_next) {
         if (tid < n) slot = state.slots[first_row * n + tid];
-        for (int i = 0, v = next.v0 + tid; i < kSliceHold; v += kT, ++i) {
+        for (int i = 0, v = next.v0 + tid; i < kHold; v += kT, ++i) {
             if (v < next.v1)
                 copy_async(buf + i * kT, next.src + v);
             else
@@ -2274,7 +2344,7 @@ __global__ void __launch_bounds__(kThreads, DC) distill_kernel(DistillArgs a, in
         const int ragged = lane < head ? lane : tail_at + lane - head;
         const bool at_end = warp == kWarps - 1 && ragged < here.len && here.a0 + ragged >= 0;
         auto copy_next = [&]() {
-            for (int i = 0; i < kSliceHold; ++i) {
+            for (int i = 0; i < kHold; ++i) {
                 if (i < next_count)
                     copy_async(buf + i * kT, src + i * kT);
                 else
@@ -2422,7 +2492,7 @@ __global__ void __launch_bounds__(kThreads, DC) distill_kernel(DistillArgs a, in
             };
             if (same_phase) {
                 uint4* at = buf;
-                for (int i = 0; i < kSliceHold; i += kChunk, at += kChunk * kT, dst += kChunk * kT, src += kChunk * kT) {
+                for (int i = 0; i < kHold; i += kChunk, at += kChunk * kT, dst += kChunk * kT, src += kChunk * kT) {
                     uint4 r[kChunk];
                     if (i + kChunk <= min(count, next_count)) {
 #pragma unroll
@@ -2475,68 +2545,22 @@ __global__ void __launch_bounds__(kThreads, DC) distill_kernel(DistillArgs a, in
         }
     }
     copies_wait<0>();
+    if (a.join_losses && team.rank == 0) {
+        // the cluster that finishes last has every row's sums
+        if (tid == 0) {
+            __threadfence();
+            sh.last = atomicAdd(state.done, 1) == static_cast<int>(step) - 1 ? 1 : 0;
+            __threadfence();
+        }
+        __syncthreads();
+        if (sh.last) {
+            double sum;
+            int rows;
+            add_losses(a, state, tid, kT, sh.d32, sh.i32, sum, rows);
+            if (tid == 0 && a.reduction != kNone) *a.loss = reduced_loss(a, sum, rows);
+        }
+    }
     cluster_sync(team.size);
-}
-
-// The rows' losses from their sums, and their sum in 64 bits and one order.
-// One cluster of 8 CTAs.
-__global__ void __cluster_dims__(8, 1, 1) __launch_bounds__(1024) losses_kernel(DistillArgs a) {
-    __shared__ double d32[32];
-    __shared__ int i32[32];
-    __shared__ double sums[8];
-    __shared__ int counts[8];
-    const Team team;
-    const DistillState state = state_of(a);
-    const double c = static_cast<double>(fminf(1.4426950408889634f / a.temperature, FLT_MAX)) * 0.69314718055994530942;
-    double sum = 0.0;
-    int count = 0;
-    for (int64_t row = team.rank + static_cast<int64_t>(threadIdx.x) * 8; row < a.in.rows; row += 8 * blockDim.x) {
-        double loss = 0.0;
-        const RowState s = state.rows[row];
-        if (state.any[row]) {
-            ++count;
-            const float all = fmaxf(s.best_listed, s.best_rest);
-            auto by = [&](float best, float v) {   // a sum by the row's maximum
-                return v == 0.0f ? 0.0 : static_cast<double>(v) *
-                           (best == all ? 1.0 : exp(c * (static_cast<double>(best) - static_cast<double>(all))));
-            };
-            const double Z = by(s.best_rest, s.rest) + by(s.best_listed, s.listed);
-            const double left = a.tail && s.rest > 0.0f ? fmax(0.0, 1.0 - s.Q) : 0.0;
-            // log P = c (x - all) - log Z
-            loss = s.C;
-            if (s.Q != 0.0) {
-                const double up = all == s.best_listed ? 0.0 : static_cast<double>(all) - static_cast<double>(s.best_listed);
-                loss += s.Q * (log(Z) + c * up);
-            }
-            if (left > 0.0) {
-                const double down = all == s.best_rest ? 0.0 : static_cast<double>(all) - static_cast<double>(s.best_rest);
-                loss += left * (log(left * Z / static_cast<double>(s.rest)) + c * down);
-            }
-            if (Z == 0.0) loss = s.Q > 0.0 ? static_cast<double>(INFINITY) : 0.0;   // nothing above -inf
-        }
-        sum += static_cast<double>(static_cast<float>(loss));
-        a.row_losses[row] = static_cast<float>(a.reduction == kNone ? loss * static_cast<double>(a.scale) : loss);
-    }
-    if (a.reduction == kNone) return;
-    sum = reduce_block(sum, Add(), d32);
-    count = reduce_block(count, Add(), i32);
-    cluster_sync(8);   // everybody has started
-    if (threadIdx.x == 0) {
-        *cg::this_cluster().map_shared_rank(sums + team.rank, 0) = sum;
-        *cg::this_cluster().map_shared_rank(counts + team.rank, 0) = count;
-    }
-    cluster_sync(8);
-    if (team.rank == 0 && threadIdx.x == 0) {
-        double all = 0.0;
-        int rows = 0;
-        for (int i = 0; i < 8; ++i) {
-            all += sums[i];
-            rows += counts[i];
-        }
-        all *= static_cast<double>(a.scale);
-        if (a.reduction == kMean) all /= static_cast<double>(max(1, rows));
-        *a.loss = static_cast<float>(all);
-    }
 }
 
 // ---------------------------------------------------------------------------
@@ -2636,8 +2660,8 @@ int list_space(int n) {
 
 template <class E>
 cudaError_t launch_distill_typed(const DistillArgs& a, cudaStream_t stream) {
-    const Shape sh = shape_of(a.in, sizeof(E), kThreads * kSliceHold * 16);
-    const size_t smem = static_cast<size_t>(kThreads) * kSliceHold * 16;
+    const Shape sh = shape_of(a.in, sizeof(E), kThreads * kHold * 16);
+    const size_t smem = static_cast<size_t>(kThreads) * kHold * 16;
     return a.grad ? launch_rows(distill_kernel<E, true>, a.in, sh.size, smem, stream, kThreads, a, sh.S)
                   : launch_rows(distill_kernel<E, false>, a.in, sh.size, smem, stream, kThreads, a, sh.S);
 }
@@ -2682,7 +2706,7 @@ constexpr int kScanTop = 256;   // longer lists are ordered faster in the cluste
 ScanShape scan_shape(const Rows& in, int es, int take) {
     const int chunk = kThreads * 16 / es;
     const int chunks = (in.V + 16 / es - 1 + chunk - 1) / chunk;
-    int parts = (chunks + kScanHold - 1) / kScanHold;
+    int parts = (chunks + kHold - 1) / kHold;
     while (parts < chunks && parts < 32 && (parts * 100 < take || in.rows * parts < 148 * 2)) ++parts;
     const float mean = static_cast<float>(take) / static_cast<float>(parts);
     const int cap = (static_cast<int>(4.0f * mean + 12.0f * sqrtf(mean)) + 96) / 2 * 2;
@@ -2703,7 +2727,7 @@ template <class E, class Args, bool kTop>
 cudaError_t launch_scan(const Args& a, ScanShape sh, bool chunks, cudaStream_t stream) {
     Rows items = a.in;   // a CTA takes a part at a time
     items.rows *= sh.parts;
-    return launch_rows(scan_kernel<E, Args, kTop>, items, 1, static_cast<size_t>(kThreads) * kScanHold * 16, stream,
+    return launch_rows(scan_kernel<E, Args, kTop>, items, 1, static_cast<size_t>(kThreads) * kHold * 16, stream,
                        kThreads, a, sh, a.space, chunks);
 }
 
@@ -2780,17 +2804,24 @@ cudaError_t launch_top(const TopArgs& given, cudaStream_t stream) {
     }
 }
 
-cudaError_t launch_distill(const DistillArgs& a, cudaStream_t stream) {
+// Rows up to which the pass itself adds up the losses at its end; a kernel of
+// its own does it for more (at 2048 rows one CTA takes 15 us for them, the
+// launch and its kernel 7 us).
+constexpr int64_t kJoinRows = 512;
+
+cudaError_t launch_distill(const DistillArgs& given, cudaStream_t stream) {
+    DistillArgs a = given;
+    a.join_losses = a.in.rows <= kJoinRows ? 1 : 0;
     if (a.in.rows > 0) {
         cudaError_t err = a.in.dtype == kF32   ? launch_slots<float>(a, stream)
                           : a.in.dtype == kF16 ? launch_slots<__half>(a, stream)
                                                : launch_slots<__nv_bfloat16>(a, stream);
         if (err == cudaSuccess) err = launch_distill_any(a, stream);
-        if (err != cudaSuccess) return err;
+        if (err != cudaSuccess || a.join_losses) return err;
     } else if (a.reduction == kNone) {
         return cudaSuccess;
     }
-    losses_kernel<<<8, a.in.rows <= 4096 ? 256 : 1024, 0, stream>>>(a);
+    losses_kernel<<<8, 1024, 0, stream>>>(a);
     return dbs_dev::count_launch(cudaGetLastError());
 }
 
@@ -2799,7 +2830,7 @@ cudaError_t launch_distill_backward(const DistillArgs& a, cudaStream_t stream) {
 }
 
 int64_t distill_state_bytes(int64_t rows, int n) {
-    return rows * (n * static_cast<int64_t>(sizeof(SlotState)) + static_cast<int64_t>(sizeof(RowState)) + 4);
+    return rows * (n * static_cast<int64_t>(sizeof(SlotState)) + static_cast<int64_t>(sizeof(RowState)) + 4) + 16;
 }
 
 }  // namespace dbs_logits

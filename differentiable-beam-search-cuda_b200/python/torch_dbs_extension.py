@@ -491,13 +491,14 @@ _MAX_DISTILL_BYTES = 1_040_000
 _MAX_LIST = 1024
 # the current stream's handle without a Stream object around it
 _RAW_STREAM = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+_CURRENT_DEVICE = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
 def _call(name: str, device: torch.device, *args) -> None:
     """One device entry point on the current stream of `device`, errors raised."""
     lib = _LIB or _library()
     stream = _RAW_STREAM(device.index) if _RAW_STREAM else torch.cuda.current_stream(device).cuda_stream
-    if torch.cuda.current_device() == device.index:
+    if _CURRENT_DEVICE() == device.index:
         rc = getattr(lib, name)(*args, stream)
     else:
         with torch.cuda.device(device):
@@ -506,15 +507,15 @@ def _call(name: str, device: torch.device, *args) -> None:
         raise RuntimeError(f"{name} failed: {lib.dbs_last_global_error().decode()}")
 
 
-def _validate_logits(logits: torch.Tensor, most: int = _MAX_ROW_BYTES) -> None:
+def _validate_logits(logits: torch.Tensor) -> None:
     if logits.dtype not in _DTYPES:
         raise ValueError("logits must be float32, float16 or bfloat16")
     if logits.dim() < 1:
         raise ValueError("logits must have shape [..., V]")
     V = logits.size(-1)
     _validate_positive_int_dim(V, "V")
-    if V * logits.element_size() > most:
-        raise ValueError(f"a row of logits takes at most {most} bytes")
+    if V * logits.element_size() > _MAX_ROW_BYTES:
+        raise ValueError(f"a row of logits takes at most {_MAX_ROW_BYTES} bytes")
 
 
 def _logits_rows(logits: torch.Tensor) -> torch.Tensor:
@@ -668,32 +669,62 @@ def top_log_probs(logits: torch.Tensor, n: int, *, temperature: float = 1.0) -> 
     return (log_probs, tokens) if logits.is_cuda else (log_probs.to(logits.device), tokens.to(logits.device))
 
 
-def _distill_forward(logits, log_probs, tokens, settings, need_grad):
-    """(loss, gradient for an incoming gradient of 1 or None, the rows' state for a backward)."""
-    x = _logits_rows(logits)
-    device, slots = x.device, tokens.size(-1)
-    temperature, tail, reduction, scale = settings
-    loss = torch.empty(logits.shape[:-1] if reduction == 0 else (), dtype=torch.float32, device=device)
-    size = _bytes_needed("dbs_device_distill_state_bytes", x.size(0), slots)
+@functools.lru_cache(maxsize=1024)
+def _distill_settings(dtype, shape, lq_dtype, lq_shape, at_dtype, at_shape, temperature, tail, reduction, scale):
+    """Checks everything of a call but its tensors' places: (C settings, the loss' shape, bytes of state, of all that it keeps)."""
+    if dtype not in _DTYPES:
+        raise ValueError("logits must be float32, float16 or bfloat16")
+    if not shape:
+        raise ValueError("logits must have shape [..., V]")
+    _validate_positive_int_dim(shape[-1], "V")
+    if shape[-1] * dtype.itemsize > _MAX_DISTILL_BYTES:
+        raise ValueError(f"a row of logits takes at most {_MAX_DISTILL_BYTES} bytes")
+    lead = shape[:-1]
+    if at_dtype not in (torch.int32, torch.int64):
+        raise ValueError("teacher_tokens must be int32 or int64")
+    if not lq_dtype.is_floating_point:
+        raise ValueError("teacher_log_probs must be floating-point")
+    if not at_shape or at_shape[:-1] != lead:
+        raise ValueError(f"teacher_tokens must have shape {(*lead, 'n')}, got {tuple(at_shape)}")
+    if lq_shape != at_shape:
+        raise ValueError("teacher_log_probs and teacher_tokens must have the same shape")
+    if not 1 <= at_shape[-1] <= _MAX_LIST:
+        raise ValueError(f"a teacher's row must have 1 .. {_MAX_LIST} slots")
+    if reduction not in dbs_ctypes.DBS_REDUCTIONS:
+        raise ValueError("reduction must be 'none', 'sum' or 'mean'")
+    _validate_positive_temperature(temperature)
+    _validate_finite_float(scale, "scale")
+    reduction = dbs_ctypes.DBS_REDUCTIONS[reduction]
+    rows = math.prod(lead)
+    size = _bytes_needed("dbs_device_distill_state_bytes", rows, at_shape[-1])
     # behind the state, where they are not asked for, the rows' losses
-    state = torch.empty((size + (0 if reduction == 0 else 4 * x.size(0)),), dtype=torch.uint8, device=device)
+    return ((at_shape[-1], temperature, tail, reduction, scale), lead if reduction == 0 else (), size,
+            size + (0 if reduction == 0 else 4 * rows))
+
+
+def _distill_forward(logits, log_probs, tokens, plan, need_grad):
+    """(loss, gradient for an incoming gradient of 1 or None, the rows' state for a backward)."""
+    settings, loss_shape, state_bytes, kept_bytes = plan
+    x = _logits_rows(logits)
+    device = x.device
+    loss = torch.empty(loss_shape, dtype=torch.float32, device=device)
+    state = torch.empty((kept_bytes,), dtype=torch.uint8, device=device)
     grad = torch.empty(logits.shape, dtype=logits.dtype, device=device) if need_grad else None
     at = state.data_ptr()
+    losses, reduced = (loss.data_ptr(), None) if settings[3] == 0 else (at + state_bytes, loss.data_ptr())
     _call("dbs_device_distill", device, *_rows_args(x), log_probs.data_ptr(), tokens.data_ptr(), tokens.element_size(),
-          slots, temperature, tail, reduction, scale, *((loss.data_ptr(), None) if reduction == 0 else
-                                                        (at + size, loss.data_ptr())), at, _ptr(grad))
+          *settings, losses, reduced, at, None if grad is None else grad.data_ptr())
     return loss, grad, state
 
 
 class _DBSDistillation(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logits: torch.Tensor, log_probs: torch.Tensor, tokens: torch.Tensor, settings):
+    def forward(ctx, logits: torch.Tensor, log_probs: torch.Tensor, tokens: torch.Tensor, plan):
         # The gradient for an incoming gradient of 1 is written in the same
         # pass; the backward keeps it, or computes it again from the logits
         # (one rounding) where the incoming gradient is another.
-        loss, ctx.grad, state = _distill_forward(logits, log_probs, tokens, settings, True)
-        ctx.settings = settings
-        ctx.slots = tokens.size(-1)
+        loss, ctx.grad, state = _distill_forward(logits, log_probs, tokens, plan, True)
+        ctx.settings = plan[0]
         ctx.save_for_backward(logits, state)
         return loss
 
@@ -718,9 +749,8 @@ class _DBSDistillation(torch.autograd.Function):
         if any(g.stride()):
             g, stride = g.contiguous(), 1
         x = _logits_rows(logits)
-        temperature, tail, reduction, scale = ctx.settings
-        _call("dbs_device_distill_backward", x.device, *_rows_args(x), ctx.slots, temperature, tail, reduction, scale,
-              state.data_ptr(), g.data_ptr(), stride, flags, grad.data_ptr())
+        _call("dbs_device_distill_backward", x.device, *_rows_args(x), *ctx.settings, state.data_ptr(), g.data_ptr(),
+              stride, flags, grad.data_ptr())
         return grad, None, None, None
 
     _backward_once = staticmethod(torch.autograd.function.once_differentiable(_backward.__func__))
@@ -745,34 +775,23 @@ def distillation_loss(logits: torch.Tensor, teacher_log_probs: torch.Tensor, tea
     the logits a second time. The loss is float32; gradients flow to the logits
     alone.
     """
-    _validate_logits(logits, _MAX_DISTILL_BYTES)
-    lead = logits.shape[:-1]
-    if teacher_tokens.dtype not in (torch.int32, torch.int64):
-        raise ValueError("teacher_tokens must be int32 or int64")
-    if not teacher_log_probs.is_floating_point():
-        raise ValueError("teacher_log_probs must be floating-point")
-    if teacher_tokens.dim() < 1 or teacher_tokens.shape[:-1] != lead:
-        raise ValueError(f"teacher_tokens must have shape {(*lead, 'n')}, got {tuple(teacher_tokens.shape)}")
-    if teacher_log_probs.shape != teacher_tokens.shape:
-        raise ValueError("teacher_log_probs and teacher_tokens must have the same shape")
-    if not 1 <= teacher_tokens.size(-1) <= _MAX_LIST:
-        raise ValueError(f"a teacher's row must have 1 .. {_MAX_LIST} slots")
-    if reduction not in dbs_ctypes.DBS_REDUCTIONS:
-        raise ValueError("reduction must be 'none', 'sum' or 'mean'")
-    _validate_positive_temperature(temperature)
-    _validate_finite_float(scale, "scale")
-    grad_on = torch.is_grad_enabled()
-    if grad_on and teacher_log_probs.requires_grad:
+    lq, at = teacher_log_probs, teacher_tokens
+    plan = _distill_settings(logits.dtype, logits.shape, lq.dtype, lq.shape, at.dtype, at.shape, float(temperature),
+                             1 if tail else 0, reduction, float(scale))
+    need_grad = torch.is_grad_enabled()
+    if need_grad and lq.requires_grad:
         raise ValueError("teacher_log_probs takes no gradient; detach it")
-    device = _cuda_device_for(logits)
-    x = logits.to(device)
-    log_probs = _beside(teacher_log_probs, "teacher_log_probs", device, torch.float32, teacher_log_probs.shape)
-    tokens = _beside(teacher_tokens, "teacher_tokens", device, teacher_tokens.dtype, teacher_tokens.shape)
-    settings = (float(temperature), 1 if tail else 0, dbs_ctypes.DBS_REDUCTIONS[reduction], float(scale))
-    if grad_on and x.requires_grad:
-        loss = _DBSDistillation.apply(x, log_probs, tokens, settings)
+    if logits.is_cuda:
+        x, device = logits, logits.device
     else:
-        loss = _distill_forward(x, log_probs, tokens, settings, False)[0]
+        device = _cuda_device_for(logits)
+        x = logits.to(device)
+    lq = _beside(lq, "teacher_log_probs", device, torch.float32, lq.shape)
+    at = _beside(at, "teacher_tokens", device, at.dtype, at.shape)
+    if need_grad and x.requires_grad:
+        loss = _DBSDistillation.apply(x, lq, at, plan)
+    else:
+        loss = _distill_forward(x, lq, at, plan, False)[0]
     return loss if logits.is_cuda else loss.to(logits.device)
 
 
