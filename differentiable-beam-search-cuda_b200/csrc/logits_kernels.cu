@@ -22,8 +22,12 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
+// Threads of the kernels that give a row to a cluster (few rows: a row's time
+// counts, and its phases are short of warps).
+constexpr int kTeam = 512;
+constexpr int kTeamWarps = kTeam / 32;
 constexpr int kMaxCluster = 16;
-constexpr int kBins = 4 * kThreads;
+constexpr int kBins = 4 * kTeam;
 constexpr int kSampleList = 512;   // longest top-k that goes through a candidate list
 constexpr uint32_t kAll = 0xFFFFFFFFu;
 
@@ -182,7 +186,7 @@ __device__ __forceinline__ float value_of(uint32_t key) {
 }
 
 // ---------------------------------------------------------------------------
-// Block reductions. `scratch` holds kWarps values; every thread gets the
+// Block reductions. `scratch` holds kTeamWarps values; every thread gets the
 // result, summed in one order.
 // ---------------------------------------------------------------------------
 template <class T, class Op>
@@ -193,7 +197,7 @@ __device__ __forceinline__ T block_reduce(T v, Op op, T* scratch) {
     __syncthreads();
     v = scratch[0];
 #pragma unroll
-    for (int w = 1; w < kWarps; ++w) v = op(v, scratch[w]);
+    for (int w = 1; w < kTeamWarps; ++w) v = op(v, scratch[w]);
     __syncthreads();
     return v;
 }
@@ -263,16 +267,16 @@ __device__ __forceinline__ Slice load_slice(const E* row, int V, int S, int c, u
     const uint4* src = reinterpret_cast<const uint4*>(reinterpret_cast<uintptr_t>(row) -
                                                       static_cast<uintptr_t>(phase) * sizeof(E)) + a0 / kVec;
     const uint4 none = vneg_inf<E>();
-    for (int base = v0 + static_cast<int>(threadIdx.x); base < v1; base += kBatch * kThreads) {
+    for (int base = v0 + static_cast<int>(threadIdx.x); base < v1; base += kBatch * kTeam) {
         uint4 r[kBatch];
 #pragma unroll
         for (int i = 0; i < kBatch; ++i) {
-            const int v = base + i * kThreads;
+            const int v = base + i * kTeam;
             r[i] = v < v1 ? ldg_once(src + v) : none;
         }
 #pragma unroll
         for (int i = 0; i < kBatch; ++i) {
-            const int v = base + i * kThreads;
+            const int v = base + i * kTeam;
             if (kClean) r[i] = vmax<E>(r[i], none);
             acc = vmax<E>(acc, r[i]);
             if (v < v1) buf[v] = r[i];
@@ -357,15 +361,16 @@ struct Shared {
     int counts[kMaxCluster];
     double masses[kMaxCluster];
     int ties[kMaxCluster];
-    double d8[kWarps];
-    unsigned long long u8[kWarps];
-    float f8[kWarps];
-    int i8[kWarps];
-    double range_mass[kWarps];
-    int range_ties[kWarps];
+    double d8[kTeamWarps];
+    unsigned long long u8[kTeamWarps];
+    float f8[kTeamWarps];
+    int i8[kTeamWarps];
+    double range_mass[kTeamWarps];
+    int range_ties[kTeamWarps];
     int listed;
     int found_bin;
     unsigned long long found_above;
+    unsigned long long totals[kMaxCluster];
 };
 
 struct Team {      // a CTA's place in its cluster
@@ -439,6 +444,22 @@ __device__ __forceinline__ unsigned long long fixed(double w) {
     return static_cast<unsigned long long>(__double_as_longlong(w + 512.0) - 0x4080000000000000LL);
 }
 
+// Adds a fixed() weight to a bin in shared memory as three limbs of 15 bits,
+// kBins apart: 32-bit additions that nothing waits for (a 64-bit one is a loop
+// of compare-and-swap), and a slice's elements, fewer than 2^17, do not overflow a limb.
+template <bool kMass>
+__device__ __forceinline__ void add_limbs(uint32_t* bin, unsigned long long w) {
+    if (!kMass) {
+        atomicAdd(bin, static_cast<uint32_t>(w));
+        return;
+    }
+    const uint32_t low = static_cast<uint32_t>(w) & 0x7FFFu, mid = static_cast<uint32_t>(w >> 15) & 0x7FFFu,
+                   high = static_cast<uint32_t>(w >> 30);
+    if (low) atomicAdd(bin, low);
+    if (mid) atomicAdd(bin + kBins, mid);
+    if (high) atomicAdd(bin + 2 * kBins, high);
+}
+
 // Where an ordered row is cut: every key above `key` is kept, and of those
 // equal to it the first `ties` by index.
 struct Cut {
@@ -451,7 +472,7 @@ struct Cut {
 template <class E, class F>
 __device__ __forceinline__ void for_elements(const uint4* buf, const Slice& s, F&& f) {
     const int lane = threadIdx.x & 31;
-    for (int base = (threadIdx.x >> 5) * 32; base < s.nv; base += kThreads) {
+    for (int base = (threadIdx.x >> 5) * 32; base < s.nv; base += kTeam) {
         const int v = base + lane;
         float x[Elem<E>::kVec];
         Elem<E>::unpack(v < s.nv ? buf[v] : vneg_inf<E>(), x);
@@ -479,7 +500,7 @@ struct Found {
 };
 
 template <class E, bool kMass>
-__device__ Found search(const Team& team, Shared& sh, unsigned long long* hist, const uint4* buf, const Slice& s,
+__device__ Found search(const Team& team, Shared& sh, uint32_t* hist, const uint4* buf, const Slice& s,
                         const Weights& weight, float span, uint32_t floor_key, double target, double extra) {
     const float scale = static_cast<float>(kBins - 1) / span;
     const float best = weight.mf;
@@ -495,50 +516,72 @@ __device__ Found search(const Team& team, Shared& sh, unsigned long long* hist, 
         return static_cast<int>(b);
     };
     for (int round = 0;; ++round) {
-        for (int b = threadIdx.x; b < kBins; b += kThreads) hist[b] = 0;
+        for (int b = threadIdx.x; b < 3 * kBins; b += kTeam) hist[b] = 0;
         __syncthreads();
         unsigned long long rest = 0;
-        for_elements<E>(buf, s, [&](float x, int) {
-            const uint32_t k = key_of<E>(x);
-            const int l = lin_bin(x);
-            bool in = k > floor_key;
-            if (round > 0) in = in && l == lin && k >= lo && k <= hi;
-            if (!__any_sync(kAll, in)) return;
-            const unsigned long long w = kMass ? fixed(weight(x)) : 1ull;
-            if (in) {
-                const int b = round == 0 ? l : static_cast<int>((hi - k) >> shift);
-                if (round == 0 && b == kBins - 1)
-                    rest += w;
+        const int lane = threadIdx.x & 31;
+        for (int base = (threadIdx.x >> 5) * 32; base < s.nv; base += kTeam) {
+            constexpr int kVec = Elem<E>::kVec;
+            float x[kVec];
+            int bin[kVec];    // -1: not a member
+            bool any = false;
+            Elem<E>::unpack(base + lane < s.nv ? buf[base + lane] : vneg_inf<E>(), x);
+#pragma unroll
+            for (int e = 0; e < kVec; ++e) {
+                const uint32_t k = key_of<E>(x[e]);
+                const int l = lin_bin(x[e]);
+                bool in = k > floor_key;
+                if (round > 0) in = in && l == lin && k >= lo && k <= hi;
+                bin[e] = in ? (round == 0 ? l : static_cast<int>((hi - k) >> shift)) : -1;
+                any = any || in;
+            }
+            if (!__any_sync(kAll, any)) continue;
+            unsigned long long w[kVec];
+#pragma unroll
+            for (int e = 0; e < kVec; ++e) w[e] = kMass ? fixed(weight(x[e])) : 1ull;
+#pragma unroll
+            for (int e = 0; e < kVec; ++e) {
+                if (bin[e] < 0) continue;
+                if (round == 0 && bin[e] == kBins - 1)
+                    rest += w[e];
                 else
-                    atomicAdd(&hist[b], w);
+                    add_limbs<kMass>(hist + bin[e], w[e]);
             }
-        });
-        if (round == 0 && rest) atomicAdd(&hist[kBins - 1], rest);
+        }
+        if (round == 0) {
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) rest += __shfl_xor_sync(kAll, rest, o);
+            if (lane == 0 && rest) add_limbs<kMass>(hist + kBins - 1, rest);
+        }
         cluster_sync(team.size);
+        // Each CTA adds up its share of the bins over the cluster (all of them
+        // in each would keep the SMs' network busy for microseconds).
+        const int share_bins = (kBins + team.size - 1) / team.size;
+        const int each = (share_bins + kTeam - 1) / kTeam;
+        const int first = team.rank * share_bins + each * static_cast<int>(threadIdx.x);
+        const int last = min(min(kBins, (team.rank + 1) * share_bins), first + each);
         unsigned long long h[4] = {0, 0, 0, 0};
-        for (int c0 = 0; c0 < team.size; c0 += 8) {
-            ulonglong2 theirs[8][2];
+        for (int c = 0; c < team.size; ++c) {
+            const uint32_t* theirs = team.of(hist, c);
 #pragma unroll
-            for (int c = 0; c < 8; ++c) {
-                theirs[c][0] = theirs[c][1] = make_ulonglong2(0, 0);
-                if (c0 + c < team.size) {
-                    const ulonglong2* of = reinterpret_cast<const ulonglong2*>(team.of(hist, c0 + c)) + 2 * threadIdx.x;
-                    theirs[c][0] = of[0];
-                    theirs[c][1] = of[1];
-                }
-            }
+            for (int q = 0; q < 4; ++q) {
+                if (first + q >= last) break;
 #pragma unroll
-            for (int c = 0; c < 8; ++c) {
-                h[0] += theirs[c][0].x;
-                h[1] += theirs[c][0].y;
-                h[2] += theirs[c][1].x;
-                h[3] += theirs[c][1].y;
+                for (int k = 0; k < (kMass ? 3 : 1); ++k)
+                    h[q] += static_cast<unsigned long long>(theirs[k * kBins + first + q]) << (15 * k);
             }
         }
         const unsigned long long own = h[0] + h[1] + h[2] + h[3];
-        const unsigned long long before = above + block_before<unsigned long long>(own, sh.u8);
+        const unsigned long long in_share = block_before<unsigned long long>(own, sh.u8);
+        const unsigned long long of_share = block_reduce(own, Add(), sh.u8);
+        team.tell(sh.totals, of_share);
+        cluster_sync(team.size);
+        unsigned long long total = 0, before = above + in_share;
+        for (int c = 0; c < team.size; ++c) {
+            if (c < team.rank) before += sh.totals[c];
+            total += sh.totals[c];
+        }
         if (round == 0) {
-            const unsigned long long total = block_reduce(own, Add(), sh.u8);
             if (kMass) {
                 out.total = static_cast<double>(total) + extra;
                 target *= out.total;
@@ -554,17 +597,16 @@ __device__ Found search(const Team& team, Shared& sh, unsigned long long* hist, 
         }
         if (static_cast<double>(before) < target && static_cast<double>(before + own) >= target) {
             unsigned long long run = before;
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
+            for (int q = 0; q < 4 && first + q < last; ++q) {
                 const bool here = static_cast<double>(run) < target && static_cast<double>(run + h[q]) >= target;
-                if (here) {
-                    sh.found_bin = 4 * static_cast<int>(threadIdx.x) + q;
-                    sh.found_above = run;
+                for (int c = 0; here && c < team.size; ++c) {
+                    *cg::this_cluster().map_shared_rank(&sh.found_bin, c) = first + q;
+                    *cg::this_cluster().map_shared_rank(&sh.found_above, c) = run;
                 }
                 run += h[q];
             }
         }
-        cluster_sync(team.size);   // also: everybody has read the bins
+        cluster_sync(team.size);
         const int b = sh.found_bin;
         above = sh.found_above;
         __syncthreads();
@@ -598,7 +640,7 @@ __device__ Found search(const Team& team, Shared& sh, unsigned long long* hist, 
 template <class E>
 __device__ __forceinline__ void append_from(Shared& sh, const uint4* buf, const Slice& s, float low, uint64_t* list,
                                             int cap) {
-    for (int v = threadIdx.x; v < s.nv; v += kThreads) {
+    for (int v = threadIdx.x; v < s.nv; v += kTeam) {
         const uint4 r = buf[v];
         if (lanes_max<E>(r) < low) continue;
         float x[Elem<E>::kVec];
@@ -644,7 +686,7 @@ __device__ int gather_best(const Team& team, Shared& sh, const uint4* buf, const
         if (!(span > 0.0f)) span = 1.0f;
         if (!(span < FLT_MAX)) span = FLT_MAX;
         // both lists' space holds the bins: what was listed is listed again below
-        const Found f = search<E, false>(team, sh, reinterpret_cast<unsigned long long*>(list), buf, s, weight, span,
+        const Found f = search<E, false>(team, sh, reinterpret_cast<uint32_t*>(list), buf, s, weight, span,
                                          key_of<E>(neg_inf()), static_cast<double>(n), 0.0);
         const int need = n - static_cast<int>(f.above);
         if (threadIdx.x == 0) sh.listed = 0;
@@ -652,7 +694,7 @@ __device__ int gather_best(const Team& team, Shared& sh, const uint4* buf, const
         append_from<E>(sh, buf, s, value_of<E>(f.key + 1), list, cap);
         // the first `need` of the equal ones, by index: a stretch of
         // neighbouring vectors per thread
-        const int per = (s.nv + kThreads - 1) / kThreads;
+        const int per = (s.nv + kTeam - 1) / kTeam;
         const int begin = min(s.nv, per * static_cast<int>(threadIdx.x)), end = min(s.nv, begin + per);
         int mine = 0;
         for (int v = begin; v < end; ++v) {
@@ -690,10 +732,10 @@ __device__ int gather_best(const Team& team, Shared& sh, const uint4* buf, const
     for (int c = 0; c < team.size; ++c) {
         const int count = sh.counts[c];
         const uint64_t* theirs = team.of(list, c);
-        for (int i = threadIdx.x; i < count; i += kThreads) sorted[at + i] = theirs[i];
+        for (int i = threadIdx.x; i < count; i += kTeam) sorted[at + i] = theirs[i];
         at += count;
     }
-    sort_by<kThreads>(sorted, total);
+    sort_by<kTeam>(sorted, total);
     return min(n, total);
 }
 
@@ -797,7 +839,7 @@ template <class E>
 __device__ __forceinline__ float sum_exp(const uint4* buf, int nv, float c2, const Reference& ref) {
     float p0 = 0.0f, p1 = 0.0f;
     if (ref.wide) {
-        for (int v = threadIdx.x; v < nv; v += kThreads) {
+        for (int v = threadIdx.x; v < nv; v += kTeam) {
             float x[Elem<E>::kVec];
             Elem<E>::unpack(buf[v], x);
 #pragma unroll
@@ -805,7 +847,7 @@ __device__ __forceinline__ float sum_exp(const uint4* buf, int nv, float c2, con
         }
         return p0;
     }
-    for (int v = threadIdx.x; v < nv; v += kThreads) {
+    for (int v = threadIdx.x; v < nv; v += kTeam) {
         float x[Elem<E>::kVec];
         Elem<E>::unpack(buf[v], x);
 #pragma unroll
@@ -821,7 +863,7 @@ __device__ __forceinline__ float sum_exp(const uint4* buf, int nv, float c2, con
 // The best log-probs of a row
 // ---------------------------------------------------------------------------
 template <class E>
-__global__ void __launch_bounds__(kThreads, 3) top_kernel(TopArgs a, int S, int cap) {
+__global__ void __launch_bounds__(kTeam) top_kernel(TopArgs a, int S, int cap) {
     extern __shared__ uint4 dyn[];
     __shared__ Shared sh;
     const Team team;
@@ -858,7 +900,7 @@ __global__ void __launch_bounds__(kThreads, 3) top_kernel(TopArgs a, int S, int 
         const int got = gather_best<E>(team, sh, buf, s, best, n, list, sorted, cap, leader);
         if (team.rank == leader) {
             const double log_z = log(Z);
-            for (int i = threadIdx.x; i < n; i += kThreads) {
+            for (int i = threadIdx.x; i < n; i += kTeam) {
                 float value = neg_inf();
                 int token = -1;
                 if (i < got) {
@@ -889,7 +931,7 @@ __device__ void pick(const Team& team, Shared& sh, const uint4* buf, const Slice
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const double tie = weight(value_of<E>(cut.key));
     // a stretch of the slice per warp
-    const int per = ((s.nv + kWarps - 1) / kWarps + 31) & ~31;
+    const int per = ((s.nv + kTeamWarps - 1) / kTeamWarps + 31) & ~31;
     const int begin = min(s.nv, per * warp), end = min(s.nv, begin + per);
     double mass = 0.0;
     int ties = 0;
@@ -920,7 +962,7 @@ __device__ void pick(const Team& team, Shared& sh, const uint4* buf, const Slice
     __syncthreads();
     double cta_mass = 0.0;
     int cta_ties = 0;
-    for (int w = 0; w < kWarps; ++w) {
+    for (int w = 0; w < kTeamWarps; ++w) {
         cta_mass += sh.range_mass[w];
         cta_ties += sh.range_ties[w];
     }
@@ -961,10 +1003,10 @@ __device__ void pick(const Team& team, Shared& sh, const uint4* buf, const Slice
     int t = 0;
     const int owner = choose(sh.masses, sh.ties, team.size, m, t);
     if (owner == team.rank) {
-        const int w = choose(sh.range_mass, sh.range_ties, kWarps, m, t);
+        const int w = choose(sh.range_mass, sh.range_ties, kTeamWarps, m, t);
         // that stretch again, by the whole CTA: neighbouring vectors per thread
         const int w_begin = min(s.nv, per * max(w, 0)), w_end = min(s.nv, w_begin + per);
-        const int each = (per + kThreads - 1) / kThreads;
+        const int each = (per + kTeam - 1) / kTeam;
         const int t_begin = min(w_end, w_begin + each * static_cast<int>(threadIdx.x));
         const int t_end = min(w_end, t_begin + each);
         double my_mass = 0.0;
@@ -985,7 +1027,7 @@ __device__ void pick(const Team& team, Shared& sh, const uint4* buf, const Slice
         const int t0 = t + block_before(my_ties, sh.i8);
         const bool mine = adds(my_mass, t0, my_ties);
         const bool past = mine && at(m0 + my_mass, t0 + my_ties) > target;
-        const int none = kThreads;
+        const int none = kTeam;
         const int first = block_reduce(past ? static_cast<int>(threadIdx.x) : none, Min(), sh.i8);
         const int last = block_reduce(mine ? static_cast<int>(threadIdx.x) : -1, Max(), sh.i8);
         const int who = first < none ? first : last;
@@ -1020,7 +1062,7 @@ __device__ void pick(const Team& team, Shared& sh, const uint4* buf, const Slice
 __device__ void pick_listed(Shared& sh, const uint64_t* sorted, int count, float best, float temperature, double p,
                             double log_q, double u, double* weight, int* token, int32_t* out) {
     // weights of the ordered entries; a thread holds neighbouring ones
-    const int each = (count + kThreads - 1) / kThreads;
+    const int each = (count + kTeam - 1) / kTeam;
     const int begin = min(count, each * static_cast<int>(threadIdx.x)), end = min(count, begin + each);
     double mine = 0.0;
     for (int i = begin; i < end; ++i) {
@@ -1049,7 +1091,7 @@ __device__ void pick_listed(Shared& sh, const uint64_t* sorted, int count, float
     const double target = u < 1.0 ? u * kept : HUGE_VAL;   // as in pick()
     // the least kept index whose sum of weights up to it passes the target
     int first = 0x7FFFFFFF, last = -1;
-    for (int i = threadIdx.x; i < keep; i += kThreads) {
+    for (int i = threadIdx.x; i < keep; i += kTeam) {
         const int own = token[i];
         double sum = 0.0;
         for (int j = 0; j < keep; ++j) sum += token[j] <= own ? weight[j] : 0.0;
@@ -1064,7 +1106,7 @@ __device__ void pick_listed(Shared& sh, const uint64_t* sorted, int count, float
 }
 
 template <class E>
-__global__ void __launch_bounds__(kThreads, 3) sample_kernel(SampleArgs a, int S, int cap) {
+__global__ void __launch_bounds__(kTeam) sample_kernel(SampleArgs a, int S, int cap) {
     extern __shared__ uint4 dyn[];
     __shared__ Shared sh;
     const Team team;
@@ -1099,7 +1141,7 @@ __global__ void __launch_bounds__(kThreads, 3) sample_kernel(SampleArgs a, int S
         int index = 0x7FFFFFFF;
         if (by_list) tau = threshold<E>(sh, acc, mine, (k + team.size - 1) / team.size);
         if (greedy) {
-            for (int v = threadIdx.x; v < s.nv; v += kThreads) {
+            for (int v = threadIdx.x; v < s.nv; v += kTeam) {
                 float x[Elem<E>::kVec];
                 Elem<E>::unpack(buf[v], x);
 #pragma unroll
@@ -1134,7 +1176,7 @@ __global__ void __launch_bounds__(kThreads, 3) sample_kernel(SampleArgs a, int S
             }
         } else {
             const Weights weight(best, temperature);
-            unsigned long long* hist = reinterpret_cast<unsigned long long*>(list);
+            uint32_t* hist = reinterpret_cast<uint32_t*>(list);
             const uint32_t none = key_of<E>(neg_inf());
             Cut cut{none, 0};
             double cut_mass = 0.0;   // of the equal ones at the top-k cut
@@ -1999,8 +2041,8 @@ template <class E, int kGroup, int kPer>
 __global__ void __launch_bounds__(256) slots_kernel(DistillArgs a, uint32_t mask) {
     constexpr int kRows = 256 / kGroup;   // of a CTA
     extern __shared__ uint32_t maps[];
-    __shared__ double d8[8];
-    __shared__ float f8[8];
+    __shared__ double d8[32];
+    __shared__ float f8[32];
     const int group = threadIdx.x / kGroup, tid = threadIdx.x % kGroup;
     uint32_t* map = maps + group * ((mask + 1) / 16);
     uint32_t* map2 = map + (mask + 1) / 32;
@@ -2020,7 +2062,7 @@ __global__ void __launch_bounds__(256) slots_kernel(DistillArgs a, uint32_t mask
             for (int o = 16; o > 0; o >>= 1) v = op(v, __shfl_xor_sync(kAll, v, o));
             return v;
         }
-        return block_reduce(v, op, scratch);
+        return reduce_block(v, op, scratch);
     };
     auto some = [&](bool v) { return kGroup == 32 ? __any_sync(kAll, v) != 0 : __syncthreads_or(v) != 0; };
     for (int i = tid; i < static_cast<int>((mask + 1) / 16); i += kGroup) map[i] = 0;
@@ -2653,9 +2695,9 @@ cudaError_t launch_rows(Kernel kernel, const Rows& in, int size, size_t smem, cu
 int element_size(int dtype) { return dtype == kF32 ? 4 : 2; }
 
 int list_space(int n) {
-    int cap = kBins / 2;   // both lists' space also holds the bins of a search
+    int cap = kBins / 2;
     while (cap < 2 * n) cap *= 2;
-    return cap;
+    return std::max(cap, 3 * kBins / 4);   // both lists' space also holds the bins of a search
 }
 
 template <class E>
@@ -2776,9 +2818,9 @@ cudaError_t launch_sample(const SampleArgs& given, cudaStream_t stream) {
     const int cap = list_space(a.top_k ? kSampleList : (a.top_k_all <= kSampleList ? std::max(a.top_k_all, 0) : 0));
     const size_t smem = static_cast<size_t>(sh.S) * es + static_cast<size_t>(cap) * 16;
     switch (a.in.dtype) {
-        case kF32: return launch_rows(sample_kernel<float>, a.in, sh.size, smem, stream, kThreads, a, sh.S, cap);
-        case kF16: return launch_rows(sample_kernel<__half>, a.in, sh.size, smem, stream, kThreads, a, sh.S, cap);
-        default: return launch_rows(sample_kernel<__nv_bfloat16>, a.in, sh.size, smem, stream, kThreads, a, sh.S, cap);
+        case kF32: return launch_rows(sample_kernel<float>, a.in, sh.size, smem, stream, kTeam, a, sh.S, cap);
+        case kF16: return launch_rows(sample_kernel<__half>, a.in, sh.size, smem, stream, kTeam, a, sh.S, cap);
+        default: return launch_rows(sample_kernel<__nv_bfloat16>, a.in, sh.size, smem, stream, kTeam, a, sh.S, cap);
     }
 }
 
@@ -2798,9 +2840,9 @@ cudaError_t launch_top(const TopArgs& given, cudaStream_t stream) {
     const int cap = list_space(a.n);
     const size_t smem = static_cast<size_t>(sh.S) * es + static_cast<size_t>(cap) * 16;
     switch (a.in.dtype) {
-        case kF32: return launch_rows(top_kernel<float>, a.in, sh.size, smem, stream, kThreads, a, sh.S, cap);
-        case kF16: return launch_rows(top_kernel<__half>, a.in, sh.size, smem, stream, kThreads, a, sh.S, cap);
-        default: return launch_rows(top_kernel<__nv_bfloat16>, a.in, sh.size, smem, stream, kThreads, a, sh.S, cap);
+        case kF32: return launch_rows(top_kernel<float>, a.in, sh.size, smem, stream, kTeam, a, sh.S, cap);
+        case kF16: return launch_rows(top_kernel<__half>, a.in, sh.size, smem, stream, kTeam, a, sh.S, cap);
+        default: return launch_rows(top_kernel<__nv_bfloat16>, a.in, sh.size, smem, stream, kTeam, a, sh.S, cap);
     }
 }
 
