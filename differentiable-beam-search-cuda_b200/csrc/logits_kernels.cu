@@ -367,6 +367,7 @@ struct Shared {
     int i8[kTeamWarps];
     double range_mass[kTeamWarps];
     int range_ties[kTeamWarps];
+    __align__(16) int steps[128];
     int listed;
     int found_bin;
     unsigned long long found_above;
@@ -735,50 +736,70 @@ __device__ int gather_best(const Team& team, Shared& sh, const uint4* buf, const
         for (int i = threadIdx.x; i < count; i += kTeam) sorted[at + i] = theirs[i];
         at += count;
     }
-    sort_by<kTeam>(sorted, total);
+    if (total > kTeam) {
+        sort_by<kTeam>(sorted, total);
+        return min(n, total);
+    }
+    __syncthreads();   // a short list in order by counting the better ones
+    const int i = threadIdx.x;
+    uint64_t mine = 0;
+    int rank = 0;
+    if (i < total) {
+        mine = sorted[i];
+        int j = 0;
+#pragma unroll 4
+        for (; j + 2 <= total; j += 2) {
+            const ulonglong2 two = *reinterpret_cast<const ulonglong2*>(sorted + j);
+            rank += (two.x > mine ? 1 : 0) + (two.y > mine ? 1 : 0);
+        }
+        if (j < total) rank += sorted[j] > mine ? 1 : 0;
+    }
+    __syncthreads();
+    if (i < total) sorted[rank] = mine;
+    __syncthreads();
     return min(n, total);
 }
 
-// A value at or below the t-th largest of this CTA's element-place maxima
-// (kVec of them per thread), so that at least t of its elements reach it;
-// -inf where fewer than t are above -inf.
+// A value that at least t of this CTA's element-place maxima (kVec of them per
+// thread) reach, and not many more; -inf where fewer than t are above -inf.
+// The maxima are counted in equal steps below `best`, down to the least of the
+// threads' own.
 template <class E>
 __device__ float threshold(Shared& sh, const uint4& acc, float best, int t) {
+    constexpr int kSteps = 128;
     float g[Elem<E>::kVec];
     Elem<E>::unpack(acc, g);
-    auto count = [&](float low) {
-        int c = 0;
-#pragma unroll
-        for (int e = 0; e < Elem<E>::kVec; ++e) c += g[e] >= low ? 1 : 0;
-        return block_reduce(c, Add(), sh.i8);
-    };
-    // the least of the threads' maxima that are above -inf
     const float mine = lanes_max<E>(acc);
-    float lo = block_reduce(mine > neg_inf() ? mine : FLT_MAX, Min(), sh.f8);
-    if (count(lo) < t) {
-        lo = FLT_MAX;
+    if (threadIdx.x < kSteps) sh.steps[threadIdx.x] = 0;
+    const float least = block_reduce(mine > neg_inf() ? mine : FLT_MAX, Min(), sh.f8);
+    const float span = fmaxf(best - least, 1.0e-30f);
+    const float scale = static_cast<float>(kSteps - 1) / span;
 #pragma unroll
-        for (int e = 0; e < Elem<E>::kVec; ++e)
-            if (g[e] > neg_inf()) lo = fminf(lo, g[e]);
-        lo = block_reduce(lo, Min(), sh.f8);
-        if (count(lo) < t) return neg_inf();
+    for (int e = 0; e < Elem<E>::kVec; ++e)
+        if (g[e] > neg_inf()) atomicAdd(&sh.steps[min(kSteps - 1, static_cast<int>((best - g[e]) * scale))], 1);
+    __syncthreads();
+    const int lane = threadIdx.x & 31;
+    const int4 four = reinterpret_cast<const int4*>(sh.steps)[lane];
+    int run = four.x + four.y + four.z + four.w;
+    const int own = run;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int up = __shfl_up_sync(kAll, run, o);
+        if (lane >= o) run += up;
     }
-    // count(lo) >= t throughout; halves the values between, or the keys where
-    // the values' range is too wide for that (masks of the lowest value)
-    float hi = best;
-    const int enough = t + t / 2 + 8;
-    for (int i = 0; i < 40; ++i) {
-        const float mid = hi - lo < 1.0e4f ? 0.5f * lo + 0.5f * hi : unord(ord(lo) + ((ord(hi) - ord(lo)) >> 1));
-        if (!(mid > lo && mid < hi)) break;
-        const int c = count(mid);
-        if (c >= t) {
-            lo = mid;
-            if (c <= enough) break;
-        } else {
-            hi = mid;
-        }
+    int step = kSteps;   // the first one up to which there are enough
+    if (run >= t) {
+        int upto = run - own + four.x;
+        step = 4 * lane;
+        if (upto < t) { ++step; upto += four.y; }
+        if (upto < t) { ++step; upto += four.z; }
+        if (upto < t) ++step;
     }
-    return lo;
+    step = __reduce_min_sync(kAll, step);
+    // the last step holds all that is further down; a hundredth of a step and
+    // the rounding down cover that of (best - g) * scale
+    if (!(best < FLT_MAX) || step >= kSteps - 1) return neg_inf();
+    return __fsub_rd(best, (static_cast<float>(step) + 1.01f) / scale);
 }
 
 __device__ __forceinline__ void copy_async(uint4* to, const uint4* from) {
