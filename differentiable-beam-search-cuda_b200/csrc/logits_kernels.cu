@@ -437,6 +437,23 @@ struct Weights {
         const double p = exp_by(static_cast<double>(x) - m, c, n, tab);
         return x == mf ? 1.0 : (n < -32686 ? 0.0 : p);   // exp(-708) and below count as nothing
     }
+    // For sums by a finite maximum and an ordinary temperature: exp(-690)
+    // stands for all that is less (`low` = m - 690 T), which no sum notices.
+    __device__ __forceinline__ double term(float x, float low) const {
+        const float v = fmaxf(x, low);
+        const int bits = __float_as_int(fmaf(v - mf, cf, 12582912.0f));   // 0x4B400000 + n
+        const double nd = __hiloint2double(0x43300000, bits + static_cast<int>(0x80000000u - 0x4B400000u)) -
+                          4503601774854144.0;
+        const double r = fma(static_cast<double>(v) - m, c, -nd);
+        constexpr double kL = 0.021660849392498290;   // ln 2 / 32
+        double p = fma(r, kL * kL * kL * kL / 24.0, kL * kL * kL / 6.0);
+        p = fma(r, p, kL * kL / 2.0);
+        p = fma(r, p, kL);
+        p = fma(r, p, 1.0);
+        p *= __shfl_sync(kAll, tab, bits & 31);
+        // n / 32 octaves; what 0x4B400000 adds to the shifted bits is beyond them
+        return __hiloint2double(__double2hiint(p) + ((bits << 15) & static_cast<int>(0xFFF00000u)), __double2loint(p));
+    }
 };
 
 // A weight as a whole number of 2^-43: sums of these do not depend on their
@@ -1332,7 +1349,7 @@ __device__ __forceinline__ Plan plan_of(const SampleArgs& a, int64_t row) {
     r.chunks = r.sum && !by_p;
     // the mass of the first k needs all of them, whatever min_p leaves of them
     r.by_low = by_q && !greedy && (r.k == 0 || !by_p);
-    r.left = r.k > kSampleList;
+    r.left = r.k > kSampleList || (r.sum && r.temperature > 1.0e30f);
     return r;
 }
 __device__ __forceinline__ Plan plan_of(const TopArgs& a, int64_t) {
@@ -1528,32 +1545,18 @@ __global__ void __launch_bounds__(kThreads, 3) scan_kernel(Args a, ScanShape sha
         }
         double mass = 0.0;
         if (again && best > neg_inf()) {
-            // Where a warp's vectors hold only terms below e^-17 of the part's
-            // maximum, they are added up in 32 bits: their error, 2^-22 of that,
-            // is lost among the others' 2e-12.
             const Weights weight(best, plan.temperature);
-            const float small_from = best - 17.0f * plan.temperature;
+            const float low = best - 690.0f * plan.temperature;
             for (int i = 0; i < per; ++i) {
                 float f[kVec];
-                Elem<E>::unpack(vmax<E>(buf[i * kThreads], none), f);
-                double w;
-                float large = f[0];
+                Elem<E>::unpack(buf[i * kThreads], f);
+                double w0 = 0.0, w1 = 0.0;
 #pragma unroll
-                for (int e = 1; e < kVec; ++e) large = fmaxf(large, f[e]);
-                if (__any_sync(kAll, large > small_from)) {
-                    double w0 = 0.0, w1 = 0.0;
-#pragma unroll
-                    for (int e = 0; e < kVec; e += 2) {
-                        w0 += weight(f[e]);
-                        w1 += weight(f[e + 1]);
-                    }
-                    w = w0 + w1;
-                } else {
-                    float small = 0.0f;
-#pragma unroll
-                    for (int e = 0; e < kVec; ++e) small += ex2((f[e] - best) * c2);
-                    w = static_cast<double>(small);
+                for (int e = 0; e < kVec; e += 2) {
+                    w0 += weight.term(f[e], low);
+                    w1 += weight.term(f[e + 1], low);
                 }
+                double w = w0 + w1;
                 mass += w;
                 if (plan.chunks) {
 #pragma unroll
@@ -1804,7 +1807,9 @@ __global__ void __launch_bounds__(512) sample_finish_kernel(SampleArgs a, ScanSh
             continue;
         }
         const double T = static_cast<double>(plan.temperature), m = static_cast<double>(best);
-        if (best > FLT_MAX && plan.take != 1) {   // the cluster's kernel knows infinities
+        // the cluster's kernel knows infinities, and maxima from which 690 T is
+        // lost in a float's rounding (see Weights::term)
+        if ((best > FLT_MAX && plan.take != 1) || (plan.sum && fabsf(best) > 1.0e6f * plan.temperature)) {
             leave();
             continue;
         }
@@ -1825,7 +1830,7 @@ __global__ void __launch_bounds__(512) sample_finish_kernel(SampleArgs a, ScanSh
             const int per = ((a.in.V + kVec - 2) / kVec + 1 + kThreads * shape.parts - 1) / (kThreads * shape.parts);
             const int used = per * shape.parts * kWarps;
             const double* sums = state.chunks + row * stretches;
-            if (!(u > 0.0)) {   // the first weight above 0 is wanted, however small
+            if (!(u > 0.0 && u < 1.0)) {   // the first or last weight above 0 is wanted, however small
                 leave();
                 continue;
             }
