@@ -1878,6 +1878,9 @@ static void check_workspace(const void* workspace, int64_t bytes) {
 static void positive_temperature(float temperature) {
     if (!(temperature > 0.0f) || !std::isfinite(temperature))
         throw std::invalid_argument("temperature must be positive and finite");
+    // differences of logits, over it, are taken in 32 bits
+    if (temperature < 1.0e-30f || temperature > 1.0e30f)
+        throw std::invalid_argument("temperature must be in [1e-30, 1e30]");
 }
 
 DBS_EXPORT int dbs_device_sample(const void* logits, int data_type, int64_t rows, int vocab_size, int64_t row_stride,

@@ -419,6 +419,7 @@ __device__ __forceinline__ double exp_by(double d, double c, int n, double tab) 
 struct Weights {
     float mf;
     float cf;
+    float half, cf2;    // m / 2 and 2 c: x - m itself can overflow in 32 bits
     double m;
     double c;
     double tab;    // 2^(lane/32)
@@ -427,12 +428,14 @@ struct Weights {
         m = static_cast<double>(best);
         c = 46.166241308446828384 / static_cast<double>(temperature);   // 32 / ln 2
         cf = static_cast<float>(c);
+        half = 0.5f * best;
+        cf2 = static_cast<float>(2.0 * c);
         tab = exp_table();
     }
     // All 32 lanes of the warp call it together.
     __device__ __forceinline__ double operator()(float x) const {
         // 0 * inf and inf - inf come out as NaN, which fmaxf drops
-        const float t = fmaxf((x - mf) * cf, -40000.0f);
+        const float t = fmaxf(fmaf(x, 0.5f, -half) * cf2, -40000.0f);
         const int n = __float_as_int(t + 12582912.0f) - 0x4B400000;
         const double p = exp_by(static_cast<double>(x) - m, c, n, tab);
         return x == mf ? 1.0 : (n < -32686 ? 0.0 : p);   // exp(-708) and below count as nothing
@@ -501,7 +504,7 @@ __device__ __forceinline__ void for_elements(const uint4* buf, const Slice& s, F
 
 // Finds the value at which the descending row reaches `target`: a count of
 // elements (kMass false) or a sum of fixed() weights. Elements with keys at or
-// below `floor_key` stay out. A round counts or adds up the members of 1024
+// below `floor_key` stay out. A round counts or adds up the members of kBins
 // bins per CTA, adds the cluster's bins and keeps the bin that reaches the
 // target; the first round's bins are equal steps of the value over
 // [best - span, best] (a last one holds the rest), later ones equal steps of
@@ -841,60 +844,23 @@ __device__ __forceinline__ float share(float x, float best, float c2) {
     return best > neg_inf() || best != best ? ex2((x - best) * c2) : 0.0f;
 }
 
-// ---------------------------------------------------------------------------
-// Softmax sums in 32 bits. An exponent is x c2 - B in one fused step, with a
-// whole number B near the maximum that the sum goes by: changing from one
-// CTA's B to the row's is a power of two, and a common rounding of c2 cancels
-// between a term and the sum. Where the maximum is so large (a mask of the
-// type's lowest value) that x c2 could overflow, a term is 1 at the maximum
-// and 0 below it, as neighbouring values there are further apart than any
-// exponent reaches.
-// ---------------------------------------------------------------------------
-struct Reference {
-    float best;
-    float B;
-    bool wide;
-    __device__ Reference(float best_, float c2) : best(best_), B(0.0f), wide(false) {
-        if (best > neg_inf()) {
-            const float b = best * c2;
-            wide = !(fabsf(b) < 1.0e30f) && fabsf(best) <= FLT_MAX;
-            B = wide || !(fabsf(b) < 1.0e30f) ? 0.0f : rintf(b);
-        }
-    }
-    __device__ __forceinline__ float exponent(float x, float c2) const {
-        return wide ? (x == best ? 0.0f : (x < best ? neg_inf() : x - x)) : fmaf(x, c2, -B);
-    }
-    // what a sum taken by `part` is multiplied by to go by this one
-    __device__ double factor(const Reference& part) const {
-        if (!(part.best > neg_inf())) return 1.0;   // nothing, or NaN
-        if (wide || part.wide) return part.best == best ? 1.0 : 0.0;
-        return exp2(static_cast<double>(part.B) - static_cast<double>(B));
-    }
-};
-
-// This thread's share of the slice's sum.
+// This thread's share of the slice's softmax sum, 2^(c2 (x - best)) each: the
+// difference is rounded first, so the same holds for maxima of any size.
 template <class E>
-__device__ __forceinline__ float sum_exp(const uint4* buf, int nv, float c2, const Reference& ref) {
-    float p0 = 0.0f, p1 = 0.0f;
-    if (ref.wide) {
-        for (int v = threadIdx.x; v < nv; v += kTeam) {
-            float x[Elem<E>::kVec];
-            Elem<E>::unpack(buf[v], x);
-#pragma unroll
-            for (int e = 0; e < Elem<E>::kVec; ++e) p0 += ex2(ref.exponent(x[e], c2));
-        }
-        return p0;
-    }
+__device__ __forceinline__ float sum_exp(const uint4* buf, int nv, float c2, float best) {
+    const float from = best > neg_inf() ? -best : 0.0f;
+    const float2 ff = make_float2(from, from), cc = make_float2(c2, c2);
+    float2 p = make_float2(0.0f, 0.0f);
     for (int v = threadIdx.x; v < nv; v += kTeam) {
         float x[Elem<E>::kVec];
         Elem<E>::unpack(buf[v], x);
 #pragma unroll
         for (int e = 0; e < Elem<E>::kVec; e += 2) {
-            p0 += ex2(fmaf(x[e], c2, -ref.B));
-            p1 += ex2(fmaf(x[e + 1], c2, -ref.B));
+            const float2 t = mul2(add2(make_float2(x[e], x[e + 1]), ff), cc);
+            p = add2(p, make_float2(ex2(t.x), ex2(t.y)));
         }
     }
-    return p0 + p1;
+    return p.x + p.y;
 }
 
 // ---------------------------------------------------------------------------
@@ -922,19 +888,20 @@ __global__ void __launch_bounds__(kTeam) top_kernel(TopArgs a, int S, int cap) {
         const Slice s = load_slice<E, true>(static_cast<const E*>(a.in.x) + row * a.in.stride, a.in.V, S, team.rank,
                                             buf, acc);
         const float mine = block_reduce(lanes_max<E>(acc), Max(), sh.f8);
-        const Reference ref(mine, c2);
-        const float part = sum_exp<E>(buf, s.nv, c2, ref);
+        const float part = sum_exp<E>(buf, s.nv, c2, mine);
         const double sum = block_reduce(static_cast<double>(part), Add(), sh.d8);
         const float tau = threshold<E>(sh, acc, mine, (n + team.size - 1) / team.size);
         team.tell(sh.box, Packet{sum, mine, tau, 0});
         cluster_sync(team.size);
         float best = sh.box[0].best;
         for (int c = 1; c < team.size; ++c) best = fmaxf(best, sh.box[c].best);
-        // the sum of 2^((x - best) c2)
-        const Reference all(best, c2);
         double Z = 0.0;
-        for (int c = 0; c < team.size; ++c) Z += sh.box[c].sum * all.factor(Reference(sh.box[c].best, c2));
-        if (!all.wide) Z *= exp2(static_cast<double>(all.B) - static_cast<double>(best) * static_cast<double>(c2));
+        for (int c = 0; c < team.size; ++c) {
+            const Packet& of = sh.box[c];
+            if (of.sum != 0.0)
+                Z += of.sum * (of.best == best ? 1.0 : exp2(static_cast<double>(c2) * (static_cast<double>(of.best) -
+                                                                                       static_cast<double>(best))));
+        }
         const int got = gather_best<E>(team, sh, buf, s, best, n, list, sorted, cap, leader);
         if (team.rank == leader) {
             const double log_z = log(Z);
@@ -1254,7 +1221,7 @@ __global__ void __launch_bounds__(kTeam) sample_kernel(SampleArgs a, int S, int 
                 // kept: x >= m + T ln q, rounded up to a float
                 const float low = __double2float_ru(static_cast<double>(best) +
                                                     static_cast<double>(temperature) * log(q));
-                const uint32_t low_key = best < FLT_MAX ? (key_of<E>(fminf(low, best))) : key_of<E>(best);
+                const uint32_t low_key = key_of<E>(fminf(low, best));
                 // a 16-bit type's key drops low bits: the least key whose value reaches `low`
                 const uint32_t least = value_of<E>(low_key) >= low ? low_key : low_key + 1;
                 if (least > cut.key) {
@@ -1303,6 +1270,7 @@ struct ScanShape {
 };
 constexpr int kHold = 16;       // most chunks of a part, and most vectors of a slice per thread
 constexpr int kScanBins = 128;
+constexpr int kMaxParts = 32;   // a part per lane where they are put together
 constexpr int kNucleus = 512;   // candidates listed for a top-p without a top-k
 
 __host__ __device__ __forceinline__ ScanState scan_of(void* space, int64_t rows, ScanShape sh, bool chunks) {
@@ -1694,7 +1662,6 @@ __device__ Gathered gather_parts(const ScanState& state, ScanShape shape, int64_
     return g;
 }
 
-
 __global__ void __launch_bounds__(256) top_finish_kernel(TopArgs a, ScanShape shape, void* space) {
     extern __shared__ uint64_t keys_space[];
     __shared__ int counters[1];
@@ -1834,7 +1801,7 @@ __global__ void __launch_bounds__(512) sample_finish_kernel(SampleArgs a, ScanSh
                 leave();
                 continue;
             }
-            __shared__ double factors[32];
+            __shared__ double factors[kMaxParts];
             if (warp == 0) factors[lane] = factor;
             __syncthreads();
             const int each = (used + kFinish - 1) / kFinish;
@@ -1986,13 +1953,15 @@ __global__ void __launch_bounds__(512) sample_finish_kernel(SampleArgs a, ScanSh
                     if (first == 0x7FFFFFFF && at > target) first = last;
                 }
             }
-        } else for (int i = tid; i < keep; i += kFinish) {
-            const int own = entry_token(keys[i]);
-            double sum = 0.0;
-            for (int j = 0; j < keep; ++j) sum += entry_token(keys[j]) <= own ? weight[j] : 0.0;
-            if (weight[i] > 0.0) {
-                last = max(last, own);
-                if (sum > target) first = min(first, own);
+        } else {
+            for (int i = tid; i < keep; i += kFinish) {
+                const int own = entry_token(keys[i]);
+                double sum = 0.0;
+                for (int j = 0; j < keep; ++j) sum += entry_token(keys[j]) <= own ? weight[j] : 0.0;
+                if (weight[i] > 0.0) {
+                    last = max(last, own);
+                    if (sum > target) first = min(first, own);
+                }
             }
         }
         first = over_ints(first, Min());
@@ -2775,10 +2744,17 @@ ScanShape scan_shape(const Rows& in, int es, int take) {
     const int chunk = kThreads * 16 / es;
     const int chunks = (in.V + 16 / es - 1 + chunk - 1) / chunk;
     int parts = (chunks + kHold - 1) / kHold;
-    while (parts < chunks && parts < 32 && (parts * 100 < take || in.rows * parts < 148 * 2)) ++parts;
+    while (parts < chunks && parts < kMaxParts && (parts * 100 < take || in.rows * parts < 148 * 2)) ++parts;
     const float mean = static_cast<float>(take) / static_cast<float>(parts);
     const int cap = (static_cast<int>(4.0f * mean + 12.0f * sqrtf(mean)) + 96) / 2 * 2;
     return ScanShape{parts, cap};
+}
+
+// Whether rows of this size are scanned.
+bool scans(const Rows& in) {
+    const int es = element_size(in.dtype);
+    return in.rows >= kScanRows && in.V >= kScanVocab &&
+           (static_cast<int64_t>(in.V) + 16 / es) * es <= static_cast<int64_t>(kMaxParts) * kHold * kThreads * 16;
 }
 
 int sample_take(const SampleArgs& a) {
@@ -2808,12 +2784,14 @@ cudaError_t launch_finish(Kernel kernel, const Args& a, ScanShape sh, int thread
 }  // namespace
 
 int64_t sample_space(const SampleArgs& a) {
-    if (a.in.rows < kScanRows || a.in.V < kScanVocab) return 0;
+    // a longer top-k is the cluster's kernel's for every row
+    const bool long_list = !a.top_k && a.top_k_all > kSampleList && a.top_k_all < a.in.V;
+    if (!scans(a.in) || long_list) return 0;
     return scan_bytes(a.in, scan_shape(a.in, element_size(a.in.dtype), sample_take(a)), true);
 }
 
 int64_t top_space(const TopArgs& a) {
-    if (a.in.rows < kScanRows || a.in.V < kScanVocab || a.n > kScanTop) return 0;
+    if (!scans(a.in) || a.n > kScanTop) return 0;
     return scan_bytes(a.in, scan_shape(a.in, element_size(a.in.dtype), a.n), false);
 }
 

@@ -605,6 +605,8 @@ def _validate_positive_temperature(temperature: float) -> None:
     _validate_finite_float(temperature, "temperature")
     if not temperature > 0.0:
         raise ValueError("temperature must be positive")
+    if not 1e-30 <= temperature <= 1e30:
+        raise ValueError("temperature must be in [1e-30, 1e30]")
 
 
 def sample(logits: torch.Tensor, uniforms: torch.Tensor, *, temperature=1.0, top_k=0, top_p=1.0,
@@ -650,7 +652,7 @@ def top_log_probs(logits: torch.Tensor, n: int, *, temperature: float = 1.0) -> 
     """The n best tokens of each row of raw logits [..., V] and their log-probs
     under softmax(logits / temperature): (float32 [..., n], int32 [..., n]).
 
-    Best first, ties by the lowest token; NaN counts as -inf; n is at most
+    The temperature is in [1e-30, 1e30]. Best first, ties by the lowest token; NaN counts as -inf; n is at most
     min(V, 1024). Places beyond the tokens above -inf hold -inf and -1, which
     `distillation_loss` reads as empty. No gradient flows through it.
     """
@@ -717,6 +719,18 @@ def _distill_forward(logits, log_probs, tokens, plan, need_grad):
     return loss, grad, state
 
 
+class _NoSecondDerivative(torch.autograd.Function):
+    """The gradient as it is, whose own derivative in the logits is an error (and not silently nothing)."""
+
+    @staticmethod
+    def forward(ctx, logits: torch.Tensor, grad: torch.Tensor):
+        return grad.detach()
+
+    @staticmethod
+    def backward(ctx, grad_output: torch.Tensor):
+        raise RuntimeError("distillation_loss cannot be differentiated twice")
+
+
 class _DBSDistillation(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits: torch.Tensor, log_probs: torch.Tensor, tokens: torch.Tensor, plan):
@@ -730,9 +744,11 @@ class _DBSDistillation(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, grad_output: torch.Tensor):
-        if torch.is_grad_enabled():   # create_graph: there is no second derivative
-            return _DBSDistillation._backward_once(ctx, grad_output)
-        return _DBSDistillation._backward(ctx, grad_output)
+        if torch.is_grad_enabled():   # create_graph
+            with torch.no_grad():
+                grad = _DBSDistillation._backward(ctx, grad_output)
+            return _NoSecondDerivative.apply(ctx.saved_tensors[0], grad), None, None, None
+        return _DBSDistillation._backward(ctx, grad_output), None, None, None
 
     @staticmethod
     def _backward(ctx, g: torch.Tensor):
@@ -751,9 +767,7 @@ class _DBSDistillation(torch.autograd.Function):
         x = _logits_rows(logits)
         _call("dbs_device_distill_backward", x.device, *_rows_args(x), *ctx.settings, state.data_ptr(), g.data_ptr(),
               stride, flags, grad.data_ptr())
-        return grad, None, None, None
-
-    _backward_once = staticmethod(torch.autograd.function.once_differentiable(_backward.__func__))
+        return grad
 
 
 def distillation_loss(logits: torch.Tensor, teacher_log_probs: torch.Tensor, teacher_tokens: torch.Tensor, *,
@@ -763,7 +777,7 @@ def distillation_loss(logits: torch.Tensor, teacher_log_probs: torch.Tensor, tea
     log-probs (as `top_log_probs` gives them), with its gradient in the logits.
 
     logits [..., V]; teacher_log_probs and teacher_tokens (int32 or int64)
-    [..., n], n <= 1024, at the same temperature. A slot whose token is outside
+    [..., n], n <= 1024, at the same temperature, in [1e-30, 1e30]. A slot whose token is outside
     [0, V) is empty. With P the student's probabilities and q the teacher's, a
     row's loss is sum q (log q - log P) over its slots; with `tail`, all tokens
     that are not listed make up one more class of mass 1 - sum q (without it,

@@ -189,7 +189,7 @@ DBS_EXPORT int dbs_device_sample_workspace_bytes(int data_type, int64_t rows, in
 
 /* The n best tokens of each row (logit desc, token asc; NaN counts as -inf)
  * and their log-probs under softmax(logits / temperature): log_probs and
- * tokens [rows, n], n <= min(vocab_size, 1024). Places beyond the tokens above
+ * tokens [rows, n], n <= min(vocab_size, 1024); temperature in [1e-30, 1e30]. Places beyond the tokens above
  * -inf hold -inf and -1. */
 DBS_EXPORT int dbs_device_top_log_probs(const void* logits, int data_type, int64_t rows, int vocab_size,
                                         int64_t row_stride, int n, float temperature, float* log_probs,
@@ -211,7 +211,8 @@ DBS_EXPORT int dbs_device_top_log_probs_workspace_bytes(int data_type, int64_t r
  * logits' type, or NULL) takes the gradient for an incoming gradient of 1, in
  * the same pass over the logits. `state` is dbs_device_distill_state_bytes
  * bytes of device memory, 16-byte aligned, that the call fills and a backward
- * of it reads. A row holds at most 1040000 bytes here. */
+ * of it reads. A row holds at most 1040000 bytes here, and the temperature is
+ * in [1e-30, 1e30]. */
 #define DBS_REDUCE_NONE 0
 #define DBS_REDUCE_SUM 1
 #define DBS_REDUCE_MEAN 2

@@ -170,3 +170,15 @@ def test_c_arguments(libdbs):
     refused(libdbs, backward(*rows, 2, 1.0, 1, 1, 1.0, P, P, 0, 1, P, None), "flags")
     refused(libdbs, backward(*rows, 2, 1.0, 1, 2, 1.0, None, P, 0, 0, P, None), "state")
     assert dc.DBS_REDUCTIONS == {"none": 0, "sum": 1, "mean": 2}
+
+
+@pytest.mark.parametrize("temperature", [1e-31, 1e31])
+def test_temperatures_beyond_32_bits(libdbs, temperature):
+    with pytest.raises(ValueError, match="1e-30"):
+        ext.top_log_probs(X, 4, temperature=temperature)
+    with pytest.raises(ValueError, match="1e-30"):
+        ext.distillation_loss(X, LQ, AT, temperature=temperature)
+    rows = (P, 0, 1, 16, 16)
+    refused(libdbs, libdbs.dbs_device_top_log_probs(*rows, 4, temperature, P, P, None, None), "1e-30")
+    refused(libdbs, libdbs.dbs_device_distill(*rows, P, P, 4, 2, temperature, 1, 1, 1.0, P, P, P, None, None), "1e-30")
+    refused(libdbs, libdbs.dbs_device_distill_backward(*rows, 2, temperature, 1, 1, 1.0, P, P, 0, 0, P, None), "1e-30")

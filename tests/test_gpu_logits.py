@@ -151,6 +151,7 @@ def test_sample_temperatures(temperature):
 
 def check_top(x, n, temperature=1.0, dev=None):
     want, tokens = ref.top_log_probs(x, n, temperature)
+    want = np.where(want < -np.finfo(np.float32).max, -np.inf, want)   # a masked value over 1e-30 is beyond float32
     got, at = ext.top_log_probs(x.cuda() if dev is None else dev, n, temperature=temperature)
     assert got.dtype == torch.float32 and at.dtype == torch.int32
     assert np.array_equal(at.cpu().numpy(), tokens)
@@ -510,3 +511,82 @@ def test_rows_behind_the_last_stay_as_they_are():
     torch.cuda.synchronize()
     assert torch.all(values[5:] == 7.0) and torch.all(tokens[5:] == 7) and torch.all(grad[5:] == 7.0) and torch.all(losses[5:] == 7.0)
     assert torch.all(tokens[:5] >= 0) and torch.all(state[size.value:] == 7)
+
+
+@pytest.mark.parametrize("N,V,dtype", [(33, 520_000, torch.float32), (32, 600_000, torch.float32), (33, 1_048_570, torch.bfloat16),
+                                       (32, 1_300_001, torch.float16)])
+def test_batches_of_long_rows(N, V, dtype):
+    """Rows of as many parts as the scan puts together, and of more."""
+    x, u = rows(N, V, dtype, V), uniforms(N, V)
+    dev = x.cuda()
+    check_sample(x, u, T=0.9, dev=dev)
+    check_sample(x, u, k=100, p=0.95, dev=dev)
+    check_sample(x, u, p=0.5, dev=dev)
+    check_top(x, 40, dev=dev)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("N", [3, 40])
+def test_sample_ratio_at_the_ends_of_the_type(N, dtype):
+    x = torch.full((N, 9001), LOWEST[dtype], dtype=dtype)
+    x[:, 77::100] = torch.finfo(dtype).max
+    x[:, 5::1000] = torch.finfo(dtype).max / 2
+    u = uniforms(N, 1)
+    for T in (1.0, torch.finfo(dtype).max):
+        for q in (0.5, 0.7, 0.99):
+            check_sample(x, u, T=T, q=q)
+            check_sample(x, u, T=T, q=q, p=0.5)
+
+
+@pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
+@pytest.mark.parametrize("N", [512, 513, 9000])
+def test_distillation_of_many_rows(N, reduction):
+    lq, at = teacher(N, 130, 5, N)
+    check_distill(rows(N, 130, torch.bfloat16, N), lq, at, reduction=reduction)
+
+
+def test_distillation_has_no_second_derivative():
+    x = rows(6, 500, torch.float32, 7).cuda().requires_grad_(True)
+    lq, at = (t.cuda() for t in teacher(6, 500, 9, 7))
+    plain, = torch.autograd.grad(ext.distillation_loss(x, lq, at), x)
+    again, = torch.autograd.grad(ext.distillation_loss(x, lq, at), x, create_graph=True)
+    assert torch.equal(plain, again)
+    with pytest.raises(RuntimeError, match="differentiated twice"):
+        torch.autograd.grad(again.sum(), x)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("N", [3, 40])
+@pytest.mark.parametrize("temperature", [1e-30, 1e30])
+def test_temperatures_at_their_ends(N, dtype, temperature):
+    x = rows(N, 9001, torch.float32, 11)
+    x[0] = 2.5
+    x[1, 3:] = LOWEST[dtype]
+    x[2, :40] = torch.finfo(dtype).max
+    x = x.to(dtype)
+    check_top(x, 20, temperature=temperature)
+    lq, at = teacher(N, 9001, 6, 11, pad=0.0)
+    x[:3] = 1.5                                   # (losses below stay finite in 32 bits)
+    if temperature > 1.0:
+        check_distill(x, lq, at, T=temperature, scale=1e30)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("N", [12, 48])
+def test_rows_far_from_zero(N, dtype):
+    """Masks of any size that leave nothing, and logits with a common offset."""
+    x = rows(N, 9001, torch.float32, 13)
+    for r, size in enumerate((1e4, 1e6, 1e8, 1e9, 1e10, 1e12, 1e15, 1e20, 1e30)):
+        x[r] = -size
+        x[r, 100 * r:100 * r + 7] = -size * (1.0 - 2.0 ** -6)
+    x[9] += 3e5
+    x[10] -= 3e5
+    x = x.to(dtype)
+    check_top(x, 30)
+    check_top(x, 30, temperature=0.3)
+    for settings in (dict(), dict(k=20), dict(p=0.7), dict(q=0.3)):
+        check_sample(x, uniforms(N, 13), **settings)
+    lq, at = teacher(N, 9001, 6, 11, pad=0.0)
+    at[:9, 0] = 100 * torch.arange(9)            # the best class
+    lq[:9, 0], lq[:9, 1:] = 0.0, -math.inf
+    check_distill(x, lq, at, reduction="none")
