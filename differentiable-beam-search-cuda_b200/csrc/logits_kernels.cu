@@ -214,9 +214,9 @@ struct Min {
     __device__ T operator()(T a, T b) const { return a < b ? a : b; }
 };
 
-// Sum of the values of the threads before this one.
+// Sum of the values of the threads before this one, and (`all`) of all.
 template <class T>
-__device__ __forceinline__ T block_before(T v, T* scratch) {
+__device__ __forceinline__ T block_before(T v, T* scratch, T* all = nullptr) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     T incl = v;
 #pragma unroll
@@ -226,9 +226,15 @@ __device__ __forceinline__ T block_before(T v, T* scratch) {
     }
     if (lane == 31) scratch[warp] = incl;
     __syncthreads();
-    T base = T(0);
-    for (int w = 0; w < warp; ++w) base += scratch[w];
+    T base = T(0), total = T(0);
+#pragma unroll
+    for (int w = 0; w < kTeamWarps; ++w) {
+        const T of = scratch[w];
+        base += w < warp ? of : T(0);
+        total += of;
+    }
     __syncthreads();
+    if (all) *all = total;
     T excl = __shfl_up_sync(kAll, incl, 1);
     if (lane == 0) excl = T(0);
     return base + excl;
@@ -557,13 +563,22 @@ __device__ Found search(const Team& team, Shared& sh, uint32_t* hist, const uint
                 any = any || in;
             }
             if (!__any_sync(kAll, any)) continue;
+            if (round > 0) {   // one bin of many: few of a vector's elements
+#pragma unroll
+                for (int e = 0; e < kVec; ++e) {
+                    if (!__any_sync(kAll, bin[e] >= 0)) continue;
+                    const unsigned long long w = kMass ? fixed(weight(x[e])) : 1ull;
+                    if (bin[e] >= 0) add_limbs<kMass>(hist + bin[e], w);
+                }
+                continue;
+            }
             unsigned long long w[kVec];
 #pragma unroll
             for (int e = 0; e < kVec; ++e) w[e] = kMass ? fixed(weight(x[e])) : 1ull;
 #pragma unroll
             for (int e = 0; e < kVec; ++e) {
                 if (bin[e] < 0) continue;
-                if (round == 0 && bin[e] == kBins - 1)
+                if (bin[e] == kBins - 1)
                     rest += w[e];
                 else
                     add_limbs<kMass>(hist + bin[e], w[e]);
@@ -582,19 +597,23 @@ __device__ Found search(const Team& team, Shared& sh, uint32_t* hist, const uint
         const int first = team.rank * share_bins + each * static_cast<int>(threadIdx.x);
         const int last = min(min(kBins, (team.rank + 1) * share_bins), first + each);
         unsigned long long h[4] = {0, 0, 0, 0};
-        for (int c = 0; c < team.size; ++c) {
-            const uint32_t* theirs = team.of(hist, c);
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                if (first + q >= last) break;
+        for (int q = 0; q < 4; ++q) {
+            if (first + q >= last) break;
+            for (int c0 = 0; c0 < team.size; c0 += 8) {
 #pragma unroll
-                for (int k = 0; k < (kMass ? 3 : 1); ++k)
-                    h[q] += static_cast<unsigned long long>(theirs[k * kBins + first + q]) << (15 * k);
+                for (int c = 0; c < 8; ++c) {   // the loads of eight CTAs' bins in flight together
+                    if (c0 + c >= team.size) continue;
+                    const uint32_t* theirs = team.of(hist, c0 + c);
+#pragma unroll
+                    for (int k = 0; k < (kMass ? 3 : 1); ++k)
+                        h[q] += static_cast<unsigned long long>(theirs[k * kBins + first + q]) << (15 * k);
+                }
             }
         }
         const unsigned long long own = h[0] + h[1] + h[2] + h[3];
-        const unsigned long long in_share = block_before<unsigned long long>(own, sh.u8);
-        const unsigned long long of_share = block_reduce(own, Add(), sh.u8);
+        unsigned long long of_share;
+        const unsigned long long in_share = block_before<unsigned long long>(own, sh.u8, &of_share);
         team.tell(sh.totals, of_share);
         cluster_sync(team.size);
         unsigned long long total = 0, before = above + in_share;
@@ -944,16 +963,19 @@ __device__ void pick(const Team& team, Shared& sh, const uint4* buf, const Slice
         const int v = base + lane;
         float x[kVec];
         Elem<E>::unpack(v < end ? buf[v] : vneg_inf<E>(), x);
+        bool any = false;
 #pragma unroll
         for (int e = 0; e < kVec; ++e) {
             const uint32_t k = key_of<E>(x[e]);
             ties += k == cut.key ? 1 : 0;
-            const bool in = k > cut.key;
-            if (__any_sync(kAll, in)) {
-                const double w = weight(x[e]);
-                mass += in ? w : 0.0;
-            }
+            any = any || k > cut.key;
         }
+        if (!__any_sync(kAll, any)) continue;
+        double w[kVec];
+#pragma unroll
+        for (int e = 0; e < kVec; ++e) w[e] = weight(x[e]);
+#pragma unroll
+        for (int e = 0; e < kVec; ++e) mass += key_of<E>(x[e]) > cut.key ? w[e] : 0.0;
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
