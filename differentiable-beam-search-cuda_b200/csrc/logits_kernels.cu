@@ -318,7 +318,8 @@ __device__ __forceinline__ float lanes_max(const uint4& v) {
 }
 
 // Descending sort of n keys in shared memory: a bitonic network whose runs
-// all have the same direction, so n need not be a power of two.
+// all have the same direction, so n need not be a power of two. Steps of up to
+// 32 places keep a warp within its own 64 keys, and wait for the warp alone.
 template <int kT>
 __device__ void sort_by(uint64_t* a, int n) {
     int n2 = 1;
@@ -339,9 +340,14 @@ __device__ void sort_by(uint64_t* a, int n) {
                     }
                 }
             }
-            __syncthreads();
+            const int next = st > 1 ? st >> 1 : size;
+            if (st > 32 || next > 32)
+                __syncthreads();
+            else
+                __syncwarp();
         }
     }
+    __syncthreads();
 }
 
 __device__ __forceinline__ uint64_t entry(float x, int token) {
@@ -1609,84 +1615,74 @@ __global__ void __launch_bounds__(kThreads, 3) scan_kernel(Args a, ScanShape sha
     copies_wait<0>();
 }
 
-// The parts' lists in `keys`, best first; how many entries, and from which
-// value on none is missing. -1: a list overflowed.
+// The entries of the parts' lists that reach every part's threshold, in `keys`,
+// best first: none is missing between them.
 struct Gathered {
-    int count;
-    int whole;     // of them, those that reach every part's threshold
+    int count;     // -1: a list overflowed
     float best;
     float tau;     // the highest of the parts' thresholds
     bool all;      // every element above -inf is there
 };
 template <int kT>
 __device__ Gathered gather_parts(const ScanState& state, ScanShape shape, int64_t row, uint64_t* keys, uint64_t* other,
-                                 int* counters) {
+                                 int* counter) {
     const PartState* parts = state.parts + row * shape.parts;
-    Gathered g = {0, 0, neg_inf(), neg_inf(), true};
+    Gathered g;
     // a part per lane, by every warp
     const int lane = threadIdx.x % 32;
     PartState mine = {0.0, neg_inf(), neg_inf(), 0, 0};
     if (lane < shape.parts) mine = parts[lane];
-    const bool over = __any_sync(kAll, mine.count > shape.cap) != 0;
-    float tau = mine.best > neg_inf() ? mine.tau : neg_inf();
     g.best = mine.best;
-    int before = mine.count;
+    g.tau = mine.best > neg_inf() ? mine.tau : neg_inf();
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
         g.best = fmaxf(g.best, __shfl_xor_sync(kAll, g.best, o));
-        tau = fmaxf(tau, __shfl_xor_sync(kAll, tau, o));
+        g.tau = fmaxf(g.tau, __shfl_xor_sync(kAll, g.tau, o));
     }
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const int up = __shfl_up_sync(kAll, before, o);
-        if (lane >= o) before += up;
-    }
-    g.count = __shfl_sync(kAll, before, 31);
-    before -= mine.count;
-    g.all = !(tau > neg_inf());
-    g.tau = tau;
-    if (over) {
-        g.count = -1;
-        return g;
-    }
-    if (threadIdx.x == 0) counters[0] = 0;
+    g.all = !(g.tau > neg_inf());
+    g.count = -1;
+    if (__any_sync(kAll, mine.count > shape.cap)) return g;
+    if (threadIdx.x == 0) *counter = 0;
     __syncthreads();
     // a part's entries by a warp
-    for (int s = 0; s < shape.parts; ++s) {
-        const int to = __shfl_sync(kAll, before, s), count = __shfl_sync(kAll, mine.count, s);
-        if (s % (kT / 32) != static_cast<int>(threadIdx.x) / 32) continue;
+    for (int s = threadIdx.x / 32; s < shape.parts; s += kT / 32) {
+        const int count = __shfl_sync(kAll, mine.count, s);
         const uint64_t* list = state.lists + (row * shape.parts + s) * shape.cap;
-        for (int i = lane; i < count; i += 32) other[to + i] = list[i];
+        for (int i = lane; i - lane < count; i += 32) {
+            const uint64_t e = i < count ? list[i] : 0;
+            const bool in = i < count && entry_value(e) >= g.tau;
+            const unsigned all = __ballot_sync(kAll, in);
+            int at = lane == 0 ? atomicAdd(counter, __popc(all)) : 0;
+            at = __shfl_sync(kAll, at, 0) + __popc(all & ((1u << lane) - 1u));
+            if (in) other[at] = e;
+        }
     }
     __syncthreads();
-    int whole = 0;
-    for (int i = threadIdx.x; i < g.count; i += kT) whole += entry_value(other[i]) >= tau ? 1 : 0;
+    g.count = *counter;
     if (g.count > kT) {
         sort_by<kT>(other, g.count);
         for (int i = threadIdx.x; i < g.count; i += kT) keys[i] = other[i];
     }
     // a short list in order by counting the better ones
-    for (int i = threadIdx.x; i < g.count && g.count <= kT; i += kT) {
-        const uint64_t mine = other[i];
+    const int i = threadIdx.x;
+    if (i < g.count && g.count <= kT) {
+        const uint64_t own = other[i];
         int rank = 0;
         int j = 0;
         for (; j + 2 <= g.count; j += 2) {
             const ulonglong2 two = *reinterpret_cast<const ulonglong2*>(other + j);
-            rank += (two.x > mine ? 1 : 0) + (two.y > mine ? 1 : 0);
+            rank += (two.x > own ? 1 : 0) + (two.y > own ? 1 : 0);
         }
-        if (j < g.count) rank += other[j] > mine ? 1 : 0;
-        keys[rank] = mine;
+        if (j < g.count) rank += other[j] > own ? 1 : 0;
+        keys[rank] = own;
     }
-    whole = __reduce_add_sync(kAll, whole);
-    if (threadIdx.x % 32 == 0) atomicAdd(&counters[0], whole);
     __syncthreads();
-    g.whole = counters[0];
     return g;
 }
 
 __global__ void __launch_bounds__(256) top_finish_kernel(TopArgs a, ScanShape shape, void* space) {
     extern __shared__ uint64_t keys_space[];
-    __shared__ int counters[1];
+    __shared__ int counter;
     constexpr int kFinish = 256;
     const ScanState state = scan_of(space, a.in.rows, shape, false);
     uint64_t* keys = keys_space;
@@ -1694,8 +1690,8 @@ __global__ void __launch_bounds__(256) top_finish_kernel(TopArgs a, ScanShape sh
     const int n = a.n;
     const double c = static_cast<double>(fminf(1.4426950408889634f / a.temperature, FLT_MAX));
     for (int64_t row = blockIdx.x; row < a.in.rows; row += gridDim.x) {
-        const Gathered g = gather_parts<kFinish>(state, shape, row, keys, other, counters);
-        if (g.count < 0 || (!g.all && g.whole < n) || !(g.best < HUGE_VALF)) {
+        const Gathered g = gather_parts<kFinish>(state, shape, row, keys, other, &counter);
+        if (g.count < 0 || (!g.all && g.count < n) || !(g.best < HUGE_VALF)) {
             if (threadIdx.x == 0) state.left[1 + atomicAdd(&state.left[0], 1)] = static_cast<int>(row);
             __syncthreads();
             continue;
@@ -1730,7 +1726,7 @@ __global__ void __launch_bounds__(512) sample_finish_kernel(SampleArgs a, ScanSh
     constexpr int kFinish = 512;
     constexpr int kW = kFinish / 32;
     extern __shared__ uint64_t keys_space[];
-    __shared__ int counters[1];
+    __shared__ int counter;
     __shared__ double d8[kW];
     __shared__ int i8[kW];
     const ScanState state = scan_of(space, a.in.rows, shape, true);
@@ -1854,12 +1850,12 @@ __global__ void __launch_bounds__(512) sample_finish_kernel(SampleArgs a, ScanSh
             if ((first_all < used && first == chosen) || (first_all >= used && last == chosen)) {
                 if (chosen >= 0) {
                     d8[0] = first_all < used ? first_run : last_run;
-                    counters[0] = chosen;
+                    counter = chosen;
                 }
             }
             __syncthreads();
             if (warp == 0) {
-                const int at = counters[0];
+                const int at = counter;
                 double base = d8[0];
                 const E* x = static_cast<const E*>(a.in.x) + row * a.in.stride;
                 const int phase = static_cast<int>((reinterpret_cast<uintptr_t>(x) & 15u) / sizeof(E));
@@ -1897,7 +1893,7 @@ __global__ void __launch_bounds__(512) sample_finish_kernel(SampleArgs a, ScanSh
             __syncthreads();
             continue;
         }
-        const Gathered g = gather_parts<kFinish>(state, shape, row, keys, other, counters);
+        const Gathered g = gather_parts<kFinish>(state, shape, row, keys, other, &counter);
         if (g.count < 0) {
             leave();
             continue;
@@ -1908,13 +1904,12 @@ __global__ void __launch_bounds__(512) sample_finish_kernel(SampleArgs a, ScanSh
             continue;
         }
         // the first k, or as many as are known
-        const int whole = g.all ? g.count : g.whole;
-        const int count = plan.k > 0 ? min(plan.k, whole) : whole;
+        const int count = plan.k > 0 ? min(plan.k, g.count) : g.count;
         // Is what lies behind the known ranks out? By rank; as everything that
         // reaches m + T ln q is known; or as p or q cut within the known ones.
         // The mass that p goes by is the row's, or that of the first k.
         const bool mass_known = plan.k == 0 || !(plan.p < 1.0);
-        const bool enough = g.all || (plan.k > 0 && whole >= plan.k) ||
+        const bool enough = g.all || (plan.k > 0 && g.count >= plan.k) ||
                             (mass_known && plan.q > 0.0 && static_cast<double>(g.tau) <= m + plan.low);
         double* weight = reinterpret_cast<double*>(other);
         const int each = (count + kFinish - 1) / kFinish;
