@@ -1581,12 +1581,16 @@ __global__ void __launch_bounds__(kThreads, 3) scan_kernel(Args a, ScanShape sha
             if (owner < 0 || i >= per || v >= (V + phase + kVec - 1) / kVec) continue;
             float f[kVec];
             Elem<E>::unpack(v >= here.v0 && v < here.v1 ? ldg_once(here.src + v) : ragged(here, v), f);
+            unsigned hits = 0;
+#pragma unroll
+            for (int e = 0; e < kVec; ++e) hits |= f[e] >= tau && f[e] > neg_inf() ? 1u << e : 0u;
+            if (hits == 0) continue;
+            int place = atomicAdd(listed, __popc(hits));
 #pragma unroll
             for (int e = 0; e < kVec; ++e) {
-                if (f[e] >= tau && f[e] > neg_inf()) {
-                    const int place = atomicAdd(listed, 1);
-                    if (place < shape.cap) list[place] = entry(f[e], v * kVec + e - phase);
-                }
+                if (!(hits >> e & 1u)) continue;
+                if (place < shape.cap) list[place] = entry(f[e], v * kVec + e - phase);
+                ++place;
             }
         }
         float all = 0.0f;
