@@ -22,12 +22,15 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
-// Threads of the kernels that give a row to a cluster (few rows: a row's time
-// counts, and its phases are short of warps).
-constexpr int kTeam = 512;
-constexpr int kTeamWarps = kTeam / 32;
+// Threads of the kernels that give a row to a cluster, their `kTeam`: lists are
+// bound by their barriers, searches and sums over a slice by arithmetic. One
+// row of 32000 bf16, top_k 50: 9.8 us with 256, 11.2 us with 512; one of
+// 128256, top_p alone: 34.3 us with 256, 32.0 us with 512.
+constexpr int kListTeam = 256;
+constexpr int kMassTeam = 512;
+constexpr int kMostWarps = kMassTeam / 32;
 constexpr int kMaxCluster = 16;
-constexpr int kBins = 4 * kTeam;
+constexpr int kBins = 2048;
 constexpr int kSampleList = 512;   // longest top-k that goes through a candidate list
 constexpr uint32_t kAll = 0xFFFFFFFFu;
 
@@ -186,10 +189,10 @@ __device__ __forceinline__ float value_of(uint32_t key) {
 }
 
 // ---------------------------------------------------------------------------
-// Block reductions. `scratch` holds kTeamWarps values; every thread gets the
+// Block reductions. `scratch` holds a value per warp; every thread gets the
 // result, summed in one order.
 // ---------------------------------------------------------------------------
-template <class T, class Op>
+template <int kTeam, class T, class Op>
 __device__ __forceinline__ T block_reduce(T v, Op op, T* scratch) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v = op(v, __shfl_xor_sync(kAll, v, o));
@@ -197,7 +200,7 @@ __device__ __forceinline__ T block_reduce(T v, Op op, T* scratch) {
     __syncthreads();
     v = scratch[0];
 #pragma unroll
-    for (int w = 1; w < kTeamWarps; ++w) v = op(v, scratch[w]);
+    for (int w = 1; w < kTeam / 32; ++w) v = op(v, scratch[w]);
     __syncthreads();
     return v;
 }
@@ -215,7 +218,7 @@ struct Min {
 };
 
 // Sum of the values of the threads before this one, and (`all`) of all.
-template <class T>
+template <int kTeam, class T>
 __device__ __forceinline__ T block_before(T v, T* scratch, T* all = nullptr) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     T incl = v;
@@ -228,7 +231,7 @@ __device__ __forceinline__ T block_before(T v, T* scratch, T* all = nullptr) {
     __syncthreads();
     T base = T(0), total = T(0);
 #pragma unroll
-    for (int w = 0; w < kTeamWarps; ++w) {
+    for (int w = 0; w < kTeam / 32; ++w) {
         const T of = scratch[w];
         base += w < warp ? of : T(0);
         total += of;
@@ -260,7 +263,7 @@ struct Slice {
 
 // Loads the slice and adds it to the elementwise maximum `acc`. kClean: NaN
 // is stored as -inf.
-template <class E, bool kClean>
+template <int kTeam, class E, bool kClean>
 __device__ __forceinline__ Slice load_slice(const E* row, int V, int S, int c, uint4* buf, uint4& acc) {
     constexpr int kVec = Elem<E>::kVec;
     constexpr int kBatch = 8;
@@ -373,12 +376,12 @@ struct Shared {
     int counts[kMaxCluster];
     double masses[kMaxCluster];
     int ties[kMaxCluster];
-    double d8[kTeamWarps];
-    unsigned long long u8[kTeamWarps];
-    float f8[kTeamWarps];
-    int i8[kTeamWarps];
-    double range_mass[kTeamWarps];
-    int range_ties[kTeamWarps];
+    double d8[kMostWarps];
+    unsigned long long u8[kMostWarps];
+    float f8[kMostWarps];
+    int i8[kMostWarps];
+    double range_mass[kMostWarps];
+    int range_ties[kMostWarps];
     __align__(16) int steps[128];
     int listed;
     int found_bin;
@@ -502,7 +505,7 @@ struct Cut {
 
 // Visits the slice's elements a warp at a time, all lanes together; lanes
 // past the end see -inf.
-template <class E, class F>
+template <int kTeam, class E, class F>
 __device__ __forceinline__ void for_elements(const uint4* buf, const Slice& s, F&& f) {
     const int lane = threadIdx.x & 31;
     for (int base = (threadIdx.x >> 5) * 32; base < s.nv; base += kTeam) {
@@ -532,7 +535,7 @@ struct Found {
     bool ok;
 };
 
-template <class E, bool kMass>
+template <int kTeam, class E, bool kMass>
 __device__ Found search(const Team& team, Shared& sh, uint32_t* hist, const uint4* buf, const Slice& s,
                         const Weights& weight, float span, uint32_t floor_key, double target, double extra) {
     const float scale = static_cast<float>(kBins - 1) / span;
@@ -602,9 +605,10 @@ __device__ Found search(const Team& team, Shared& sh, uint32_t* hist, const uint
         const int each = (share_bins + kTeam - 1) / kTeam;
         const int first = team.rank * share_bins + each * static_cast<int>(threadIdx.x);
         const int last = min(min(kBins, (team.rank + 1) * share_bins), first + each);
-        unsigned long long h[4] = {0, 0, 0, 0};
+        constexpr int kEach = kBins / kTeam;
+        unsigned long long h[kEach] = {};
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
+        for (int q = 0; q < kEach; ++q) {
             if (first + q >= last) break;
             for (int c0 = 0; c0 < team.size; c0 += 8) {
 #pragma unroll
@@ -617,9 +621,11 @@ __device__ Found search(const Team& team, Shared& sh, uint32_t* hist, const uint
                 }
             }
         }
-        const unsigned long long own = h[0] + h[1] + h[2] + h[3];
+        unsigned long long own = 0;
+#pragma unroll
+        for (int q = 0; q < kEach; ++q) own += h[q];
         unsigned long long of_share;
-        const unsigned long long in_share = block_before<unsigned long long>(own, sh.u8, &of_share);
+        const unsigned long long in_share = block_before<kTeam>(own, sh.u8, &of_share);
         team.tell(sh.totals, of_share);
         cluster_sync(team.size);
         unsigned long long total = 0, before = above + in_share;
@@ -643,7 +649,9 @@ __device__ Found search(const Team& team, Shared& sh, uint32_t* hist, const uint
         }
         if (static_cast<double>(before) < target && static_cast<double>(before + own) >= target) {
             unsigned long long run = before;
-            for (int q = 0; q < 4 && first + q < last; ++q) {
+#pragma unroll
+            for (int q = 0; q < kEach; ++q) {
+                if (first + q >= last) break;
                 const bool here = static_cast<double>(run) < target && static_cast<double>(run + h[q]) >= target;
                 for (int c = 0; here && c < team.size; ++c) {
                     *cg::this_cluster().map_shared_rank(&sh.found_bin, c) = first + q;
@@ -683,7 +691,7 @@ __device__ Found search(const Team& team, Shared& sh, uint32_t* hist, const uint
 
 // Appends every element that reaches `low` (and is above -inf) to the CTA's
 // list; `listed` counts on where the list is full.
-template <class E>
+template <int kTeam, class E>
 __device__ __forceinline__ void append_from(Shared& sh, const uint4* buf, const Slice& s, float low, uint64_t* list,
                                             int cap) {
     for (int v = threadIdx.x; v < s.nv; v += kTeam) {
@@ -706,12 +714,12 @@ __device__ __forceinline__ void append_from(Shared& sh, const uint4* buf, const 
 // other CTAs. box[] holds every CTA's `tau` below which it needs to list
 // nothing. Every CTA lists what is at or above the least of these; where ties
 // make that too many, the exact cut is searched.
-template <class E>
+template <int kTeam, class E>
 __device__ int gather_best(const Team& team, Shared& sh, const uint4* buf, const Slice& s, float best, int n,
                            uint64_t* list, uint64_t* sorted, int cap, int leader) {
     float tau = sh.box[0].tau;
     for (int c = 1; c < team.size; ++c) tau = fminf(tau, sh.box[c].tau);
-    append_from<E>(sh, buf, s, tau, list, cap);
+    append_from<kTeam, E>(sh, buf, s, tau, list, cap);
     __syncthreads();
     team.tell(sh.counts, sh.listed);
     cluster_sync(team.size);
@@ -722,8 +730,8 @@ __device__ int gather_best(const Team& team, Shared& sh, const uint4* buf, const
         // above -inf are members, and they are more than n.
         const Weights weight(best, 1.0f);
         float low = best;
-        for_elements<E>(buf, s, [&](float x, int) { low = x > neg_inf() ? fminf(low, x) : low; });
-        low = block_reduce(low, Min(), sh.f8);
+        for_elements<kTeam, E>(buf, s, [&](float x, int) { low = x > neg_inf() ? fminf(low, x) : low; });
+        low = block_reduce<kTeam>(low, Min(), sh.f8);
         cluster_sync(team.size);          // box is read by everybody
         team.tell(sh.box, Packet{0.0, 0.0f, low, 0});
         cluster_sync(team.size);
@@ -732,12 +740,12 @@ __device__ int gather_best(const Team& team, Shared& sh, const uint4* buf, const
         if (!(span > 0.0f)) span = 1.0f;
         if (!(span < FLT_MAX)) span = FLT_MAX;
         // both lists' space holds the bins: what was listed is listed again below
-        const Found f = search<E, false>(team, sh, reinterpret_cast<uint32_t*>(list), buf, s, weight, span,
+        const Found f = search<kTeam, E, false>(team, sh, reinterpret_cast<uint32_t*>(list), buf, s, weight, span,
                                          key_of<E>(neg_inf()), static_cast<double>(n), 0.0);
         const int need = n - static_cast<int>(f.above);
         if (threadIdx.x == 0) sh.listed = 0;
         __syncthreads();
-        append_from<E>(sh, buf, s, value_of<E>(f.key + 1), list, cap);
+        append_from<kTeam, E>(sh, buf, s, value_of<E>(f.key + 1), list, cap);
         // the first `need` of the equal ones, by index: a stretch of
         // neighbouring vectors per thread
         const int per = (s.nv + kTeam - 1) / kTeam;
@@ -749,8 +757,8 @@ __device__ int gather_best(const Team& team, Shared& sh, const uint4* buf, const
 #pragma unroll
             for (int e = 0; e < Elem<E>::kVec; ++e) mine += key_of<E>(x[e]) == f.key;
         }
-        const int all = block_reduce(mine, Add(), sh.i8);
-        int at = block_before(mine, sh.i8);
+        const int all = block_reduce<kTeam>(mine, Add(), sh.i8);
+        int at = block_before<kTeam>(mine, sh.i8);
         team.tell(sh.ties, all);
         cluster_sync(team.size);
         int ahead = 0;
@@ -809,14 +817,14 @@ __device__ int gather_best(const Team& team, Shared& sh, const uint4* buf, const
 // thread) reach, and not many more; -inf where fewer than t are above -inf.
 // The maxima are counted in equal steps below `best`, down to the least of the
 // threads' own.
-template <class E>
+template <int kTeam, class E>
 __device__ float threshold(Shared& sh, const uint4& acc, float best, int t) {
     constexpr int kSteps = 128;
     float g[Elem<E>::kVec];
     Elem<E>::unpack(acc, g);
     const float mine = lanes_max<E>(acc);
     if (threadIdx.x < kSteps) sh.steps[threadIdx.x] = 0;
-    const float least = block_reduce(mine > neg_inf() ? mine : FLT_MAX, Min(), sh.f8);
+    const float least = block_reduce<kTeam>(mine > neg_inf() ? mine : FLT_MAX, Min(), sh.f8);
     const float span = fmaxf(best - least, 1.0e-30f);
     const float scale = static_cast<float>(kSteps - 1) / span;
 #pragma unroll
@@ -871,7 +879,7 @@ __device__ __forceinline__ float share(float x, float best, float c2) {
 
 // This thread's share of the slice's softmax sum, 2^(c2 (x - best)) each: the
 // difference is rounded first, so the same holds for maxima of any size.
-template <class E>
+template <int kTeam, class E>
 __device__ __forceinline__ float sum_exp(const uint4* buf, int nv, float c2, float best) {
     const float from = best > neg_inf() ? -best : 0.0f;
     const float2 ff = make_float2(from, from), cc = make_float2(c2, c2);
@@ -891,7 +899,7 @@ __device__ __forceinline__ float sum_exp(const uint4* buf, int nv, float c2, flo
 // ---------------------------------------------------------------------------
 // The best log-probs of a row
 // ---------------------------------------------------------------------------
-template <class E>
+template <int kTeam, class E>
 __global__ void __launch_bounds__(kTeam) top_kernel(TopArgs a, int S, int cap) {
     extern __shared__ uint4 dyn[];
     __shared__ Shared sh;
@@ -910,12 +918,12 @@ __global__ void __launch_bounds__(kTeam) top_kernel(TopArgs a, int S, int cap) {
         __syncthreads();
         if (threadIdx.x == 0) sh.listed = 0;
         uint4 acc = vneg_inf<E>();
-        const Slice s = load_slice<E, true>(static_cast<const E*>(a.in.x) + row * a.in.stride, a.in.V, S, team.rank,
+        const Slice s = load_slice<kTeam, E, true>(static_cast<const E*>(a.in.x) + row * a.in.stride, a.in.V, S, team.rank,
                                             buf, acc);
-        const float mine = block_reduce(lanes_max<E>(acc), Max(), sh.f8);
-        const float part = sum_exp<E>(buf, s.nv, c2, mine);
-        const double sum = block_reduce(static_cast<double>(part), Add(), sh.d8);
-        const float tau = threshold<E>(sh, acc, mine, (n + team.size - 1) / team.size);
+        const float mine = block_reduce<kTeam>(lanes_max<E>(acc), Max(), sh.f8);
+        const float part = sum_exp<kTeam, E>(buf, s.nv, c2, mine);
+        const double sum = block_reduce<kTeam>(static_cast<double>(part), Add(), sh.d8);
+        const float tau = threshold<kTeam, E>(sh, acc, mine, (n + team.size - 1) / team.size);
         team.tell(sh.box, Packet{sum, mine, tau, 0});
         cluster_sync(team.size);
         float best = sh.box[0].best;
@@ -927,7 +935,7 @@ __global__ void __launch_bounds__(kTeam) top_kernel(TopArgs a, int S, int cap) {
                 Z += of.sum * (of.best == best ? 1.0 : exp2(static_cast<double>(c2) * (static_cast<double>(of.best) -
                                                                                        static_cast<double>(best))));
         }
-        const int got = gather_best<E>(team, sh, buf, s, best, n, list, sorted, cap, leader);
+        const int got = gather_best<kTeam, E>(team, sh, buf, s, best, n, list, sorted, cap, leader);
         if (team.rank == leader) {
             const double log_z = log(Z);
             for (int i = threadIdx.x; i < n; i += kTeam) {
@@ -954,14 +962,15 @@ __global__ void __launch_bounds__(kTeam) top_kernel(TopArgs a, int S, int cap) {
 
 // The token that index order and the uniform number give among the elements
 // that the cut keeps. `out` is written by the CTA that holds it.
-template <class E>
+template <int kTeam, class E>
 __device__ void pick(const Team& team, Shared& sh, const uint4* buf, const Slice& s, const Weights& weight, Cut cut,
                      double u, int32_t* out) {
     constexpr int kVec = Elem<E>::kVec;
+    constexpr int kWarps = kTeam / 32;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const double tie = weight(value_of<E>(cut.key));
     // a stretch of the slice per warp
-    const int per = ((s.nv + kTeamWarps - 1) / kTeamWarps + 31) & ~31;
+    const int per = ((s.nv + kWarps - 1) / kWarps + 31) & ~31;
     const int begin = min(s.nv, per * warp), end = min(s.nv, begin + per);
     double mass = 0.0;
     int ties = 0;
@@ -995,7 +1004,7 @@ __device__ void pick(const Team& team, Shared& sh, const uint4* buf, const Slice
     __syncthreads();
     double cta_mass = 0.0;
     int cta_ties = 0;
-    for (int w = 0; w < kTeamWarps; ++w) {
+    for (int w = 0; w < kTeam / 32; ++w) {
         cta_mass += sh.range_mass[w];
         cta_ties += sh.range_ties[w];
     }
@@ -1036,7 +1045,7 @@ __device__ void pick(const Team& team, Shared& sh, const uint4* buf, const Slice
     int t = 0;
     const int owner = choose(sh.masses, sh.ties, team.size, m, t);
     if (owner == team.rank) {
-        const int w = choose(sh.range_mass, sh.range_ties, kTeamWarps, m, t);
+        const int w = choose(sh.range_mass, sh.range_ties, kTeam / 32, m, t);
         // that stretch again, by the whole CTA: neighbouring vectors per thread
         const int w_begin = min(s.nv, per * max(w, 0)), w_end = min(s.nv, w_begin + per);
         const int each = (per + kTeam - 1) / kTeam;
@@ -1056,13 +1065,13 @@ __device__ void pick(const Team& team, Shared& sh, const uint4* buf, const Slice
                 my_ties += k == cut.key ? 1 : 0;
             }
         }
-        const double m0 = m + block_before(my_mass, sh.d8);
-        const int t0 = t + block_before(my_ties, sh.i8);
+        const double m0 = m + block_before<kTeam>(my_mass, sh.d8);
+        const int t0 = t + block_before<kTeam>(my_ties, sh.i8);
         const bool mine = adds(my_mass, t0, my_ties);
         const bool past = mine && at(m0 + my_mass, t0 + my_ties) > target;
         const int none = kTeam;
-        const int first = block_reduce(past ? static_cast<int>(threadIdx.x) : none, Min(), sh.i8);
-        const int last = block_reduce(mine ? static_cast<int>(threadIdx.x) : -1, Max(), sh.i8);
+        const int first = block_reduce<kTeam>(past ? static_cast<int>(threadIdx.x) : none, Min(), sh.i8);
+        const int last = block_reduce<kTeam>(mine ? static_cast<int>(threadIdx.x) : -1, Max(), sh.i8);
         const int who = first < none ? first : last;
         // its warp walks along its elements
         if (warp == (who >> 5) && who >= 0) {
@@ -1092,6 +1101,7 @@ __device__ void pick(const Team& team, Shared& sh, const uint4* buf, const Slice
 }
 
 // A top-k row: its k best entries in order are all that is needed.
+template <int kTeam>
 __device__ void pick_listed(Shared& sh, const uint64_t* sorted, int count, float best, float temperature, double p,
                             double log_q, double u, double* weight, int* token, int32_t* out) {
     // weights of the ordered entries; a thread holds neighbouring ones
@@ -1107,8 +1117,8 @@ __device__ void pick_listed(Shared& sh, const uint64_t* sorted, int count, float
         token[i] = entry_token(sorted[i]);
         mine += w;
     }
-    const double total = block_reduce(mine, Add(), sh.d8);
-    double run = block_before(mine, sh.d8);
+    const double total = block_reduce<kTeam>(mine, Add(), sh.d8);
+    double run = block_before<kTeam>(mine, sh.d8);
     int keep = 0;
     for (int i = begin; i < end; ++i) {
         const float x = entry_value(sorted[i]);
@@ -1117,10 +1127,10 @@ __device__ void pick_listed(Shared& sh, const uint64_t* sorted, int count, float
         keep += (i == 0 || ((!(p < 1.0) || run < p * total) && z >= log_q)) ? 1 : 0;
         run += weight[i];
     }
-    keep = block_reduce(keep, Add(), sh.i8);   // the kept ones are the first
+    keep = block_reduce<kTeam>(keep, Add(), sh.i8);   // the kept ones are the first
     mine = 0.0;
     for (int i = begin; i < min(end, keep); ++i) mine += weight[i];
-    const double kept = block_reduce(mine, Add(), sh.d8);
+    const double kept = block_reduce<kTeam>(mine, Add(), sh.d8);
     const double target = u < 1.0 ? u * kept : HUGE_VAL;   // as in pick()
     // the least kept index whose sum of weights up to it passes the target
     int first = 0x7FFFFFFF, last = -1;
@@ -1133,12 +1143,12 @@ __device__ void pick_listed(Shared& sh, const uint64_t* sorted, int count, float
             if (sum > target) first = min(first, own);
         }
     }
-    first = block_reduce(first, Min(), sh.i8);
-    last = block_reduce(last, Max(), sh.i8);
+    first = block_reduce<kTeam>(first, Min(), sh.i8);
+    last = block_reduce<kTeam>(last, Max(), sh.i8);
     if (threadIdx.x == 0) *out = first < 0x7FFFFFFF ? first : last;
 }
 
-template <class E>
+template <int kTeam, class E>
 __global__ void __launch_bounds__(kTeam) sample_kernel(SampleArgs a, int S, int cap) {
     extern __shared__ uint4 dyn[];
     __shared__ Shared sh;
@@ -1167,12 +1177,12 @@ __global__ void __launch_bounds__(kTeam) sample_kernel(SampleArgs a, int S, int 
         const bool greedy = !(given > 0.0f) || k == 1 || p <= 0.0;
         const bool by_list = !greedy && cut_k && k <= kSampleList;
         uint4 acc = vneg_inf<E>();
-        const Slice s = load_slice<E, true>(static_cast<const E*>(a.in.x) + row * a.in.stride, V, S, team.rank, buf,
+        const Slice s = load_slice<kTeam, E, true>(static_cast<const E*>(a.in.x) + row * a.in.stride, V, S, team.rank, buf,
                                             acc);
-        const float mine = block_reduce(lanes_max<E>(acc), Max(), sh.f8);
+        const float mine = block_reduce<kTeam>(lanes_max<E>(acc), Max(), sh.f8);
         float tau = neg_inf();
         int index = 0x7FFFFFFF;
-        if (by_list) tau = threshold<E>(sh, acc, mine, (k + team.size - 1) / team.size);
+        if (by_list) tau = threshold<kTeam, E>(sh, acc, mine, (k + team.size - 1) / team.size);
         if (greedy) {
             for (int v = threadIdx.x; v < s.nv; v += kTeam) {
                 float x[Elem<E>::kVec];
@@ -1181,7 +1191,7 @@ __global__ void __launch_bounds__(kTeam) sample_kernel(SampleArgs a, int S, int 
                 for (int e = 0; e < Elem<E>::kVec; ++e)
                     if (x[e] == mine) index = min(index, s.first + v * Elem<E>::kVec + e);
             }
-            index = block_reduce(index, Min(), sh.i8);
+            index = block_reduce<kTeam>(index, Min(), sh.i8);
         }
         team.tell(sh.box, Packet{0.0, mine, tau, index});
         cluster_sync(team.size);
@@ -1200,12 +1210,12 @@ __global__ void __launch_bounds__(kTeam) sample_kernel(SampleArgs a, int S, int 
             }
             cluster_sync(team.size);
         } else if (by_list) {
-            const int got = gather_best<E>(team, sh, buf, s, best, k, list, sorted, cap, leader);
+            const int got = gather_best<kTeam, E>(team, sh, buf, s, best, k, list, sorted, cap, leader);
             if (team.rank == leader) {
                 // the leader's own list has been copied: its space holds the weights
                 double* weight = reinterpret_cast<double*>(list);
                 int* token = reinterpret_cast<int*>(weight + got);
-                pick_listed(sh, sorted, got, best, temperature, p, q > 0.0 ? log(q) : -HUGE_VAL, u, weight, token, out);
+                pick_listed<kTeam>(sh, sorted, got, best, temperature, p, q > 0.0 ? log(q) : -HUGE_VAL, u, weight, token, out);
             }
         } else {
             const Weights weight(best, temperature);
@@ -1215,8 +1225,8 @@ __global__ void __launch_bounds__(kTeam) sample_kernel(SampleArgs a, int S, int 
             double cut_mass = 0.0;   // of the equal ones at the top-k cut
             if (cut_k) {
                 float low = best;
-                for_elements<E>(buf, s, [&](float x, int) { low = x > neg_inf() ? fminf(low, x) : low; });
-                low = block_reduce(low, Min(), sh.f8);
+                for_elements<kTeam, E>(buf, s, [&](float x, int) { low = x > neg_inf() ? fminf(low, x) : low; });
+                low = block_reduce<kTeam>(low, Min(), sh.f8);
                 cluster_sync(team.size);
                 team.tell(sh.box, Packet{0.0, 0.0f, low, 0});
                 cluster_sync(team.size);
@@ -1224,7 +1234,7 @@ __global__ void __launch_bounds__(kTeam) sample_kernel(SampleArgs a, int S, int 
                 float span = best - low;
                 if (!(span > 0.0f)) span = 1.0f;
                 if (!(span < FLT_MAX)) span = FLT_MAX;
-                const Found f = search<E, false>(team, sh, hist, buf, s, weight, span, none,
+                const Found f = search<kTeam, E, false>(team, sh, hist, buf, s, weight, span, none,
                                                  static_cast<double>(k), 0.0);
                 if (f.ok) {
                     cut.key = f.key;
@@ -1234,7 +1244,7 @@ __global__ void __launch_bounds__(kTeam) sample_kernel(SampleArgs a, int S, int 
             }
             if (p < 1.0) {
                 const float span = fminf(fmaxf(32.0f * temperature, FLT_MIN), FLT_MAX);
-                const Found f = search<E, true>(team, sh, hist, buf, s, weight, span, cut.key, p,
+                const Found f = search<kTeam, E, true>(team, sh, hist, buf, s, weight, span, cut.key, p,
                                                 static_cast<double>(cut.ties) * cut_mass);
                 if (f.ok) {
                     cut.key = f.key;
@@ -1257,7 +1267,7 @@ __global__ void __launch_bounds__(kTeam) sample_kernel(SampleArgs a, int S, int 
                     cut.ties = 0;
                 }
             }
-            pick<E>(team, sh, buf, s, weight, cut, u, out);
+            pick<kTeam, E>(team, sh, buf, s, weight, cut, u, out);
             cluster_sync(team.size);
         }
         leader = leader + 1 == team.size ? 0 : leader + 1;
@@ -2802,6 +2812,17 @@ cudaError_t launch_finish(Kernel kernel, const Args& a, ScanShape sh, int thread
     return launch_rows(kernel, a.in, 1, smem, stream, threads, a, sh, a.space);
 }
 
+template <int kTeam>
+cudaError_t launch_sample_rows(const SampleArgs& a, Shape sh, int cap, cudaStream_t stream) {
+    const size_t smem = static_cast<size_t>(sh.S) * element_size(a.in.dtype) + static_cast<size_t>(cap) * 16;
+    auto launch = [&](auto kernel) { return launch_rows(kernel, a.in, sh.size, smem, stream, kTeam, a, sh.S, cap); };
+    switch (a.in.dtype) {
+        case kF32: return launch(sample_kernel<kTeam, float>);
+        case kF16: return launch(sample_kernel<kTeam, __half>);
+        default: return launch(sample_kernel<kTeam, __nv_bfloat16>);
+    }
+}
+
 }  // namespace
 
 int64_t sample_space(const SampleArgs& a) {
@@ -2841,12 +2862,8 @@ cudaError_t launch_sample(const SampleArgs& given, cudaStream_t stream) {
     const Shape sh = shape_of(a.in, es, 68 * 1024, a.left != nullptr);
     // lists for rows that may take that path, bins for the others
     const int cap = list_space(a.top_k ? kSampleList : (a.top_k_all <= kSampleList ? std::max(a.top_k_all, 0) : 0));
-    const size_t smem = static_cast<size_t>(sh.S) * es + static_cast<size_t>(cap) * 16;
-    switch (a.in.dtype) {
-        case kF32: return launch_rows(sample_kernel<float>, a.in, sh.size, smem, stream, kTeam, a, sh.S, cap);
-        case kF16: return launch_rows(sample_kernel<__half>, a.in, sh.size, smem, stream, kTeam, a, sh.S, cap);
-        default: return launch_rows(sample_kernel<__nv_bfloat16>, a.in, sh.size, smem, stream, kTeam, a, sh.S, cap);
-    }
+    const bool lists = !a.top_k && a.top_k_all > 0 && a.top_k_all <= kSampleList && a.top_k_all < a.in.V;
+    return lists ? launch_sample_rows<kListTeam>(a, sh, cap, stream) : launch_sample_rows<kMassTeam>(a, sh, cap, stream);
 }
 
 cudaError_t launch_top(const TopArgs& given, cudaStream_t stream) {
@@ -2865,9 +2882,9 @@ cudaError_t launch_top(const TopArgs& given, cudaStream_t stream) {
     const int cap = list_space(a.n);
     const size_t smem = static_cast<size_t>(sh.S) * es + static_cast<size_t>(cap) * 16;
     switch (a.in.dtype) {
-        case kF32: return launch_rows(top_kernel<float>, a.in, sh.size, smem, stream, kTeam, a, sh.S, cap);
-        case kF16: return launch_rows(top_kernel<__half>, a.in, sh.size, smem, stream, kTeam, a, sh.S, cap);
-        default: return launch_rows(top_kernel<__nv_bfloat16>, a.in, sh.size, smem, stream, kTeam, a, sh.S, cap);
+        case kF32: return launch_rows(top_kernel<kListTeam, float>, a.in, sh.size, smem, stream, kListTeam, a, sh.S, cap);
+        case kF16: return launch_rows(top_kernel<kListTeam, __half>, a.in, sh.size, smem, stream, kListTeam, a, sh.S, cap);
+        default: return launch_rows(top_kernel<kListTeam, __nv_bfloat16>, a.in, sh.size, smem, stream, kListTeam, a, sh.S, cap);
     }
 }
 
