@@ -2763,11 +2763,7 @@ cudaError_t launch_distill_any(const DistillArgs& a, cudaStream_t stream) {
 
 namespace {
 
-// Rows from which the scan is worth its three launches, and the least of a row
-// that it is worth for.
-constexpr int64_t kScanRows = 32;
-constexpr int kScanVocab = 8192;
-constexpr int kScanTop = 256;   // longer lists are ordered faster in the cluster's kernel
+constexpr int kScanTop = 256;   // the longest list of top_log_probs that a scan gathers
 
 // Parts of at most 16 chunks; more of them where the rows are few or the lists
 // long (a list of its part's share should take less than half of its threads).
@@ -2781,11 +2777,28 @@ ScanShape scan_shape(const Rows& in, int es, int take) {
     return ScanShape{parts, cap};
 }
 
-// Whether rows of this size are scanned.
-bool scans(const Rows& in) {
+// Which batches are scanned, by three launches, and which go to the cluster's
+// kernel at once. Where a list is enough (`lists`) its clusters are many on an
+// SM, and only rows of more than a CTA's slice gain, once they are many, or
+// where a row needs more than eight CTAs. Sums in 64 bits (a top-p without a
+// top-k, temperature alone) gain earlier; with settings of each row (`both`)
+// rows have to be longer. Measured in us, scan against cluster's kernel, bf16:
+//   top_k 50: 512 x 32000 36 / 26, 64 x 128256 18 / 14, 128 x 128256 23 / 28, 512 x 128256 58 / 101
+//   n = 64: 2048 x 32000 78 / 88, 48 x 128256 15 / 15, 2048 x 128256 185 / 383; one row of 256000 fp32 12.5 / 16.8
+//   temperature alone: 128 x 32000 19 / 16, 400 x 16384 26 / 34, 512 x 128256 109 / 269; one of 200000 12.4 / 18.5
+//   top_p 0.9: 64 x 32000 46 / 36, 32 x 128256 40 / 50, 64 x 128256 51 / 91; one of 200000 20 / 47
+//   each row's own: 1024 x 8192 141 / 124, 64 x 32000 51 / 35, 256 x 32000 82 / 85, 256 x 128256 113 / 221
+bool scans(const Rows& in, bool lists, bool both) {
     const int es = element_size(in.dtype);
-    return in.rows >= kScanRows && in.V >= kScanVocab &&
-           (static_cast<int64_t>(in.V) + 16 / es) * es <= static_cast<int64_t>(kMaxParts) * kHold * kThreads * 16;
+    const int64_t row = static_cast<int64_t>(in.V) * es, all = in.rows * row;
+    if (row + 16 > static_cast<int64_t>(kMaxParts) * kHold * kThreads * 16) return false;
+    if (lists) return row > 520 * 1024 || (row > 68 * 1024 && all >= 20000000);
+    return row > 256 * 1024 || (row >= (both ? 48 : 16) * 1024 && all >= 10000000);
+}
+
+// A top-k for every row, short enough for a list.
+bool by_lists(const SampleArgs& a) {
+    return !a.top_k && a.top_k_all > 0 && a.top_k_all <= kSampleList && a.top_k_all < a.in.V;
 }
 
 int sample_take(const SampleArgs& a) {
@@ -2828,18 +2841,23 @@ cudaError_t launch_sample_rows(const SampleArgs& a, Shape sh, int cap, cudaStrea
 int64_t sample_space(const SampleArgs& a) {
     // a longer top-k is the cluster's kernel's for every row
     const bool long_list = !a.top_k && a.top_k_all > kSampleList && a.top_k_all < a.in.V;
-    if (!scans(a.in) || long_list) return 0;
+    if (long_list || !scans(a.in, by_lists(a), a.top_k != nullptr)) return 0;
     return scan_bytes(a.in, scan_shape(a.in, element_size(a.in.dtype), sample_take(a)), true);
 }
 
 int64_t top_space(const TopArgs& a) {
-    if (!scans(a.in) || a.n > kScanTop) return 0;
+    if (a.n > kScanTop || !scans(a.in, true, false)) return 0;
     return scan_bytes(a.in, scan_shape(a.in, element_size(a.in.dtype), a.n), false);
 }
 
 cudaError_t launch_sample(const SampleArgs& given, cudaStream_t stream) {
     SampleArgs a = given;
-    if (sample_space(a) > 0) {
+    // a ratio alone, or the best token, needs no sum of its row: as lists do
+    const bool greedy = !a.temperature && !(a.temperature_all > 0.0f);
+    const bool ratio = !a.top_k && (a.top_k_all <= 0 || a.top_k_all >= a.in.V) && !a.top_p && a.top_p_all >= 1.0f &&
+                       !a.min_p && a.min_p_all > 0.0f;
+    const bool lists = greedy || by_lists(a);
+    if (sample_space(a) > 0 && !ratio && scans(a.in, lists, a.top_k != nullptr)) {
         const ScanShape scan = scan_shape(a.in, element_size(a.in.dtype), sample_take(a));
         cudaError_t err;
         switch (a.in.dtype) {
@@ -2862,8 +2880,7 @@ cudaError_t launch_sample(const SampleArgs& given, cudaStream_t stream) {
     const Shape sh = shape_of(a.in, es, 68 * 1024, a.left != nullptr);
     // lists for rows that may take that path, bins for the others
     const int cap = list_space(a.top_k ? kSampleList : (a.top_k_all <= kSampleList ? std::max(a.top_k_all, 0) : 0));
-    const bool lists = !a.top_k && a.top_k_all > 0 && a.top_k_all <= kSampleList && a.top_k_all < a.in.V;
-    return lists ? launch_sample_rows<kListTeam>(a, sh, cap, stream) : launch_sample_rows<kMassTeam>(a, sh, cap, stream);
+    return lists || ratio ? launch_sample_rows<kListTeam>(a, sh, cap, stream) : launch_sample_rows<kMassTeam>(a, sh, cap, stream);
 }
 
 cudaError_t launch_top(const TopArgs& given, cudaStream_t stream) {

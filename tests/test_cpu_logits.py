@@ -138,13 +138,13 @@ def test_c_arguments(libdbs):
     refused(libdbs, top(*rows, 17, 1.0, P, P, None, None), "n must be")
     refused(libdbs, top(*rows, 4, 0.0, P, P, None, None), "temperature")
     refused(libdbs, top(*rows, 4, 1.0, None, P, None, None), "cannot be null")
-    wide = (P, 0, 64, 32000, 32000)      # the rows' own scan passes its lists on
+    wide = (P, 0, 400, 32000, 32000)     # the rows' own scan passes its lists on
     refused(libdbs, sample(*wide, P, None, 1.0, None, 0, None, 1.0, None, 0.0, P, None, None), "workspace cannot be null")
     refused(libdbs, sample(*wide, P, None, 1.0, None, 0, None, 1.0, None, 0.0, P, ODD, None), "workspace is not aligned")
     refused(libdbs, top(*wide, 4, 1.0, P, P, None, None), "workspace cannot be null")
     size = ctypes.c_int64()
     for query, given in ((libdbs.dbs_device_sample_workspace_bytes, (8, 0.9)), (libdbs.dbs_device_top_log_probs_workspace_bytes, (8,))):
-        assert query(0, 64, 32000, *given, ctypes.byref(size)) == 0 and size.value > 0
+        assert query(0, 400, 32000, *given, ctypes.byref(size)) == 0 and size.value > 0
         assert query(0, 1, 32000, *given, ctypes.byref(size)) == 0 and size.value == 0
         refused(libdbs, query(0, 64, 32000, *given, None), "bytes cannot be null")
         refused(libdbs, query(9, 64, 32000, *given, ctypes.byref(size)), "data type")

@@ -590,3 +590,114 @@ def test_rows_far_from_zero(N, dtype):
     at[:9, 0] = 100 * torch.arange(9)            # the best class
     lq[:9, 0], lq[:9, 1:] = 0.0, -math.inf
     check_distill(x, lq, at, reduction="none")
+
+
+def scanned(dtype, V=40003):
+    """Twelve rows (the kinds of the tests above), and as often as a batch is repeated that is scanned."""
+    g = torch.Generator().manual_seed(8)
+    x = rows(12, V, torch.float32, 8)
+    x[0] = torch.round(x[0])
+    x[1] = -math.inf
+    x[2, 10:] = -math.inf
+    x[3, 40:] = LOWEST[dtype]
+    x[4] = LOWEST[dtype]
+    x[5, ::3] = math.nan
+    x[6, [70, 4000]] = math.inf
+    x[7] = torch.where(torch.rand(V, generator=g) < 0.5, -math.inf, 4.0)
+    x[8] = torch.arange(V, 0, -1) / 100.0
+    x[9] = torch.where(torch.arange(V) < 300, 2.0, 1.0)
+    x = x.to(dtype)
+    return x, -(-21_000_000 // (12 * V * x.element_size()))
+
+
+@pytest.mark.parametrize("settings", SETTINGS, ids=str)
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_sample_scanned(dtype, settings):
+    x, times = scanned(dtype)
+    dev = x.cuda().repeat(times, 1)
+
+    def col(name, default, of):
+        return np.full(12, settings.get(name, default), dtype=of)
+
+    for u in (torch.zeros(12), torch.full((12,), 1.0 - 2.0 ** -24), torch.ones(12), uniforms(12, 4)):
+        want = ref.sample(x, u.numpy(), col("T", 1.0, np.float32), col("k", 0, np.int32), col("p", 1.0, np.float32), col("q", 0.0, np.float32))
+        got = ext.sample(dev, u.cuda().repeat(times), temperature=settings.get("T", 1.0), top_k=settings.get("k", 0),
+                         top_p=settings.get("p", 1.0), min_p=settings.get("q", 0.0))
+        assert got.cpu().view(times, 12).tolist() == [want.tolist()] * times
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_sample_scanned_with_settings_of_each_row(dtype):
+    N = 130 if dtype == torch.float32 else 260
+    g = torch.Generator().manual_seed(N)
+    T = torch.rand(N, generator=g) * 1.5
+    T[::7] = 0.0
+    k = torch.randint(0, 80, (N,), generator=g, dtype=torch.int32)
+    k[::5] = 0
+    k[3::11] = 700
+    p = torch.rand(N, generator=g) * 1.3
+    q = torch.rand(N, generator=g) * 0.2
+    q[::3] = 0.0
+    check_sample(rows(N, 40003, dtype, N), uniforms(N, N), T, k, p, q)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n", [1, 13, 64, 256])
+def test_top_log_probs_scanned(n, dtype):
+    x, times = scanned(dtype)
+    x[6] = -50.0
+    x[6, 4321] = 60.0
+    dev = x.cuda().repeat(times, 1)
+    check_top(x, n)
+    want = ext.top_log_probs(x.cuda(), n)
+    got = ext.top_log_probs(dev, n)
+    assert torch.equal(got[1].view(times, 12, n), want[1].expand(times, 12, n))
+    values = got[0].view(times, 12, n).double().cpu().numpy()
+    want, _ = ref.top_log_probs(x, n, 1.0)
+    fine = np.broadcast_to(np.isfinite(want), values.shape)
+    assert np.array_equal(np.isfinite(values), fine)
+    assert np.all(np.abs(values - want)[fine] <= np.broadcast_to(ref.top_bound(want), values.shape)[fine])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("N,V", [(1, 300_001), (3, 555_555)])
+def test_few_long_rows(N, V, dtype):
+    x, u = rows(N, V, dtype, 6), uniforms(N, 6)
+    for settings in (dict(), dict(k=30, p=0.9), dict(p=0.6), dict(q=0.2), dict(p=0.9, q=0.05), dict(T=0.0)):
+        check_sample(x, u, **settings)
+    for n in (1, 128):
+        check_top(x, n)
+
+
+def test_scanned_on_two_streams_and_captured():
+    x = rows(300, 20011, torch.float32, 40).cuda()
+    u = uniforms(300, 40).cuda()
+
+    def step():
+        return ext.sample(x, u, top_k=30), ext.sample(x, u, top_p=0.9, min_p=0.02), ext.sample(x, u), *ext.top_log_probs(x, 30)
+
+    want = step()
+    side = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    got = []
+    for s in side:
+        with torch.cuda.stream(s):
+            for _ in range(3):
+                got.append(step())
+    torch.cuda.synchronize()
+    for many in got:
+        assert all(torch.equal(a, b) for a, b in zip(many, want))
+    graphs = [torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()]
+    held = []
+    for graph in graphs:
+        with torch.cuda.graph(graph):
+            held.append(step())
+    x.copy_(rows(300, 20011, torch.float32, 41))
+    want = step()
+    for s, graph in zip(side, graphs):
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            graph.replay()
+    torch.cuda.synchronize()
+    for many in held:
+        assert all(torch.equal(a, b) for a, b in zip(many, want))
