@@ -1,11 +1,14 @@
 // Operators on rows of raw logits [rows, V]: sampling, the best log-probs of
 // a row, and the distillation loss from a teacher's best log-probs.
 //
-// Every kernel gives one row to one thread-block cluster. The row is cut into
-// equal slices, one per CTA, each read from HBM once into that CTA's shared
-// memory; whatever needs the whole row (maximum, sums, thresholds, candidate
-// counts) crosses the cluster through distributed shared memory. Clusters are
-// persistent: cluster c takes rows c, c + n, c + 2n, ...
+// Two forms. A row to a thread-block cluster: the row is cut into equal slices,
+// one per CTA, each read from HBM once into that CTA's shared memory, and what
+// needs the whole row (maximum, sums, thresholds, candidate counts) crosses the
+// cluster through distributed shared memory; clusters are persistent, cluster c
+// takes rows c, c + n, c + 2n, ... The distillation, and small batches of the
+// others. And a scan: CTAs list the candidates of parts of rows without
+// waiting for one another, a second kernel finishes each row from its lists,
+// and rows that lists do not settle go to the clusters.
 #pragma once
 
 #include <cstdint>
@@ -18,8 +21,8 @@ enum DataType : int { kF32 = 0, kF16 = 1, kBF16 = 2 };
 
 // Limits of this implementation.
 constexpr int kMaxTop = 1024;                 // entries of a top list, slots of a teacher's row
-constexpr int64_t kMaxRowBytes = 3000000;      // a row has to fit 16 CTAs' shared memory,
-constexpr int64_t kMaxDistillBytes = 1040000;  // three times where it is distilled
+constexpr int64_t kMaxRowBytes = 3000000;      // a row has to fit 16 CTAs' shared memory;
+constexpr int64_t kMaxDistillBytes = 1040000;  // 64 KB of each where it is distilled
 
 struct Rows {
     const void* x = nullptr;
@@ -68,7 +71,7 @@ struct DistillArgs {
     int tail = 1;
     int reduction = kSum;
     float scale = 1.0f;
-    float* row_losses = nullptr;                // [rows]; null: not written
+    float* row_losses = nullptr;                // [rows]
     float* loss = nullptr;                      // the reduced loss; null with kNone
     void* state = nullptr;                      // distill_state_bytes(); written forward, read backward
     int skip_state = 0;                         // backward: the sums are there already

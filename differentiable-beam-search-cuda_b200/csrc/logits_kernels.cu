@@ -410,9 +410,10 @@ struct Team {      // a CTA's place in its cluster
 };
 
 // 2^(d c / 32) in 64 bits, relative error below 2e-12: 2^(n/32 + r/32) with n
-// the whole number nearest to d c (within -2^15 and 2^15), a table of 2^(j/32) (an entry per lane) and
-// the Taylor polynomial of 2^(r/32) to the fourth power. All 32 lanes of a
-// warp call it together.
+// the whole number nearest to d c (within -2^15 and 2^15), a table of 2^(j/32)
+// (an entry per lane) and the Taylor polynomial of 2^(r/32) to the fourth
+// power: what it leaves out is at most (ln 2 / 64)^5 / 120 = 1.3e-12. All 32
+// lanes of a warp call it together.
 __device__ __forceinline__ double exp_table() { return exp2(static_cast<double>(threadIdx.x & 31) * 0.03125); }
 __device__ __forceinline__ double exp_by(double d, double c, int n, double tab) {
     constexpr double kL = 0.021660849392498290;   // ln 2 / 32
@@ -897,7 +898,11 @@ __device__ __forceinline__ float sum_exp(const uint4* buf, int nv, float c2, flo
 }
 
 // ---------------------------------------------------------------------------
-// The best log-probs of a row
+// The best log-probs of a row: x / T - log sum exp(x / T) = (x - m) / T - log Z
+// with Z summed in 32 bits by each slice's maximum (a slice's own sum in 64
+// bits, and all that follows). Bound by latency: one pass over a slice in
+// shared memory, 6 barriers of the CTA and 3 of the cluster. 8 rows of 32000
+// fp32, n = 20: 9.8 us, of which a launch is 3.
 // ---------------------------------------------------------------------------
 template <int kTeam, class E>
 __global__ void __launch_bounds__(kTeam) top_kernel(TopArgs a, int S, int cap) {
@@ -957,7 +962,14 @@ __global__ void __launch_bounds__(kTeam) top_kernel(TopArgs a, int S, int cap) {
 }
 
 // ---------------------------------------------------------------------------
-// Sampling
+// Sampling. One token is chosen by whole rows' order and mass: the cut is found
+// as a key and a number of ties (a list for short top-k, else a search by
+// bins), then the token by a sum in index order over the cluster, the CTAs'
+// warps and a warp's elements. Bound by latency where a list is enough (one
+// row of 32000 bf16, top_k 50: 10.0 us), else by the weights in 64 bits,
+// about 40 instructions each and taken three times (twice by the search, once
+// by the choice): one row of 128256 bf16, top_p 0.9 alone, 32 us, of a
+// floor of 0.04.
 // ---------------------------------------------------------------------------
 
 // The token that index order and the uniform number give among the elements
@@ -1286,8 +1298,16 @@ __global__ void __launch_bounds__(kTeam) sample_kernel(SampleArgs a, int S, int 
 // do not lie. No part waits for another, so that the scan runs at the memory's
 // pace. The finish accepts a list where its last wanted entry reaches every
 // part's threshold: then nothing unlisted could have come before it. Rows that
-// fail (or whose ties overflow a list) go to the cluster's kernel below, by
+// fail (or whose ties overflow a list) go to the cluster's kernel above, by
 // the list `left`.
+//
+// A part's vectors are a thread's own from the copy to the last use, so that
+// copies need no barrier, and are copied ahead by cp.async, 64 KB a CTA, three
+// CTAs on an SM; that keeps HBM busy while others count. Bound by issue: 11
+// instructions an element with the exponential (2048 rows of 128256 bf16, n =
+// 64: 160 of 185 us, 3.3 TB/s), 25 with a weight in 64 bits (512 rows of them,
+// temperature alone: 95 of 109 us). Also measured there, in us: a warp per
+// part without barriers 236, the cluster's kernel for all rows 383 and 269.
 // ---------------------------------------------------------------------------
 struct PartState {
     double sum;
@@ -1309,7 +1329,10 @@ struct ScanShape {
 constexpr int kHold = 16;       // most chunks of a part, and most vectors of a slice per thread
 constexpr int kScanBins = 128;
 constexpr int kMaxParts = 32;   // a part per lane where they are put together
-constexpr int kNucleus = 512;   // candidates listed for a top-p without a top-k
+// Candidates listed for a top-p without a top-k: 64 rows of 50257 fp32, top_p
+// 0.95, min_p 0.02 take 42 us with 512, 56 with 256 and 57 with 1024; 256 rows
+// of 128256 with their own settings 113, 96 and 117.
+constexpr int kNucleus = 512;
 
 __host__ __device__ __forceinline__ ScanState scan_of(void* space, int64_t rows, ScanShape sh, bool chunks) {
     ScanState s;
@@ -1694,6 +1717,8 @@ __device__ Gathered gather_parts(const ScanState& state, ScanShape shape, int64_
     return g;
 }
 
+// A row's lists in order, and its sums joined. Bound by latency: a row takes
+// about 7 us, 2048 rows of n = 64 about 20 us.
 __global__ void __launch_bounds__(256) top_finish_kernel(TopArgs a, ScanShape shape, void* space) {
     extern __shared__ uint64_t keys_space[];
     __shared__ int counter;
@@ -1734,6 +1759,10 @@ __global__ void __launch_bounds__(256) top_finish_kernel(TopArgs a, ScanShape sh
     }
 }
 
+// A row's token from its lists, or from its stretches' sums where every token
+// can come. Bound by latency, as above: 7 us for a row of 100 candidates (12000
+// to 14000 cycles: reading the lists 4000, the cut 2800, the choice 2200), 15
+// us for one of 1000, most of it for two sorts.
 template <class E>
 __global__ void __launch_bounds__(512) sample_finish_kernel(SampleArgs a, ScanShape shape, void* space) {
     constexpr int kVec = Elem<E>::kVec;
@@ -1964,7 +1993,8 @@ __global__ void __launch_bounds__(512) sample_finish_kernel(SampleArgs a, ScanSh
         const double target = u < 1.0 ? u * kept : HUGE_VAL;
         int first = 0x7FFFFFFF, last = -1;
         if (keep > kFinish / 4) {
-            // by index: token and rank in one key, then running sums
+            // by index: token and rank in one key, then running sums (by
+            // pairs, as below, 64 rows of 50257 take 48 us and not 42)
             __syncthreads();
             for (int i = tid; i < keep; i += kFinish) {
                 const uint64_t token = static_cast<uint64_t>(entry_token(keys[i]));
@@ -2303,7 +2333,12 @@ struct DistillShared {
 // into gradients the same vectors of its CTA's slice in shared memory, and
 // starts the copy of the next row's vector as soon as it has used one, so
 // there are two barriers a row: for the row's sum, and before the listed
-// places are written a second time.
+// places are written a second time. 64 KB of slice a CTA, three CTAs on an SM.
+// Bound by issue, near the memory's rate: 12 instructions an element for sum
+// and gradient; 4096 rows of 128256 bf16 take 410 of the call's 435 us, 5.1
+// TB/s. Also measured there, in us: 655 with the slots and losses in this
+// kernel (20 barriers a row), 666 by one CTA a row reading it twice (9 % of the
+// second reads hit L2), 582 with the exponentials kept in registers.
 // What the teacher lists is not part of the sum, which must not be a
 // difference of two sums (a tail of 1e-6 would be lost in it): a row ahead,
 // the slots' threads name the listed elements to the threads that hold them,
@@ -2644,10 +2679,12 @@ struct Shape {
     int S;
 };
 
-// Slices of up to 68 KB let three CTAs share an SM, so that one's loads, one's
-// arithmetic and one's stores overlap. Few rows are cut finer, down to 8 KB,
-// so that they reach more SMs; 16 CTAs (more than every GPU grants a cluster)
-// are taken only for rows that need them.
+// Slices of up to 64 KB (distillation; 68 KB else) let two or three CTAs share
+// an SM, so that one's loads, one's arithmetic and one's stores overlap. Few
+// rows are cut finer, down to 8 KB, so that they reach more SMs; 16 CTAs (more
+// than every GPU grants a cluster) are taken only for rows that need them (256
+// rows with their own settings, of which 3 are left to clusters: 116 us with 8
+// CTAs, 119 with 16).
 Shape shape_of(const Rows& in, int es, int most, bool few = false) {
     const int vec = 16 / es;
     auto slice = [&](int size) {
