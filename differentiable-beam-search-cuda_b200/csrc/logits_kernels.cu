@@ -967,8 +967,7 @@ __global__ void __launch_bounds__(kTeam) top_kernel(TopArgs a, int S, int cap) {
 // bins), then the token by a sum in index order over the cluster, the CTAs'
 // warps and a warp's elements. Bound by latency where a list is enough (one
 // row of 32000 bf16, top_k 50: 10.0 us), else by the weights in 64 bits,
-// about 40 instructions each and taken three times (twice by the search, once
-// by the choice): one row of 128256 bf16, top_p 0.9 alone, 32 us, of a
+// taken three times (twice by the search, once by the choice): one row of 128256 bf16, top_p 0.9 alone, 32 us, of a
 // floor of 0.04.
 // ---------------------------------------------------------------------------
 
@@ -1305,8 +1304,8 @@ __global__ void __launch_bounds__(kTeam) sample_kernel(SampleArgs a, int S, int 
 // copies need no barrier, and are copied ahead by cp.async, 64 KB a CTA, three
 // CTAs on an SM; that keeps HBM busy while others count. Bound by issue: 11
 // instructions an element with the exponential (2048 rows of 128256 bf16, n =
-// 64: 160 of 185 us, 3.3 TB/s), 25 with a weight in 64 bits (512 rows of them,
-// temperature alone: 95 of 109 us). Also measured there, in us: a warp per
+// 64: about 160 of 185 us, 3.3 TB/s), 34 with a weight in 64 bits (512 rows of
+// them, temperature alone: about 95 of 109 us). Also measured there, in us: a warp per
 // part without barriers 236, the cluster's kernel for all rows 383 and 269.
 // ---------------------------------------------------------------------------
 struct PartState {
@@ -2334,11 +2333,12 @@ struct DistillShared {
 // starts the copy of the next row's vector as soon as it has used one, so
 // there are two barriers a row: for the row's sum, and before the listed
 // places are written a second time. 64 KB of slice a CTA, three CTAs on an SM.
-// Bound by issue, near the memory's rate: 12 instructions an element for sum
-// and gradient; 4096 rows of 128256 bf16 take 410 of the call's 435 us, 5.1
-// TB/s. Also measured there, in us: 655 with the slots and losses in this
+// Bound by issue, near the memory's rate: 14 instructions an element for sum
+// and gradient; 4096 rows of 128256 bf16 take about 410 of the call's 435 us,
+// 5.1 TB/s. Also measured there, in us: 655 with the slots and losses in this
 // kernel (20 barriers a row), 666 by one CTA a row reading it twice (9 % of the
-// second reads hit L2), 582 with the exponentials kept in registers.
+// second reads hit L2), 582 with the exponentials kept in registers, 518 with
+// slices of 48 KB.
 // What the teacher lists is not part of the sum, which must not be a
 // difference of two sums (a tail of 1e-6 would be lost in it): a row ahead,
 // the slots' threads name the listed elements to the threads that hold them,
