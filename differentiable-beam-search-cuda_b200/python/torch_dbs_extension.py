@@ -507,14 +507,13 @@ def _call(name: str, device: torch.device, *args) -> None:
         raise RuntimeError(f"{name} failed: {lib.dbs_last_global_error().decode()}")
 
 
-def _validate_logits(logits: torch.Tensor) -> None:
-    if logits.dtype not in _DTYPES:
+def _validate_logits(dtype: torch.dtype, shape) -> None:
+    if dtype not in _DTYPES:
         raise ValueError("logits must be float32, float16 or bfloat16")
-    if logits.dim() < 1:
+    if not shape:
         raise ValueError("logits must have shape [..., V]")
-    V = logits.size(-1)
-    _validate_positive_int_dim(V, "V")
-    if V * logits.element_size() > _MAX_ROW_BYTES:
+    _validate_positive_int_dim(shape[-1], "V")
+    if shape[-1] * dtype.itemsize > _MAX_ROW_BYTES:
         raise ValueError(f"a row of logits takes at most {_MAX_ROW_BYTES} bytes")
 
 
@@ -553,12 +552,6 @@ def _bytes_needed(name: str, *args) -> int:
     return size.value
 
 
-def _workspace(name: str, x: torch.Tensor, *settings) -> Optional[torch.Tensor]:
-    """Device memory for what passes between a call's kernels, or None."""
-    size = _bytes_needed(name, _DTYPES[x.dtype], x.size(0), x.size(1), *settings)
-    return torch.empty((size,), dtype=torch.uint8, device=x.device) if size else None
-
-
 def _beside(t: torch.Tensor, name: str, device: torch.device, dtype: torch.dtype, shape) -> torch.Tensor:
     """`t` broadcast to `shape`, contiguous on the logits' device; a tensor on another GPU is refused."""
     if t.dtype == dtype and t.device == device and t.shape == shape and t.is_contiguous():
@@ -570,14 +563,6 @@ def _beside(t: torch.Tensor, name: str, device: torch.device, dtype: torch.dtype
     except RuntimeError:
         raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}") from None
     return t.contiguous()
-
-
-def _row_setting(value, name: str, device: torch.device, dtype: torch.dtype, lead, check):
-    """A sampling setting as (per-row tensor or None, scalar): numbers are checked, tensors are read on the device."""
-    if isinstance(value, torch.Tensor):
-        return _beside(value, name, device, dtype, lead), 0
-    check(value)
-    return None, value
 
 
 def _check_temperature(value) -> None:
@@ -609,6 +594,24 @@ def _validate_positive_temperature(temperature: float) -> None:
         raise ValueError("temperature must be in [1e-30, 1e30]")
 
 
+@functools.lru_cache(maxsize=1024)
+def _sample_settings(dtype, shape, u_dtype, u_shape, temperature, top_k, top_p, min_p):
+    """Checks everything of a call but its tensors' places, None standing for a setting of each row: (C settings, bytes of workspace)."""
+    _validate_logits(dtype, shape)
+    lead = shape[:-1]
+    if u_dtype != torch.float32:
+        raise ValueError("uniforms must be float32")
+    if u_shape != lead:
+        raise ValueError(f"uniforms must have shape {tuple(lead)}, got {tuple(u_shape)}")
+    for value, check in ((temperature, _check_temperature), (top_k, _check_top_k), (top_p, _check_top_p), (min_p, _check_min_p)):
+        if value is not None:
+            check(value)
+    k = 0 if top_k is None else min(int(top_k), _INT_MAX)
+    size = _bytes_needed("dbs_device_sample_workspace_bytes", _DTYPES[dtype], math.prod(lead), shape[-1],
+                         -1 if top_k is None else k, -1.0 if top_p is None else float(top_p))
+    return (temperature or 0.0, k, top_p or 0.0, min_p or 0.0), size
+
+
 def sample(logits: torch.Tensor, uniforms: torch.Tensor, *, temperature=1.0, top_k=0, top_p=1.0,
            min_p=0.0) -> torch.Tensor:
     """One token per row of raw logits [..., V] from uniform numbers [...] in [0, 1): int32 [...].
@@ -626,26 +629,40 @@ def sample(logits: torch.Tensor, uniforms: torch.Tensor, *, temperature=1.0, top
     positive is 0, a top_k that is not positive keeps all, a top_p of 1 or more
     keeps all and one of 0 or less the best, a min_p above 1 is 1.
     """
-    _validate_logits(logits)
-    lead = logits.shape[:-1]
-    if uniforms.dtype != torch.float32:
-        raise ValueError("uniforms must be float32")
-    if uniforms.shape != lead:
-        raise ValueError(f"uniforms must have shape {tuple(lead)}, got {tuple(uniforms.shape)}")
-    device = _cuda_device_for(logits)
-    t_rows, t_all = _row_setting(temperature, "temperature", device, torch.float32, lead, _check_temperature)
-    k_rows, k_all = _row_setting(top_k, "top_k", device, torch.int32, lead, _check_top_k)
-    p_rows, p_all = _row_setting(top_p, "top_p", device, torch.float32, lead, _check_top_p)
-    q_rows, q_all = _row_setting(min_p, "min_p", device, torch.float32, lead, _check_min_p)
-    x = _logits_rows(logits.to(device))
+    given = (temperature, top_k, top_p, min_p)
+    tensors = tuple(isinstance(v, torch.Tensor) for v in given)
+    per_row = any(tensors)
+    numbers = tuple(None if t else v for t, v in zip(tensors, given)) if per_row else given
+    (t_all, k_all, p_all, q_all), size = _sample_settings(logits.dtype, logits.shape, uniforms.dtype, uniforms.shape, *numbers)
+    lead = uniforms.shape
+    if logits.is_cuda:
+        x, device = logits, logits.device
+    else:
+        device = _cuda_device_for(logits)
+        x = logits.to(device)
+    x = _logits_rows(x)
     u = _beside(uniforms, "uniforms", device, torch.float32, lead)
+    rows = (None,) * 4
+    if per_row:
+        rows = tuple(_beside(v, name, device, dtype, lead) if t else None
+                     for t, v, name, dtype in zip(tensors, given, ("temperature", "top_k", "top_p", "min_p"),
+                                                  (torch.float32, torch.int32, torch.float32, torch.float32)))
     tokens = torch.empty(lead, dtype=torch.int32, device=device)
-    k_all = min(int(k_all), _INT_MAX)
-    space = _workspace("dbs_device_sample_workspace_bytes", x, k_all if k_rows is None else -1,
-                       float(p_all) if p_rows is None else -1.0)
-    _call("dbs_device_sample", device, *_rows_args(x), u.data_ptr(), _ptr(t_rows), t_all, _ptr(k_rows), k_all,
-          _ptr(p_rows), p_all, _ptr(q_rows), q_all, tokens.data_ptr(), _ptr(space))
+    space = torch.empty((size,), dtype=torch.uint8, device=device) if size else None
+    _call("dbs_device_sample", device, *_rows_args(x), u.data_ptr(), _ptr(rows[0]), t_all, _ptr(rows[1]), k_all,
+          _ptr(rows[2]), p_all, _ptr(rows[3]), q_all, tokens.data_ptr(), _ptr(space))
     return tokens if logits.is_cuda else tokens.to(logits.device)
+
+
+@functools.lru_cache(maxsize=1024)
+def _top_settings(dtype, shape, n, temperature):
+    """Checks a call: (n, the results' shape, bytes of workspace)."""
+    _validate_logits(dtype, shape)
+    if n != int(n) or not 1 <= n <= min(shape[-1], _MAX_LIST):
+        raise ValueError(f"n must be in 1 .. {min(shape[-1], _MAX_LIST)}")
+    _validate_positive_temperature(temperature)
+    size = _bytes_needed("dbs_device_top_log_probs_workspace_bytes", _DTYPES[dtype], math.prod(shape[:-1]), shape[-1], int(n))
+    return int(n), (*shape[:-1], int(n)), size
 
 
 def top_log_probs(logits: torch.Tensor, n: int, *, temperature: float = 1.0) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -656,18 +673,19 @@ def top_log_probs(logits: torch.Tensor, n: int, *, temperature: float = 1.0) -> 
     min(V, 1024). Places beyond the tokens above -inf hold -inf and -1, which
     `distillation_loss` reads as empty. No gradient flows through it.
     """
-    _validate_logits(logits)
-    if n != int(n) or not 1 <= n <= min(logits.size(-1), _MAX_LIST):
-        raise ValueError(f"n must be in 1 .. {min(logits.size(-1), _MAX_LIST)}")
-    _validate_positive_temperature(temperature)
-    device = _cuda_device_for(logits)
-    x = _logits_rows(logits.to(device))
-    shape = (*logits.shape[:-1], int(n))
+    temperature = float(temperature)
+    n, shape, size = _top_settings(logits.dtype, logits.shape, int(n) if n == int(n) else n, temperature)
+    if logits.is_cuda:
+        x, device = logits, logits.device
+    else:
+        device = _cuda_device_for(logits)
+        x = logits.to(device)
+    x = _logits_rows(x)
     log_probs = torch.empty(shape, dtype=torch.float32, device=device)
     tokens = torch.empty(shape, dtype=torch.int32, device=device)
-    space = _workspace("dbs_device_top_log_probs_workspace_bytes", x, int(n))
-    _call("dbs_device_top_log_probs", device, *_rows_args(x), int(n), temperature, log_probs.data_ptr(),
-          tokens.data_ptr(), _ptr(space))
+    space = torch.empty((size,), dtype=torch.uint8, device=device) if size else None
+    _call("dbs_device_top_log_probs", device, *_rows_args(x), n, temperature, log_probs.data_ptr(), tokens.data_ptr(),
+          _ptr(space))
     return (log_probs, tokens) if logits.is_cuda else (log_probs.to(logits.device), tokens.to(logits.device))
 
 

@@ -701,3 +701,17 @@ def test_scanned_on_two_streams_and_captured():
     torch.cuda.synchronize()
     for many in held:
         assert all(torch.equal(a, b) for a, b in zip(many, want))
+
+
+def test_settings_given_as_tensors_are_read_at_each_call():
+    x, u = rows(4, 900, torch.float32, 3).cuda(), uniforms(4, 3).cuda()
+    n, T = torch.tensor(3), torch.tensor(0.5)
+    k = torch.tensor(2, dtype=torch.int32, device="cuda")
+    for i in range(3):
+        values, tokens = ext.top_log_probs(x, n, temperature=T)
+        want = ext.top_log_probs(x, 3 + i, temperature=0.5 + i)
+        assert torch.equal(values, want[0]) and torch.equal(tokens, want[1])
+        assert torch.equal(ext.sample(x, u, temperature=T, top_k=k), ext.sample(x, u, temperature=0.5 + i, top_k=2 + i))
+        n += 1
+        T += 1.0
+        k += 1
