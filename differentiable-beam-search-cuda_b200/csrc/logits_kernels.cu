@@ -456,7 +456,7 @@ struct Weights {
         const double p = exp_by(static_cast<double>(x) - m, c, n, tab);
         return x == mf ? 1.0 : (n < -32686 ? 0.0 : p);   // exp(-708) and below count as nothing
     }
-    // For sums by a finite maximum and an ordinary temperature: exp(-690)
+    // For sums by a finite maximum and a temperature in [1e-36, 1e30]: exp(-690)
     // stands for all that is less (`low` = m - 690 T), which no sum notices.
     __device__ __forceinline__ double term(float x, float low) const {
         const float v = fmaxf(x, low);
@@ -1377,7 +1377,8 @@ __device__ __forceinline__ Plan plan_of(const SampleArgs& a, int64_t row) {
     r.chunks = r.sum && !by_p;
     // the mass of the first k needs all of them, whatever min_p leaves of them
     r.by_low = by_q && !greedy && (r.k == 0 || !by_p);
-    r.left = r.k > kSampleList || (r.sum && r.temperature > 1.0e30f);
+    // at such temperatures 690 T or 32 / (T ln 2) is beyond 32 bits (see Weights::term)
+    r.left = r.k > kSampleList || (r.sum && !(r.temperature >= 1.0e-36f && r.temperature <= 1.0e30f));
     return r;
 }
 __device__ __forceinline__ Plan plan_of(const TopArgs& a, int64_t) {

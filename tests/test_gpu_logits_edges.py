@@ -1,0 +1,48 @@
+"""Rows, settings and lists at the ends of what the operators on rows of logits
+accept (sample, top_log_probs, distillation_loss), against their definitions
+in 64 bits."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import logits_reference as ref
+import torch_dbs_extension as ext
+from test_gpu_logits import DTYPES, rows, uniforms
+
+pytestmark = pytest.mark.gpu
+
+
+def below_zero(N, V, dtype, seed):
+    """Rows whose maximum is exactly 0 (once, or several times), as logits are after their maximum has been taken off."""
+    x = rows(N, V, torch.float32, seed)
+    x = (x - x.amax(dim=1, keepdim=True)).to(dtype)
+    x[1, 5::1000] = 0.0
+    x[2, :] = 0.0
+    x[3, 1:] = -math.inf
+    x[3, 0] = 0.0
+    return x
+
+
+def check_sample_repeated(x, times, u, T, p=1.0):
+    """A batch of `times` copies of the rows x, for rows that only a large batch gives to the scan."""
+    N = len(x)
+    want = ref.sample(x, u.numpy(), T.numpy(), np.zeros(N, dtype=np.int32), np.full(N, p, dtype=np.float32), np.zeros(N, dtype=np.float32))
+    dev, du = x.cuda().repeat(times, 1), u.cuda().repeat(times)
+    alike = bool((T == T[0]).all())
+    for given in [T.cuda().repeat(times)] + ([float(T[0])] if alike else []):
+        got = ext.sample(dev, du, temperature=given, top_p=p)
+        assert got.cpu().view(times, N).tolist() == [want.tolist()] * times
+
+
+@pytest.mark.parametrize("p", [1.0, 0.9])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_sample_scanned_temperatures_at_their_ends(dtype, p):
+    """12 rows of 20011, 25 times over: 12 MB and more, which is scanned."""
+    x, u = below_zero(12, 20011, dtype, 5), uniforms(12, 5)
+    ends = [2.0 ** -149, 1e-38, 1.3e-37, 1.4e-37, 1e-33, 1e-30, 1e-3, 1e3, 1e30, 3e38]
+    for T in ends:
+        check_sample_repeated(x, 25, u, torch.full((12,), T), p)
+    mixed = torch.tensor((ends + [0.0, 1.0]), dtype=torch.float32)
+    check_sample_repeated(x, 25, u, mixed, p)
