@@ -435,7 +435,9 @@ __device__ __forceinline__ double exp_by(double d, double c, int n, double tab) 
 struct Weights {
     float mf;
     float cf;
-    float half, cf2;    // m / 2 and 2 c: x - m itself can overflow in 32 bits
+    // The table's step goes by (x s - m s) (c / s): with s = 1/2 because x - m
+    // itself can overflow in 32 bits, with 2^99 where T is so small that c does.
+    float s, ms, cs;
     double m;
     double c;
     double tab;    // 2^(lane/32)
@@ -444,14 +446,17 @@ struct Weights {
         m = static_cast<double>(best);
         c = 46.166241308446828384 / static_cast<double>(temperature);   // 32 / ln 2
         cf = static_cast<float>(c);
-        half = 0.5f * best;
-        cf2 = static_cast<float>(2.0 * c);
+        const bool tiny = temperature < 1.0e-36f;
+        s = tiny ? 6.338253e29f : 0.5f;
+        // x <= m: where m s is below all floats, x s - m s stays negative
+        ms = fmaxf(s * best, -FLT_MAX);
+        cs = static_cast<float>(c / static_cast<double>(s));
         tab = exp_table();
     }
     // All 32 lanes of the warp call it together.
     __device__ __forceinline__ double operator()(float x) const {
         // 0 * inf and inf - inf come out as NaN, which fmaxf drops
-        const float t = fmaxf(fmaf(x, 0.5f, -half) * cf2, -40000.0f);
+        const float t = fmaxf(fmaf(x, s, -ms) * cs, -40000.0f);
         const int n = __float_as_int(t + 12582912.0f) - 0x4B400000;
         const double p = exp_by(static_cast<double>(x) - m, c, n, tab);
         return x == mf ? 1.0 : (n < -32686 ? 0.0 : p);   // exp(-708) and below count as nothing

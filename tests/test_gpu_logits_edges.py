@@ -9,7 +9,7 @@ import torch
 
 import logits_reference as ref
 import torch_dbs_extension as ext
-from test_gpu_logits import DTYPES, rows, uniforms
+from test_gpu_logits import DTYPES, check_sample, rows, uniforms
 
 pytestmark = pytest.mark.gpu
 
@@ -46,3 +46,17 @@ def test_sample_scanned_temperatures_at_their_ends(dtype, p):
         check_sample_repeated(x, 25, u, torch.full((12,), T), p)
     mixed = torch.tensor((ends + [0.0, 1.0]), dtype=torch.float32)
     check_sample_repeated(x, 25, u, mixed, p)
+
+
+@pytest.mark.parametrize("N,times", [(8, 1), (12, 40)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("T", [3e-39, 1e-38, 1e-37, 2.6e-37, 3e-37, 1e-36])
+def test_sample_logits_as_small_as_the_temperature(N, times, dtype, T):
+    """Logits of a few T, so that several tokens have a weight whatever T is."""
+    g = torch.Generator().manual_seed(3)
+    x = (-8.0 * T * torch.rand((N, 20011), generator=g, dtype=torch.float64)).to(dtype)
+    x[0] = torch.where(torch.rand(20011, generator=g) < 0.5, -T, 2.0 * T).to(dtype)
+    x[1] += 1.0          # what is left of the differences are ties, or steps of many T
+    for p in (1.0, 0.7):
+        check_sample_repeated(x, times, uniforms(N, 9), torch.full((N,), T), p)
+    check_sample(x, uniforms(N, 9), T=T, k=700)
