@@ -2097,7 +2097,13 @@ __device__ __forceinline__ T reduce_block(T v, Op op, T* scratch) {   // any num
 // pass. The first slot of a token stands for all of its slots. Two bit maps of
 // the tokens' hashes (a bit for each of `mask` + 1 values) tell that no token
 // is listed twice; where they cannot (one row in 250 with 64 slots), the
-// tokens are compared.
+// tokens are compared. Atomics of several threads may come in any order, so
+// the maps are filled in three steps: all slots enter the first one; those
+// that were the first on their bit enter the second; the others, of which
+// every token listed twice has at least one, are looked up there and entered.
+// Of two slots of a token the later one in this order meets the earlier one's
+// bits in both maps. (Both maps in one step let two threads each be the first
+// in one of them, and none saw the other.)
 template <class E, int kGroup, int kPer>
 __global__ void __launch_bounds__(256) slots_kernel(DistillArgs a, uint32_t mask) {
     constexpr int kRows = 256 / kGroup;   // of a CTA
@@ -2160,6 +2166,7 @@ __global__ void __launch_bounds__(256) slots_kernel(DistillArgs a, uint32_t mask
         double Q = 0.0;
         bool maybe = false;
         uint32_t h[kPer];
+        bool met[kPer];    // not the first on its bit of the first map
 #pragma unroll
         for (int k = 0; k < kPer; ++k) {
             // log-probs above 709 are infinite, those below -708 nothing
@@ -2172,12 +2179,23 @@ __global__ void __launch_bounds__(256) slots_kernel(DistillArgs a, uint32_t mask
                 slot[k].q = static_cast<float>(q);
                 Q += q;
                 h[k] = static_cast<uint32_t>(slot[k].token) * 2654435761u;
-                const uint32_t h1 = h[k] >> 7 & mask, h2 = h[k] >> 15 & mask;
-                const bool was1 = atomicOr(&map[h1 >> 5], 1u << (h1 & 31u)) >> (h1 & 31u) & 1u;
-                const bool was2 = atomicOr(&map2[h2 >> 5], 1u << (h2 & 31u)) >> (h2 & 31u) & 1u;
-                maybe = maybe || (was1 && was2);
+                const uint32_t h1 = h[k] >> 7 & mask;
+                met[k] = atomicOr(&map[h1 >> 5], 1u << (h1 & 31u)) >> (h1 & 31u) & 1u;
             }
             best = fmaxf(best, slot[k].x);
+        }
+        sync();
+#pragma unroll
+        for (int k = 0; k < kPer; ++k) {
+            const uint32_t h2 = h[k] >> 15 & mask;
+            if (slot[k].token >= 0 && !met[k]) atomicOr(&map2[h2 >> 5], 1u << (h2 & 31u));
+        }
+        sync();
+#pragma unroll
+        for (int k = 0; k < kPer; ++k) {
+            const uint32_t h2 = h[k] >> 15 & mask;
+            if (slot[k].token >= 0 && met[k])
+                maybe = (atomicOr(&map2[h2 >> 5], 1u << (h2 & 31u)) >> (h2 & 31u) & 1u) || maybe;
         }
         any = some(any);
         best = over(best, Max(), f8);

@@ -9,7 +9,7 @@ import torch
 
 import logits_reference as ref
 import torch_dbs_extension as ext
-from test_gpu_logits import DTYPES, check_sample, rows, uniforms
+from test_gpu_logits import DTYPES, check_distill, check_sample, rows, uniforms
 
 pytestmark = pytest.mark.gpu
 
@@ -60,3 +60,24 @@ def test_sample_logits_as_small_as_the_temperature(N, times, dtype, T):
     for p in (1.0, 0.7):
         check_sample_repeated(x, times, uniforms(N, 9), torch.full((N,), T), p)
     check_sample(x, uniforms(N, 9), T=T, k=700)
+
+
+@pytest.mark.parametrize("n", [2, 64, 128, 129, 1024])
+def test_distillation_one_token_twice_among_many(n):
+    """In each row two slots far from or next to one another have one token; the others have tokens of their own."""
+    N, V = 512, 9000
+    g = torch.Generator().manual_seed(n)
+    at = torch.stack([torch.randperm(V, generator=g)[:n] for _ in range(N)])
+    pair = torch.stack([torch.randperm(n, generator=g)[:2] for _ in range(N)])
+    at[torch.arange(N), pair[:, 1]] = at[torch.arange(N), pair[:, 0]]
+    lq = torch.log_softmax(torch.randn((N, n), generator=g), dim=1) - 0.5
+    x = rows(N, V, torch.float32, n)
+    check_distill(x, lq, at, reduction="none")
+    leaf = x.cuda().requires_grad_(True)
+    lq, at = lq.cuda(), at.cuda()
+    first = None
+    for _ in range(200):     # what the slots' threads see of one another may come in any order
+        loss = ext.distillation_loss(leaf, lq, at, reduction="none")
+        now = loss.detach(), torch.autograd.grad(loss.sum(), leaf)[0]
+        first = first or now
+        assert torch.equal(first[0], now[0]) and torch.equal(first[1], now[1])
