@@ -1725,11 +1725,11 @@ __device__ Gathered gather_parts(const ScanState& state, ScanShape shape, int64_
 // A row's lists in order, and its sums joined. Bound by latency: a row takes
 // about 7 us, 2048 rows of n = 64 about 20 us.
 __global__ void __launch_bounds__(256) top_finish_kernel(TopArgs a, ScanShape shape, void* space) {
-    extern __shared__ uint64_t keys_space[];
+    extern __shared__ uint4 dyn[];
     __shared__ int counter;
     constexpr int kFinish = 256;
     const ScanState state = scan_of(space, a.in.rows, shape, false);
-    uint64_t* keys = keys_space;
+    uint64_t* keys = reinterpret_cast<uint64_t*>(dyn);
     uint64_t* other = keys + shape.parts * shape.cap;
     const int n = a.n;
     const double c = static_cast<double>(fminf(1.4426950408889634f / a.temperature, FLT_MAX));
@@ -1773,12 +1773,12 @@ __global__ void __launch_bounds__(512) sample_finish_kernel(SampleArgs a, ScanSh
     constexpr int kVec = Elem<E>::kVec;
     constexpr int kFinish = 512;
     constexpr int kW = kFinish / 32;
-    extern __shared__ uint64_t keys_space[];
+    extern __shared__ uint4 dyn[];
     __shared__ int counter;
     __shared__ double d8[kW];
     __shared__ int i8[kW];
     const ScanState state = scan_of(space, a.in.rows, shape, true);
-    uint64_t* keys = keys_space;
+    uint64_t* keys = reinterpret_cast<uint64_t*>(dyn);
     uint64_t* other = keys + shape.parts * shape.cap;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     auto total_of = [&](double v) {
@@ -2107,11 +2107,11 @@ __device__ __forceinline__ T reduce_block(T v, Op op, T* scratch) {   // any num
 template <class E, int kGroup, int kPer>
 __global__ void __launch_bounds__(256) slots_kernel(DistillArgs a, uint32_t mask) {
     constexpr int kRows = 256 / kGroup;   // of a CTA
-    extern __shared__ uint32_t maps[];
+    extern __shared__ uint4 dyn[];
     __shared__ double d8[32];
     __shared__ float f8[32];
     const int group = threadIdx.x / kGroup, tid = threadIdx.x % kGroup;
-    uint32_t* map = maps + group * ((mask + 1) / 16);
+    uint32_t* map = reinterpret_cast<uint32_t*>(dyn) + group * ((mask + 1) / 16);
     uint32_t* map2 = map + (mask + 1) / 32;
     const DistillState state = state_of(a);
     const int n = a.n;
