@@ -441,16 +441,17 @@ struct Weights {
     double m;
     double c;
     double tab;    // 2^(lane/32)
-    __device__ Weights(float best, float temperature) {
+    // ordinary: the temperature is known to be at least 1e-36
+    __device__ Weights(float best, float temperature, bool ordinary) {
         mf = best;
         m = static_cast<double>(best);
         c = 46.166241308446828384 / static_cast<double>(temperature);   // 32 / ln 2
         cf = static_cast<float>(c);
-        const bool tiny = temperature < 1.0e-36f;
+        const bool tiny = !ordinary && temperature < 1.0e-36f;
         s = tiny ? 6.338253e29f : 0.5f;
         // x <= m: where m s is below all floats, x s - m s stays negative
         ms = fmaxf(s * best, -FLT_MAX);
-        cs = static_cast<float>(c / static_cast<double>(s));
+        cs = static_cast<float>(c * (tiny ? 1.5777218104420236e-30 : 2.0));
         tab = exp_table();
     }
     // All 32 lanes of the warp call it together.
@@ -734,7 +735,7 @@ __device__ int gather_best(const Team& team, Shared& sh, const uint4* buf, const
     if (total > cap) {
         // Too many: find the n-th value itself. All of the row's elements
         // above -inf are members, and they are more than n.
-        const Weights weight(best, 1.0f);
+        const Weights weight(best, 1.0f, true);
         float low = best;
         for_elements<kTeam, E>(buf, s, [&](float x, int) { low = x > neg_inf() ? fminf(low, x) : low; });
         low = block_reduce<kTeam>(low, Min(), sh.f8);
@@ -1234,7 +1235,7 @@ __global__ void __launch_bounds__(kTeam) sample_kernel(SampleArgs a, int S, int 
                 pick_listed<kTeam>(sh, sorted, got, best, temperature, p, q > 0.0 ? log(q) : -HUGE_VAL, u, weight, token, out);
             }
         } else {
-            const Weights weight(best, temperature);
+            const Weights weight(best, temperature, false);
             uint32_t* hist = reinterpret_cast<uint32_t*>(list);
             const uint32_t none = key_of<E>(neg_inf());
             Cut cut{none, 0};
@@ -1579,7 +1580,7 @@ __global__ void __launch_bounds__(kThreads, 3) scan_kernel(Args a, ScanShape sha
         }
         double mass = 0.0;
         if (again && best > neg_inf()) {
-            const Weights weight(best, plan.temperature);
+            const Weights weight(best, plan.temperature, true);
             const float low = best - 690.0f * plan.temperature;
             for (int i = 0; i < per; ++i) {
                 float f[kVec];
@@ -1908,7 +1909,7 @@ __global__ void __launch_bounds__(512) sample_finish_kernel(SampleArgs a, ScanSh
                 const E* x = static_cast<const E*>(a.in.x) + row * a.in.stride;
                 const int phase = static_cast<int>((reinterpret_cast<uintptr_t>(x) & 15u) / sizeof(E));
                 const int64_t start = (static_cast<int64_t>(at / kWarps) * kThreads + at % kWarps * 32 + lane) * kVec - phase;
-                const Weights weight(best, plan.temperature);
+                const Weights weight(best, plan.temperature, true);
                 double w[kVec], own = 0.0;
 #pragma unroll
                 for (int e = 0; e < kVec; ++e) {
