@@ -885,28 +885,36 @@ __device__ __forceinline__ float share(float x, float best, float c2) {
 }
 
 // This thread's share of the slice's softmax sum, 2^(c2 (x - best)) each: the
-// difference is rounded first, so the same holds for maxima of any size.
+// difference is rounded first, so the same holds for maxima of any size. Two
+// sums of up to 64 terms in 32 bits at a time, and those in 64: a slice of the
+// longest rows has 184 terms for each, and next to a large one as many small
+// terms as that, all below half a step of the sum, would be lost.
 template <int kTeam, class E>
-__device__ __forceinline__ float sum_exp(const uint4* buf, int nv, float c2, float best) {
+__device__ __forceinline__ double sum_exp(const uint4* buf, int nv, float c2, float best) {
+    constexpr int kVectors = 128 / Elem<E>::kVec;   // of 64 terms in each sum
     const float from = best > neg_inf() ? -best : 0.0f;
     const float2 ff = make_float2(from, from), cc = make_float2(c2, c2);
-    float2 p = make_float2(0.0f, 0.0f);
-    for (int v = threadIdx.x; v < nv; v += kTeam) {
-        float x[Elem<E>::kVec];
-        Elem<E>::unpack(buf[v], x);
+    double sum = 0.0;
+    for (int v0 = threadIdx.x; v0 < nv; v0 += kVectors * kTeam) {
+        float2 p = make_float2(0.0f, 0.0f);
+        for (int v = v0; v < min(nv, v0 + kVectors * kTeam); v += kTeam) {
+            float x[Elem<E>::kVec];
+            Elem<E>::unpack(buf[v], x);
 #pragma unroll
-        for (int e = 0; e < Elem<E>::kVec; e += 2) {
-            const float2 t = mul2(add2(make_float2(x[e], x[e + 1]), ff), cc);
-            p = add2(p, make_float2(ex2(t.x), ex2(t.y)));
+            for (int e = 0; e < Elem<E>::kVec; e += 2) {
+                const float2 t = mul2(add2(make_float2(x[e], x[e + 1]), ff), cc);
+                p = add2(p, make_float2(ex2(t.x), ex2(t.y)));
+            }
         }
+        sum += static_cast<double>(p.x + p.y);
     }
-    return p.x + p.y;
+    return sum;
 }
 
 // ---------------------------------------------------------------------------
 // The best log-probs of a row: x / T - log sum exp(x / T) = (x - m) / T - log Z
-// with Z summed in 32 bits by each slice's maximum (a slice's own sum in 64
-// bits, and all that follows). Bound by latency: one pass over a slice in
+// with Z summed in 32 bits by each slice's maximum, 64 terms at a time (in 64
+// bits from there on). Bound by latency: one pass over a slice in
 // shared memory, 6 barriers of the CTA and 3 of the cluster. 8 rows of 32000
 // fp32, n = 20: 9.8 us, of which a launch is 3.
 // ---------------------------------------------------------------------------
@@ -932,8 +940,7 @@ __global__ void __launch_bounds__(kTeam) top_kernel(TopArgs a, int S, int cap) {
         const Slice s = load_slice<kTeam, E, true>(static_cast<const E*>(a.in.x) + row * a.in.stride, a.in.V, S, team.rank,
                                             buf, acc);
         const float mine = block_reduce<kTeam>(lanes_max<E>(acc), Max(), sh.f8);
-        const float part = sum_exp<kTeam, E>(buf, s.nv, c2, mine);
-        const double sum = block_reduce<kTeam>(static_cast<double>(part), Add(), sh.d8);
+        const double sum = block_reduce<kTeam>(sum_exp<kTeam, E>(buf, s.nv, c2, mine), Add(), sh.d8);
         const float tau = threshold<kTeam, E>(sh, acc, mine, (n + team.size - 1) / team.size);
         team.tell(sh.box, Packet{sum, mine, tau, 0});
         cluster_sync(team.size);

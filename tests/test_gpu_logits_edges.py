@@ -9,7 +9,7 @@ import torch
 
 import logits_reference as ref
 import torch_dbs_extension as ext
-from test_gpu_logits import DTYPES, check_distill, check_sample, rows, uniforms
+from test_gpu_logits import DTYPES, check_distill, check_sample, check_top, rows, uniforms
 
 pytestmark = pytest.mark.gpu
 
@@ -81,3 +81,12 @@ def test_distillation_one_token_twice_among_many(n):
         now = loss.detach(), torch.autograd.grad(loss.sum(), leaf)[0]
         first = first or now
         assert torch.equal(first[0], now[0]) and torch.equal(first[1], now[1])
+
+
+def test_top_log_probs_long_sums():
+    """A row of the most elements: a large term, then more small ones than a sum in 32 bits may take (each below half a step of it)."""
+    V, S = 1_499_999, 93760          # 16 slices; a thread's first vector is one of a slice's first 256
+    i = torch.arange(V)
+    x = torch.full((1, V), -16.640625)
+    x[0, (i % S < 2048) & (i % 8 < 2)] = 0.0
+    check_top(x.to(torch.float16), 3)
