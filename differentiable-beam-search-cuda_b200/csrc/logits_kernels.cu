@@ -2526,7 +2526,9 @@ __global__ void __launch_bounds__(kThreads, 3) distill_kernel(DistillArgs a, int
         float end_x = neg_inf();
         if (at_end && !(sh.end_marks[par] >> lane & 1u)) end_x = Elem<E>::widen(in[row * a.in.stride + here.a0 + ragged]);
         // The sum goes by the maximum of the thread's first vectors; where the
-        // others run so far beyond it that the sum overflows, by all of them.
+        // others run so far beyond it that the sum passes 1e18, by all of them.
+        // (Factors between such maxima come out as 0 below 2^-126, so what is
+        // lost of the row's sum is below 2^-50.)
         auto best_of = [&](int chunks) {
             uint4 top = none;
             for (int i = 0; i < chunks * kChunk; ++i) top = vmax<E>(top, buf[i * kT]);
@@ -2558,7 +2560,7 @@ __global__ void __launch_bounds__(kThreads, 3) distill_kernel(DistillArgs a, int
         };
         best = fmaxf(best_of(min(chunks, 1)), end_x);
         add_up();
-        if (!(best > neg_inf()) || !(sum < 1.0e30f)) {
+        if (!(best > neg_inf()) || !(sum < 1.0e18f)) {
             best = fmaxf(best_of(chunks), end_x);
             add_up();
         }
@@ -2606,12 +2608,16 @@ __global__ void __launch_bounds__(kThreads, 3) distill_kernel(DistillArgs a, int
                 a.tail && rest.y > 0.0f ? static_cast<float>(fmax(0.0, 1.0 - known.Q)) : 0.0f;
             const float w = unit * g;
             const float G = (static_cast<float>(known.Q) + q_rest) * (Z == 0.0f ? 0.0f : __fdividef(1.0f, Z));
-            // by the thread's reference: P = exponential * share by the row's / Z,
-            // P / P_r = exponential * share by the rest's / its sum
-            float scale = G * share(best, all, c2);
-            if (q_rest > 0.0f) scale -= __fdividef(q_rest, rest.y) * share(best, rest.x, c2);
-            scale = best > neg_inf() ? scale * w : 0.0f;
-            const float from = best > neg_inf() ? -best : 0.0f;
+            // P / P_r = exponential by the rest's reference / its sum, and P =
+            // exponential by the row's / Z. With a rest's class both go by the
+            // rest's, where P may be lost next to P / P_r; without one by the
+            // row's, so that the smallest P stays. (By a thread's own, a factor
+            // to the row's of 2^-126 took all of its elements' gradients.)
+            const float by = q_rest > 0.0f ? rest.x : all;
+            float scale = G;
+            if (q_rest > 0.0f) scale = G * share(rest.x, all, c2) - __fdividef(q_rest, rest.y);
+            scale *= w;
+            const float from = by > neg_inf() ? -by : 0.0f;
             const float2 ff = make_float2(from, from), ss = make_float2(scale, scale);
             auto gradient = [&](const uint4& r) {
                 float f[kVec];

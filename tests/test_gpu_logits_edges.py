@@ -83,6 +83,25 @@ def test_distillation_one_token_twice_among_many(n):
         assert torch.equal(first[0], now[0]) and torch.equal(first[1], now[1])
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("high", [40.0, 62.0, 64.5])
+@pytest.mark.parametrize("tail", [True, False])
+def test_distillation_rows_that_rise(dtype, high, tail):
+    """Each thread's first vectors at 0, the others far above them, and a listed token so far above both that a factor between
+    the first vectors' scale and the row's is below 2^-126."""
+    V = 16000 if dtype == torch.float32 else 32000
+    x = torch.full((80, V), high)
+    x[:, :V // 4 + 96] = 0.0
+    x += 0.25 * torch.rand((80, V), generator=torch.Generator().manual_seed(1))
+    x[:, V - 7] = 90.0
+    x[::2, V - 9] = 89.0
+    lq = torch.tensor([math.log(0.999), -math.inf]).expand(80, 2).contiguous()
+    at = torch.tensor([V - 7, -1]).expand(80, 2).contiguous()
+    check_distill(x.to(dtype), lq, at, tail=tail, reduction="none")
+    at = torch.tensor([3, V // 2]).expand(80, 2).contiguous()
+    check_distill(x.to(dtype), lq, at, tail=tail, reduction="none")
+
+
 def test_top_log_probs_long_sums():
     """A row of the most elements: a large term, then more small ones than a sum in 32 bits may take (each below half a step of it)."""
     V, S = 1_499_999, 93760          # 16 slices; a thread's first vector is one of a slice's first 256
