@@ -565,6 +565,17 @@ def _beside(t: torch.Tensor, name: str, device: torch.device, dtype: torch.dtype
     return t.contiguous()
 
 
+def _row_top_k(k: torch.Tensor) -> torch.Tensor:
+    """A top_k of each row within int32, as a number is (a cast would wrap what is beyond it into another list's length)."""
+    if k.dtype in (torch.int32, torch.int16, torch.int8, torch.uint8, torch.bool):
+        return k
+    if k.is_floating_point():
+        k = k.detach().to(torch.float64).nan_to_num(0.0)
+    else:
+        k = k.to(torch.int64)
+    return k.clamp(0, _INT_MAX)
+
+
 def _check_temperature(value) -> None:
     _validate_finite_float(value, "temperature")
     if value < 0.0:
@@ -644,6 +655,8 @@ def sample(logits: torch.Tensor, uniforms: torch.Tensor, *, temperature=1.0, top
     u = _beside(uniforms, "uniforms", device, torch.float32, lead)
     rows = (None,) * 4
     if per_row:
+        if tensors[1]:
+            given = (temperature, _row_top_k(top_k), top_p, min_p)
         rows = tuple(_beside(v, name, device, dtype, lead) if t else None
                      for t, v, name, dtype in zip(tensors, given, ("temperature", "top_k", "top_p", "min_p"),
                                                   (torch.float32, torch.int32, torch.float32, torch.float32)))

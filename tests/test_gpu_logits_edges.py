@@ -109,3 +109,13 @@ def test_top_log_probs_long_sums():
     x = torch.full((1, V), -16.640625)
     x[0, (i % S < 2048) & (i % 8 < 2)] = 0.0
     check_top(x.to(torch.float16), 3)
+
+
+def test_sample_top_k_beyond_32_bits():
+    x, u = rows(40, 5000, torch.float32, 1), uniforms(40, 1)
+    for k in (2 ** 32 + 5, 2 ** 40, 2 ** 63 - 1, -2 ** 32 + 5, -2 ** 63, 2 ** 31, 7):
+        every = ext.sample(x.cuda(), u.cuda(), top_k=torch.full((40,), k, dtype=torch.int64, device="cuda"))
+        assert torch.equal(every, ext.sample(x.cuda(), u.cuda(), top_k=max(k, 0)))
+    for k in (math.inf, 3e9, -math.inf, -3e9, math.nan, 7.0):
+        every = ext.sample(x.cuda(), u.cuda(), top_k=torch.full((40,), k, device="cuda"))
+        assert torch.equal(every, ext.sample(x.cuda(), u.cuda(), top_k=7 if k == 7.0 else 0))
