@@ -491,6 +491,7 @@ _MAX_DISTILL_BYTES = 1_040_000
 _MAX_LIST = 1024
 # the current stream's handle without a Stream object around it
 _RAW_STREAM = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+_FORWARD_AD = torch.autograd.forward_ad
 _CURRENT_DEVICE = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
@@ -801,6 +802,11 @@ class _DBSDistillation(torch.autograd.Function):
         return grad
 
 
+def _has_tangent(t: torch.Tensor) -> bool:
+    # outside of every dual level there are none (unpack_dual alone takes half a microsecond to say so)
+    return getattr(_FORWARD_AD, "_current_level", 0) >= 0 and _FORWARD_AD.unpack_dual(t).tangent is not None
+
+
 def distillation_loss(logits: torch.Tensor, teacher_log_probs: torch.Tensor, teacher_tokens: torch.Tensor, *,
                       temperature: float = 1.0, tail: bool = True, reduction: str = "mean",
                       scale: float = 1.0) -> torch.Tensor:
@@ -818,14 +824,16 @@ def distillation_loss(logits: torch.Tensor, teacher_log_probs: torch.Tensor, tea
     multiplies the loss (temperature ** 2 is usual); a factor given here costs
     nothing, while one applied to the loss afterwards makes the backward read
     the logits a second time. The loss is float32; gradients flow to the logits
-    alone.
+    alone, backward and once (a tangent of forward mode is refused).
     """
     lq, at = teacher_log_probs, teacher_tokens
     plan = _distill_settings(logits.dtype, logits.shape, lq.dtype, lq.shape, at.dtype, at.shape, float(temperature),
                              1 if tail else 0, reduction, float(scale))
     need_grad = torch.is_grad_enabled()
-    if need_grad and lq.requires_grad:
+    if (need_grad and lq.requires_grad) or _has_tangent(lq):
         raise ValueError("teacher_log_probs takes no gradient; detach it")
+    if _has_tangent(logits):
+        raise RuntimeError("distillation_loss has no forward-mode derivative")
     if logits.is_cuda:
         x, device = logits, logits.device
     else:

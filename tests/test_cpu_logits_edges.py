@@ -38,3 +38,14 @@ def test_sample_top_k_of_each_row_reaches_the_library_unwrapped(values, dtype, w
     monkeypatch.setattr(ext, "_call", call)
     ext.sample(torch.randn(3, 16), torch.rand(3), top_k=torch.tensor(values, dtype=dtype))
     assert seen == want
+
+
+@pytest.mark.parametrize("grad", [True, False])
+def test_distillation_refuses_tangents(grad):
+    x, lq, at = torch.randn(3, 16), torch.full((3, 4), -2.0), torch.arange(4).expand(3, 4)
+    ad = torch.autograd.forward_ad
+    with ad.dual_level(), torch.set_grad_enabled(grad):
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            ext.distillation_loss(ad.make_dual(x, torch.ones_like(x)), lq, at)
+        with pytest.raises(ValueError, match="takes no gradient"):
+            ext.distillation_loss(x, ad.make_dual(lq, torch.ones_like(lq)), at)

@@ -9,7 +9,7 @@ import torch
 
 import logits_reference as ref
 import torch_dbs_extension as ext
-from test_gpu_logits import DTYPES, check_distill, check_sample, check_top, rows, uniforms
+from test_gpu_logits import DTYPES, check_distill, check_sample, check_top, rows, teacher, uniforms
 
 pytestmark = pytest.mark.gpu
 
@@ -119,3 +119,14 @@ def test_sample_top_k_beyond_32_bits():
     for k in (math.inf, 3e9, -math.inf, -3e9, math.nan, 7.0):
         every = ext.sample(x.cuda(), u.cuda(), top_k=torch.full((40,), k, device="cuda"))
         assert torch.equal(every, ext.sample(x.cuda(), u.cuda(), top_k=7 if k == 7.0 else 0))
+
+
+def test_no_forward_derivative():
+    x = rows(6, 500, torch.float32, 7).cuda()
+    lq, at = (t.cuda() for t in teacher(6, 500, 9, 7))
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(x, torch.ones_like(x))
+        for grad in (True, False):
+            with torch.set_grad_enabled(grad), pytest.raises(RuntimeError, match="forward-mode"):
+                ext.distillation_loss(dual, lq, at)
+        assert torch.equal(ext.distillation_loss(x, lq, at), ext.distillation_loss(x.clone(), lq, at))
