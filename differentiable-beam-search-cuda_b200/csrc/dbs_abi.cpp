@@ -1875,6 +1875,11 @@ static void check_workspace(const void* workspace, int64_t bytes) {
         throw std::invalid_argument("workspace is not aligned to 16 bytes");
 }
 
+static void check_aligned(const void* p, size_t size, const char* name) {
+    if (reinterpret_cast<uintptr_t>(p) % size != 0)
+        throw std::invalid_argument(std::string(name) + " is not aligned to its type");
+}
+
 static void positive_temperature(float temperature) {
     if (!(temperature > 0.0f) || !std::isfinite(temperature))
         throw std::invalid_argument("temperature must be positive and finite");
@@ -1898,6 +1903,12 @@ DBS_EXPORT int dbs_device_sample(const void* logits, int data_type, int64_t rows
         if (!min_ps && !(min_p >= 0.0f && min_p <= 1.0f)) throw std::invalid_argument("min_p must be in [0, 1]");
         if (rows == 0) return 0;
         if (!uniforms || !tokens) throw std::invalid_argument("uniforms and tokens cannot be null");
+        check_aligned(uniforms, 4, "uniforms");
+        check_aligned(temperatures, 4, "temperatures");
+        check_aligned(top_ks, 4, "top_ks");
+        check_aligned(top_ps, 4, "top_ps");
+        check_aligned(min_ps, 4, "min_ps");
+        check_aligned(tokens, 4, "tokens");
         a.uniforms = uniforms;
         a.temperature = temperatures;
         a.temperature_all = temperature;
@@ -1959,6 +1970,8 @@ DBS_EXPORT int dbs_device_top_log_probs(const void* logits, int data_type, int64
             throw std::invalid_argument("n must be in 1 .. min(vocab_size, 1024)");
         if (rows == 0) return 0;
         if (!log_probs || !tokens) throw std::invalid_argument("log_probs and tokens cannot be null");
+        check_aligned(log_probs, 4, "log_probs");
+        check_aligned(tokens, 4, "tokens");
         a.n = n;
         a.temperature = temperature;
         a.log_probs = log_probs;
@@ -2014,6 +2027,10 @@ DBS_EXPORT int dbs_device_distill(const void* logits, int data_type, int64_t row
         a.token_bytes = token_bytes;
         if (rows > 0 && !row_losses) throw std::invalid_argument("row_losses cannot be null");
         if (reduction != DBS_REDUCE_NONE && !loss) throw std::invalid_argument("a reduced loss needs a place");
+        check_aligned(teacher_log_probs, 4, "teacher_log_probs");
+        check_aligned(teacher_tokens, static_cast<size_t>(token_bytes), "teacher_tokens");
+        check_aligned(row_losses, 4, "row_losses");
+        check_aligned(loss, 4, "loss");
         a.row_losses = row_losses;
         a.loss = loss;
         dbs_host::check_cuda(dbs_logits::launch_distill(a, static_cast<cudaStream_t>(cuda_stream)), "distill");
@@ -2042,6 +2059,7 @@ DBS_EXPORT int dbs_device_distill_backward(const void* logits, int data_type, in
         if ((flags & ~DBS_DEVICE_GRAD_UNIT) != 0) throw std::invalid_argument("unknown flags");
         if (rows == 0) return 0;
         if (!grad_loss || !grad_logits) throw std::invalid_argument("grad_loss and grad_logits cannot be null");
+        check_aligned(grad_loss, 4, "grad_loss");
         a.skip_state = 1;
         a.grad_loss = grad_loss;
         a.grad_loss_stride = grad_loss_stride;

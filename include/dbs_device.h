@@ -160,7 +160,7 @@ DBS_EXPORT int dbs_device_backward_sparse_noalloc(DBSDecoderHandle* handle, int 
  * alone. Common arguments: `logits` holds `rows` rows of `vocab_size`
  * elements of DBS_DTYPE_F32 / F16 / BF16 (`data_type`), row r at
  * r * row_stride elements (0 repeats one row); rows need no alignment beyond
- * their element's. A row holds at most 3000000 bytes. No handle: errors are
+ * their element's, as all arrays of these calls (others are refused). A row holds at most 3000000 bytes. No handle: errors are
  * in dbs_last_global_error. No call allocates, waits or keeps state, so calls
  * may overlap on several streams and be captured into graphs, each with a
  * workspace of its own: device memory, 16-byte aligned, of at least the bytes

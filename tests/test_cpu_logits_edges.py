@@ -49,3 +49,35 @@ def test_distillation_refuses_tangents(grad):
             ext.distillation_loss(ad.make_dual(x, torch.ones_like(x)), lq, at)
         with pytest.raises(ValueError, match="takes no gradient"):
             ext.distillation_loss(x, ad.make_dual(lq, torch.ones_like(lq)), at)
+
+
+# Host memory stands in for the device's: every call here is refused before a kernel is launched.
+BUF = (ctypes.c_float * 64)()
+P = ctypes.c_void_p((ctypes.addressof(BUF) + 15) // 16 * 16)
+ODD, FOUR = ctypes.c_void_p(P.value + 2), ctypes.c_void_p(P.value + 4)
+ROWS = (P, 0, 1, 16, 16)
+
+
+def refused(lib, rc, message):
+    assert rc == -2
+    assert message in lib.dbs_last_global_error().decode()
+
+
+def changed(args, at, value):
+    return [value if i == at else a for i, a in enumerate(args)]
+
+
+@pytest.mark.parametrize("entry,args,names", [
+    ("dbs_device_sample", [*ROWS, P, P, 1.0, P, 0, P, 1.0, P, 0.0, P, P, None],
+     {5: "uniforms", 6: "temperatures", 8: "top_ks", 10: "top_ps", 12: "min_ps", 14: "tokens"}),
+    ("dbs_device_top_log_probs", [*ROWS, 4, 1.0, P, P, None, None], {7: "log_probs", 8: "tokens"}),
+    ("dbs_device_distill", [*ROWS, P, P, 4, 2, 1.0, 1, 1, 1.0, P, P, P, P, None],
+     {5: "teacher_log_probs", 6: "teacher_tokens", 13: "row_losses", 14: "loss"}),
+    ("dbs_device_distill_backward", [*ROWS, 2, 1.0, 1, 1, 1.0, P, P, 0, 0, P, None], {11: "grad_loss"}),
+])
+def test_c_pointers_that_are_not_aligned(libdbs, entry, args, names):
+    """A kernel that reads or writes there would fault."""
+    for at, name in names.items():
+        refused(libdbs, getattr(libdbs, entry)(*changed(args, at, ODD)), name + " is not aligned")
+    if entry == "dbs_device_distill":
+        refused(libdbs, libdbs.dbs_device_distill(*changed(changed(args, 7, 8), 6, FOUR)), "teacher_tokens is not aligned")
