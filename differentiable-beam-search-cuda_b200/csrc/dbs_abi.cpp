@@ -1991,6 +1991,8 @@ static dbs_logits::DistillArgs distill_args(const void* logits, int data_type, i
     a.in = logits_rows(logits, data_type, rows, vocab_size, row_stride);
     if (vocab_size * (data_type == DBS_DTYPE_F32 ? 4LL : 2LL) > dbs_logits::kMaxDistillBytes)
         throw std::invalid_argument("a row to distill takes at most 1040000 bytes");
+    if (rows > std::numeric_limits<int>::max())   // rows with slots are counted in an int
+        throw std::invalid_argument("a loss takes at most 2147483647 rows");
     positive_temperature(temperature);
     if (slots <= 0 || slots > dbs_logits::kMaxTop) throw std::invalid_argument("slots must be in 1 .. 1024");
     if (reduction != DBS_REDUCE_NONE && reduction != DBS_REDUCE_SUM && reduction != DBS_REDUCE_MEAN)
@@ -2040,8 +2042,8 @@ DBS_EXPORT int dbs_device_distill(const void* logits, int data_type, int64_t row
 }
 
 DBS_EXPORT int dbs_device_distill_state_bytes(int64_t rows, int slots, int64_t* bytes) {
-    if (!bytes || rows < 0 || slots <= 0 || slots > dbs_logits::kMaxTop) {
-        set_error(nullptr, "rows cannot be negative and slots must be in 1 .. 1024");
+    if (!bytes || rows < 0 || rows > std::numeric_limits<int>::max() || slots <= 0 || slots > dbs_logits::kMaxTop) {
+        set_error(nullptr, "rows must be in 0 .. 2147483647 and slots in 1 .. 1024");
         return -1;
     }
     *bytes = dbs_logits::distill_state_bytes(rows, slots);

@@ -8,6 +8,7 @@
 
 #include <algorithm>
 #include <cfloat>
+#include <climits>
 #include <cmath>
 #include <mutex>
 #include <tuple>
@@ -2864,6 +2865,7 @@ ScanShape scan_shape(const Rows& in, int es, int take) {
 //   top_p 0.9: 64 x 32000 46 / 36, 32 x 128256 40 / 50, 64 x 128256 51 / 91; one of 200000 20 / 47
 //   each row's own: 1024 x 8192 141 / 124, 64 x 32000 51 / 35, 256 x 32000 82 / 85, 256 x 128256 113 / 221
 bool scans(const Rows& in, bool lists, bool both) {
+    if (in.rows > INT_MAX) return false;   // the list of rows left over holds ints
     const int es = element_size(in.dtype);
     const int64_t row = static_cast<int64_t>(in.V) * es, all = in.rows * row;
     if (row + 16 > static_cast<int64_t>(kMaxParts) * kHold * kThreads * 16) return false;

@@ -211,8 +211,8 @@ DBS_EXPORT int dbs_device_top_log_probs_workspace_bytes(int data_type, int64_t r
  * logits' type, or NULL) takes the gradient for an incoming gradient of 1, in
  * the same pass over the logits. `state` is dbs_device_distill_state_bytes
  * bytes of device memory, 16-byte aligned, that the call fills and a backward
- * of it reads. A row holds at most 1040000 bytes here, and the temperature is
- * in [1e-30, 1e30]. */
+ * of it reads. A row holds at most 1040000 bytes here, there are at most
+ * 2147483647 rows, and the temperature is in [1e-30, 1e30]. */
 #define DBS_REDUCE_NONE 0
 #define DBS_REDUCE_SUM 1
 #define DBS_REDUCE_MEAN 2

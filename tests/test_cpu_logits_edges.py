@@ -81,3 +81,16 @@ def test_c_pointers_that_are_not_aligned(libdbs, entry, args, names):
         refused(libdbs, getattr(libdbs, entry)(*changed(args, at, ODD)), name + " is not aligned")
     if entry == "dbs_device_distill":
         refused(libdbs, libdbs.dbs_device_distill(*changed(changed(args, 7, 8), 6, FOUR)), "teacher_tokens is not aligned")
+
+
+def test_c_more_rows_than_an_int_counts(libdbs):
+    """The loss' rows are counted in an int, a scan's rows are listed as ints: 2^31 rows (of one repeated row, or without a gradient) fit
+    the memory of a GPU. A workspace for them is not asked for, as they are not scanned."""
+    many, size = (P, 0, 2 ** 31, 16, 0), ctypes.c_int64(-1)
+    refused(libdbs, libdbs.dbs_device_distill(*many, P, P, 4, 2, 1.0, 1, 2, 1.0, P, P, P, None, None), "at most 2147483647 rows")
+    refused(libdbs, libdbs.dbs_device_distill_backward(*many, 2, 1.0, 1, 2, 1.0, P, P, 0, 0, P, None), "at most 2147483647 rows")
+    assert libdbs.dbs_device_distill_state_bytes(2 ** 31, 1, ctypes.byref(size)) == -1
+    assert libdbs.dbs_device_distill_state_bytes(2 ** 31 - 1, 1024, ctypes.byref(size)) == 0 and size.value > 2 ** 45
+    for rows in (2 ** 31, 2 ** 62):
+        assert libdbs.dbs_device_sample_workspace_bytes(0, rows, 32000, 8, 0.9, ctypes.byref(size)) == 0 and size.value == 0
+        assert libdbs.dbs_device_top_log_probs_workspace_bytes(0, rows, 32000, 8, ctypes.byref(size)) == 0 and size.value == 0
