@@ -1733,11 +1733,11 @@ __device__ Gathered gather_parts(const ScanState& state, ScanShape shape, int64_
 
 // A row's lists in order, and its sums joined. Bound by latency: a row takes
 // about 7 us, 2048 rows of n = 64 about 20 us.
-__global__ void __launch_bounds__(256) top_finish_kernel(TopArgs a, ScanShape shape, void* space) {
+__global__ void __launch_bounds__(256) top_finish_kernel(TopArgs a, ScanShape shape, void* space, bool with_chunks) {
     extern __shared__ uint4 dyn[];
     __shared__ int counter;
     constexpr int kFinish = 256;
-    const ScanState state = scan_of(space, a.in.rows, shape, false);
+    const ScanState state = scan_of(space, a.in.rows, shape, with_chunks);
     uint64_t* keys = reinterpret_cast<uint64_t*>(dyn);
     uint64_t* other = keys + shape.parts * shape.cap;
     const int n = a.n;
@@ -1778,7 +1778,7 @@ __global__ void __launch_bounds__(256) top_finish_kernel(TopArgs a, ScanShape sh
 // to 14000 cycles: reading the lists 4000, the cut 2800, the choice 2200), 15
 // us for one of 1000, most of it for two sorts.
 template <class E>
-__global__ void __launch_bounds__(512) sample_finish_kernel(SampleArgs a, ScanShape shape, void* space) {
+__global__ void __launch_bounds__(512) sample_finish_kernel(SampleArgs a, ScanShape shape, void* space, bool with_chunks) {
     constexpr int kVec = Elem<E>::kVec;
     constexpr int kFinish = 512;
     constexpr int kW = kFinish / 32;
@@ -1786,7 +1786,7 @@ __global__ void __launch_bounds__(512) sample_finish_kernel(SampleArgs a, ScanSh
     __shared__ int counter;
     __shared__ double d8[kW];
     __shared__ int i8[kW];
-    const ScanState state = scan_of(space, a.in.rows, shape, true);
+    const ScanState state = scan_of(space, a.in.rows, shape, with_chunks);
     uint64_t* keys = reinterpret_cast<uint64_t*>(dyn);
     uint64_t* other = keys + shape.parts * shape.cap;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -2897,9 +2897,9 @@ cudaError_t launch_scan(const Args& a, ScanShape sh, bool chunks, cudaStream_t s
 }
 
 template <class Kernel, class Args>
-cudaError_t launch_finish(Kernel kernel, const Args& a, ScanShape sh, int threads, cudaStream_t stream) {
+cudaError_t launch_finish(Kernel kernel, const Args& a, ScanShape sh, bool chunks, int threads, cudaStream_t stream) {
     const size_t smem = static_cast<size_t>(sh.parts) * sh.cap * 16;
-    return launch_rows(kernel, a.in, 1, smem, stream, threads, a, sh, a.space);
+    return launch_rows(kernel, a.in, 1, smem, stream, threads, a, sh, a.space, chunks);
 }
 
 template <int kTeam>
@@ -2919,7 +2919,8 @@ int64_t sample_space(const SampleArgs& a) {
     // a longer top-k is the cluster's kernel's for every row
     const bool long_list = !a.top_k && a.top_k_all > kSampleList && a.top_k_all < a.in.V;
     if (long_list || !scans(a.in, by_lists(a), a.top_k != nullptr)) return 0;
-    return scan_bytes(a.in, scan_shape(a.in, element_size(a.in.dtype), sample_take(a)), true);
+    // the chunks' sums are for rows with a temperature alone
+    return scan_bytes(a.in, scan_shape(a.in, element_size(a.in.dtype), sample_take(a)), !by_lists(a));
 }
 
 int64_t top_space(const TopArgs& a) {
@@ -2936,22 +2937,23 @@ cudaError_t launch_sample(const SampleArgs& given, cudaStream_t stream) {
     const bool lists = greedy || by_lists(a);
     if (sample_space(a) > 0 && !ratio && scans(a.in, lists, a.top_k != nullptr)) {
         const ScanShape scan = scan_shape(a.in, element_size(a.in.dtype), sample_take(a));
+        const bool chunks = !by_lists(a);
         cudaError_t err;
         switch (a.in.dtype) {
             case kF32:
-                err = launch_scan<float, SampleArgs, false>(a, scan, true, stream);
-                if (err == cudaSuccess) err = launch_finish(sample_finish_kernel<float>, a, scan, 512, stream);
+                err = launch_scan<float, SampleArgs, false>(a, scan, chunks, stream);
+                if (err == cudaSuccess) err = launch_finish(sample_finish_kernel<float>, a, scan, chunks, 512, stream);
                 break;
             case kF16:
-                err = launch_scan<__half, SampleArgs, false>(a, scan, true, stream);
-                if (err == cudaSuccess) err = launch_finish(sample_finish_kernel<__half>, a, scan, 512, stream);
+                err = launch_scan<__half, SampleArgs, false>(a, scan, chunks, stream);
+                if (err == cudaSuccess) err = launch_finish(sample_finish_kernel<__half>, a, scan, chunks, 512, stream);
                 break;
             default:
-                err = launch_scan<__nv_bfloat16, SampleArgs, false>(a, scan, true, stream);
-                if (err == cudaSuccess) err = launch_finish(sample_finish_kernel<__nv_bfloat16>, a, scan, 512, stream);
+                err = launch_scan<__nv_bfloat16, SampleArgs, false>(a, scan, chunks, stream);
+                if (err == cudaSuccess) err = launch_finish(sample_finish_kernel<__nv_bfloat16>, a, scan, chunks, 512, stream);
         }
         if (err != cudaSuccess) return err;
-        a.left = scan_of(a.space, a.in.rows, scan, true).left;
+        a.left = scan_of(a.space, a.in.rows, scan, chunks).left;
     }
     const int es = element_size(a.in.dtype);
     const Shape sh = shape_of(a.in, es, 68 * 1024, a.left != nullptr);
@@ -2967,7 +2969,7 @@ cudaError_t launch_top(const TopArgs& given, cudaStream_t stream) {
         cudaError_t err = a.in.dtype == kF32   ? launch_scan<float, TopArgs, true>(a, scan, false, stream)
                           : a.in.dtype == kF16 ? launch_scan<__half, TopArgs, true>(a, scan, false, stream)
                                                : launch_scan<__nv_bfloat16, TopArgs, true>(a, scan, false, stream);
-        if (err == cudaSuccess) err = launch_finish(top_finish_kernel, a, scan, 256, stream);
+        if (err == cudaSuccess) err = launch_finish(top_finish_kernel, a, scan, false, 256, stream);
         if (err != cudaSuccess) return err;
         a.left = scan_of(a.space, a.in.rows, scan, false).left;
     }

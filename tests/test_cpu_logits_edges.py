@@ -94,3 +94,15 @@ def test_c_more_rows_than_an_int_counts(libdbs):
     for rows in (2 ** 31, 2 ** 62):
         assert libdbs.dbs_device_sample_workspace_bytes(0, rows, 32000, 8, 0.9, ctypes.byref(size)) == 0 and size.value == 0
         assert libdbs.dbs_device_top_log_probs_workspace_bytes(0, rows, 32000, 8, ctypes.byref(size)) == 0 and size.value == 0
+
+
+def test_c_workspace_of_a_common_top_k_holds_no_chunk_sums(libdbs):
+    """128 sums of 8 bytes for each part of a row are for rows that every token can come from; a top-k for all rows leaves none."""
+    def bytes_of(rows, V, top_k, top_p):
+        size = ctypes.c_int64()
+        assert libdbs.dbs_device_sample_workspace_bytes(2, rows, V, top_k, top_p, ctypes.byref(size)) == 0
+        return size.value
+
+    # 4 parts of 128256 bf16 with the least share each: state and list, below 2 KB, and the row's place in the list of those left over
+    assert 0 < bytes_of(2048, 128256, 8, 1.0) < 2048 * 4 * 1024 < bytes_of(2048, 128256, 0, 1.0)
+    assert bytes_of(2048, 128256, 50, 1.0) == bytes_of(2048, 128256, 50, 0.9)
