@@ -2352,7 +2352,6 @@ __global__ void __cluster_dims__(8, 1, 1) __launch_bounds__(1024) losses_kernel(
 struct DistillShared {
     float2 box[2][kMaxCluster];   // reference and sum of the CTAs' slices
     float2 part[kWarps];          // and of the warps' vectors
-    float ends[32];               // the slice's elements that no whole vector holds
     uint32_t end_marks[2];        // which of these are listed
     int i32[32];
     uint4 marks[2][kThreads];     // a bit for each of a thread's elements: those that are listed
