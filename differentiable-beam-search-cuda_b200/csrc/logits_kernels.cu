@@ -2270,6 +2270,15 @@ __global__ void __launch_bounds__(256) slots_kernel(DistillArgs a, uint32_t mask
     }
 }
 
+// Is there a rest's class: is P_r, a sum `rest` of exponentials by the reference
+// `best_rest` beside the row's `all`, above 0? As in 64 bits: what is below
+// 2^-1075 of the row's maximum (to the octave) is nothing, so that tokens
+// masked by their type's lowest value make no class of their own.
+__device__ __forceinline__ bool has_rest(float rest, float best_rest, float all, float c2) {
+    const int octaves = (__float_as_int(rest) >> 23) - 127;
+    return rest > 0.0f && (all == best_rest || (all - best_rest) * c2 < static_cast<float>(1075 + octaves));
+}
+
 // A row's loss from its sums. Other CTAs have written them: past L1.
 __device__ double row_loss(const DistillArgs& a, const DistillState& state, int64_t row, double c) {
     const RowState* at = state.rows + row;
@@ -2282,7 +2291,8 @@ __device__ double row_loss(const DistillArgs& a, const DistillState& state, int6
     };
     const double Z = by(s.best_rest, s.rest) + by(s.best_listed, s.listed);
     if (Z == 0.0) return s.Q > 0.0 ? static_cast<double>(INFINITY) : 0.0;   // nothing above -inf
-    const double left = a.tail && s.rest > 0.0f ? fmax(0.0, 1.0 - s.Q) : 0.0;
+    const float c2 = fminf(1.4426950408889634f / a.temperature, FLT_MAX);
+    const double left = a.tail && has_rest(s.rest, s.best_rest, all, c2) ? fmax(0.0, 1.0 - s.Q) : 0.0;
     // log P = c (x - all) - log Z
     double loss = s.C;
     if (s.Q != 0.0) {
@@ -2605,7 +2615,7 @@ __global__ void __launch_bounds__(kThreads, 3) distill_kernel(DistillArgs a, int
             const float Z = (rest.y == 0.0f ? 0.0f : rest.y * share(rest.x, all, c2)) +
                             (known.listed == 0.0f ? 0.0f : known.listed * share(known.best_listed, all, c2));
             const float q_rest =
-                a.tail && rest.y > 0.0f ? static_cast<float>(fmax(0.0, 1.0 - known.Q)) : 0.0f;
+                a.tail && has_rest(rest.y, rest.x, all, c2) ? static_cast<float>(fmax(0.0, 1.0 - known.Q)) : 0.0f;
             const float w = unit * g;
             const float G = (static_cast<float>(known.Q) + q_rest) * (Z == 0.0f ? 0.0f : __fdividef(1.0f, Z));
             // P / P_r = exponential by the rest's reference / its sum, and P =

@@ -818,7 +818,8 @@ def distillation_loss(logits: torch.Tensor, teacher_log_probs: torch.Tensor, tea
     [0, V) is empty. With P the student's probabilities and q the teacher's, a
     row's loss is sum q (log q - log P) over its slots; with `tail`, all tokens
     that are not listed make up one more class of mass 1 - sum q (without it,
-    that mass is left out). A row without slots has loss 0 and gradient 0
+    that mass is left out); where all of these are masked, by -inf or some 745
+    temperatures below the row's maximum, there is no such class. A row without slots has loss 0 and gradient 0
     whatever its logits hold, and "mean" divides by the number of the others;
     "sum" and "none" (each row's, [...]) are the other reductions. `scale`
     multiplies the loss (temperature ** 2 is usual); a factor given here costs

@@ -204,7 +204,9 @@ DBS_EXPORT int dbs_device_top_log_probs_workspace_bytes(int data_type, int64_t r
  * slot's log-prob, P_r = sum of P outside S, and q_r = max(0, 1 - sum q)
  * where `tail` is set and P_r > 0, else 0, a row's loss is
  *   sum_j q_j (log q_j - log P_j) + q_r (log q_r - log P_r),   0 log 0 = 0,
- * and 0 for a row without slots, whatever its logits hold. `reduction`:
+ * and 0 for a row without slots, whatever its logits hold. P_r > 0 is meant as
+ * in 64 bits: exponentials by the row's maximum that add up to less than
+ * 2^-1075 (masks by the type's lowest value) are none. `reduction`:
  * DBS_REDUCE_NONE (row_losses [rows] alone; loss NULL), _SUM, or _MEAN over
  * the rows with slots; `scale` multiplies the result. row_losses [rows] is
  * needed for every reduction. grad_logits ([rows, vocab_size] contiguous, the

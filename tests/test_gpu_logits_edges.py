@@ -130,3 +130,44 @@ def test_no_forward_derivative():
             with torch.set_grad_enabled(grad), pytest.raises(RuntimeError, match="forward-mode"):
                 ext.distillation_loss(dual, lq, at)
         assert torch.equal(ext.distillation_loss(x, lq, at), ext.distillation_loss(x.clone(), lq, at))
+
+
+def distill_by_logarithms(x, lq, listed, T, tail):
+    """Row losses and gradients where the first `listed` tokens are listed: from logarithms, as exponentials near 2^-1074 have few bits
+    in 64 (exp(-740) is 85 steps of 2^-1074). A rest's class is one whose exponentials by the row's maximum add up to 2^-1075."""
+    z = x.double() / T
+    log_P = z - torch.logsumexp(z, dim=1, keepdim=True)
+    log_rest = torch.logsumexp(log_P[:, listed:], dim=1)
+    q = lq.double().exp()
+    q_rest = (1.0 - q.sum(dim=1)).clamp(min=0.0) * (tail and 1.0) * (torch.logsumexp(z[:, listed:], dim=1) - z.amax(dim=1) > -1075.0 * math.log(2.0))
+    loss = (q * (lq.double() - log_P[:, :listed])).sum(dim=1)
+    loss = loss + torch.where(q_rest > 0, q_rest * (q_rest.log() - log_rest), 0.0)
+    total = (q.sum(dim=1) + q_rest)[:, None]
+    share = torch.where(q_rest[:, None] > 0, q_rest[:, None] * (log_P - log_rest[:, None]).exp(), 0.0)
+    share[:, :listed] = q
+    return loss.numpy(), ((total * log_P.exp() - share) / T).numpy(), ((total * log_P.exp() + share) / T).numpy()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("tail", [True, False])
+def test_distillation_all_but_masked_tokens_listed(dtype, tail):
+    """What no slot lists is masked: by the lowest value or another far below the rest there is no rest's class (its mass is 0 in 64
+    bits), and no gradient there; from 745 T below the maximum on (750 for 3300 tokens together) there is one."""
+    V, n = 4000, 700
+    masks = [torch.finfo(dtype).min, -math.inf, -3e4, -800.0, -750.0, -740.0, -700.0, -100.0, -5.0]
+    x = rows(2 * len(masks), V, dtype, 3).clamp(-20.0, 0.0)
+    x[:, 17] = 0.0
+    for r, mask in enumerate(masks):
+        x[2 * r:2 * r + 2, n:] = mask
+    at = torch.arange(n).expand(len(x), n).contiguous()
+    lq = torch.log_softmax(x[:, :n].float() + torch.randn((1, n), generator=torch.Generator().manual_seed(2)), dim=1) - 0.7
+    for T, one_left in ((1.0, False), (2.0, False), (1.0, True)):
+        if one_left:
+            x[1::2, n + 9] = -30.0                # one token of the rest is not masked
+        want, grad, size = distill_by_logarithms(x, lq, n, T, tail)
+        leaf = x.cuda().requires_grad_(True)
+        loss = ext.distillation_loss(leaf, lq.cuda(), at.cuda(), temperature=T, tail=tail, reduction="none")
+        got, = torch.autograd.grad(loss.sum(), leaf)
+        off = np.abs(loss.detach().cpu().double().numpy() - want) - ref.loss_bound(want, 745.0)
+        assert off.max() <= 0.0, (off.max(), off.argmax())
+        assert np.all(np.abs(got.cpu().double().numpy() - grad) <= ref.grad_bound(grad, size, 1.0, dtype))
