@@ -218,6 +218,13 @@ struct Min {
     __device__ T operator()(T a, T b) const { return a < b ? a : b; }
 };
 
+template <class T>
+__device__ __forceinline__ T shuffle_up(T v, int o) { return __shfl_up_sync(kAll, v, o); }
+__device__ __forceinline__ unsigned __int128 shuffle_up(unsigned __int128 v, int o) {
+    const uint64_t high = __shfl_up_sync(kAll, static_cast<uint64_t>(v >> 64), o);
+    return static_cast<unsigned __int128>(high) << 64 | __shfl_up_sync(kAll, static_cast<uint64_t>(v), o);
+}
+
 // Sum of the values of the threads before this one, and (`all`) of all.
 template <int kTeam, class T>
 __device__ __forceinline__ T block_before(T v, T* scratch, T* all = nullptr) {
@@ -225,7 +232,7 @@ __device__ __forceinline__ T block_before(T v, T* scratch, T* all = nullptr) {
     T incl = v;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const T up = __shfl_up_sync(kAll, incl, o);
+        const T up = shuffle_up(incl, o);
         if (lane >= o) incl += up;
     }
     if (lane == 31) scratch[warp] = incl;
@@ -239,7 +246,7 @@ __device__ __forceinline__ T block_before(T v, T* scratch, T* all = nullptr) {
     }
     __syncthreads();
     if (all) *all = total;
-    T excl = __shfl_up_sync(kAll, incl, 1);
+    T excl = shuffle_up(incl, 1);
     if (lane == 0) excl = T(0);
     return base + excl;
 }
@@ -378,7 +385,7 @@ struct Shared {
     double masses[kMaxCluster];
     int ties[kMaxCluster];
     double d8[kMostWarps];
-    unsigned long long u8[kMostWarps];
+    unsigned __int128 u16[kMostWarps];
     float f8[kMostWarps];
     int i8[kMostWarps];
     double range_mass[kMostWarps];
@@ -386,8 +393,8 @@ struct Shared {
     __align__(16) int steps[128];
     int listed;
     int found_bin;
-    unsigned long long found_above;
-    unsigned long long totals[kMaxCluster];
+    unsigned __int128 found_above;
+    unsigned __int128 totals[kMaxCluster];
 };
 
 struct Team {      // a CTA's place in its cluster
@@ -414,9 +421,9 @@ struct Team {      // a CTA's place in its cluster
 // the whole number nearest to d c (within -2^15 and 2^15), a table of 2^(j/32)
 // (an entry per lane) and the Taylor polynomial of 2^(r/32) to the fourth
 // power: what it leaves out is at most (ln 2 / 64)^5 / 120 = 1.3e-12. All 32
-// lanes of a warp call it together.
+// lanes of a warp call it together. `up` octaves are added.
 __device__ __forceinline__ double exp_table() { return exp2(static_cast<double>(threadIdx.x & 31) * 0.03125); }
-__device__ __forceinline__ double exp_by(double d, double c, int n, double tab) {
+__device__ __forceinline__ double exp_by(double d, double c, int n, double tab, int up = 0) {
     constexpr double kL = 0.021660849392498290;   // ln 2 / 32
     const double nd = __hiloint2double(0x43300000, n ^ static_cast<int>(0x80000000)) - 4503601774854144.0;
     const double r = fma(d, c, -nd);
@@ -425,7 +432,7 @@ __device__ __forceinline__ double exp_by(double d, double c, int n, double tab) 
     p = fma(r, p, kL);
     p = fma(r, p, 1.0);
     p *= __shfl_sync(kAll, tab, n & 31);
-    return __hiloint2double(__double2hiint(p) + ((n >> 5) << 20), __double2loint(p));
+    return __hiloint2double(__double2hiint(p) + (((n >> 5) + up) << 20), __double2loint(p));
 }
 
 // ---------------------------------------------------------------------------
@@ -455,12 +462,13 @@ struct Weights {
         cs = static_cast<float>(c * (tiny ? 1.5777218104420236e-30 : 2.0));
         tab = exp_table();
     }
-    // All 32 lanes of the warp call it together.
-    __device__ __forceinline__ double operator()(float x) const {
+    // All 32 lanes of the warp call it together. `up`: octaves by which a weight
+    // other than the best one's is taken up.
+    __device__ __forceinline__ double operator()(float x, int up = 0) const {
         // 0 * inf and inf - inf come out as NaN, which fmaxf drops
         const float t = fmaxf(fmaf(x, s, -ms) * cs, -40000.0f);
         const int n = __float_as_int(t + 12582912.0f) - 0x4B400000;
-        const double p = exp_by(static_cast<double>(x) - m, c, n, tab);
+        const double p = exp_by(static_cast<double>(x) - m, c, n, tab, up);
         return x == mf ? 1.0 : (n < -32686 ? 0.0 : p);   // exp(-708) and below count as nothing
     }
     // For sums by a finite maximum and a temperature in [1e-36, 1e30]: exp(-690)
@@ -482,8 +490,9 @@ struct Weights {
     }
 };
 
-// A weight as a whole number of 2^-43: sums of these do not depend on their
-// order, and 2^20 of them stay below 2^63.
+// A weight (or one taken up by some octaves, at most about 1) as a whole number
+// of 2^-43: sums of these do not depend on their order, and 2^20 of them stay
+// below 2^63.
 __device__ __forceinline__ unsigned long long fixed(double w) {
     return static_cast<unsigned long long>(__double_as_longlong(w + 512.0) - 0x4080000000000000LL);
 }
@@ -502,6 +511,24 @@ __device__ __forceinline__ void add_limbs(uint32_t* bin, unsigned long long w) {
     if (low) atomicAdd(bin, low);
     if (mid) atomicAdd(bin + kBins, mid);
     if (high) atomicAdd(bin + 2 * kBins, high);
+}
+
+// What a search adds up: elements, or weights as whole numbers of 2^-89, so
+// that weights 46 octaves below the best one still have 43 bits (a target p *
+// mass may lie on the border between two equal best tokens but for the mass of
+// all the small ones).
+template <bool kMass>
+struct SumOf {
+    using T = unsigned long long;
+};
+template <>
+struct SumOf<true> {
+    using T = unsigned __int128;
+};
+constexpr int kOctaves = 46;
+__device__ __forceinline__ double real(unsigned long long v) { return static_cast<double>(v); }
+__device__ __forceinline__ double real(unsigned __int128 v) {   // times 2^-89; rounded twice, but never out of order
+    return fma(static_cast<double>(static_cast<uint64_t>(v >> 64)), 0x1p-25, static_cast<double>(static_cast<uint64_t>(v)) * 0x1p-89);
 }
 
 // Where an ordered row is cut: every key above `key` is kept, and of those
@@ -531,7 +558,8 @@ __device__ __forceinline__ void for_elements(const uint4* buf, const Slice& s, F
 // bins per CTA, adds the cluster's bins and keeps the bin that reaches the
 // target; the first round's bins are equal steps of the value over
 // [best - span, best] (a last one holds the rest), later ones equal steps of
-// the key, until a bin is one value.
+// the key, until a bin is one value. Weights are taken up by whole octaves, as
+// many as their bin of the first round lies below the best value.
 // For kMass, `target` comes in as the share p, and becomes p * (all members'
 // mass + extra); where the members fall short of it, ok is false.
 // Returns the key reached, and the count or mass above it.
@@ -551,9 +579,18 @@ __device__ Found search(const Team& team, Shared& sh, uint32_t* hist, const uint
     int lin = -1;                 // the first round's bin, once known
     uint32_t lo = floor_key + 1, hi = key_of<E>(best);
     int shift = 0;
-    unsigned long long above = 0;
+    using Sum = typename SumOf<kMass>::T;
+    Sum above = 0;
+    Sum* totals = reinterpret_cast<Sum*>(sh.totals);
+    Sum* found_above = reinterpret_cast<Sum*>(&sh.found_above);
     Found out;
     out.total = 0.0;
+    // octaves between bins of the first round, in 2^-14, rounded down
+    const int bin_octaves =
+        kMass ? static_cast<int>(fmin(static_cast<double>(span) / (kBins - 1) * weight.c * 0.03125, 1.0 * kOctaves) * 16384.0) : 0;
+    auto octaves = [&](int l) { return min(kOctaves, l * bin_octaves >> 14); };
+    // by all lanes of the warp together; what is asked for with a bin of -1 is not used
+    auto taken_up = [&](float x, int l) { return kMass ? fixed(weight(x, octaves(l))) : 1ull; };
     auto lin_bin = [&](float x) {
         // also right for infinite operands: inf - inf is NaN, and fminf drops it
         const float b = x == best ? 0.0f : fminf((best - x) * scale, static_cast<float>(kBins - 1));
@@ -584,14 +621,14 @@ __device__ Found search(const Team& team, Shared& sh, uint32_t* hist, const uint
 #pragma unroll
                 for (int e = 0; e < kVec; ++e) {
                     if (!__any_sync(kAll, bin[e] >= 0)) continue;
-                    const unsigned long long w = kMass ? fixed(weight(x[e])) : 1ull;
+                    const unsigned long long w = taken_up(x[e], lin);
                     if (bin[e] >= 0) add_limbs<kMass>(hist + bin[e], w);
                 }
                 continue;
             }
             unsigned long long w[kVec];
 #pragma unroll
-            for (int e = 0; e < kVec; ++e) w[e] = kMass ? fixed(weight(x[e])) : 1ull;
+            for (int e = 0; e < kVec; ++e) w[e] = taken_up(x[e], bin[e]);
 #pragma unroll
             for (int e = 0; e < kVec; ++e) {
                 if (bin[e] < 0) continue;
@@ -629,48 +666,51 @@ __device__ Found search(const Team& team, Shared& sh, uint32_t* hist, const uint
                 }
             }
         }
-        unsigned long long own = 0;
+        auto in_bin = [&](int q) {
+            return static_cast<Sum>(h[q]) << (kMass ? kOctaves - octaves(round == 0 ? first + q : lin) : 0);
+        };
+        Sum own = 0;
 #pragma unroll
-        for (int q = 0; q < kEach; ++q) own += h[q];
-        unsigned long long of_share;
-        const unsigned long long in_share = block_before<kTeam>(own, sh.u8, &of_share);
-        team.tell(sh.totals, of_share);
+        for (int q = 0; q < kEach; ++q) own += in_bin(q);
+        Sum of_share;
+        const Sum in_share = block_before<kTeam>(own, reinterpret_cast<Sum*>(sh.u16), &of_share);
+        team.tell(totals, of_share);
         cluster_sync(team.size);
-        unsigned long long total = 0, before = above + in_share;
+        Sum total = 0, before = above + in_share;
         for (int c = 0; c < team.size; ++c) {
-            if (c < team.rank) before += sh.totals[c];
-            total += sh.totals[c];
+            if (c < team.rank) before += totals[c];
+            total += totals[c];
         }
         if (round == 0) {
             if (kMass) {
-                out.total = static_cast<double>(total) + extra;
+                out.total = real(total) + extra;
                 target *= out.total;
             }
             out.target = target;
-            out.ok = static_cast<double>(total) >= target && total > 0;
+            out.ok = real(total) >= target && total > 0;
             if (!out.ok) {
                 cluster_sync(team.size);
                 out.key = floor_key;
-                out.above = static_cast<double>(total);
+                out.above = real(total);
                 return out;
             }
         }
-        if (static_cast<double>(before) < target && static_cast<double>(before + own) >= target) {
-            unsigned long long run = before;
+        if (real(before) < target && real(before + own) >= target) {
+            Sum run = before;
 #pragma unroll
             for (int q = 0; q < kEach; ++q) {
                 if (first + q >= last) break;
-                const bool here = static_cast<double>(run) < target && static_cast<double>(run + h[q]) >= target;
+                const bool here = real(run) < target && real(run + in_bin(q)) >= target;
                 for (int c = 0; here && c < team.size; ++c) {
                     *cg::this_cluster().map_shared_rank(&sh.found_bin, c) = first + q;
-                    *cg::this_cluster().map_shared_rank(&sh.found_above, c) = run;
+                    *cg::this_cluster().map_shared_rank(found_above, c) = run;
                 }
-                run += h[q];
+                run += in_bin(q);
             }
         }
         cluster_sync(team.size);
         const int b = sh.found_bin;
-        above = sh.found_above;
+        above = *found_above;
         __syncthreads();
         if (round == 0) {
             lin = b;
@@ -684,7 +724,7 @@ __device__ Found search(const Team& team, Shared& sh, uint32_t* hist, const uint
         } else {
             if (shift == 0) {
                 out.key = hi - static_cast<uint32_t>(b);
-                out.above = static_cast<double>(above);
+                out.above = real(above);
                 return out;
             }
             hi = hi - (static_cast<uint32_t>(b) << shift);
@@ -1264,17 +1304,18 @@ __global__ void __launch_bounds__(kTeam) sample_kernel(SampleArgs a, int S, int 
                 if (f.ok) {
                     cut.key = f.key;
                     cut.ties = k - static_cast<int>(f.above);
-                    cut_mass = static_cast<double>(fixed(weight(value_of<E>(f.key))));
+                    cut_mass = weight(value_of<E>(f.key));
                 }
             }
             if (p < 1.0) {
-                const float span = fminf(fmaxf(32.0f * temperature, FLT_MIN), FLT_MAX);
+                // (2047 / span has to stay finite)
+                const float span = fminf(fmaxf(32.0f * temperature, 1.0e-35f), FLT_MAX);
                 const Found f = search<kTeam, E, true>(team, sh, hist, buf, s, weight, span, cut.key, p,
                                                 static_cast<double>(cut.ties) * cut_mass);
                 if (f.ok) {
                     cut.key = f.key;
                     cut.ties = 0x7FFFFFFF;
-                    cut_mass = static_cast<double>(fixed(weight(value_of<E>(f.key))));
+                    cut_mass = weight(value_of<E>(f.key));
                 }
                 // of the equal ones, as many as reach the target
                 const double left = ceil((f.target - f.above) / cut_mass);

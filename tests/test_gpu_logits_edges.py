@@ -171,3 +171,18 @@ def test_distillation_all_but_masked_tokens_listed(dtype, tail):
         off = np.abs(loss.detach().cpu().double().numpy() - want) - ref.loss_bound(want, 745.0)
         assert off.max() <= 0.0, (off.max(), off.argmax())
         assert np.all(np.abs(got.cpu().double().numpy() - grad) <= ref.grad_bound(grad, size, 1.0, dtype))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("N,V", [(4, 60), (4, 3000), (3, 60000), (200, 60000)])
+def test_sample_top_p_at_a_border_that_small_weights_move(N, V, dtype):
+    """`ties` best tokens, and 40 whose mass (from 1.8e-13 on) times p makes a token more than p * ties of the best ones stay: their
+    part of the target is 4e-14 and more, 200 steps of a sum in 64 bits."""
+    for ties, p in ((2, 0.5), (4, 0.25), (4, 0.75), (8, 0.875)):
+        for low in (-33.0, -31.75, -24.0, -20.5):
+            x = torch.full((N, V), -math.inf)
+            x[:, 3:3 + ties] = 0.0
+            x[:, V - 41:V - 1] = low
+            for u in (0.05, 0.3, 0.6, 0.95):
+                check_sample(x.to(dtype), torch.full((N,), u), p=p)
+                check_sample(x.to(dtype), torch.full((N,), u), p=p, k=V - 30)
