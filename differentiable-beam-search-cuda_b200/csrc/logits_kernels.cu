@@ -26,7 +26,7 @@ constexpr int kWarps = kThreads / 32;
 // Threads of the kernels that give a row to a cluster, their `kTeam`: lists are
 // bound by their barriers, searches and sums over a slice by arithmetic. One
 // row of 32000 bf16, top_k 50: 9.8 us with 256, 11.2 us with 512; one of
-// 128256, top_p alone: 34.3 us with 256, 32.0 us with 512.
+// 128256, top_p alone: 38.3 us with 256, 37.7 us with 512.
 constexpr int kListTeam = 256;
 constexpr int kMassTeam = 512;
 constexpr int kMostWarps = kMassTeam / 32;
@@ -1021,8 +1021,8 @@ __global__ void __launch_bounds__(kTeam) top_kernel(TopArgs a, int S, int cap) {
 // bins), then the token by a sum in index order over the cluster, the CTAs'
 // warps and a warp's elements. Bound by latency where a list is enough (one
 // row of 32000 bf16, top_k 50: 10.0 us), else by the weights in 64 bits,
-// taken three times (twice by the search, once by the choice): one row of 128256 bf16, top_p 0.9 alone, 32 us, of a
-// floor of 0.04.
+// taken three times (twice by the search, once by the choice): one row of 128256 bf16, top_p 0.9 alone, 37.7 us, of a
+// floor of 0.04 (34.4 with weights as whole numbers of 2^-43, see SumOf).
 // ---------------------------------------------------------------------------
 
 // The token that index order and the uniform number give among the elements
@@ -1357,11 +1357,14 @@ __global__ void __launch_bounds__(kTeam) sample_kernel(SampleArgs a, int S, int 
 //
 // A part's vectors are a thread's own from the copy to the last use, so that
 // copies need no barrier, and are copied ahead by cp.async, 64 KB a CTA, three
-// CTAs on an SM; that keeps HBM busy while others count. Bound by issue: 11
+// CTAs on an SM; the next part's begin when this part's last vector has been
+// used. Bound by latency at 24 warps an SM (barriers, the loads that follow one
+// another in a part) with issue next, active in 52 % of the cycles: 11
 // instructions an element with the exponential (2048 rows of 128256 bf16, n =
-// 64: about 160 of 185 us, 3.3 TB/s), 34 with a weight in 64 bits (512 rows of
-// them, temperature alone: about 95 of 109 us). Also measured there, in us: a warp per
-// part without barriers 236, the cluster's kernel for all rows 383 and 269.
+// 64: about 160 of 185 us, 3.3 TB/s). With a weight in 64 bits it is 34, active
+// in 65 % (512 rows of them, temperature alone: about 95 of 109 us). Also
+// measured there, in us: a warp per part without barriers 236, the cluster's
+// kernel for all rows 385 and 264.
 // ---------------------------------------------------------------------------
 struct PartState {
     double sum;
@@ -1384,8 +1387,9 @@ constexpr int kHold = 16;       // most chunks of a part, and most vectors of a 
 constexpr int kScanBins = 128;
 constexpr int kMaxParts = 32;   // a part per lane where they are put together
 // Candidates listed for a top-p without a top-k: 64 rows of 50257 fp32, top_p
-// 0.95, min_p 0.02 take 42 us with 512, 56 with 256 and 57 with 1024; 256 rows
-// of 128256 with their own settings 113, 96 and 117.
+// 0.95, min_p 0.02 take 42 us with 512, 57 with 256 and 46 with 1024; 256 rows
+// of 128256 with their own settings 114, 98 and 112: there 256 would be the
+// better choice, and nothing known before the call separates the two.
 constexpr int kNucleus = 512;
 
 __host__ __device__ __forceinline__ ScanState scan_of(void* space, int64_t rows, ScanShape sh, bool chunks) {
@@ -2416,9 +2420,14 @@ struct DistillShared {
 // starts the copy of the next row's vector as soon as it has used one, so
 // there are two barriers a row: for the row's sum, and before the listed
 // places are written a second time. 64 KB of slice a CTA, three CTAs on an SM.
-// Bound by issue, near the memory's rate: 14 instructions an element for sum
-// and gradient; 4096 rows of 128256 bf16 take about 410 of the call's 435 us,
-// 5.1 TB/s. Also measured there, in us: 655 with the slots and losses in this
+// Bound by latency at 24 warps an SM (barriers, the exponentials' pipe), with
+// 14 instructions an element for sum and gradient, issue active in half of the
+// cycles; 4096 rows of 128256 bf16, a tenth of them without a teacher, take
+// about 410 of the call's 435 us, 4.9 TB/s of what is read and written. A slice
+// that is not full costs nearly what a full one does (1025 rows of fp32: 12
+// vectors a thread, 49152 elements a row, 93 us; 16 vectors, 65536, 115 us), and
+// ends out of phase with 16 bytes 7 us there (50257 against 50256 elements).
+// Also measured on the 4096 rows, in us: 655 with the slots and losses in this
 // kernel (20 barriers a row), 666 by one CTA a row reading it twice (9 % of the
 // second reads hit L2), 582 with the exponentials kept in registers, 518 with
 // slices of 48 KB.
@@ -2909,11 +2918,16 @@ ScanShape scan_shape(const Rows& in, int es, int take) {
 // where a row needs more than eight CTAs. Sums in 64 bits (a top-p without a
 // top-k, temperature alone) gain earlier; with settings of each row (`both`)
 // rows have to be longer. Measured in us, scan against cluster's kernel, bf16:
-//   top_k 50: 512 x 32000 36 / 26, 64 x 128256 18 / 14, 128 x 128256 23 / 28, 512 x 128256 58 / 101
-//   n = 64: 2048 x 32000 78 / 88, 48 x 128256 15 / 15, 2048 x 128256 185 / 383; one row of 256000 fp32 12.5 / 16.8
-//   temperature alone: 128 x 32000 19 / 16, 400 x 16384 26 / 34, 512 x 128256 109 / 269; one of 200000 12.4 / 18.5
-//   top_p 0.9: 64 x 32000 46 / 36, 32 x 128256 40 / 50, 64 x 128256 51 / 91; one of 200000 20 / 47
-//   each row's own: 1024 x 8192 141 / 124, 64 x 32000 51 / 35, 256 x 32000 82 / 85, 256 x 128256 113 / 221
+//   top_k 50: 512 x 32000 37 / 26, 64 x 128256 18 / 14, 128 x 128256 23 / 28, 512 x 128256 59 / 101
+//   n = 64: 512 x 32000 31 / 28, 1024 x 32000 47 / 50, 2048 x 32000 79 / 89, 4096 x 32000 150 / 172, 48 x 128256 16 / 15,
+//     2048 x 128256 186 / 385; one row of 256000 fp32, n = 128, 12.7 / 16.6
+//   temperature alone: 128 x 32000 19 / 16, 400 x 16384 26 / 33, 512 x 128256 109 / 264; one of 200000 12.6 / 18.0
+//   top_p 0.9, min_p 0.02: 64 x 32000 47 / 37, 16 x 128256 35 / 70, 32 x 128256 40 / 53, 64 x 128256 52 / 99; one of 200000 20 / 52
+//   top_p 0.9 alone: 64 x 32000 92 / 38, 16 x 128256 74 / 71, 32 x 128256 82 / 54, 64 x 128256 128 / 104; one of 200000 61 / 56
+//   each row's own: 1024 x 8192 142 / 131, 64 x 32000 52 / 37, 256 x 32000 84 / 89, 256 x 128256 114 / 225
+// Where the rule takes the slower side: n = 64 of 1024 rows of 32000 and more (by 6 to 15 %; one border serves top_k and n,
+// and top_k loses there), up to 38 rows of 128256 with top-p and min-p, and a top-p alone whose rows are flat, as these are
+// (their nuclei are longer than the list, so that they are looked through twice), which a rule on sizes cannot tell.
 bool scans(const Rows& in, bool lists, bool both) {
     if (in.rows > INT_MAX) return false;   // the list of rows left over holds ints
     const int es = element_size(in.dtype);
