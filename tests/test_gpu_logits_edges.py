@@ -183,6 +183,10 @@ def test_sample_top_p_at_a_border_that_small_weights_move(N, V, dtype):
             x = torch.full((N, V), -math.inf)
             x[:, 3:3 + ties] = 0.0
             x[:, V - 41:V - 1] = low
+            x = x.to(dtype)
+            dev = x.cuda()
             for u in (0.05, 0.3, 0.6, 0.95):
-                check_sample(x.to(dtype), torch.full((N,), u), p=p)
-                check_sample(x.to(dtype), torch.full((N,), u), p=p, k=V - 30)
+                for k in (0, V - 30):     # (the rows are the same)
+                    want = ref.sample(x[:1], [np.float32(u)], [1.0], [k], [np.float32(p)], [0.0])
+                    got = ext.sample(dev, torch.full((N,), u, device="cuda", dtype=torch.float32), top_p=p, top_k=k)
+                    assert got.cpu().tolist() == [int(want[0])] * N
